@@ -457,6 +457,78 @@ int wrnn_wavernn_set_path(wrnn_wavernn* h, int path);
 int wrnn_mol_sample(const float* y, const float* u_mix, const float* u_logistic, int B, int nr_mix, int T,
                     float log_scale_min, float* out, int32_t* mix_out, void* stream);
 
+/* ------------------------------------------------------- self-attention of the forward models' transformers */
+
+/* The core of nn.MultiheadAttention in FFTBlock (models/common_layers.py:148-185), between its projections, with what the
+ * reference's module cannot do: shared key heads, causality, a relative position bias without a dense mask.
+ *   S[b,h,i,j] = scale * q[b,h,i,:] . k[b, h / (heads / kv_heads), j, :] + bias_table[bucket(j - (i + start_b)), h]
+ *   out = softmax over the allowed keys of S, times v;  lse = log of the sum of exp(S) over them
+ * Key j is allowed for query i of row b if j < key_lens[b], key_mask[b, j] == 0 and, with `causal`, j <= i + start_b;
+ * start_b = q_start[b], or k_len - q_len if q_start is NULL (the queries are the last positions).  A query without any
+ * allowed key gets out = 0, lse = -inf and takes part in no gradient.  Keys and values at places that lengths, mask or (for
+ * every query of the row) causality leave out are never used, whatever they hold.
+ *
+ * All pointers are device pointers of `dtype` unless stated; strides count elements for [batch, head, position], the head
+ * dimension is contiguous.  Sums, maxima and exponentials are held in 32 bits; with WRNN_BFLOAT16 the probabilities and the
+ * scores' gradients are rounded to bfloat16 where they enter a matrix product.
+ *
+ * Buckets: a distance d = |j - (i + start_b)| below E = side / 2 has a bucket of its own, above it a bucket E + (number of
+ * bucket_edges <= d); side = num_buckets, or num_buckets / 2 with `bidirectional`, where keys behind the query (positive
+ * j - position) use the second half of the table; one-sided tables give them bucket 0.  bucket_edges is a HOST array of
+ * side - E - 1 ascending distances in [E, max_distance]; wavernn_amd.attention.bucket_edges() gives the usual logarithmic ones. */
+#define WRNN_FLOAT32 0
+#define WRNN_BFLOAT16 1
+typedef struct wrnn_attention_desc {
+  int32_t dtype;      /* WRNN_FLOAT32 or WRNN_BFLOAT16: q, k, v, out and their gradients */
+  int32_t batch, heads, kv_heads, q_len, k_len;
+  int32_t head_dim;   /* 1 .. 256 */
+  int32_t causal;
+  int32_t num_buckets, max_distance, bidirectional; /* used with bias_table; max_distance <= 1024 */
+  float scale;
+  const void* q;      /* [batch, heads, q_len, head_dim] */
+  const void* k;      /* [batch, kv_heads, k_len, head_dim] */
+  const void* v;
+  int64_t q_stride[3], k_stride[3], v_stride[3];
+  const uint8_t* key_mask; /* [batch, k_len], non-zero leaves a key out, or NULL */
+  int64_t key_mask_stride; /* of a batch row */
+  const int32_t* key_lens; /* [batch] or NULL; values are clamped to 0 .. k_len */
+  const int32_t* q_start;  /* [batch] or NULL */
+  const float* bias_table; /* [num_buckets, heads] fp32 or NULL */
+  const int32_t* bucket_edges; /* host */
+} wrnn_attention_desc;
+
+/* lse [batch, heads, q_len] fp32 or NULL.  The workspace (device) is needed for calls with few queries, whose keys are divided
+ * over workgroups: the other size is 0.  It is free again once the call's work on `stream` is done. */
+size_t wrnn_attention_workspace_bytes(const wrnn_attention_desc* desc);
+int wrnn_attention_forward(const wrnn_attention_desc* desc, void* out, const int64_t out_stride[3], float* lse, void* workspace,
+                           size_t workspace_bytes, void* stream);
+
+/* The backward pass; recomputes the probabilities from lse, so nothing of size q_len x k_len is kept or written.  All
+ * sums have a fixed order: the same inputs give the same bits. */
+typedef struct wrnn_attention_grads {
+  const void* out;   /* of the forward pass */
+  const float* lse;  /* of the forward pass */
+  const void* dout;  /* [batch, heads, q_len, head_dim] */
+  void* dq;
+  void* dk;          /* [batch, kv_heads, k_len, head_dim], summed over the heads that share them; dk and dv may both be NULL */
+  void* dv;
+  float* dtable;     /* [num_buckets, heads] or NULL */
+  int64_t out_stride[3], dout_stride[3], dq_stride[3], dk_stride[3], dv_stride[3];
+} wrnn_attention_grads;
+size_t wrnn_attention_backward_workspace_bytes(const wrnn_attention_desc* desc);
+int wrnn_attention_backward(const wrnn_attention_desc* desc, const wrnn_attention_grads* grads, void* workspace, size_t workspace_bytes,
+                            void* stream);
+
+/* The same bias as a dense [heads, q_len, k_len] tensor, as the additive attn_mask of nn.MultiheadAttention takes it, and its
+ * table's gradient: out[h,i,j] = table[bucket(j - (i + start)), h];  dtable[n,h] = sum of dout[h,i,j] over the pairs of bucket n.
+ * table, out, dout, dtable: contiguous, all of `dtype`; sums in 32 bits or more, in a fixed order.  `start`: position of query 0 among the keys. */
+int wrnn_relative_bias_forward(const void* table, int dtype, int heads, int q_len, int k_len, int start, int num_buckets,
+                               int max_distance, int bidirectional, const int32_t* bucket_edges, void* out, void* stream);
+size_t wrnn_relative_bias_workspace_bytes(int heads, int q_len, int k_len, int num_buckets, int max_distance);
+int wrnn_relative_bias_backward(const void* dout, int dtype, int heads, int q_len, int k_len, int start, int num_buckets,
+                                int max_distance, int bidirectional, const int32_t* bucket_edges, void* dtable, void* workspace,
+                                size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

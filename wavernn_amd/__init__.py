@@ -5,7 +5,7 @@ of them (SURVEY.md section 8, rows a-e and f1-f4) live here; everything runs thr
 Importing the package does not need a GPU; calling an op without one, or without the built
 library, raises.
 """
-__all__ = ["Decoder", "LengthRegulator", "Tacotron", "BiLSTM", "BiGRU", "DurationExtractor", "ForwardTacotron", "FastPitch", "MultiFastPitch", "MultiForwardTacotron", "WaveRNN", "synth"]
+__all__ = ["Decoder", "LengthRegulator", "Tacotron", "BiLSTM", "BiGRU", "DurationExtractor", "ForwardTacotron", "FastPitch", "MultiFastPitch", "MultiForwardTacotron", "WaveRNN", "RelativePositionBias", "synth"]
 
 
 def __getattr__(name):  # lazy: `import wavernn_amd.synth` must not need torch
@@ -36,4 +36,7 @@ def __getattr__(name):  # lazy: `import wavernn_amd.synth` must not need torch
     if name == "DurationExtractor":
         from .duration_extractor import DurationExtractor
         return DurationExtractor
+    if name == "RelativePositionBias":
+        from .attention import RelativePositionBias
+        return RelativePositionBias
     raise AttributeError(name)

@@ -89,6 +89,23 @@ class WaveRnnWeights(C.Structure):
     _fields_ = [(name, C.c_void_p) for name, _ in WAVERNN_FIELDS]
 
 
+I64x3 = C.c_int64 * 3
+
+
+class AttentionDesc(C.Structure):
+    _fields_ = ([(n, C.c_int32) for n in ("dtype", "batch", "heads", "kv_heads", "q_len", "k_len", "head_dim", "causal",
+                                          "num_buckets", "max_distance", "bidirectional")]
+                + [("scale", C.c_float)] + [(n, C.c_void_p) for n in ("q", "k", "v")]
+                + [(n, I64x3) for n in ("q_stride", "k_stride", "v_stride")]
+                + [("key_mask", C.c_void_p), ("key_mask_stride", C.c_int64), ("key_lens", C.c_void_p), ("q_start", C.c_void_p),
+                   ("bias_table", C.c_void_p), ("bucket_edges", C.POINTER(C.c_int32))])
+
+
+class AttentionGrads(C.Structure):
+    _fields_ = ([(n, C.c_void_p) for n in ("out", "lse", "dout", "dq", "dk", "dv", "dtable")]
+                + [(n, I64x3) for n in ("out_stride", "dout_stride", "dq_stride", "dk_stride", "dv_stride")])
+
+
 # every symbol include/wrnn_mi355.h declares: name -> (restype, argtypes)
 _P, _I, _F = C.c_void_p, C.c_int, C.c_float
 SYMBOLS = {
@@ -123,6 +140,13 @@ SYMBOLS = {
     "wrnn_bilstm_set_path": (_I, [_P, _I]),
     "wrnn_bigru_create": (_I, [_I, _I, C.POINTER(BiGruWeights), _I, C.POINTER(_P)]),
     "wrnn_bigru_destroy": (_I, [_P]),
+    "wrnn_attention_workspace_bytes": (C.c_size_t, [C.POINTER(AttentionDesc)]),
+    "wrnn_attention_forward": (_I, [C.POINTER(AttentionDesc), _P, I64x3, _P, _P, C.c_size_t, _P]),
+    "wrnn_attention_backward_workspace_bytes": (C.c_size_t, [C.POINTER(AttentionDesc)]),
+    "wrnn_attention_backward": (_I, [C.POINTER(AttentionDesc), C.POINTER(AttentionGrads), _P, C.c_size_t, _P]),
+    "wrnn_relative_bias_forward": (_I, [_P] + [_I] * 8 + [C.POINTER(C.c_int32), _P, _P]),
+    "wrnn_relative_bias_workspace_bytes": (C.c_size_t, [_I] * 5),
+    "wrnn_relative_bias_backward": (_I, [_P] + [_I] * 8 + [C.POINTER(C.c_int32), _P, _P, C.c_size_t, _P]),
     "wrnn_bigru_forward": (_I, [_P, _P, _P, _I, _I, _F, _P, _P, _P]),
 }
 

@@ -1,0 +1,267 @@
+"""Self-attention of the forward models' transformer blocks (models/common_layers.py:148-185), forward and backward, and the
+learned relative position bias by buckets that it applies without a dense mask.
+
+``attention(q, k, v, ...)`` is the part of ``nn.MultiheadAttention`` between its projections; ``forward_models.FFTBlock`` calls
+it with the attention path ``'fused'``.  ``RelativePositionBias`` holds the table of a position bias: called, it gives the dense
+``[heads, q_len, k_len]`` tensor that ``nn.MultiheadAttention`` takes as an additive mask; given to ``attention`` as ``bias_table`` it
+never becomes one.  The kernels run in libwrnn_mi355.so (include/wrnn_mi355.h states the formulas); there is no CPU fallback.
+
+Types: float32 and bfloat16.  All sums, maxima and exponentials are held in 32 bits; in bfloat16 the probabilities and the scores'
+gradients are rounded where they enter a matrix product.  The same inputs give the same bits, gradients included.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import functools
+import math
+from typing import Optional
+
+import torch
+import torch.nn as nn
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1}   # WRNN_FLOAT32, WRNN_BFLOAT16
+MAX_DISTANCE, MAX_BUCKETS, MAX_HEAD_DIM = 1024, 256, 256
+
+
+@functools.lru_cache(maxsize=64)
+def _edges(num_buckets: int, max_distance: int, bidirectional: bool):
+    """(edges as a list, the same as a host int32 array).  A distance d at or above E = side / 2 goes to bucket
+    E + floor(log(d / E) / log(max_distance / E) * (side - E)); edge k is the first d with d^n E^k >= max_distance^k E^n, n = side - E,
+    found in whole numbers because the logarithms come out a hair low or high where a border falls on a whole distance."""
+    side = num_buckets // 2 if bidirectional else num_buckets
+    if not 2 <= num_buckets <= MAX_BUCKETS or (bidirectional and (num_buckets % 2 or side < 2)):
+        raise ValueError(f"num_buckets must be in 2..{MAX_BUCKETS}, and even and at least 4 with two sides, got {num_buckets}")
+    if not side // 2 < max_distance <= MAX_DISTANCE:
+        raise ValueError(f"max_distance must be in {side // 2 + 1}..{MAX_DISTANCE}, got {max_distance}")
+    e = side // 2
+    n = side - e
+    edges, d = [], e
+    for k in range(1, n):
+        while d ** n * e ** k < max_distance ** k * e ** n:
+            d += 1
+        edges.append(d)
+    return edges, (C.c_int32 * max(1, len(edges)))(*edges)
+
+
+def bucket_edges(num_buckets: int = 32, max_distance: int = 128, bidirectional: bool = True) -> list:
+    """The distances at which each bucket above the exact ones begins (``bucket_edges`` of the C ABI)."""
+    return list(_edges(num_buckets, max_distance, bidirectional)[0])
+
+
+def _on_gpu(t: torch.Tensor, what: str) -> None:
+    if t.device.type != 'cuda':
+        raise RuntimeError(f"wavernn_amd.{what} runs only on an MI355X (HIP) device; there is no CPU fallback")
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """The kernels take any strides but that of the last dimension."""
+    return t if t.stride(3) == 1 or t.shape[3] == 1 else t.contiguous()
+
+
+def _strides(t: torch.Tensor):
+    return t.stride()[:3]
+
+
+def _empty_like(t: torch.Tensor) -> torch.Tensor:
+    """Dense, its batch / head / position order in memory as t's: the projections around attention then need no copy."""
+    if t.is_contiguous():
+        return torch.empty_like(t)
+    s = t.stride()
+    order = sorted(range(3), key=lambda i: (-s[i], i)) + [3]
+    return torch.empty([t.shape[i] for i in order], dtype=t.dtype, device=t.device).permute([order.index(i) for i in range(4)])
+
+
+def _desc(q, k, v, table, key_mask, key_lens, q_start, causal, scale, max_distance, bidirectional):
+    B, H, Tq, D = q.shape
+    edges = None
+    if table is not None:
+        edges = _edges(table.shape[0], max_distance, bidirectional)[1]
+    I3 = _lib.I64x3
+    return _lib.AttentionDesc(_DTYPES[q.dtype], B, H, k.shape[1], Tq, k.shape[2], D, causal, 0 if table is None else table.shape[0],
+                              max_distance, bidirectional, scale, q.data_ptr(), k.data_ptr(), v.data_ptr(), I3(*_strides(q)),
+                              I3(*_strides(k)), I3(*_strides(v)), None if key_mask is None else key_mask.data_ptr(),
+                              0 if key_mask is None else key_mask.stride(0), None if key_lens is None else key_lens.data_ptr(),
+                              None if q_start is None else q_start.data_ptr(), None if table is None else table.data_ptr(), edges)
+
+
+def _forward(desc, q, lse):
+    lib = _lib.load()
+    out = _empty_like(q)
+    size = lib.wrnn_attention_workspace_bytes(C.byref(desc))
+    space = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
+    _lib.check(lib.wrnn_attention_forward(C.byref(desc), out.data_ptr(), _lib.I64x3(*_strides(out)), None if lse is None else lse.data_ptr(),
+                                          None if space is None else space.data_ptr(), size,
+                                          torch.cuda.current_stream(q.device).cuda_stream), "wrnn_attention_forward")
+    return out
+
+
+class _Attention(torch.autograd.Function):
+
+    @staticmethod
+    def forward(ctx, q, k, v, table, key_mask, key_lens, q_start, causal, scale, max_distance, bidirectional):
+        ctx.rule = (causal, scale, max_distance, bidirectional)
+        with torch.cuda.device(q.device):
+            lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device)
+            out = _forward(_desc(q, k, v, table, key_mask, key_lens, q_start, *ctx.rule), q, lse)
+        ctx.save_for_backward(q, k, v, table, key_mask, key_lens, q_start, out, lse)
+        ctx.mark_non_differentiable(lse)
+        return out, lse
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout, _):
+        q, k, v, table, key_mask, key_lens, q_start, out, lse = ctx.saved_tensors
+        want_table = table is not None and ctx.needs_input_grad[3]
+        B, H, Tq, _ = q.shape
+        if not (B and H and Tq):
+            return (torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v), torch.zeros_like(table) if want_table else None) + (None,) * 7
+        lib = _lib.load()
+        want_keys = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
+        with torch.cuda.device(q.device):
+            dout = _rows(dout)
+            dq = _empty_like(q)
+            dk, dv = (_empty_like(k), _empty_like(v)) if want_keys else (None, None)
+            dtable = torch.empty_like(table) if want_table else None
+            desc = _desc(q, k, v, table, key_mask, key_lens, q_start, *ctx.rule)
+            I3 = _lib.I64x3
+            none = I3(0, 0, 0)
+            grads = _lib.AttentionGrads(out.data_ptr(), lse.data_ptr(), dout.data_ptr(), dq.data_ptr(), dk.data_ptr() if want_keys else None,
+                                        dv.data_ptr() if want_keys else None, dtable.data_ptr() if want_table else None,
+                                        I3(*_strides(out)), I3(*_strides(dout)), I3(*_strides(dq)),
+                                        I3(*_strides(dk)) if want_keys else none, I3(*_strides(dv)) if want_keys else none)
+            size = lib.wrnn_attention_backward_workspace_bytes(C.byref(desc))
+            space = torch.empty(size, dtype=torch.uint8, device=q.device)
+            _lib.check(lib.wrnn_attention_backward(C.byref(desc), C.byref(grads), space.data_ptr(), size,
+                                                   torch.cuda.current_stream(q.device).cuda_stream), "wrnn_attention_backward")
+        return (dq, dk, dv, dtable) + (None,) * 7
+
+
+def _whole(t: Optional[torch.Tensor], B: int, q: torch.Tensor, name: str) -> Optional[torch.Tensor]:
+    if t is None:
+        return None
+    if t.dtype not in (torch.int32, torch.int64) or tuple(t.shape) != (B,) or t.device != q.device:
+        raise ValueError(f"{name} must be an int32 or int64 tensor [{B}] on {q.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.clamp(-(1 << 30), 1 << 30).to(torch.int32) if t.dtype == torch.int64 else t.contiguous()
+
+
+def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, key_mask: Optional[torch.Tensor] = None,
+              key_lens: Optional[torch.Tensor] = None, q_start: Optional[torch.Tensor] = None, causal: bool = False,
+              scale: Optional[float] = None, bias_table: Optional[torch.Tensor] = None, max_distance: int = 128,
+              bidirectional: bool = True, return_lse: bool = False):
+    """softmax(scale * q k^T + bias) v over the allowed keys; differentiable in q, k, v and bias_table.
+
+    q [B, H, Tq, D], k and v [B, Hkv, Tk, D] with H a multiple of Hkv (head h reads key head h // (H // Hkv)), D up to 256, any
+    strides.  The result has q's shape and its order in memory.
+
+    key_mask [B, Tk] bool: True leaves a key out (``key_padding_mask`` of nn.MultiheadAttention).  key_lens [B]: keys at or past a
+    row's length are left out.  causal: query i of row b sees keys up to position i + q_start[b]; q_start [B] defaults to Tk - Tq, the
+    queries being the last positions.  A query that is left no key gives zeros and takes part in no gradient.  What lies at keys that are left
+    out for a whole row is never used, NaN and infinities included.
+    scale: 1 / sqrt(D) by default.
+    bias_table [num_buckets, H] (``RelativePositionBias.weight``) adds table[bucket(j - (i + q_start[b])), h]; max_distance and
+    bidirectional are its rule.  -inf in a table leaves its distances out.
+    return_lse: also the log of each query's sum of exponentials, [B, H, Tq] float32, -inf for a query without keys (no gradient)."""
+    _on_gpu(q, "attention")
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
+        raise ValueError(f"expected q [B,H,Tq,D] and k, v [B,Hkv,Tk,D], got {tuple(q.shape)}, {tuple(k.shape)} and {tuple(v.shape)}")
+    if q.dtype not in _DTYPES or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError(f"attention takes float32 or bfloat16, the same for q, k and v, got {q.dtype}, {k.dtype} and {v.dtype}")
+    dev = q.device
+    if k.device != dev or v.device != dev:
+        raise RuntimeError("q, k and v must be on the same device")
+    B, H, Tq, D = q.shape
+    if not 1 <= D <= MAX_HEAD_DIM:
+        raise ValueError(f"head dimension {D} is outside 1..{MAX_HEAD_DIM}")
+    if k.shape[1] == 0 or H % k.shape[1]:
+        raise ValueError(f"{H} heads do not share {k.shape[1]} key heads evenly")
+    if key_mask is not None:
+        if key_mask.dtype != torch.bool or tuple(key_mask.shape) != (B, k.shape[2]) or key_mask.device != dev:
+            raise ValueError(f"key_mask must be a bool tensor [{B}, {k.shape[2]}] on {dev}, got {key_mask.dtype} {tuple(key_mask.shape)} "
+                             f"on {key_mask.device}")
+        if key_mask.stride(1) != 1 and key_mask.shape[1] > 1:
+            key_mask = key_mask.contiguous()
+    key_lens, q_start = _whole(key_lens, B, q, "key_lens"), _whole(q_start, B, q, "q_start")
+    if bias_table is not None:
+        if bias_table.dim() != 2 or bias_table.shape[1] != H or bias_table.device != dev or bias_table.dtype not in _DTYPES:
+            raise ValueError(f"bias_table must be a float32 or bfloat16 tensor [num_buckets, {H}] on {dev}, got {bias_table.dtype} "
+                             f"{tuple(bias_table.shape)} on {bias_table.device}")
+        bias_table = bias_table.float().contiguous()
+        _edges(bias_table.shape[0], max_distance, bidirectional)   # checks the rule
+    if scale is None:
+        scale = 1.0 / math.sqrt(D)
+    q, k, v = _rows(q), _rows(k), _rows(v)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
+                                    or (bias_table is not None and bias_table.requires_grad)):
+        out, lse = _Attention.apply(q, k, v, bias_table, key_mask, key_lens, q_start, causal, scale, max_distance, bidirectional)
+        return (out, lse) if return_lse else out
+    with torch.cuda.device(dev):
+        lse = torch.empty(q.shape[:3], dtype=torch.float32, device=dev) if return_lse else None
+        out = _forward(_desc(q, k, v, bias_table, key_mask, key_lens, q_start, causal, scale, max_distance, bidirectional), q, lse)
+    return (out, lse) if return_lse else out
+
+
+class _RelativeBias(torch.autograd.Function):
+
+    @staticmethod
+    def forward(ctx, table, q_len, k_len, start, max_distance, bidirectional):
+        ctx.rule = (table.shape[1], q_len, k_len, start, table.shape[0], max_distance, bidirectional)
+        lib = _lib.load()
+        with torch.cuda.device(table.device):
+            out = torch.empty(table.shape[1], q_len, k_len, dtype=table.dtype, device=table.device)
+            _lib.check(lib.wrnn_relative_bias_forward(table.data_ptr(), _DTYPES[table.dtype], *ctx.rule, _edges(table.shape[0], max_distance, bidirectional)[1],
+                                                      out.data_ptr(), torch.cuda.current_stream(table.device).cuda_stream),
+                       "wrnn_relative_bias_forward")
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        H, q_len, k_len, _, buckets, max_distance, bidirectional = ctx.rule
+        if not (H and q_len and k_len):
+            return (dout.new_zeros(buckets, H),) + (None,) * 5
+        lib = _lib.load()
+        with torch.cuda.device(dout.device):
+            dout = dout.contiguous()
+            dtable = torch.empty(buckets, H, dtype=dout.dtype, device=dout.device)
+            size = lib.wrnn_relative_bias_workspace_bytes(H, q_len, k_len, buckets, max_distance)
+            space = torch.empty(size, dtype=torch.uint8, device=dout.device)
+            _lib.check(lib.wrnn_relative_bias_backward(dout.data_ptr(), _DTYPES[dout.dtype], *ctx.rule, _edges(buckets, max_distance, bidirectional)[1],
+                                                       dtable.data_ptr(), space.data_ptr(), size,
+                                                       torch.cuda.current_stream(dout.device).cuda_stream), "wrnn_relative_bias_backward")
+        return (dtable,) + (None,) * 5
+
+
+def relative_position_bias(table: torch.Tensor, q_len: int, k_len: int, *, q_start: Optional[int] = None, max_distance: int = 128,
+                           bidirectional: bool = True) -> torch.Tensor:
+    """table [num_buckets, H] -> [H, q_len, k_len] of the table's type: table[bucket(j - (i + q_start)), h]; q_start defaults to
+    k_len - q_len.  Differentiable in the table."""
+    _on_gpu(table, "relative_position_bias")
+    if table.dim() != 2 or table.dtype not in _DTYPES:
+        raise TypeError(f"expected a float32 or bfloat16 table [num_buckets, heads], got {table.dtype} {tuple(table.shape)}")
+    if q_len < 0 or k_len < 0:
+        raise ValueError(f"negative length ({q_len}, {k_len})")
+    _edges(table.shape[0], max_distance, bidirectional)
+    return _RelativeBias.apply(table.contiguous(), int(q_len), int(k_len), int(k_len - q_len if q_start is None else q_start),
+                               max_distance, bool(bidirectional))
+
+
+class RelativePositionBias(nn.Module):
+    """A learned bias on attention scores by the distance from query to key: exact buckets near, logarithmic ones up to
+    ``max_distance``, one for everything beyond; with ``bidirectional`` half of them for keys behind the query.  Build extension, not
+    in the reference."""
+
+    def __init__(self, heads: int, num_buckets: int = 32, max_distance: int = 128, bidirectional: bool = True):
+        super().__init__()
+        _edges(num_buckets, max_distance, bidirectional)
+        self.max_distance, self.bidirectional = max_distance, bidirectional
+        self.weight = nn.Parameter(torch.empty(num_buckets, heads).normal_(std=0.02))
+
+    def forward(self, q_len: int, k_len: int, q_start: Optional[int] = None) -> torch.Tensor:
+        return relative_position_bias(self.weight, q_len, k_len, q_start=q_start, max_distance=self.max_distance,
+                                      bidirectional=self.bidirectional)
+
+    def extra_repr(self) -> str:
+        return f"heads={self.weight.shape[1]}, num_buckets={self.weight.shape[0]}, max_distance={self.max_distance}, bidirectional={self.bidirectional}"

@@ -15,8 +15,13 @@ LIB_DIR = os.path.join(HERE, "lib")
 OBJ_DIR = os.path.join(LIB_DIR, "obj")
 LIB_PATH = os.path.join(LIB_DIR, "libwrnn_mi355.so")
 SOURCES = ["taco_decoder.hip", "length_regulator.hip", "bilstm.hip", "bigru.hip", "durations.hip", "wavernn.hip",
-           "aligner.hip", "mol.hip"]
+           "aligner.hip", "mol.hip", "attention.hip", "attention_backward.hip", "relative_bias.hip"]
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function"]
+# The attention kernels are built without packed fp32 instructions: some of their forms have given wrong results on this
+# hardware, with no error.  (The host pass does not know the feature and says so; harmless.)  The older kernels keep the code they were
+# verified with: the teacher-forced loop loses 5.5 % without them (13.7 -> 14.5 us per decoder step at B=64).
+NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+SOURCE_FLAGS = {s: NO_PACKED_FP32 for s in ("attention.hip", "attention_backward.hip", "relative_bias.hip")}
 
 
 def _hipcc() -> str:
@@ -53,7 +58,7 @@ def build(force: bool = False, verbose: bool = True) -> str:
     for s in SOURCES:
         src, obj = os.path.join(CSRC, s), os.path.join(OBJ_DIR, s[:-4] + ".o")
         if force or _stale(obj, [src] + hdrs):
-            jobs.append([_hipcc()] + FLAGS + ["-c", src, "-o", obj])
+            jobs.append([_hipcc()] + FLAGS + SOURCE_FLAGS.get(s, []) + ["-c", src, "-o", obj])
 
     def run(cmd):
         if verbose:
