@@ -57,8 +57,10 @@ def _on_gpu(t: torch.Tensor, what: str) -> None:
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
-    """The kernels take any strides but that of the last dimension."""
-    return t if t.stride(3) == 1 or t.shape[3] == 1 else t.contiguous()
+    """The kernels take any strides but that of the last dimension (and positions no further apart than 2^26 elements)."""
+    if (t.stride(3) == 1 or t.shape[3] == 1) and t.stride(2) < 1 << 26:
+        return t
+    return t.contiguous()
 
 
 def _strides(t: torch.Tensor):

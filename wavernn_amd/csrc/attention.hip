@@ -11,12 +11,14 @@ namespace attn {
 // The maximum only moves when a score exceeds it by more than 8 (a factor 256, far inside float's range): most tiles rescale nothing.
 struct Running {
   float m = -3e38f, l = 0.f;
-  template <int DT>
-  __device__ __forceinline__ void step(float (&s)[16], f32x16 (&acc)[DT]) {
-    float mx = s[0];
+  template <int NS, int DT>
+  __device__ __forceinline__ void step(float (&s)[NS][16], f32x16 (&acc)[DT]) {
+    float mx = s[0][0];
 #pragma unroll
-    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
-    mx = fmaxf(mx, other_half(mx));
+    for (int n = 0; n < NS; ++n)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[n][i]);
+    mx = both_max(mx);
     if (__any(mx > m + 8.f)) {
       const float mn = fmaxf(m, mx), a = exp2f(m - mn);
       m = mn;
@@ -25,23 +27,35 @@ struct Running {
       for (int dt = 0; dt < DT; ++dt) acc[dt] *= a;
     }
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      s[i] = __builtin_amdgcn_exp2f(s[i] - m);
-      l += s[i];
-    }
+    for (int n = 0; n < NS; ++n)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[n][i] = __builtin_amdgcn_exp2f(s[n][i] - m);
+        l += s[n][i];
+      }
   }
 };
 
+// Keys of a tile in LDS.
+template <class T>
+constexpr int key_tile() {
+  return sizeof(T) == 2 ? 64 : 32;
+}
+// Two buffers for each tile where they fit.
+template <class T, int DP>
+constexpr int forward_buffers() {
+  return sizeof(T) == 4 && DP == 256 ? 1 : 2;
+}
+
 // 128 queries of one head per workgroup, 32 per wave, against key tiles shared through LDS (two buffers, one barrier a tile).
 template <class T, int DP, bool BIAS>
-__global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attention_forward_kernel(Params p) {
-  using TL = Tile<T, DP>;
-  constexpr int BN = sizeof(T) == 2 ? 64 : 32, NC2 = TL::NCH / 2, DT = DP / 32;
+__global__ __launch_bounds__(256, DP * Type<T>::NP <= 192 ? 2 : 1) void attention_forward_kernel(Params p) {
+  constexpr int BN = key_tile<T>(), NS = BN / 32, NC2 = DP / 16, DT = DP / 32, BUFS = forward_buffers<T, DP>();
+  using TL = Tile<T, DP, BN>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   char* kt = smem;
-  char* vt = smem + 2 * BN * TL::ROWB;
-  float* add = reinterpret_cast<float*>(smem + 4 * BN * TL::ROWB);  // [2][BN]
-  int* word = reinterpret_cast<int*>(add + 2 * BN);
+  char* vt = smem + BUFS * TL::BYTES;
+  int* word = reinterpret_cast<int*>(smem + 2 * BUFS * TL::BYTES);
   float* lut = reinterpret_cast<float*>(word + 4);
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = tid >> 6;
   const int nt = (p.Tq + 127) / 128, n = p.B * p.H * nt, item = xcd_item(n);
@@ -54,60 +68,61 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attention_forward_kerne
   const uint8_t* mask = p.key_mask ? p.key_mask + b * p.mask_b : nullptr;
   const int qi = q0 + wave * 32 + (lane & 31), pos = qi + off;
   const int pos_lo = q0 + wave * 32 + off, pos_hi = pos_lo + 31;
-  typename TL::chunk q[NC2];
-  {
-    const T* row = reinterpret_cast<const T*>(p.q) + b * p.q_b + h * p.q_h + min(qi, p.Tq - 1) * p.q_t;
-#pragma unroll
-    for (int c = 0; c < NC2; ++c) q[c] = load_chunk<T>(row, 2 * c + half, p.D, p.vec);
-  }
+  Stationary<T, DP, false> q;
+  q.load(reinterpret_cast<const T*>(p.q) + b * p.q_b + h * p.q_h + min(qi, p.Tq - 1) * p.q_t, half, p.D, p.vec, true);
   if constexpr (BIAS) fill_lut(p, h, lut, tid, 256);
   const int end = key_end(p, b, min(q0 + 127, p.Tq - 1) + off, word, tid, 256);
   const int tiles = (end + BN - 1) / BN;
   f32x16 acc[DT] = {};
   Running run;
   Stage<T, DP, BN> sk, sv;
+  KeyBits bits(mask, end, lane);
   auto load = [&](int t) {
-    sk.load(kb, p.k_t, t * BN, end, mask, p.D, p.vec, tid);
-    sv.load(vb, p.v_t, t * BN, end, mask, p.D, p.vec, tid);
+    sk.load(kb, p.k_t, t * BN, end, p.D, p.vec, tid);
+    sv.load(vb, p.v_t, t * BN, end, p.D, p.vec, tid);
+    bits.load(t * BN);
   };
   auto store = [&](int t) {
-    const int o = t & 1;
-    sk.store(kt + o * BN * TL::ROWB, tid);
-    sv.store(vt + o * BN * TL::ROWB, tid);
-    if (tid < BN) {
-      const int j = t * BN + tid;
-      add[o * BN + tid] = j < end && !(mask && mask[j]) ? 0.f : -INFINITY;
-    }
+    const uint64_t use = bits.get(t * BN);
+    const int o = t & (BUFS - 1);
+    sk.store(kt + o * TL::BYTES, use, tid);
+    sv.store(vt + o * TL::BYTES, use, tid);
+    return use;
   };
+  uint64_t use = 0, next = 0;
   if (tiles) {
     load(0);
-    store(0);
+    use = store(0);
   }
   __syncthreads();
   for (int t = 0; t < tiles; ++t) {
     if (t + 1 < tiles) load(t + 1);
-    const int o = t & 1;
-    const bool masked = mask || (t + 1) * BN > end;
-    if (q0 + wave * 32 < p.Tq) {
+    const char *kk = kt + (t & (BUFS - 1)) * TL::BYTES, *vv = vt + (t & (BUFS - 1)) * TL::BYTES;
+    const int key0 = t * BN;
+    if (q0 + wave * 32 < p.Tq && !(p.causal && key0 > pos_hi)) {
+      f32x16 raw[NS] = {};
 #pragma unroll
-      for (int sub = 0; sub < BN / 32; ++sub) {
-        const int key0 = t * BN + sub * 32;
-        if (key0 >= end || (p.causal && key0 > pos_hi)) break;
-        const char* kk = kt + o * BN * TL::ROWB;
-        f32x16 raw = {};
+      for (int c = 0; c < NC2; ++c)
 #pragma unroll
-        for (int c = 0; c < NC2; ++c) raw = Type<T>::mma(TL::row_chunk(kk, sub * 32 + (lane & 31), 2 * c + half), q[c], raw);
-        float s[16];
-        finish_scores<BIAS>(p, raw, s, key0, pos, pos_lo, pos_hi, masked ? add + o * BN + sub * 32 : nullptr, lut, half);
-        run.step(s, acc);
-        ColumnProduct<T, DP, DT>::run(vt + o * BN * TL::ROWB, sub * 32, 0, s, acc, lane);
+        for (int s = 0; s < NS; ++s) raw[s] = mma(TL::row_chunk(kk, s * 32 + (lane & 31), 2 * c + half), q.get(c), raw[s]);
+      float s[NS][16];
+#pragma unroll
+      for (int x = 0; x < NS; ++x) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[x][i] = raw[x][i];
+        finish_scores<BIAS>(p, s[x], key0 + 32 * x, pos, pos_lo, pos_hi, (uint32_t)(use >> (32 * x)), lut, half);
       }
+      run.step(s, acc);
+#pragma unroll
+      for (int x = 0; x < NS; ++x) column_product<T, TL>(vv, 32 * x, 0, Weights<T>(s[x]), acc, lane);
     }
-    if (t + 1 < tiles) store(t + 1);
+    if (BUFS == 1) __syncthreads();
+    if (t + 1 < tiles) next = store(t + 1);
+    use = next;
     __syncthreads();
   }
   if (qi >= p.Tq) return;
-  const float l = run.l + other_half(run.l), inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+  const float l = both_sum(run.l), inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
   T* orow = reinterpret_cast<T*>(p.out) + b * p.o_b + h * p.o_h + qi * p.o_t;
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
@@ -121,22 +136,32 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attention_forward_kerne
 // Few queries, or too few workgroups of the kernel above: 32 query columns per workgroup (with p.pack the queries of a whole group
 // of heads that share k and v), its four waves on different 32-key tiles and further splits of the keys on other workgroups.  A
 // wave is on its own until the join: keys go from memory to the matrix instructions' registers, values through a
-// private LDS tile, both requested one tile ahead.
+// private LDS tile of at most 128 columns, both requested one tile ahead where registers allow.
+template <class T, int DP>
+constexpr int split_columns() {
+  return DP > 128 ? 128 : DP;
+}
+template <class T, int DP>
+constexpr size_t split_wave_bytes() {  // a wave's value tile, and later its sums
+  const size_t tile = Tile<T, split_columns<T, DP>(), 32>::BYTES, sums = 32 * (DP + 4) * sizeof(float);
+  return tile > sums ? tile : sums;
+}
 template <class T, int DP, bool BIAS>
 __global__ __launch_bounds__(256, 1) void attention_split_kernel(Params p) {
-  using TL = Tile<T, DP>;
-  constexpr int NC2 = TL::NCH / 2, DT = DP / 32, NV = 32 * TL::NCH / 64;
+  constexpr int NC2 = DP / 16, DT = DP / 32, DV = split_columns<T, DP>(), VP = DP / DV, NCV = DV / 8, NV = 32 * NCV / 64;
+  constexpr bool AHEAD = DP * sizeof(T) <= 512;
+  using TL = Tile<T, DV, 32>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  float* ml = reinterpret_cast<float*>(smem + 4 * 32 * (DP + 4) * sizeof(float));  // [4][2][32]
+  float* ml = reinterpret_cast<float*>(smem + 4 * split_wave_bytes<T, DP>());  // [4][2][32]
   int* word = reinterpret_cast<int*>(ml + 4 * 2 * 32);
   float* lut = reinterpret_cast<float*>(word + 4);
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = tid >> 6, col = lane & 31;
-  char* vt = smem + wave * 32 * (DP + 4) * sizeof(float);
+  char* vt = smem + wave * split_wave_bytes<T, DP>();
   const int heads = p.pack ? p.Hkv : p.H, nq = p.pack ? 1 : (p.Tq + 31) / 32;
   const int n = p.B * heads * nq * p.splits, item = xcd_item(n);
   if (item >= n) return;
   const int split = item % p.splits, r = item / p.splits, qt = r % nq, bh = r / nq, b = bh / heads, hh = bh - b * heads;
-  const int lh = p.pack ? col / p.Tq : 0;                        // the column's head within the group
+  const int lh = p.pack ? col / p.Tq : 0;  // the column's head within the group
   const int h = p.pack ? hh * p.group + min(lh, p.group - 1) : hh, kvh = p.pack ? hh : hh / p.group;
   const int qi = p.pack ? col - lh * p.Tq : qt * 32 + col;
   const int off = start_of(p, b), pos = qi + off;
@@ -144,12 +169,8 @@ __global__ __launch_bounds__(256, 1) void attention_split_kernel(Params p) {
   const T* kb = reinterpret_cast<const T*>(p.k) + b * p.k_b + kvh * p.k_h;
   const T* vb = reinterpret_cast<const T*>(p.v) + b * p.v_b + kvh * p.v_h;
   const uint8_t* mask = p.key_mask ? p.key_mask + b * p.mask_b : nullptr;
-  typename TL::chunk q[NC2];
-  {
-    const T* row = reinterpret_cast<const T*>(p.q) + b * p.q_b + h * p.q_h + min(qi, p.Tq - 1) * p.q_t;
-#pragma unroll
-    for (int c = 0; c < NC2; ++c) q[c] = load_chunk<T>(row, 2 * c + half, p.D, p.vec);
-  }
+  Stationary<T, DP, false> q;
+  q.load(reinterpret_cast<const T*>(p.q) + b * p.q_b + h * p.q_h + min(qi, p.Tq - 1) * p.q_t, half, p.D, p.vec, true);
   const int lut_len = 2 * p.max_distance + 1;
   if constexpr (BIAS) {
     if (p.pack)
@@ -164,51 +185,67 @@ __global__ __launch_bounds__(256, 1) void attention_split_kernel(Params p) {
 
   f32x16 acc[DT] = {};
   Running run;
-  typename TL::chunk k[NC2], v[NV];
-  uint32_t keys = 0;  // of the requested tile: bit r = key r may be used
-  auto load = [&](int t) {
+  Raw<T> k[NC2], v[VP][NV];
+  uint64_t keys = 0;  // of the requested tile: bit r = key r may be used
+  auto load_k = [&](int t) {
     const int row = t * 32 + col, rc = min(row, end - 1);
-    const bool ok = row < end && !(mask && mask[rc]);
-    keys = (uint32_t)__ballot(ok);
+    keys = __ballot(row < end && !(mask && mask[rc]));
+    const T* kr = kb + rc * p.k_t;
 #pragma unroll
-    for (int c = 0; c < NC2; ++c) {
-      const auto x = load_chunk<T>(kb + rc * p.k_t, 2 * c + half, p.D, p.vec);
-      k[c] = ok ? x : typename TL::chunk{};
-    }
+    for (int c = 0; c < NC2; ++c) k[c] = load_chunk<T>(kr, 2 * c + half, p.D, p.vec);
+  };
+  auto load_v = [&](int t, int part) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int id = i * 64 + lane, vr = t * 32 + id / TL::NCH, vc = min(vr, end - 1);
-      const auto x = load_chunk<T>(vb + vc * p.v_t, id % TL::NCH, p.D, p.vec);
-      v[i] = vr < end && !(mask && mask[vc]) ? x : typename TL::chunk{};
+      const int id = i * 64 + lane, vr = t * 32 + id / NCV;
+      v[part][i] = load_chunk<T>(vb + min(vr, end - 1) * p.v_t, part * NCV + id % NCV, p.D, p.vec);
     }
   };
   int t = split * per + wave;
-  if (t < t1) load(t);
+  if (t < t1) {
+    load_k(t);
+    if (AHEAD)
+#pragma unroll
+      for (int part = 0; part < VP; ++part) load_v(t, part);
+  }
   for (; t < t1; t += 4) {
     const int key0 = t * 32;
-    const uint32_t use = keys;
-    // every lane's private-tile reads of the last round are done before this round's writes: LDS operations of a wave stay in order
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-#pragma unroll
-    for (int i = 0; i < NV; ++i) TL::put(vt, (i * 64 + lane) / TL::NCH, (i * 64 + lane) % TL::NCH, v[i]);
+    const uint32_t use = (uint32_t)keys;
     f32x16 raw = {};
+    if (use != ~0u && !((use >> col) & 1)) {
 #pragma unroll
-    for (int c = 0; c < NC2; ++c) raw = Type<T>::mma(k[c], q[c], raw);
-    if (t + 4 < t1) load(t + 4);
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    float s[16];
-    finish_scores<BIAS>(p, raw, s, key0, pos, pos_lo, pos_hi, nullptr, my_lut, half);
-    if (use != ~0u) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] = (use >> moving_row(i, half)) & 1 ? s[i] : -INFINITY;
+      for (int c = 0; c < NC2; ++c) k[c].x = {};
     }
+#pragma unroll
+    for (int c = 0; c < NC2; ++c) raw = mma(operand(k[c]), q.get(c), raw);
+    float s[1][16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[0][i] = raw[i];
+    if (t + 4 < t1) load_k(t + 4);
+    finish_scores<BIAS>(p, s[0], key0, pos, pos_lo, pos_hi, use, my_lut, half);
     run.step(s, acc);
-    ColumnProduct<T, DP, DT>::run(vt, 0, 0, s, acc, lane);
+    const Weights<T> w(s[0]);
+#pragma unroll
+    for (int part = 0; part < VP; ++part) {
+      if (!AHEAD) load_v(t, part);
+      // LDS operations of a wave stay in order: the last reads of the private tile come before these writes
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int vr = (i * 64 + lane) / NCV;
+        if (use != ~0u && !((use >> vr) & 1)) v[part][i].x = {};
+        TL::put(vt, vr, (i * 64 + lane) % NCV, operand(v[part][i]));
+      }
+      if (AHEAD && t + 4 < t1) load_v(t + 4, part);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      f32x16(&mine)[DV / 32] = *reinterpret_cast<f32x16(*)[DV / 32]>(&acc[part * (DV / 32)]);
+      column_product<T, TL>(vt, 0, 0, w, mine, lane);
+    }
   }
   // join the four waves: a common maximum per column, then sums over the waves in their order
-  const float l = run.l + other_half(run.l);
+  const float l = both_sum(run.l);
   if (half == 0) {
     ml[(wave * 2) * 32 + col] = run.m;
     ml[(wave * 2 + 1) * 32 + col] = l;
@@ -236,26 +273,24 @@ __global__ __launch_bounds__(256, 1) void attention_split_kernel(Params p) {
   for (int w = 0; w < 4; ++w) l2 += ml[(w * 2 + 1) * 32 + c2] * exp2f(ml[(w * 2) * 32 + c2] - m2);
   const int lh2 = p.pack ? c2 / p.Tq : 0, h2 = p.pack ? hh * p.group + lh2 : hh, qi2 = p.pack ? c2 - lh2 * p.Tq : qt * 32 + c2;
   if (p.pack ? lh2 >= p.group : qi2 >= p.Tq) return;
-  const float* all4 = reinterpret_cast<const float*>(smem);
   const int64_t row = ((int64_t)b * p.H + h2) * p.Tq + qi2;
+  auto sum = [&](int d) {
+    f32x4 x = {};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) x += *reinterpret_cast<const f32x4*>(smem + w * split_wave_bytes<T, DP>() + (c2 * LD + d) * 4);
+    return x;
+  };
   if (p.splits == 1) {
     const float inv = l2 > 0.f ? 1.f / l2 : (l2 == 0.f ? 0.f : l2);
     T* orow = reinterpret_cast<T*>(p.out) + b * p.o_b + h2 * p.o_h + qi2 * p.o_t;
     for (int d = (tid & 7) * 4; d < DP; d += 32) {
-      f32x4 x = {};
-#pragma unroll
-      for (int w = 0; w < 4; ++w) x += *reinterpret_cast<const f32x4*>(all4 + (w * 32 + c2) * LD + d);
+      const f32x4 x = sum(d);
       store4<T>(orow, d, p.D, p.vec, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
     }
     if ((tid & 7) == 0 && p.lse) p.lse[row] = l2 == 0.f ? -INFINITY : (m2 + log2f(l2)) * kLn2;
   } else {
     float* part = p.part + (row * p.splits + split) * (DP + 4);
-    for (int d = (tid & 7) * 4; d < DP; d += 32) {
-      f32x4 x = {};
-#pragma unroll
-      for (int w = 0; w < 4; ++w) x += *reinterpret_cast<const f32x4*>(all4 + (w * 32 + c2) * LD + d);
-      *reinterpret_cast<f32x4*>(part + 4 + d) = x;
-    }
+    for (int d = (tid & 7) * 4; d < DP; d += 32) *reinterpret_cast<f32x4*>(part + 4 + d) = sum(d);
     if ((tid & 7) == 0) {
       part[0] = m2;
       part[1] = l2;
@@ -318,17 +353,15 @@ static size_t split_workspace(const Params& p) {
 
 template <class T, int DP, bool BIAS>
 static int launch_forward(const Params& p, hipStream_t st) {
-  using TL = Tile<T, DP>;
   static std::atomic<uint64_t> wide_done{0}, split_done{0};
   const size_t lut = BIAS ? lut_floats(p) * sizeof(float) : 0;
   if (p.splits == 0) {
-    constexpr int BN = sizeof(T) == 2 ? 64 : 32;
     return launch(&attention_forward_kernel<T, DP, BIAS>, &wide_done, (int64_t)p.B * p.H * ((p.Tq + 127) / 128),
-                  4 * BN * TL::ROWB + 2 * BN * 4 + 16 + lut, p, st);
+                  2 * forward_buffers<T, DP>() * Tile<T, DP, key_tile<T>()>::BYTES + 16 + lut, p, st);
   }
   const int64_t n = (p.pack ? (int64_t)p.B * p.Hkv : (int64_t)p.B * p.H * ((p.Tq + 31) / 32)) * p.splits;
   if (launch(&attention_split_kernel<T, DP, BIAS>, &split_done, n,
-             4 * 32 * (DP + 4) * sizeof(float) + 4 * 2 * 32 * 4 + 16 + lut * (p.pack ? p.group : 1), p, st))
+             4 * split_wave_bytes<T, DP>() + 4 * 2 * 32 * 4 + 16 + lut * (p.pack ? p.group : 1), p, st))
     return 1;
   if (p.splits > 1) {
     const int64_t rows = (int64_t)p.B * p.H * p.Tq;
@@ -374,6 +407,9 @@ int attention_params(const wrnn_attention_desc* d, attn::Params* p, const char* 
   p->q_b = st(d->batch, d->q_stride[0]), p->q_h = st(d->heads, d->q_stride[1]), p->q_t = st(d->q_len, d->q_stride[2]);
   p->k_b = st(d->batch, d->k_stride[0]), p->k_h = st(d->kv_heads, d->k_stride[1]), p->k_t = st(d->k_len, d->k_stride[2]);
   p->v_b = st(d->batch, d->v_stride[0]), p->v_h = st(d->kv_heads, d->v_stride[1]), p->v_t = st(d->k_len, d->v_stride[2]);
+  // a lane's rows inside a tile are found with 32-bit offsets
+  for (int64_t s : {p->q_t, p->k_t, p->v_t})
+    WRNN_REQUIRE(s > -kMaxRowStride && s < kMaxRowStride, "%s: position strides are below 2^26 elements", who);
   p->B = d->batch, p->H = d->heads, p->Hkv = d->kv_heads, p->group = d->heads ? d->heads / d->kv_heads : 1;
   p->Tq = d->q_len, p->Tk = d->k_len, p->D = d->head_dim;
   p->causal = d->causal != 0;

@@ -48,9 +48,13 @@ struct BiasGrad {
   }
 };
 
+template <class T, int DP>
+constexpr int back_tile() {  // moving rows of a tile in LDS
+  return sizeof(T) == 2 && DP < 256 ? 64 : 32;
+}
 // Two buffers for each tile where they leave room for the position bias's tables.
 template <class T, int DP>
-constexpr int dq_buffers() {
+constexpr int back_buffers() {
   return sizeof(T) == 4 && DP == 256 ? 1 : 2;
 }
 
@@ -60,20 +64,18 @@ constexpr int dq_buffers() {
 // holds most of a row's keys adds that error up over all rows.  There the table's gradient takes delta = sum_j P dP from a first walk over the
 // keys instead.
 template <class T, int DP, int BIAS>
-__global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attention_dq_kernel(Params p) {
-  using TL = Tile<T, DP>;
-  constexpr int BN = sizeof(T) == 2 && DP < 256 ? 64 : 32, NC2 = TL::NCH / 2, DA = DP > 128 ? 128 : DP, DT = DA / 32, PARTS = DP / DA;
-  constexpr bool TWICE = BIAS == 2 && sizeof(T) == 2;
-  constexpr int BUFS = dq_buffers<T, DP>();
+__global__ __launch_bounds__(256, DP * Type<T>::NP <= 128 ? 2 : 1) void attention_dq_kernel(Params p) {
+  constexpr int BN = back_tile<T, DP>(), NC2 = DP / 16, DA = DP > 128 ? 128 : DP, DT = DA / 32, PARTS = DP / DA, BUFS = back_buffers<T, DP>();
+  constexpr bool TWICE = BIAS == 2 && sizeof(T) == 2, RAW = sizeof(T) == 4 && DP == 256;
+  using TL = Tile<T, DP, BN>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   char* kt = smem;
-  char* vt = smem + BUFS * BN * TL::ROWB;
-  float* add = reinterpret_cast<float*>(smem + 2 * BUFS * BN * TL::ROWB);  // [2][BN]
-  int* word = reinterpret_cast<int*>(add + 2 * BN);
+  char* vt = smem + BUFS * TL::BYTES;
+  int* word = reinterpret_cast<int*>(smem + 2 * BUFS * TL::BYTES);
   float* lut = reinterpret_cast<float*>(word + 4);
   const int lut_len = BIAS ? 2 * p.max_distance + 1 : 0, lut_pad = (lut_len + 3) & ~3;
-  float* scratch = lut + lut_pad;                          // [4][32 * LD]
-  float* sums = scratch + 4 * 32 * BiasGrad::LD;           // [4][lut_pad]
+  float* scratch = lut + lut_pad;                 // [4][32 * LD]
+  float* sums = scratch + 4 * 32 * BiasGrad::LD;  // [4][lut_pad]
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = tid >> 6;
   const int nt = (p.Tq + 127) / 128, n = p.B * p.H * nt * PARTS;
   int item = xcd_item(n);
@@ -88,23 +90,22 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attention_dq_kernel(Par
   const uint8_t* mask = p.key_mask ? p.key_mask + b * p.mask_b : nullptr;
   const int qi = q0 + wave * 32 + (lane & 31), qc = min(qi, p.Tq - 1), pos = qi + off;
   const int pos_lo = q0 + wave * 32 + off, pos_hi = pos_lo + 31;
-  typename TL::chunk q[NC2], go[NC2];
+  Stationary<T, DP, RAW> q, go;
   float delta = 0.f;
   {
-    const T* qr = reinterpret_cast<const T*>(p.q) + b * p.q_b + h * p.q_h + qc * p.q_t;
     const T* gr = reinterpret_cast<const T*>(p.dout) + b * p.do_b + h * p.do_h + qc * p.do_t;
-    const T* orow = reinterpret_cast<const T*>(p.o_in) + b * p.oi_b + h * p.oi_h + qc * p.oi_t;
+    q.load(reinterpret_cast<const T*>(p.q) + b * p.q_b + h * p.q_h + qc * p.q_t, half, p.D, p.vec, true);
+    go.load(gr, half, p.D, p.vec, true);
+    if (!TWICE) {
+      const T* orow = reinterpret_cast<const T*>(p.o_in) + b * p.oi_b + h * p.oi_h + qc * p.oi_t;
 #pragma unroll
-    for (int c = 0; c < NC2; ++c) {
-      q[c] = load_chunk<T>(qr, 2 * c + half, p.D, p.vec);
-      go[c] = load_chunk<T>(gr, 2 * c + half, p.D, p.vec);
-      if (!TWICE) {
-        const auto o = load_chunk<T>(orow, 2 * c + half, p.D, p.vec);
+      for (int c = 0; c < NC2; ++c) {
+        const Raw<T> g = load_chunk<T>(gr, 2 * c + half, p.D, p.vec), o = load_chunk<T>(orow, 2 * c + half, p.D, p.vec);
 #pragma unroll
-        for (int e = 0; e < TL::CE; ++e) delta += (float)go[c][e] * (float)o[e];
+        for (int e = 0; e < 8; ++e) delta += (float)g.x[e] * (float)o.x[e];
       }
+      delta = both_sum(delta);
     }
-    delta += other_half(delta);
   }
   const float lse = qi < p.Tq ? p.lse[(int64_t)bh * p.Tq + qi] : -INFINITY;
   const float lse2 = lse == -INFINITY ? INFINITY : lse * kLog2e;  // a row without keys, or none at all: P = exp2(.. - inf) = 0
@@ -116,53 +117,48 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attention_dq_kernel(Par
   f32x16 acc[DT] = {};
   BiasGrad bias_grad;
   Stage<T, DP, BN> sk, sv;
+  KeyBits bits(mask, end, lane);
   auto load = [&](int t) {
-    sk.load(kb, p.k_t, t * BN, end, mask, p.D, p.vec, tid);
-    sv.load(vb, p.v_t, t * BN, end, mask, p.D, p.vec, tid);
+    sk.load(kb, p.k_t, t * BN, end, p.D, p.vec, tid);
+    sv.load(vb, p.v_t, t * BN, end, p.D, p.vec, tid);
+    bits.load(t * BN);
   };
   auto store = [&](int t) {
+    const uint64_t use = bits.get(t * BN);
     const int o = t & (BUFS - 1);
-    sk.store(kt + o * BN * TL::ROWB, tid);
-    sv.store(vt + o * BN * TL::ROWB, tid);
-    if (tid < BN) {
-      const int j = t * BN + tid;
-      add[o * BN + tid] = j < end && !(mask && mask[j]) ? 0.f : -INFINITY;
-    }
-  };
-  // P and dP of one subtile
-  auto pair = [&](int o, int sub, int key0, bool masked, float (&pr)[16], f32x16& dp) {
-    const char *kk = kt + o * BN * TL::ROWB, *vv = vt + o * BN * TL::ROWB;
-    f32x16 raw = {};
-    dp = f32x16{};
-#pragma unroll
-    for (int c = 0; c < NC2; ++c) {
-      raw = Type<T>::mma(TL::row_chunk(kk, sub * 32 + (lane & 31), 2 * c + half), q[c], raw);
-      dp = Type<T>::mma(TL::row_chunk(vv, sub * 32 + (lane & 31), 2 * c + half), go[c], dp);
-    }
-    finish_scores<BIAS != 0>(p, raw, pr, key0, pos, pos_lo, pos_hi, masked ? add + o * BN + sub * 32 : nullptr, lut, half);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) pr[i] = __builtin_amdgcn_exp2f(pr[i] - lse2);
+    sk.store(kt + o * TL::BYTES, use, tid);
+    sv.store(vt + o * TL::BYTES, use, tid);
+    return use;
   };
   const bool live = q0 + wave * 32 < p.Tq;
 #pragma unroll
   for (int walk = TWICE ? 0 : 1; walk < 2; ++walk) {
+    uint64_t use = 0, next = 0;
     if (tiles) {
       load(0);
-      store(0);
+      use = store(0);
     }
     __syncthreads();
     for (int t = 0; t < tiles; ++t) {
       if (t + 1 < tiles) load(t + 1);
-      const int o = t & (BUFS - 1);
-      const bool masked = mask || (t + 1) * BN > end;
+      const char *kk = kt + (t & (BUFS - 1)) * TL::BYTES, *vv = vt + (t & (BUFS - 1)) * TL::BYTES;
       if (live) {
 #pragma unroll
         for (int sub = 0; sub < BN / 32; ++sub) {
           const int key0 = t * BN + sub * 32;
           if (key0 >= end || (p.causal && key0 > pos_hi)) break;
+          f32x16 raw = {}, dp = {};
+#pragma unroll
+          for (int c = 0; c < NC2; ++c) {
+            raw = mma(TL::row_chunk(kk, sub * 32 + (lane & 31), 2 * c + half), q.get(c), raw);
+            dp = mma(TL::row_chunk(vv, sub * 32 + (lane & 31), 2 * c + half), go.get(c), dp);
+          }
           float pr[16];
-          f32x16 dp;
-          pair(o, sub, key0, masked, pr, dp);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) pr[i] = raw[i];
+          finish_scores<BIAS != 0>(p, pr, key0, pos, pos_lo, pos_hi, (uint32_t)(use >> (32 * sub)), lut, half);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) pr[i] = __builtin_amdgcn_exp2f(pr[i] - lse2);
           if (TWICE && walk == 0) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) delta += pr[i] * dp[i];
@@ -171,15 +167,16 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attention_dq_kernel(Par
             for (int i = 0; i < 16; ++i) pr[i] *= dp[i] - delta;
             if constexpr (BIAS == 2)
               if (d0 == 0) bias_grad.add(pr, key0 - pos_lo, p.max_distance, scratch + wave * 32 * BiasGrad::LD, sums + wave * lut_pad, lane);
-            ColumnProduct<T, DP, DT>::run(kt + o * BN * TL::ROWB, sub * 32, d0, pr, acc, lane);
+            column_product<T, TL>(kk, sub * 32, d0, Weights<T>(pr), acc, lane);
           }
         }
       }
       if (BUFS == 1) __syncthreads();
-      if (t + 1 < tiles) store(t + 1);
+      if (t + 1 < tiles) next = store(t + 1);
+      use = next;
       __syncthreads();
     }
-    if (TWICE && walk == 0) delta += other_half(delta);
+    if (TWICE && walk == 0) delta = both_sum(delta);
   }
   if (qi < p.Tq) {
     T* row = reinterpret_cast<T*>(p.dq) + b * p.dq_b + h * p.dq_h + qi * p.dq_t;
@@ -219,15 +216,15 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attention_dq_kernel(Par
 // dk, dv: 128 keys of one key head per workgroup, 32 per wave; tiles of queries and their output gradients through LDS, over all heads of
 // the group.
 template <class T, int DP, bool BIAS>
-__global__ __launch_bounds__(256, 1) void attention_dkv_kernel(Params p) {
-  using TL = Tile<T, DP>;
-  constexpr int BM = sizeof(T) == 2 && DP < 256 ? 64 : 32, NC2 = TL::NCH / 2, DA = DP > 128 ? 128 : DP, DT = DA / 32, PARTS = DP / DA;
+__global__ __launch_bounds__(256, DP * Type<T>::NP <= 64 ? 2 : 1) void attention_dkv_kernel(Params p) {
+  constexpr int BM = back_tile<T, DP>(), NC2 = DP / 16, DA = DP > 128 ? 128 : DP, DT = DA / 32, PARTS = DP / DA, BUFS = back_buffers<T, DP>();
+  constexpr bool RAW = sizeof(T) == 4 && DP == 256;
+  using TL = Tile<T, DP, BM>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   char* qt = smem;
-  char* gt = smem + 2 * BM * TL::ROWB;
-  float* stat = reinterpret_cast<float*>(smem + 4 * BM * TL::ROWB);  // [2][2][BM]: lse in log2 units, delta
-  int* word = reinterpret_cast<int*>(stat + 4 * BM);
-  float* lut = reinterpret_cast<float*>(word + 4);
+  char* gt = smem + BUFS * TL::BYTES;
+  float* stat = reinterpret_cast<float*>(smem + 2 * BUFS * TL::BYTES);  // [BUFS][2][BM]: lse in log2 units, delta
+  float* lut = stat + 4 * BM;
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = tid >> 6;
   const int nt = (p.Tk + 127) / 128, n = p.B * p.Hkv * nt * PARTS;
   int item = xcd_item(n);
@@ -241,17 +238,9 @@ __global__ __launch_bounds__(256, 1) void attention_dkv_kernel(Params p) {
   if (p.key_lens) end = min(end, max(p.key_lens[b], 0));
   if (p.causal) end = min(end, max(p.Tq + off, 0));  // past the last query's reach
   const bool ok = key < end && !(mask && mask[kc]);
-  typename TL::chunk k[NC2], v[NC2];
-  {
-    const T* kr = reinterpret_cast<const T*>(p.k) + b * p.k_b + kvh * p.k_h + kc * p.k_t;
-    const T* vr = reinterpret_cast<const T*>(p.v) + b * p.v_b + kvh * p.v_h + kc * p.v_t;
-#pragma unroll
-    for (int c = 0; c < NC2; ++c) {
-      const auto x = load_chunk<T>(kr, 2 * c + half, p.D, p.vec), y = load_chunk<T>(vr, 2 * c + half, p.D, p.vec);
-      k[c] = ok ? x : typename TL::chunk{};
-      v[c] = ok ? y : typename TL::chunk{};
-    }
-  }
+  Stationary<T, DP, RAW> k, v;
+  k.load(reinterpret_cast<const T*>(p.k) + b * p.k_b + kvh * p.k_h + kc * p.k_t, half, p.D, p.vec, ok);
+  v.load(reinterpret_cast<const T*>(p.v) + b * p.v_b + kvh * p.v_h + kc * p.v_t, half, p.D, p.vec, ok);
   const float add = ok ? 0.f : -INFINITY;
   f32x16 dk[DT] = {}, dv[DT] = {};
   // under causality queries before key - off see nothing of this block
@@ -261,8 +250,8 @@ __global__ __launch_bounds__(256, 1) void attention_dkv_kernel(Params p) {
   float s_lse = 0.f, s_delta = 0.f;
   auto load = [&](int it) {
     const int h = kvh * p.group + it / per, r0 = (qt_0 + it % per) * BM;
-    sq.load(reinterpret_cast<const T*>(p.q) + b * p.q_b + h * p.q_h, p.q_t, r0, p.Tq, nullptr, p.D, p.vec, tid);
-    sg.load(reinterpret_cast<const T*>(p.dout) + b * p.do_b + h * p.do_h, p.do_t, r0, p.Tq, nullptr, p.D, p.vec, tid);
+    sq.load(reinterpret_cast<const T*>(p.q) + b * p.q_b + h * p.q_h, p.q_t, r0, p.Tq, p.D, p.vec, tid);
+    sg.load(reinterpret_cast<const T*>(p.dout) + b * p.do_b + h * p.do_h, p.do_t, r0, p.Tq, p.D, p.vec, tid);
     if (tid < BM) {
       const int64_t row = ((int64_t)b * p.H + h) * p.Tq + r0 + tid;
       const float l = r0 + tid < p.Tq ? p.lse[row] : -INFINITY;
@@ -271,9 +260,9 @@ __global__ __launch_bounds__(256, 1) void attention_dkv_kernel(Params p) {
     }
   };
   auto store = [&](int it) {
-    const int o = it & 1;
-    sq.store(qt + o * BM * TL::ROWB, tid);
-    sg.store(gt + o * BM * TL::ROWB, tid);
+    const int o = it & (BUFS - 1);
+    sq.store(qt + o * TL::BYTES, ~0ull, tid);
+    sg.store(gt + o * TL::BYTES, ~0ull, tid);
     if (tid < BM) {
       stat[o * 2 * BM + tid] = s_lse;
       stat[(o * 2 + 1) * BM + tid] = s_delta;
@@ -292,8 +281,8 @@ __global__ __launch_bounds__(256, 1) void attention_dkv_kernel(Params p) {
     }
     __syncthreads();
     if (it + 1 < steps) load(it + 1);
-    const int o = it & 1, r0 = (qt_0 + it % per) * BM;
-    const char *qq = qt + o * BM * TL::ROWB, *gg = gt + o * BM * TL::ROWB;
+    const int o = it & (BUFS - 1), r0 = (qt_0 + it % per) * BM;
+    const char *qq = qt + o * TL::BYTES, *gg = gt + o * TL::BYTES;
     if (kw < end) {
 #pragma unroll
       for (int sub = 0; sub < BM / 32; ++sub) {
@@ -303,27 +292,28 @@ __global__ __launch_bounds__(256, 1) void attention_dkv_kernel(Params p) {
         f32x16 raw = {}, dp = {};
 #pragma unroll
         for (int c = 0; c < NC2; ++c) {
-          raw = Type<T>::mma(TL::row_chunk(qq, sub * 32 + (lane & 31), 2 * c + half), k[c], raw);
-          dp = Type<T>::mma(TL::row_chunk(gg, sub * 32 + (lane & 31), 2 * c + half), v[c], dp);
+          raw = mma(TL::row_chunk(qq, sub * 32 + (lane & 31), 2 * c + half), k.get(c), raw);
+          dp = mma(TL::row_chunk(gg, sub * 32 + (lane & 31), 2 * c + half), v.get(c), dp);
         }
         float s[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = raw[i] * p.scale2 + add;
         if constexpr (BIAS) {
           const int md = p.max_distance;
           if (kw + 31 - p0 <= -md || kw - (p0 + 31) >= md) {
-            const float far = lut[kw > p0 ? 2 * md : 0];
+            const float far = lut[kw > p0 ? 2 * md : 0] + add;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] += far;
+            for (int i = 0; i < 16; ++i) s[i] = fmaf(raw[i], p.scale2, far);
           } else {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] += lut[min(max(key - p0 - moving_row(i, half), -md), md) + md];
+            for (int i = 0; i < 16; ++i) s[i] = fmaf(raw[i], p.scale2, lut[min(max(key - p0 - moving_row(i, half), -md), md) + md] + add);
           }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[i] = fmaf(raw[i], p.scale2, add);
         }
         if (p.causal && kw + 31 > p0) {
+          const int first = key - p0 - 4 * half;
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (key > p0 + moving_row(i, half)) s[i] = -INFINITY;
+          for (int i = 0; i < 16; ++i) s[i] = first > moving_row(i, 0) ? -INFINITY : s[i];
         }
         const float* l2 = stat + o * 2 * BM + sub * 32 + 4 * half;
         float ds[16];
@@ -337,10 +327,11 @@ __global__ __launch_bounds__(256, 1) void attention_dkv_kernel(Params p) {
             ds[i] = s[i] * (dp[i] - de[e]);
           }
         }
-        ColumnProduct<T, DP, DT>::run(gg, sub * 32, d0, s, dv, lane);
-        ColumnProduct<T, DP, DT>::run(qq, sub * 32, d0, ds, dk, lane);
+        column_product<T, TL>(gg, sub * 32, d0, Weights<T>(s), dv, lane);
+        column_product<T, TL>(qq, sub * 32, d0, Weights<T>(ds), dk, lane);
       }
     }
+    if (BUFS == 1) __syncthreads();
     if (it + 1 < steps) store(it + 1);
   }
   if (key >= p.Tk) return;
@@ -364,15 +355,15 @@ static int dtable_rows(const Params& p) { return p.B * ((p.Tq + 127) / 128); }
 
 template <class T, int DP, int BIAS>
 static int launch_backward(const Params& p, float* dtable, hipStream_t st) {
-  using TL = Tile<T, DP>;
-  constexpr int BN = sizeof(T) == 2 && DP < 256 ? 64 : 32, PARTS = DP > 128 ? 2 : 1;
+  constexpr int PARTS = DP > 128 ? 2 : 1;
+  constexpr size_t tiles = 2 * back_buffers<T, DP>() * Tile<T, DP, back_tile<T, DP>()>::BYTES;
   const size_t lut = BIAS ? (size_t)(2 * p.max_distance + 4) * 4 : 0;
   static std::atomic<uint64_t> dq_done{0}, dkv_done{0};
   if (launch(&attention_dq_kernel<T, DP, BIAS>, &dq_done, (int64_t)p.B * p.H * ((p.Tq + 127) / 128) * PARTS,
-             2 * dq_buffers<T, DP>() * BN * TL::ROWB + 2 * BN * 4 + 16 + lut + (BIAS == 2 ? 4 * (32 * BiasGrad::LD * 4 + lut) : 0), p, st))
+             tiles + 16 + lut + (BIAS == 2 ? 4 * (32 * BiasGrad::LD * 4 + lut) : 0), p, st))
     return 1;
   if (p.dk && p.Tk && launch(&attention_dkv_kernel<T, DP, BIAS != 0>, &dkv_done, (int64_t)p.B * p.Hkv * ((p.Tk + 127) / 128) * PARTS,
-                     4 * BN * TL::ROWB + 4 * BN * 4 + 16 + lut, p, st))
+                             tiles + 4 * back_tile<T, DP>() * 4 + lut, p, st))
     return 1;
   if (BIAS == 2) {
     return launch_table_sum<float>(p.dtable_part, dtable_rows(p), p.H, p.buckets, dtable, st);
@@ -418,6 +409,8 @@ extern "C" int wrnn_attention_backward(const wrnn_attention_desc* desc, const wr
   auto on16 = [&](const void* x, const int64_t* st) { return attn::rows_on_16(x, st[0], st[1], st[2], es); };
   p.vec = p.vec && on16(g->out, g->out_stride) && on16(g->dout, g->dout_stride) && on16(g->dq, g->dq_stride) &&
           on16(g->dk, g->dk_stride) && on16(g->dv, g->dv_stride);
+  for (const int64_t* x : {g->out_stride, g->dout_stride, g->dq_stride, g->dk_stride, g->dv_stride})
+    WRNN_REQUIRE(x[2] > -attn::kMaxRowStride && x[2] < attn::kMaxRowStride, "wrnn_attention_backward: position strides are below 2^26 elements");
   p.o_in = g->out, p.oi_b = g->out_stride[0], p.oi_h = g->out_stride[1], p.oi_t = g->out_stride[2];
   p.dout = g->dout, p.do_b = g->dout_stride[0], p.do_h = g->dout_stride[1], p.do_t = g->dout_stride[2];
   p.dq = g->dq, p.dq_b = g->dq_stride[0], p.dq_h = g->dq_stride[1], p.dq_t = g->dq_stride[2];

@@ -1,15 +1,20 @@
 // Shared device pieces of the attention kernels (attention.hip, attention_backward.hip).
 //
 // Everything is built on one wave tile: 32 "stationary" rows (queries in the forward pass and for dq, keys for dk / dv), one per
-// lane column, against 32 "moving" rows.  With v_mfma_f32_32x32x* the product  X(moving) * Y(stationary)^T  leaves a lane with ONE
-// stationary row and 16 moving rows,
+// lane column, against 32 "moving" rows.  With v_mfma_f32_32x32x16_bf16 the product  X(moving) * Y(stationary)^T  leaves a lane with
+// ONE stationary row and 16 moving rows,
 //     moving row of register i = 8 * (i / 4) + 4 * (lane / 32) + i % 4,
 // so row statistics of the stationary side are sums inside a lane plus one exchange between the wave's halves, and those 16
 // registers are already the right-hand operand of the second product  Z(moving)^T * P : its sum runs over the moving rows, whose
 // order is free as long as both operands use the same one.  No score ever goes through shared memory.
 //
-// Moving tiles lie in LDS row by row in 16-byte chunks.  The first product reads chunk 2c + half of a row per lane; the second
-// reads columns: bfloat16 with ds_read_b64_tr_b16 (four rows x 16 columns transposed per 16 lanes), float32 one word per lane.
+// float32 goes through the same instructions: a value is the sum of three bfloat16 (8 bits of mantissa each, rounded to nearest, so 24 and a
+// sign in each remainder), and a product the six partial products down to 2^-24 of it, added in 32 bits, smallest first.  What is left out
+// is below 2^-25: the result is as exact as the 32-bit matrix instruction's and takes 6 x 32 cycles for 16 columns of a 32 x 32
+// tile where that one takes 8 x 64.
+//
+// Moving tiles lie in LDS row by row in 16-byte chunks of 8 bfloat16 (three planes for float32).  The first product reads chunk 2c + half of
+// a row per lane; the second reads columns with ds_read_b64_tr_b16 (four rows x 16 columns transposed per 16 lanes).
 // swizzle() spreads both kinds of read over the banks.
 #pragma once
 #include <stdint.h>
@@ -31,6 +36,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int kMaxEdges = 128;
 constexpr int kMaxDistance = 1024;
+constexpr int64_t kMaxRowStride = 1 << 26;
 
 // What the kernels get, by value.  Strides count elements; the last dimension is contiguous.
 struct Params {
@@ -57,55 +63,125 @@ struct Params {
   float* part;
 };
 
+// A chunk of 8 elements as the matrix instruction takes it: one bfloat16 plane, or three.
 template <class T>
 struct Type;
 template <>
 struct Type<__bf16> {
-  using chunk = bf16x8;
-  static constexpr int CE = 8;  // elements of a 16-byte chunk
-  static __device__ __forceinline__ f32x16 mma(chunk a, chunk b, f32x16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
-  }
+  static constexpr int NP = 1;
 };
 template <>
 struct Type<float> {
-  using chunk = f32x4;
-  static constexpr int CE = 4;
-  // element e of the two halves' chunks makes one K = 2 product
-  static __device__ __forceinline__ f32x16 mma(chunk a, chunk b, f32x16 c) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
-    return c;
-  }
+  static constexpr int NP = 3;
 };
+template <class T>
+struct Operand {
+  bf16x8 p[Type<T>::NP];
+};
+template <class T>
+struct Raw {  // 8 elements as they come from memory
+  typedef T vec __attribute__((ext_vector_type(8)));
+  vec x;
+};
+
+__device__ __forceinline__ Operand<__bf16> operand(const Raw<__bf16>& r) { return {{r.x}}; }
+__device__ __forceinline__ void split(f32x8 x, bf16x8 (&p)[3]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    p[i] = __builtin_convertvector(x, bf16x8);
+    x -= __builtin_convertvector(p[i], f32x8);  // exact
+  }
+  p[2] = __builtin_convertvector(x, bf16x8);
+}
+__device__ __forceinline__ Operand<float> operand(const Raw<float>& r) {
+  Operand<float> o;
+  split(r.x, o.p);
+  return o;
+}
+
+__device__ __forceinline__ f32x16 mma1(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x16 mma(const Operand<__bf16>& a, const Operand<__bf16>& b, f32x16 c) { return mma1(a.p[0], b.p[0], c); }
+__device__ __forceinline__ f32x16 mma(const Operand<float>& a, const Operand<float>& b, f32x16 c) {
+  c = mma1(a.p[2], b.p[0], c);
+  c = mma1(a.p[0], b.p[2], c);
+  c = mma1(a.p[1], b.p[1], c);
+  c = mma1(a.p[1], b.p[0], c);
+  c = mma1(a.p[0], b.p[1], c);
+  return mma1(a.p[0], b.p[0], c);
+}
 
 __device__ __forceinline__ int moving_row(int i, int half) { return 8 * (i >> 2) + 4 * half + (i & 3); }
 
-// the other half-wave's value
-__device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32); }
+// x combined with the other half-wave's: lane l and lane l ^ 32 get the same
+__device__ __forceinline__ float both_max(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float both_sum(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
 
+// Chunk ch (8 elements) of a row of D; what lies past D is zero and not read.  vec: rows start on 16 bytes and D is a multiple of
+// 16 bytes.
 template <class T>
-__device__ __forceinline__ typename Type<T>::chunk load_chunk(const T* row, int ch, int D, bool vec) {
-  using chunk = typename Type<T>::chunk;
-  constexpr int CE = Type<T>::CE;
-  chunk r = {};
+__device__ __forceinline__ Raw<T> load_chunk(const T* row, int ch, int D, bool vec) {
+  Raw<T> r;
+  r.x = {};
   if (vec) {
-    if (ch * CE < D) r = *reinterpret_cast<const chunk*>(row + ch * CE);
+    if constexpr (sizeof(T) == 2) {
+      if (ch * 8 < D) r.x = *reinterpret_cast<const bf16x8*>(row + ch * 8);
+    } else {
+      f32x4 a = {}, b = {};
+      if (ch * 8 < D) a = *reinterpret_cast<const f32x4*>(row + ch * 8);
+      if (ch * 8 + 4 < D) b = *reinterpret_cast<const f32x4*>(row + ch * 8 + 4);
+      r.x = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
   } else {
 #pragma unroll
-    for (int e = 0; e < CE; ++e)
-      if (ch * CE + e < D) r[e] = row[ch * CE + e];
+    for (int e = 0; e < 8; ++e)
+      if (ch * 8 + e < D) r.x[e] = row[ch * 8 + e];
   }
   return r;
 }
 
-// A tile of ROWS rows of DP elements in LDS.
+// The wave's stationary rows: lane column's row in chunks 2c + half.  RAW keeps float32 as it is and splits at every use: half the
+// registers of the three planes.
+template <class T, int DP, bool RAW>
+struct Stationary {
+  static constexpr int NC2 = DP / 16;
+  Operand<T> o[NC2];
+  __device__ __forceinline__ void load(const T* row, int half, int D, bool vec, bool ok) {
+#pragma unroll
+    for (int c = 0; c < NC2; ++c) {
+      Raw<T> r = load_chunk<T>(row, 2 * c + half, D, vec);
+      if (!ok) r.x = {};
+      o[c] = operand(r);
+    }
+  }
+  __device__ __forceinline__ const Operand<T>& get(int c) const { return o[c]; }
+};
 template <class T, int DP>
+struct Stationary<T, DP, true> {
+  static constexpr int NC2 = DP / 16;
+  Raw<T> o[NC2];
+  __device__ __forceinline__ void load(const T* row, int half, int D, bool vec, bool ok) {
+#pragma unroll
+    for (int c = 0; c < NC2; ++c) {
+      o[c] = load_chunk<T>(row, 2 * c + half, D, vec);
+      if (!ok) o[c].x = {};
+    }
+  }
+  __device__ __forceinline__ Operand<T> get(int c) const { return operand(o[c]); }
+};
+
+// A tile of ROWS rows of DP elements in LDS, plane after plane.
+template <class T, int DP, int ROWS>
 struct Tile {
-  using chunk = typename Type<T>::chunk;
-  static constexpr int CE = Type<T>::CE;
-  static constexpr int NCH = DP / CE;       // chunks of a row
-  static constexpr int ROWB = DP * sizeof(T);
+  static constexpr int NP = Type<T>::NP;
+  static constexpr int NCH = DP / 8;   // chunks of a row
+  static constexpr int ROWB = DP * 2;  // bytes of a row of a plane
+  static constexpr int PLANE = ROWS * ROWB, BYTES = NP * PLANE;
   static_assert(ROWB >= 128 && (ROWB & (ROWB - 1)) == 0, "rows of 128 bytes or a power of two more");
 
   // Chunk position of chunk ch of row r.  Column reads take two neighbouring chunks of four neighbouring rows, row reads one
@@ -115,93 +191,89 @@ struct Tile {
     if (ROWB >= 256) return ch ^ (((r & 7) << 1) | ((r >> 3) & 1));
     return ch ^ ((((r >> 1) & 3) << 1) | ((r >> 3) & 1));
   }
-  static __device__ __forceinline__ chunk row_chunk(const char* tile, int r, int ch) {
-    return *reinterpret_cast<const chunk*>(tile + r * ROWB + swizzle(r, ch) * 16);
+  static __device__ __forceinline__ Operand<T> row_chunk(const char* tile, int r, int ch) {
+    Operand<T> o;
+#pragma unroll
+    for (int n = 0; n < NP; ++n) o.p[n] = *reinterpret_cast<const bf16x8*>(tile + n * PLANE + r * ROWB + swizzle(r, ch) * 16);
+    return o;
   }
-  static __device__ __forceinline__ void put(char* tile, int r, int ch, chunk x) {
-    *reinterpret_cast<chunk*>(tile + r * ROWB + swizzle(r, ch) * 16) = x;
+  static __device__ __forceinline__ void put(char* tile, int r, int ch, const Operand<T>& x) {
+#pragma unroll
+    for (int n = 0; n < NP; ++n) *reinterpret_cast<bf16x8*>(tile + n * PLANE + r * ROWB + swizzle(r, ch) * 16) = x.p[n];
   }
 };
 
-// acc[dt] += X^T P over 32 moving rows from `r0` of the tile; p holds a lane's 16 values in register order.
-template <class T, int DP, int DT>
-struct ColumnProduct;
-template <int DP, int DT>
-struct ColumnProduct<__bf16, DP, DT> {
-  static __device__ __forceinline__ void run(const char* tile, int r0, int d0, const float (&p)[16], f32x16 (&acc)[DT], int lane) {
-    using TL = Tile<__bf16, DP>;
-    bf16x8 b[2];
+// 16 values of a lane (P or dS) as right-hand operands over 2 x 16 moving rows; rounded to bfloat16, or split.
+template <class T>
+struct Weights {
+  Operand<T> o[2];
+  __device__ __forceinline__ explicit Weights(const float (&p)[16]) {
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       f32x8 f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) f[e] = p[8 * s + e];
-      b[s] = __builtin_convertvector(f, bf16x8);  // round to nearest even
-    }
-    // lane l of a 16-lane group hands in row l / 4, columns 4 (l % 4) .. + 3 and gets column l of the four rows
-    const int half = lane >> 5, sub = lane & 15, colgrp = (lane >> 4) & 1;
-    const int rr = r0 + 4 * half + (sub >> 2);
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) {
-      const int col = d0 + dt * 32 + colgrp * 16 + 4 * (sub & 3);
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        bf16x8 a;
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int r = rr + 16 * s + 8 * u;
-          const char* at = tile + r * TL::ROWB + TL::swizzle(r, col >> 3) * 16 + (col & 7) * 2;
-          const bf16x4 t = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
-              (__attribute__((address_space(3))) bf16x4*)(uintptr_t)(uint32_t)(uintptr_t)at);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) a[4 * u + e] = t[e];
-        }
-        acc[dt] = Type<__bf16>::mma(a, b[s], acc[dt]);
-      }
-    }
-  }
-};
-template <int DP, int DT>
-struct ColumnProduct<float, DP, DT> {
-  static __device__ __forceinline__ void run(const char* tile, int r0, int d0, const float (&p)[16], f32x16 (&acc)[DT], int lane) {
-    using TL = Tile<float, DP>;
-    const int half = lane >> 5;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int r = r0 + moving_row(i, half);
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) {
-        const int col = d0 + dt * 32 + (lane & 31);
-        const float a = *reinterpret_cast<const float*>(tile + r * TL::ROWB + TL::swizzle(r, col >> 2) * 16 + (col & 3) * 4);
-        acc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, p[i], acc[dt], 0, 0, 0);
-      }
+      if constexpr (sizeof(T) == 2) o[s].p[0] = __builtin_convertvector(f, bf16x8);  // round to nearest even
+      else split(f, o[s].p);
     }
   }
 };
 
-// Rows of a tensor's [.., T, D] slice on their way to an LDS tile: loaded to registers before a tile's arithmetic, written to the
-// other buffer after it.  Rows at or past `limit` and masked ones become zero: what lies there (another sequence's values, infinities, NaN)
-// must not reach a product, where 0 * NaN would.
-template <class T, int DP, int ROWS, int NT = 256>
-struct Stage {
-  using TL = Tile<T, DP>;
-  static constexpr int N = ROWS * TL::NCH / NT, STEP = NT / TL::NCH;
-  static_assert(N >= 1 && NT % TL::NCH == 0, "whole rows per pass");
-  typename TL::chunk r[N];
-  __device__ __forceinline__ void load(const T* base, int64_t stride, int row0, int limit, const uint8_t* mask, int D, bool vec, int tid) {
-    const int ch = tid % TL::NCH;
+// acc[dt] += X^T W over 32 moving rows from row r0 of the tile, output rows d0 + 32 dt ..
+template <class T, class TL, int DT>
+__device__ __forceinline__ void column_product(const char* tile, int r0, int d0, const Weights<T>& w, f32x16 (&acc)[DT], int lane) {
+  // lane l of a 16-lane group hands in row l / 4, columns 4 (l % 4) .. + 3 and gets column l of the four rows
+  const int half = lane >> 5, sub = lane & 15, colgrp = (lane >> 4) & 1;
+  const int rr = r0 + 4 * half + (sub >> 2);
 #pragma unroll
-    for (int n = 0; n < N; ++n) {
-      const int row = row0 + tid / TL::NCH + n * STEP, rc = min(row, limit - 1);
-      typename TL::chunk x = load_chunk<T>(base + rc * stride, ch, D, vec);
-      const bool ok = row < limit && !(mask && mask[rc]);
-      r[n] = ok ? x : typename TL::chunk{};
+  for (int dt = 0; dt < DT; ++dt) {
+    const int col = d0 + dt * 32 + colgrp * 16 + 4 * (sub & 3);
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      Operand<T> a;
+#pragma unroll
+      for (int n = 0; n < TL::NP; ++n)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int r = rr + 16 * s + 8 * u;
+          const char* at = tile + n * TL::PLANE + r * TL::ROWB + TL::swizzle(r, col >> 3) * 16 + (col & 7) * 2;
+          const bf16x4 t = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)(uintptr_t)(uint32_t)(uintptr_t)at);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) a.p[n][4 * u + e] = t[e];
+        }
+      acc[dt] = mma(a, w.o[s], acc[dt]);
     }
   }
-  __device__ __forceinline__ void store(char* tile, int tid) const {
-    const int ch = tid % TL::NCH;
+}
+
+// Rows of a tensor's [.., T, D] slice on their way to an LDS tile: requested before a tile's arithmetic, written to LDS after it.
+// `bits` says which rows of the tile may be used; the others become zero: what lies there (another sequence's values,
+// infinities, NaN) must not reach a product, where 0 * NaN would.
+template <class T, int DP, int ROWS, int NT = 256>
+struct Stage {
+  using TL = Tile<T, DP, ROWS>;
+  static constexpr int N = ROWS * TL::NCH / NT, STEP = NT / TL::NCH;
+  static_assert(N >= 1 && NT % TL::NCH == 0, "whole rows per pass");
+  Raw<T> r[N];
+  __device__ __forceinline__ void load(const T* base, int64_t stride, int row0, int limit, int D, bool vec, int tid) {
+    const int ch = tid % TL::NCH, mine = tid / TL::NCH;
 #pragma unroll
-    for (int n = 0; n < N; ++n) TL::put(tile, tid / TL::NCH + n * STEP, ch, r[n]);
+    for (int n = 0; n < N; ++n) {
+      const T* rows = base + (int64_t)(row0 + n * STEP) * stride;  // the same for all lanes
+      r[n].x = {};
+      if (row0 + n * STEP + mine < limit) r[n] = load_chunk<T>(rows + mine * (int)stride, ch, D, vec);
+    }
+  }
+  __device__ __forceinline__ void store(char* tile, uint64_t bits, int tid) {
+    const int ch = tid % TL::NCH, mine = tid / TL::NCH;
+    constexpr uint64_t kAll = ROWS == 64 ? ~0ull : (1ull << ROWS) - 1;
+    if ((bits & kAll) != kAll) {
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+        if (!((bits >> (mine + n * STEP)) & 1)) r[n].x = {};
+    }
+#pragma unroll
+    for (int n = 0; n < N; ++n) TL::put(tile, mine + n * STEP, ch, operand(r[n]));
   }
 };
 
@@ -249,33 +321,46 @@ __device__ __forceinline__ void fill_lut(const Params& p, int h, float* lut, int
   }
 }
 
-// s (raw products of one 32-key subtile) -> scores in log2 units with bias, and -inf where a pair is left out.
-// key0: first key of the subtile; pos: the lane's query position; add: 0 / -inf by key, from LDS, or null.
-template <bool BIAS>
-__device__ __forceinline__ void finish_scores(const Params& p, const f32x16& raw, float (&s)[16], int key0, int pos, int pos_lo, int pos_hi,
-                                              const float* add, const float* lut, int half) {
-#pragma unroll
-  for (int g = 0; g < 4; ++g) {
-    f32x4 km = {};
-    if (add) km = *reinterpret_cast<const f32x4*>(add + 8 * g + 4 * half);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) s[4 * g + e] = raw[4 * g + e] * p.scale2 + km[e];
+// Which keys of a tile of up to 64 may be used, one bit each: lane l looks at key l.
+struct KeyBits {
+  const uint8_t* mask;
+  int end, lane;
+  uint8_t m = 0;
+  __device__ __forceinline__ KeyBits(const uint8_t* mask_, int end_, int lane_) : mask(mask_), end(end_), lane(lane_) {}
+  __device__ __forceinline__ void load(int key0) {
+    if (mask) m = mask[min(key0 + lane, end - 1)];
   }
+  __device__ __forceinline__ uint64_t get(int key0) const { return __ballot(key0 + lane < end && m == 0); }
+};
+
+// s = raw products of one 32-key subtile -> scores in log2 units with the bias; -inf where a pair is left out.
+// key0: first key of the subtile; pos: the lane's query position, pos_lo .. pos_hi the wave's; use: bit r = key key0 + r may be used.
+template <bool BIAS>
+__device__ __forceinline__ void finish_scores(const Params& p, float (&s)[16], int key0, int pos, int pos_lo, int pos_hi, uint32_t use,
+                                              const float* lut, int half) {
   if constexpr (BIAS) {
     const int md = p.max_distance;
     if (key0 + 31 - pos_lo <= -md || key0 - pos_hi >= md) {
       const float far = lut[key0 - pos_hi >= md ? 2 * md : 0];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] += far;
+      for (int i = 0; i < 16; ++i) s[i] = fmaf(s[i], p.scale2, far);
     } else {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] += lut[min(max(key0 + moving_row(i, half) - pos, -md), md) + md];
+      for (int i = 0; i < 16; ++i) s[i] = fmaf(s[i], p.scale2, lut[min(max(key0 + moving_row(i, half) - pos, -md), md) + md]);
     }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] *= p.scale2;
   }
   if (p.causal && key0 + 31 > pos_lo) {
+    const int last = pos - key0 - 4 * half;
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-      if (key0 + moving_row(i, half) > pos) s[i] = -INFINITY;
+    for (int i = 0; i < 16; ++i) s[i] = moving_row(i, 0) > last ? -INFINITY : s[i];
+  }
+  if (use != ~0u) {
+    const uint32_t mine = use >> (4 * half);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = (mine >> moving_row(i, 0)) & 1 ? s[i] : -INFINITY;
   }
 }
 
