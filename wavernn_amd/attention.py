@@ -57,10 +57,15 @@ def _on_gpu(t: torch.Tensor, what: str) -> None:
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
-    """The kernels take any strides but that of the last dimension (and positions no further apart than 2^26 elements)."""
-    if (t.stride(3) == 1 or t.shape[3] == 1) and t.stride(2) < 1 << 26:
+    """The kernels take any strides of batch, head and position; rows are contiguous, start on 16 bytes and are whole in them.  A
+    copy, padded with zeros, where that does not hold."""
+    e = t.element_size()
+    s, n = t.stride(), t.shape
+    if ((s[3] == 1 or n[3] == 1) and n[3] * e % 16 == 0 and t.data_ptr() % 16 == 0 and s[2] < 1 << 26
+            and all(s[i] * e % 16 == 0 or n[i] == 1 for i in range(3))):
         return t
-    return t.contiguous()
+    pad = -n[3] % (16 // e)
+    return nn.functional.pad(t, (0, pad)) if pad else t.contiguous() if not t.is_contiguous() else t.clone()
 
 
 def _strides(t: torch.Tensor):
@@ -195,14 +200,19 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, key_mask: Op
     if scale is None:
         scale = 1.0 / math.sqrt(D)
     q, k, v = _rows(q), _rows(k), _rows(v)
+    out, lse = _run(q, k, v, bias_table, key_mask, key_lens, q_start, causal, scale, max_distance, bidirectional, return_lse)
+    out = out if out.shape[3] == D else out[..., :D]
+    return (out, lse) if return_lse else out
+
+
+def _run(q, k, v, bias_table, key_mask, key_lens, q_start, causal, scale, max_distance, bidirectional, want_lse):
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
                                     or (bias_table is not None and bias_table.requires_grad)):
-        out, lse = _Attention.apply(q, k, v, bias_table, key_mask, key_lens, q_start, causal, scale, max_distance, bidirectional)
-        return (out, lse) if return_lse else out
-    with torch.cuda.device(dev):
-        lse = torch.empty(q.shape[:3], dtype=torch.float32, device=dev) if return_lse else None
+        return _Attention.apply(q, k, v, bias_table, key_mask, key_lens, q_start, causal, scale, max_distance, bidirectional)
+    with torch.cuda.device(q.device):
+        lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) if want_lse else None
         out = _forward(_desc(q, k, v, bias_table, key_mask, key_lens, q_start, causal, scale, max_distance, bidirectional), q, lse)
-    return (out, lse) if return_lse else out
+    return out, lse
 
 
 class _RelativeBias(torch.autograd.Function):

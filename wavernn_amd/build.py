@@ -15,13 +15,14 @@ LIB_DIR = os.path.join(HERE, "lib")
 OBJ_DIR = os.path.join(LIB_DIR, "obj")
 LIB_PATH = os.path.join(LIB_DIR, "libwrnn_mi355.so")
 SOURCES = ["taco_decoder.hip", "length_regulator.hip", "bilstm.hip", "bigru.hip", "durations.hip", "wavernn.hip",
-           "aligner.hip", "mol.hip", "attention.hip", "attention_backward.hip", "relative_bias.hip"]
+           "aligner.hip", "mol.hip", "relative_bias.hip", "attention.hip", "attention_forward_bf16.hip",
+           "attention_forward_f32.hip", "attention_backward_bf16.hip", "attention_backward_f32.hip"]
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function"]
 # The attention kernels are built without packed fp32 instructions: some of their forms have given wrong results on this
 # hardware, with no error.  (The host pass does not know the feature and says so; harmless.)  The older kernels keep the code they were
 # verified with: the teacher-forced loop loses 5.5 % without them (13.7 -> 14.5 us per decoder step at B=64).
 NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-SOURCE_FLAGS = {s: NO_PACKED_FP32 for s in ("attention.hip", "attention_backward.hip", "relative_bias.hip")}
+SOURCE_FLAGS = {s: NO_PACKED_FP32 for s in SOURCES if s.startswith(("attention", "relative_bias"))}
 
 
 def _hipcc() -> str:

@@ -1,0 +1,290 @@
+// Self-attention, forward:  out = softmax(scale * q k^T + bias) v  over the keys that lengths, mask and causality leave.
+//
+// One pass over the keys with a running maximum and sum per query (kept in 32 bits, in units of log2 so that the exponential is
+// one v_exp_f32).  The [Tq, Tk] scores only ever exist as 32 x 32 tiles in registers (attention_tile.h).
+#pragma once
+#include "attention_tile.h"
+
+namespace wrnn {
+namespace attn {
+
+// Running softmax of one query per lane: maximum, sum (this half-wave's share), and the accumulators it scales.
+// The maximum only moves when a score exceeds it by more than 8 (a factor 256, far inside float's range): most tiles rescale nothing.
+struct Running {
+  float m = -3e38f, l = 0.f;
+  template <int NS, int DT>
+  __device__ __forceinline__ void step(float (&s)[NS][16], f32x16 (&acc)[DT]) {
+    float mx = s[0][0];
+#pragma unroll
+    for (int n = 0; n < NS; ++n)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[n][i]);
+    mx = both_max(mx);
+    if (__any(mx > m + 8.f)) {
+      const float mn = fmaxf(m, mx), a = exp2f(m - mn);
+      m = mn;
+      l *= a;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) acc[dt] *= a;
+    }
+#pragma unroll
+    for (int n = 0; n < NS; ++n)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[n][i] = __builtin_amdgcn_exp2f(s[n][i] - m);
+        l += s[n][i];
+      }
+  }
+};
+
+// Shapes of a workgroup.
+//   wide   4 waves, 32 queries each, all against every 32 keys of a tile: a tile in LDS serves 128 queries.
+//   narrow 32 queries, the waves on different 32 keys of a tile, joined at the end; the keys may further be split over
+//          workgroups, and the 32 columns may hold the queries of all heads that share k and v (p.pack).  For calls with few
+//          queries, or too few workgroups of the wide shape to fill the compute units.
+template <class T, int DP, bool WIDE>
+struct ForwardShape {
+  static constexpr int NP = Type<T>::NP;
+  // narrow: as many waves as tiles of 32 keys fit the LDS beside each other (three planes of float32 are 6 bytes an element)
+  static constexpr int WQ = WIDE ? 4 : 1, WK = WIDE ? 1 : NP == 1 ? 4 : DP == 64 ? 4 : DP == 128 ? 2 : 1;
+  static constexpr int NS = WIDE && NP == 1 ? 2 : 1;  // 32-key subtiles of a tile per wave
+  static constexpr int THREADS = 64 * WQ * WK, BN = 32 * WK * NS;
+  static constexpr int BUFS = WIDE && !(NP == 3 && DP == 256) ? 2 : 1;  // two where they fit
+  static constexpr int WAVES = WIDE ? (DP * NP <= 192 ? 2 : 1) : (DP * NP <= 128 ? 2 : 1);  // per SIMD
+  using TL = Tile<T, DP, BN>;
+  static constexpr size_t TILES = 2 * BUFS * TL::BYTES, SUMS = WK > 1 ? (size_t)WK * 32 * (DP + 4) * 4 : 0;
+  static constexpr size_t BODY = TILES > SUMS ? TILES : SUMS;
+  static constexpr size_t LDS = BODY + 2 * 32 * 4 * 4 + 16;  // + statistics of the waves, a word; the position bias's table follows
+};
+
+template <class T, int DP, bool BIAS, bool WIDE>
+__global__ __launch_bounds__((ForwardShape<T, DP, WIDE>::THREADS), (ForwardShape<T, DP, WIDE>::WAVES)) void attention_forward_kernel(Params p) {
+  using S = ForwardShape<T, DP, WIDE>;
+  using TL = typename S::TL;
+  constexpr int BN = S::BN, NS = S::NS, NC2 = DP / 16, DT = DP / 32, BUFS = S::BUFS, NT = S::THREADS;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  char* kt = smem;
+  char* vt = smem + BUFS * TL::BYTES;
+  float* ml = reinterpret_cast<float*>(smem + S::BODY);  // [WK][2][32]
+  int* word = reinterpret_cast<int*>(ml + 4 * 2 * 32);
+  float* lut = reinterpret_cast<float*>(word + 4);
+  const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wq = WIDE ? wave : 0, wk = WIDE ? 0 : wave;
+  const bool pack = !WIDE && p.pack;
+  const int heads = pack ? p.Hkv : p.H, splits = WIDE ? 1 : p.splits;
+  const int nt = pack ? 1 : (p.Tq + 32 * S::WQ - 1) / (32 * S::WQ), n = p.B * heads * nt * splits;
+  int item = xcd_item(n);
+  if (item >= n) return;
+  const int part = item % splits;
+  item /= splits;
+  const int bh = item / nt, b = bh / heads, hh = bh - b * heads;
+  const int q0 = (p.causal ? nt - 1 - item % nt : item % nt) * 32 * S::WQ + 32 * wq;  // under causality the long rows start first
+  const int lh = pack ? col / p.Tq : 0;                                              // the column's head within the group
+  const int h = pack ? hh * p.group + min(lh, p.group - 1) : hh, kvh = pack ? hh : hh / p.group;
+  const int qi = pack ? col - lh * p.Tq : q0 + col;
+  const int off = start_of(p, b), pos = qi + off;
+  const int pos_lo = q0 + off, pos_hi = (pack ? p.Tq - 1 : q0 + 31) + off;
+  const T* kb = reinterpret_cast<const T*>(p.k) + b * p.k_b + kvh * p.k_h;
+  const T* vb = reinterpret_cast<const T*>(p.v) + b * p.v_b + kvh * p.v_h;
+  const uint8_t* mask = p.key_mask ? p.key_mask + b * p.mask_b : nullptr;
+  Stationary<T, DP, false> q;
+  q.load(reinterpret_cast<const T*>(p.q) + b * p.q_b + h * p.q_h + min(qi, p.Tq - 1) * p.q_t, half, p.D, true);
+  const int lut_len = 2 * p.max_distance + 1;
+  const float* my_lut = lut;
+  if constexpr (BIAS) {
+    if (pack) {
+      for (int g = 0; g < p.group; ++g) fill_lut(p, hh * p.group + g, lut + g * lut_len, tid, NT);
+      my_lut += min(lh, p.group - 1) * lut_len;
+    } else {
+      fill_lut(p, h, lut, tid, NT);
+    }
+  }
+  const int last_pos = min(q0 - 32 * wq + 32 * S::WQ - 1, p.Tq - 1) + off;
+  const int end = key_end(p, b, last_pos, word, tid, NT);
+  const int all = (end + BN - 1) / BN, per = (all + splits - 1) / splits, t0 = part * per, t1 = min(all, t0 + per);
+  f32x16 acc[DT] = {};
+  Running run;
+  Stage<T, DP, BN, NT> sk, sv;
+  KeyBits<BN> keys(mask, end, lane);
+  auto load = [&](int t) {
+    sk.load(kb, p.k_t, t * BN, end, p.D, tid);
+    sv.load(vb, p.v_t, t * BN, end, p.D, tid);
+    keys.load(t * BN);
+  };
+  auto store = [&](int t) {
+    const RowBits use = keys.get(t * BN);
+    const int o = t & (BUFS - 1);
+    sk.drop(use, tid);
+    sv.drop(use, tid);
+    sk.store(kt + o * TL::BYTES, tid);
+    sv.store(vt + o * TL::BYTES, tid);
+    return use;
+  };
+  // round r requests tile r, works on tile r - 1 and puts tile r into LDS: one copy of each piece of code, for a call's time on few
+  // tiles is the time to fetch its instructions
+  RowBits use;
+  if constexpr (BIAS) __syncthreads();
+  for (int r = t0; r <= t1; ++r) {
+    if (r < t1) load(r);
+    const int t = r - 1;
+    const char *kk = kt + (t & (BUFS - 1)) * TL::BYTES, *vv = vt + (t & (BUFS - 1)) * TL::BYTES;
+    const int sub0 = NS * wk, key0 = t * BN + 32 * sub0;
+    if (r > t0 && q0 < p.Tq && key0 < end && !(p.causal && key0 > pos_hi)) {
+      f32x16 raw[NS] = {};
+#pragma unroll
+      for (int c = 0; c < NC2; ++c)
+#pragma unroll
+        for (int s = 0; s < NS; ++s) raw[s] = mma(TL::row_chunk(kk, (sub0 + s) * 32 + col, 2 * c + half), q.get(c), raw[s]);
+      float s[NS][16];
+#pragma unroll
+      for (int x = 0; x < NS; ++x) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[x][i] = raw[x][i];
+        finish_scores<BIAS>(p, s[x], key0 + 32 * x, pos, pos_lo, pos_hi, use.of(sub0 + x), my_lut, half);
+      }
+      run.step(s, acc);
+#pragma unroll
+      for (int x = 0; x < NS; ++x) column_product<T, TL>(vv, (sub0 + x) * 32, 0, Weights<T>(s[x]), acc, lane);
+    }
+    if (BUFS == 1) __syncthreads();
+    if (r < t1) use = store(r);
+    __syncthreads();
+  }
+  const float l = both_sum(run.l);
+  if constexpr (S::WK == 1) {
+    if (qi >= p.Tq || (pack && lh >= p.group)) return;
+    const int64_t row = ((int64_t)b * p.H + h) * p.Tq + qi;
+    if (splits == 1) {
+      const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+      T* orow = reinterpret_cast<T*>(p.out) + b * p.o_b + h * p.o_h + qi * p.o_t;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          store4<T>(orow, dt * 32 + 8 * g + 4 * half, p.D, acc[dt][4 * g] * inv, acc[dt][4 * g + 1] * inv, acc[dt][4 * g + 2] * inv,
+                    acc[dt][4 * g + 3] * inv);
+      if (half == 0 && p.lse) p.lse[row] = l == 0.f ? -INFINITY : (run.m + log2f(l)) * kLn2;
+    } else {
+      float* to = p.part + (row * splits + part) * (DP + 4);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<f32x4*>(to + 4 + dt * 32 + 8 * g + 4 * half) = f32x4{acc[dt][4 * g], acc[dt][4 * g + 1], acc[dt][4 * g + 2], acc[dt][4 * g + 3]};
+      if (half == 0) {
+        to[0] = run.m;
+        to[1] = l;
+      }
+    }
+  } else {
+    // join the waves: a common maximum per column, then sums over the waves in their order
+    if (half == 0) {
+      ml[(wk * 2) * 32 + col] = run.m;
+      ml[(wk * 2 + 1) * 32 + col] = l;
+    }
+    __syncthreads();
+    float m = ml[col];
+#pragma unroll
+    for (int w = 1; w < S::WK; ++w) m = fmaxf(m, ml[(w * 2) * 32 + col]);
+    const float a = exp2f(run.m - m);
+    constexpr int LD = DP + 4;
+    float* sums = reinterpret_cast<float*>(smem);  // [WK][32][LD], in the tiles' place
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<f32x4*>(sums + (wk * 32 + col) * LD + dt * 32 + 8 * g + 4 * half) =
+            f32x4{acc[dt][4 * g] * a, acc[dt][4 * g + 1] * a, acc[dt][4 * g + 2] * a, acc[dt][4 * g + 3] * a};
+    __syncthreads();
+    constexpr int TPC = NT / 32;  // threads a column
+    const int c2 = tid / TPC, d_first = (tid % TPC) * 4;
+    float m2 = ml[c2], l2 = 0.f;
+#pragma unroll
+    for (int w = 1; w < S::WK; ++w) m2 = fmaxf(m2, ml[(w * 2) * 32 + c2]);
+#pragma unroll
+    for (int w = 0; w < S::WK; ++w) l2 += ml[(w * 2 + 1) * 32 + c2] * exp2f(ml[(w * 2) * 32 + c2] - m2);
+    const int lh2 = pack ? c2 / p.Tq : 0, h2 = pack ? hh * p.group + lh2 : hh, qi2 = pack ? c2 - lh2 * p.Tq : q0 + c2;
+    if (pack ? lh2 >= p.group : qi2 >= p.Tq) return;
+    const int64_t row = ((int64_t)b * p.H + h2) * p.Tq + qi2;
+    const float inv = splits > 1 ? 1.f : l2 > 0.f ? 1.f / l2 : (l2 == 0.f ? 0.f : l2);
+    T* orow = reinterpret_cast<T*>(p.out) + b * p.o_b + h2 * p.o_h + qi2 * p.o_t;
+    float* to = p.part + (row * splits + part) * (DP + 4);
+#pragma unroll
+    for (int d = d_first; d < DP; d += TPC * 4) {
+      f32x4 x = *reinterpret_cast<const f32x4*>(sums + c2 * LD + d);
+#pragma unroll
+      for (int w = 1; w < S::WK; ++w) x += *reinterpret_cast<const f32x4*>(sums + (w * 32 + c2) * LD + d);
+      if (splits == 1)
+        store4<T>(orow, d, p.D, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+      else
+        *reinterpret_cast<f32x4*>(to + 4 + d) = x;
+    }
+    if (d_first == 0) {
+      if (splits > 1) {
+        to[0] = m2;
+        to[1] = l2;
+      } else if (p.lse) {
+        p.lse[row] = l2 == 0.f ? -INFINITY : (m2 + log2f(l2)) * kLn2;
+      }
+    }
+  }
+}
+
+// Joins the splits of a query: one wave per query, splits in their order.
+template <class T, int DP>
+__global__ __launch_bounds__(256) void attention_join_kernel(Params p) {
+  const int lane = threadIdx.x & 63;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= (int64_t)p.B * p.H * p.Tq) return;
+  const float* part = p.part + row * p.splits * (DP + 4);
+  float m = -3e38f, l = 0.f;
+  for (int s = 0; s < p.splits; ++s) m = fmaxf(m, part[s * (DP + 4)]);
+  constexpr int E = DP / 64;
+  float x[E] = {};
+  for (int s = 0; s < p.splits; ++s) {
+    const float* ps = part + s * (DP + 4);
+    const float a = exp2f(ps[0] - m);
+    l += ps[1] * a;
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[e] += ps[4 + e * 64 + lane] * a;
+  }
+  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+  const int qi = row % p.Tq, h = (row / p.Tq) % p.H, b = row / p.Tq / p.H;
+  T* orow = reinterpret_cast<T*>(p.out) + b * p.o_b + h * p.o_h + qi * p.o_t;
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    if (e * 64 + lane < p.D) orow[e * 64 + lane] = (T)(x[e] * inv);
+  if (lane == 0 && p.lse) p.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+}
+
+template <class T, int DP, bool BIAS>
+static int launch_forward(const Params& p, hipStream_t st) {
+  static std::atomic<uint64_t> wide_done{0}, narrow_done{0};
+  const size_t lut = BIAS ? (2 * p.max_distance + 1) * sizeof(float) : 0;
+  if (p.splits == 0) {
+    using S = ForwardShape<T, DP, true>;
+    return launch(&attention_forward_kernel<T, DP, BIAS, true>, &wide_done, (int64_t)p.B * p.H * ((p.Tq + 127) / 128), S::THREADS, S::LDS + lut, p, st);
+  }
+  using S = ForwardShape<T, DP, false>;
+  const int64_t n = (p.pack ? (int64_t)p.B * p.Hkv : (int64_t)p.B * p.H * ((p.Tq + 31) / 32)) * p.splits;
+  if (launch(&attention_forward_kernel<T, DP, BIAS, false>, &narrow_done, n, S::THREADS, S::LDS + lut * (p.pack ? p.group : 1), p, st)) return 1;
+  if (p.splits > 1) {
+    const int64_t rows = (int64_t)p.B * p.H * p.Tq;
+    hipLaunchKernelGGL((attention_join_kernel<T, DP>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, p);
+    WRNN_LAUNCH_CHECK();
+  }
+  return 0;
+}
+
+template <class T, int DP>
+static int launch_bias(const Params& p, hipStream_t st) {
+  return p.table ? launch_forward<T, DP, true>(p, st) : launch_forward<T, DP, false>(p, st);
+}
+
+template <class T>
+int forward(const Params& p, hipStream_t st) {
+  return p.D <= 64 ? launch_bias<T, 64>(p, st) : p.D <= 128 ? launch_bias<T, 128>(p, st) : launch_bias<T, 256>(p, st);
+}
+
+}  // namespace attn
+}  // namespace wrnn

@@ -45,7 +45,7 @@ struct Params {
   float* lse;  // [B, H, Tq], natural logarithm; -inf where a row has no key
   int64_t q_b, q_h, q_t, k_b, k_h, k_t, v_b, v_h, v_t, o_b, o_h, o_t;
   int B, H, Hkv, group, Tq, Tk, D;
-  int causal, vec;          // vec: every row of every tensor starts on 16 bytes and D fills whole chunks
+  int causal;
   float scale, scale2;      // scale, scale * log2(e)
   const uint8_t* key_mask;  // [B, Tk], non-zero = left out
   int64_t mask_b;
@@ -57,6 +57,7 @@ struct Params {
   const void *dout, *o_in;
   void *dq, *dk, *dv;
   float *delta, *dtable_part;
+  int wide_dq, wide_dkv;  // 128 stationary rows per workgroup, not 32
   int64_t do_b, do_h, do_t, oi_b, oi_h, oi_t, dq_b, dq_h, dq_t, dk_b, dk_h, dk_t, dv_b, dv_h, dv_t;
   // keys split over workgroups (few queries)
   int splits, pack;
@@ -85,13 +86,28 @@ struct Raw {  // 8 elements as they come from memory
 };
 
 __device__ __forceinline__ Operand<__bf16> operand(const Raw<__bf16>& r) { return {{r.x}}; }
+// Two values at a time: one packed conversion, and the two roundings back as bits (a shift, a mask).
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)a, (__bf16)b});
+}
 __device__ __forceinline__ void split(f32x8 x, bf16x8 (&p)[3]) {
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  u32x4 w[3];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    p[i] = __builtin_convertvector(x, bf16x8);
-    x -= __builtin_convertvector(p[i], f32x8);  // exact
+  for (int j = 0; j < 4; ++j) {
+    float a = x[2 * j], b = x[2 * j + 1];
+#pragma unroll
+    for (int n = 0; n < 3; ++n) {
+      uint32_t u = pack2(a, b);
+      asm("" : "+v"(u));  // keeps it one conversion: without this the low half is converted a second time on its own
+      w[n][j] = u;
+      a -= __uint_as_float(u << 16);  // exact
+      b -= __uint_as_float(u & 0xffff0000u);
+    }
   }
-  p[2] = __builtin_convertvector(x, bf16x8);
+#pragma unroll
+  for (int n = 0; n < 3; ++n) p[n] = __builtin_bit_cast(bf16x8, w[n]);
 }
 __device__ __forceinline__ Operand<float> operand(const Raw<float>& r) {
   Operand<float> o;
@@ -122,25 +138,18 @@ __device__ __forceinline__ float both_sum(float x) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// Chunk ch (8 elements) of a row of D; what lies past D is zero and not read.  vec: rows start on 16 bytes and D is a multiple of
-// 16 bytes.
+// Chunk ch (8 elements) of a row of D; what lies past D is zero and not read.  Rows start on 16 bytes and D is whole in them.
 template <class T>
-__device__ __forceinline__ Raw<T> load_chunk(const T* row, int ch, int D, bool vec) {
+__device__ __forceinline__ Raw<T> load_chunk(const T* row, int ch, int D) {
   Raw<T> r;
   r.x = {};
-  if (vec) {
-    if constexpr (sizeof(T) == 2) {
-      if (ch * 8 < D) r.x = *reinterpret_cast<const bf16x8*>(row + ch * 8);
-    } else {
-      f32x4 a = {}, b = {};
-      if (ch * 8 < D) a = *reinterpret_cast<const f32x4*>(row + ch * 8);
-      if (ch * 8 + 4 < D) b = *reinterpret_cast<const f32x4*>(row + ch * 8 + 4);
-      r.x = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
-    }
+  if constexpr (sizeof(T) == 2) {
+    if (ch * 8 < D) r.x = *reinterpret_cast<const bf16x8*>(row + ch * 8);
   } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (ch * 8 + e < D) r.x[e] = row[ch * 8 + e];
+    f32x4 a = {}, b = {};
+    if (ch * 8 < D) a = *reinterpret_cast<const f32x4*>(row + ch * 8);
+    if (ch * 8 + 4 < D) b = *reinterpret_cast<const f32x4*>(row + ch * 8 + 4);
+    r.x = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
   }
   return r;
 }
@@ -151,10 +160,10 @@ template <class T, int DP, bool RAW>
 struct Stationary {
   static constexpr int NC2 = DP / 16;
   Operand<T> o[NC2];
-  __device__ __forceinline__ void load(const T* row, int half, int D, bool vec, bool ok) {
+  __device__ __forceinline__ void load(const T* row, int half, int D, bool ok) {
 #pragma unroll
     for (int c = 0; c < NC2; ++c) {
-      Raw<T> r = load_chunk<T>(row, 2 * c + half, D, vec);
+      Raw<T> r = load_chunk<T>(row, 2 * c + half, D);
       if (!ok) r.x = {};
       o[c] = operand(r);
     }
@@ -165,10 +174,10 @@ template <class T, int DP>
 struct Stationary<T, DP, true> {
   static constexpr int NC2 = DP / 16;
   Raw<T> o[NC2];
-  __device__ __forceinline__ void load(const T* row, int half, int D, bool vec, bool ok) {
+  __device__ __forceinline__ void load(const T* row, int half, int D, bool ok) {
 #pragma unroll
     for (int c = 0; c < NC2; ++c) {
-      o[c] = load_chunk<T>(row, 2 * c + half, D, vec);
+      o[c] = load_chunk<T>(row, 2 * c + half, D);
       if (!ok) o[c].x = {};
     }
   }
@@ -246,52 +255,76 @@ __device__ __forceinline__ void column_product(const char* tile, int r0, int d0,
   }
 }
 
+// Which rows of a tile of up to 128 may be used, one bit each.
+struct RowBits {
+  uint64_t lo = 0, hi = 0;
+  __device__ __forceinline__ uint32_t of(int sub) const { return (uint32_t)((sub & 2 ? +hi : +lo) >> (32 * (sub & 1))); }
+  __device__ __forceinline__ bool at(int r) const { return ((r & 64 ? +hi : +lo) >> (r & 63)) & 1; }
+  template <int ROWS>
+  __device__ __forceinline__ bool all() const {
+    constexpr uint64_t first = ROWS >= 64 ? ~0ull : (1ull << (ROWS & 63)) - 1;
+    return (lo & first) == first && (ROWS <= 64 || hi == ~0ull);
+  }
+};
+
+// The keys of a tile that lengths, reach (end) and mask leave: lane l looks at keys l and l + 64.
+template <int ROWS>
+struct KeyBits {
+  const uint8_t* mask;
+  int end, lane;
+  uint32_t out_lo = 0, out_hi = 0;
+  __device__ __forceinline__ KeyBits(const uint8_t* mask_, int end_, int lane_) : mask(mask_), end(end_), lane(lane_) {}
+  __device__ __forceinline__ void load(int key0) {
+    if (!mask) return;
+    out_lo = mask[min(key0 + lane, end - 1)];
+    if (ROWS > 64) out_hi = mask[min(key0 + 64 + lane, end - 1)];
+  }
+  __device__ __forceinline__ RowBits get(int key0) const {
+    RowBits r;
+    r.lo = __ballot(key0 + lane < end && out_lo == 0);
+    if (ROWS > 64) r.hi = __ballot(key0 + 64 + lane < end && out_hi == 0);
+    return r;
+  }
+};
+
 // Rows of a tensor's [.., T, D] slice on their way to an LDS tile: requested before a tile's arithmetic, written to LDS after it.
-// `bits` says which rows of the tile may be used; the others become zero: what lies there (another sequence's values,
-// infinities, NaN) must not reach a product, where 0 * NaN would.
-template <class T, int DP, int ROWS, int NT = 256>
+// Rows that may not be used become zero: what lies there (another sequence's values, infinities, NaN) must not reach a
+// product, where 0 * NaN would.
+template <class T, int DP, int ROWS, int NT>
 struct Stage {
   using TL = Tile<T, DP, ROWS>;
   static constexpr int N = ROWS * TL::NCH / NT, STEP = NT / TL::NCH;
   static_assert(N >= 1 && NT % TL::NCH == 0, "whole rows per pass");
   Raw<T> r[N];
-  __device__ __forceinline__ void load(const T* base, int64_t stride, int row0, int limit, int D, bool vec, int tid) {
+  __device__ __forceinline__ void load(const T* base, int64_t stride, int row0, int limit, int D, int tid) {
     const int ch = tid % TL::NCH, mine = tid / TL::NCH;
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       const T* rows = base + (int64_t)(row0 + n * STEP) * stride;  // the same for all lanes
       r[n].x = {};
-      if (row0 + n * STEP + mine < limit) r[n] = load_chunk<T>(rows + mine * (int)stride, ch, D, vec);
+      if (row0 + n * STEP + mine < limit) r[n] = load_chunk<T>(rows + mine * (int)stride, ch, D);
     }
   }
-  __device__ __forceinline__ void store(char* tile, uint64_t bits, int tid) {
-    const int ch = tid % TL::NCH, mine = tid / TL::NCH;
-    constexpr uint64_t kAll = ROWS == 64 ? ~0ull : (1ull << ROWS) - 1;
-    if ((bits & kAll) != kAll) {
+  __device__ __forceinline__ void drop(const RowBits& bits, int tid) {
+    if (bits.all<ROWS>()) return;
 #pragma unroll
-      for (int n = 0; n < N; ++n)
-        if (!((bits >> (mine + n * STEP)) & 1)) r[n].x = {};
-    }
+    for (int n = 0; n < N; ++n)
+      if (!bits.at(tid / TL::NCH + n * STEP)) r[n].x = {};
+  }
+  __device__ __forceinline__ void store(char* tile, int tid) {
 #pragma unroll
-    for (int n = 0; n < N; ++n) TL::put(tile, mine + n * STEP, ch, operand(r[n]));
+    for (int n = 0; n < N; ++n) TL::put(tile, tid / TL::NCH + n * STEP, tid % TL::NCH, operand(r[n]));
   }
 };
 
 // A lane's 32 columns x 4 rows of an accumulator as output: column = stationary row, 4 neighbouring d per register group.
 template <class T>
-__device__ __forceinline__ void store4(T* row, int d, int D, bool vec, float a, float b, float c, float e) {
-  const float x[4] = {a, b, c, e};
-  if (vec) {  // D is a whole number of chunks, so of fours
-    if (d >= D) return;
-    if constexpr (sizeof(T) == 4) {
-      *reinterpret_cast<f32x4*>(row + d) = f32x4{a, b, c, e};
-    } else {
-      *reinterpret_cast<bf16x4*>(row + d) = bf16x4{(__bf16)a, (__bf16)b, (__bf16)c, (__bf16)e};
-    }
+__device__ __forceinline__ void store4(T* row, int d, int D, float a, float b, float c, float e) {
+  if (d >= D) return;  // D is a whole number of fours
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<f32x4*>(row + d) = f32x4{a, b, c, e};
   } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (d + i < D) row[d + i] = (T)x[i];
+    *reinterpret_cast<bf16x4*>(row + d) = bf16x4{(__bf16)a, (__bf16)b, (__bf16)c, (__bf16)e};
   }
 }
 
@@ -320,18 +353,6 @@ __device__ __forceinline__ void fill_lut(const Params& p, int h, float* lut, int
     lut[i] = x * kLog2e;
   }
 }
-
-// Which keys of a tile of up to 64 may be used, one bit each: lane l looks at key l.
-struct KeyBits {
-  const uint8_t* mask;
-  int end, lane;
-  uint8_t m = 0;
-  __device__ __forceinline__ KeyBits(const uint8_t* mask_, int end_, int lane_) : mask(mask_), end(end_), lane(lane_) {}
-  __device__ __forceinline__ void load(int key0) {
-    if (mask) m = mask[min(key0 + lane, end - 1)];
-  }
-  __device__ __forceinline__ uint64_t get(int key0) const { return __ballot(key0 + lane < end && m == 0); }
-};
 
 // s = raw products of one 32-key subtile -> scores in log2 units with the bias; -inf where a pair is left out.
 // key0: first key of the subtile; pos: the lane's query position, pos_lo .. pos_hi the wave's; use: bit r = key key0 + r may be used.
@@ -432,10 +453,10 @@ static int allow_lds(K kernel, std::atomic<uint64_t>* done) {
 }
 
 template <class K>
-static int launch(K kernel, std::atomic<uint64_t>* done, int64_t items, size_t lds, const Params& p, hipStream_t st) {
+static int launch(K kernel, std::atomic<uint64_t>* done, int64_t items, int threads, size_t lds, const Params& p, hipStream_t st) {
   if (allow_lds(kernel, done)) return 1;
   WRNN_REQUIRE(lds <= kLdsBytes, "attention: %zu bytes of LDS", lds);
-  hipLaunchKernelGGL(kernel, dim3((unsigned)(8 * ((items + 7) / 8))), dim3(256), lds, st, p);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)(8 * ((items + 7) / 8))), dim3(threads), lds, st, p);
   WRNN_LAUNCH_CHECK();
   return 0;
 }
@@ -445,6 +466,11 @@ static inline bool rows_on_16(const void* ptr, int64_t b, int64_t h, int64_t t, 
   return ((reinterpret_cast<uintptr_t>(ptr) | (uintptr_t)(b * es) | (uintptr_t)(h * es) | (uintptr_t)(t * es)) & 15) == 0;
 }
 
+}  // namespace attn
+
+// Query tiles of a head in the dq kernel: rows of the table gradient's partial sums.
+namespace attn {
+static inline int dq_tiles(const Params& p) { return p.wide_dq ? (p.Tq + 127) / 128 : (p.Tq + 31) / 32; }
 }  // namespace attn
 
 // dtable[n, h] = sum over r of part[r][h][n] (relative_bias.hip).
