@@ -61,7 +61,7 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     copy, padded with zeros, where that does not hold."""
     e = t.element_size()
     s, n = t.stride(), t.shape
-    if ((s[3] == 1 or n[3] == 1) and n[3] * e % 16 == 0 and t.data_ptr() % 16 == 0 and s[2] < 1 << 26
+    if ((s[3] == 1 or n[3] == 1) and n[3] * e % 16 == 0 and t.data_ptr() % 16 == 0 and s[2] < 1 << 22
             and all(s[i] * e % 16 == 0 or n[i] == 1 for i in range(3))):
         return t
     pad = -n[3] % (16 // e)

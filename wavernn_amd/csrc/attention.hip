@@ -64,7 +64,7 @@ int attention_params(const wrnn_attention_desc* d, attn::Params* p, const char* 
   p->v_b = st(d->batch, d->v_stride[0]), p->v_h = st(d->kv_heads, d->v_stride[1]), p->v_t = st(d->k_len, d->v_stride[2]);
   // a lane's rows inside a tile are found with 32-bit offsets
   for (int64_t s : {p->q_t, p->k_t, p->v_t})
-    WRNN_REQUIRE(s > -kMaxRowStride && s < kMaxRowStride, "%s: position strides are below 2^26 elements", who);
+    WRNN_REQUIRE(s >= 0 && s < kMaxRowStride, "%s: position strides are in 0 .. 2^22 - 1 elements", who);
   p->B = d->batch, p->H = d->heads, p->Hkv = d->kv_heads, p->group = d->heads ? d->heads / d->kv_heads : 1;
   p->Tq = d->q_len, p->Tk = d->k_len, p->D = d->head_dim;
   p->causal = d->causal != 0;
@@ -134,7 +134,7 @@ extern "C" int wrnn_attention_backward(const wrnn_attention_desc* desc, const wr
   WRNN_REQUIRE(on16(g->out, g->out_stride) && on16(g->dout, g->dout_stride) && on16(g->dq, g->dq_stride) && on16(g->dk, g->dk_stride) && on16(g->dv, g->dv_stride),
                "wrnn_attention_backward: rows have to start on 16 bytes");
   for (const int64_t* x : {g->out_stride, g->dout_stride, g->dq_stride, g->dk_stride, g->dv_stride})
-    WRNN_REQUIRE(x[2] > -attn::kMaxRowStride && x[2] < attn::kMaxRowStride, "wrnn_attention_backward: position strides are below 2^26 elements");
+    WRNN_REQUIRE(x[2] >= 0 && x[2] < attn::kMaxRowStride, "wrnn_attention_backward: position strides are in 0 .. 2^22 - 1 elements");
   p.o_in = g->out, p.oi_b = g->out_stride[0], p.oi_h = g->out_stride[1], p.oi_t = g->out_stride[2];
   p.dout = g->dout, p.do_b = g->dout_stride[0], p.do_h = g->dout_stride[1], p.do_t = g->dout_stride[2];
   p.dq = g->dq, p.dq_b = g->dq_stride[0], p.dq_h = g->dq_stride[1], p.dq_t = g->dq_stride[2];

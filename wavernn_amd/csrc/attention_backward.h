@@ -59,6 +59,7 @@ struct BackwardShape {
   static constexpr int WAVES = WS * WM, THREADS = 64 * WAVES, BM = 32 * WM * NS;
   static constexpr int BUFS = WIDE && !(NP == 3 && DP == 256) ? 2 : 1;  // two where they leave room for the position bias's tables
   static constexpr bool AHEAD = WIDE || DP * NP <= 256;                 // the next tile is requested before this one's arithmetic
+  static constexpr bool EARLY = NP == 3 && BUFS == 2;                   // it goes to LDS beside the arithmetic (forward pass)
   static constexpr bool RAW = NP == 3 && DP == 256;
   // output columns of a workgroup: both sums and both stationary operands have to fit the registers
   static constexpr int DA = DP > 128 ? 128 : DP, PARTS = DP / DA, DT = DA / 32;
@@ -165,42 +166,60 @@ __global__ __launch_bounds__((BackwardShape<T, DP, WIDE>::THREADS), (BackwardSha
   f32x16 acc[S::DT] = {};
   BiasGrad bias_grad;
   Stage<T, DP, BN, NT> sk, sv;
+  sk.start(kb, p.k_t, end, p.D, tid);
+  sv.start(vb, p.v_t, end, p.D, tid);
   KeyBits<BN> keys(mask, end, lane);
   auto load = [&](int t) {
-    sk.load(kb, p.k_t, t * BN, end, p.D, tid);
-    sv.load(vb, p.v_t, t * BN, end, p.D, tid);
+    sk.load(t * BN);
+    sv.load(t * BN);
     keys.load(t * BN);
   };
+  auto drop = [&](const RowBits& use) {
+    if (mask && !use.template all<BN>()) {
+      sk.drop(use, tid);
+      sv.drop(use, tid);
+    }
+  };
   auto store = [&](int t) {
-    const RowBits use = keys.get(t * BN);
     const int o = t & (BUFS - 1);
-    sk.drop(use, tid);
-    sv.drop(use, tid);
     sk.store(kt + o * TL::BYTES, tid);
     sv.store(vt + o * TL::BYTES, tid);
-    return use;
   };
-  const bool live = q0 < p.Tq;
 #pragma unroll
   for (int walk = TWICE ? 0 : 1; walk < 2; ++walk) {
-    // round r requests tile r, works on tile r - 1 and puts tile r into LDS (one copy of each piece of code)
-    RowBits use;
+    // the order of a round: as in the forward pass
+    RowBits use, next;
+    load(0);
+    use = keys.get(0);
+    drop(use);
+    store(0);
+    if (S::EARLY) load(1);
     __syncthreads();
-    for (int r = 0; r <= tiles; ++r) {
-      if (S::AHEAD && r < tiles) load(r);
-      const int t = r - 1;
+    for (int t = 0; t < tiles; ++t) {
       const char *kk = kt + (t & (BUFS - 1)) * TL::BYTES, *vv = vt + (t & (BUFS - 1)) * TL::BYTES;
-      if (live && r > 0) {
+      if (S::EARLY) {
+        next = keys.get((t + 1) * BN);
+        drop(next);
+      } else if (S::AHEAD) {
+        load(t + 1);
+      }
 #pragma unroll
-        for (int x = 0; x < S::NS; ++x) {
-          const int sub = S::NS * wm + x, key0 = t * BN + sub * 32;
-          if (key0 >= end || (p.causal && key0 > pos_hi)) break;
-          f32x16 raw = {}, dp = {};
+      for (int x = 0; x < S::NS; ++x) {
+        const int sub = S::NS * wm + x, key0 = t * BN + sub * 32;
+        const bool work = key0 < end && !(p.causal && key0 > pos_hi);
+        f32x16 raw = {}, dp = {};
+        if (work) {
 #pragma unroll
           for (int c = 0; c < NC2; ++c) {
             raw = mma(TL::row_chunk(kk, sub * 32 + col, 2 * c + half), q.get(c), raw);
             dp = mma(TL::row_chunk(vv, sub * 32 + col, 2 * c + half), go.get(c), dp);
           }
+        }
+        if (x == 0 && S::EARLY) {
+          store(t + 1);
+          load(t + 2);
+        }
+        if (work) {
           float pr[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) pr[i] = raw[i];
@@ -219,9 +238,14 @@ __global__ __launch_bounds__((BackwardShape<T, DP, WIDE>::THREADS), (BackwardSha
           }
         }
       }
-      if (BUFS == 1) __syncthreads();
-      if (!S::AHEAD && r < tiles) load(r);
-      if (r < tiles) use = store(r);
+      if (!S::EARLY) {
+        if (BUFS == 1) __syncthreads();
+        if (!S::AHEAD) load(t + 1);
+        next = keys.get((t + 1) * BN);
+        drop(next);
+        store(t + 1);
+      }
+      use = next;
       __syncthreads();
     }
     if (TWICE && walk == 0) {
@@ -296,11 +320,16 @@ __global__ __launch_bounds__((BackwardShape<T, DP, WIDE>::THREADS), (BackwardSha
   const int qt_n = (p.Tq + BM - 1) / BM, qt_0 = p.causal ? min(max(k0 - off, 0) / BM, qt_n) : 0, per = qt_n - qt_0;
   const int steps = k0 < end ? per * p.group : 0;
   Stage<T, DP, BM, NT> sq, sg;
+  sq.start(nullptr, p.q_t, p.Tq, p.D, tid);
+  sg.start(nullptr, p.do_t, p.Tq, p.D, tid);
   float s_lse = 0.f, s_delta = 0.f;
   auto load = [&](int it) {
+    if (it >= steps) return;
     const int h = kvh * p.group + it / per, r0 = (qt_0 + it % per) * BM;
-    sq.load(reinterpret_cast<const T*>(p.q) + b * p.q_b + h * p.q_h, p.q_t, r0, p.Tq, p.D, tid);
-    sg.load(reinterpret_cast<const T*>(p.dout) + b * p.do_b + h * p.do_h, p.do_t, r0, p.Tq, p.D, tid);
+    sq.base = reinterpret_cast<const char*>(reinterpret_cast<const T*>(p.q) + b * p.q_b + h * p.q_h);
+    sg.base = reinterpret_cast<const char*>(reinterpret_cast<const T*>(p.dout) + b * p.do_b + h * p.do_h);
+    sq.load(r0);
+    sg.load(r0);
     if (tid < BM) {
       const int64_t row = ((int64_t)b * p.H + h) * p.Tq + r0 + tid;
       const float l = r0 + tid < p.Tq ? p.lse[row] : -INFINITY;
@@ -317,29 +346,37 @@ __global__ __launch_bounds__((BackwardShape<T, DP, WIDE>::THREADS), (BackwardSha
       stat[(o * 2 + 1) * BM + tid] = s_delta;
     }
   };
-  for (int r = 0; r <= steps; ++r) {
-    const int it = r - 1;
+  load(0);
+  store(0);
+  if (S::EARLY) load(1);
+  __syncthreads();
+  for (int it = 0; it < steps; ++it) {
     if constexpr (BIAS) {
-      if (r > 0 && r <= steps && it % per == 0) {
+      if (it % per == 0) {
         fill_lut(p, kvh * p.group + it / per, lut, tid, NT);
         __syncthreads();
       }
     }
-    if (S::AHEAD && r < steps) load(r);
     const int o = it & (BUFS - 1), r0 = (qt_0 + it % per) * BM;
     const char *qq = qt + o * TL::BYTES, *gg = gt + o * TL::BYTES;
-    if (r > 0 && kw < end) {
+    if (!S::EARLY && S::AHEAD) load(it + 1);
 #pragma unroll
-      for (int x = 0; x < S::NS; ++x) {
-        const int sub = S::NS * wm + x, i0 = r0 + sub * 32, p0 = i0 + off;  // position of the subtile's first query
-        if (i0 >= p.Tq) break;
-        if (p.causal && kw > p0 + 31) continue;
-        f32x16 raw = {}, dp = {};
+    for (int x = 0; x < S::NS; ++x) {
+      const int sub = S::NS * wm + x, i0 = r0 + sub * 32, p0 = i0 + off;  // position of the subtile's first query
+      const bool work = kw < end && i0 < p.Tq && !(p.causal && kw > p0 + 31);
+      f32x16 raw = {}, dp = {};
+      if (work) {
 #pragma unroll
         for (int c = 0; c < NC2; ++c) {
           raw = mma(TL::row_chunk(qq, sub * 32 + col, 2 * c + half), k.get(c), raw);
           dp = mma(TL::row_chunk(gg, sub * 32 + col, 2 * c + half), v.get(c), dp);
         }
+      }
+      if (x == 0 && S::EARLY) {
+        store(it + 1);
+        load(it + 2);
+      }
+      if (work) {
         float s[16];
         if constexpr (BIAS) {
           const int md = p.max_distance;
@@ -376,9 +413,11 @@ __global__ __launch_bounds__((BackwardShape<T, DP, WIDE>::THREADS), (BackwardSha
         column_product<T, TL>(qq, sub * 32, d0, Weights<T>(ds), dk, lane);
       }
     }
-    if (BUFS == 1) __syncthreads();
-    if (!S::AHEAD && r < steps) load(r);
-    if (r < steps) store(r);
+    if (!S::EARLY) {
+      if (BUFS == 1) __syncthreads();
+      if (!S::AHEAD) load(it + 1);
+      store(it + 1);
+    }
     __syncthreads();
   }
   T* kout = reinterpret_cast<T*>(p.dk) + b * p.dk_b + kvh * p.dk_h;

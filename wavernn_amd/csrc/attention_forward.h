@@ -51,6 +51,7 @@ struct ForwardShape {
   static constexpr int THREADS = 64 * WQ * WK, BN = 32 * WK * NS;
   static constexpr int BUFS = WIDE && !(NP == 3 && DP == 256) ? 2 : 1;  // two where they fit
   static constexpr int WAVES = WIDE ? (DP * NP <= 192 ? 2 : 1) : (DP * NP <= 128 ? 2 : 1);  // per SIMD
+  static constexpr bool EARLY = NP == 3 && BUFS == 2;
   using TL = Tile<T, DP, BN>;
   static constexpr size_t TILES = 2 * BUFS * TL::BYTES, SUMS = WK > 1 ? (size_t)WK * 32 * (DP + 4) * 4 : 0;
   static constexpr size_t BODY = TILES > SUMS ? TILES : SUMS;
@@ -105,36 +106,54 @@ __global__ __launch_bounds__((ForwardShape<T, DP, WIDE>::THREADS), (ForwardShape
   f32x16 acc[DT] = {};
   Running run;
   Stage<T, DP, BN, NT> sk, sv;
+  sk.start(kb, p.k_t, end, p.D, tid);
+  sv.start(vb, p.v_t, end, p.D, tid);
   KeyBits<BN> keys(mask, end, lane);
   auto load = [&](int t) {
-    sk.load(kb, p.k_t, t * BN, end, p.D, tid);
-    sv.load(vb, p.v_t, t * BN, end, p.D, tid);
+    sk.load(t * BN);
+    sv.load(t * BN);
     keys.load(t * BN);
   };
+  auto drop = [&](const RowBits& use) {
+    if (mask && !use.template all<BN>()) {
+      sk.drop(use, tid);
+      sv.drop(use, tid);
+    }
+  };
   auto store = [&](int t) {
-    const RowBits use = keys.get(t * BN);
     const int o = t & (BUFS - 1);
-    sk.drop(use, tid);
-    sv.drop(use, tid);
     sk.store(kt + o * TL::BYTES, tid);
     sv.store(vt + o * TL::BYTES, tid);
-    return use;
   };
-  // round r requests tile r, works on tile r - 1 and puts tile r into LDS: one copy of each piece of code, for a call's time on few
-  // tiles is the time to fetch its instructions
-  RowBits use;
-  if constexpr (BIAS) __syncthreads();
-  for (int r = t0; r <= t1; ++r) {
-    if (r < t1) load(r);
-    const int t = r - 1;
+  // float32 (EARLY): tile t is worked on while tile t + 1 goes from registers to LDS (its conversion fills the matrix instructions' shadow)
+  // and tile t + 2 is requested.  Otherwise tile t + 1 is requested before tile t's arithmetic and goes to LDS after it; with one buffer
+  // that waits for everybody to be done with tile t.
+  RowBits use, next;
+  load(t0);
+  use = keys.get(t0 * BN);
+  drop(use);
+  store(t0);
+  if (S::EARLY) load(t0 + 1);
+  __syncthreads();
+  for (int t = t0; t < t1; ++t) {
     const char *kk = kt + (t & (BUFS - 1)) * TL::BYTES, *vv = vt + (t & (BUFS - 1)) * TL::BYTES;
     const int sub0 = NS * wk, key0 = t * BN + 32 * sub0;
-    if (r > t0 && q0 < p.Tq && key0 < end && !(p.causal && key0 > pos_hi)) {
+    if (S::EARLY) {
+      next = keys.get((t + 1) * BN);
+      drop(next);
+    } else {
+      load(t + 1);
+    }
+    if (key0 < end && !(p.causal && key0 > pos_hi)) {
       f32x16 raw[NS] = {};
 #pragma unroll
       for (int c = 0; c < NC2; ++c)
 #pragma unroll
         for (int s = 0; s < NS; ++s) raw[s] = mma(TL::row_chunk(kk, (sub0 + s) * 32 + col, 2 * c + half), q.get(c), raw[s]);
+      if (S::EARLY) {
+        store(t + 1);
+        load(t + 2);
+      }
       float s[NS][16];
 #pragma unroll
       for (int x = 0; x < NS; ++x) {
@@ -145,9 +164,17 @@ __global__ __launch_bounds__((ForwardShape<T, DP, WIDE>::THREADS), (ForwardShape
       run.step(s, acc);
 #pragma unroll
       for (int x = 0; x < NS; ++x) column_product<T, TL>(vv, (sub0 + x) * 32, 0, Weights<T>(s[x]), acc, lane);
+    } else if (S::EARLY) {
+      store(t + 1);
+      load(t + 2);
     }
-    if (BUFS == 1) __syncthreads();
-    if (r < t1) use = store(r);
+    if (!S::EARLY) {
+      if (BUFS == 1) __syncthreads();
+      next = keys.get((t + 1) * BN);
+      drop(next);
+      store(t + 1);
+    }
+    use = next;
     __syncthreads();
   }
   const float l = both_sum(run.l);

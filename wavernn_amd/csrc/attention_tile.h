@@ -36,7 +36,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int kMaxEdges = 128;
 constexpr int kMaxDistance = 1024;
-constexpr int64_t kMaxRowStride = 1 << 26;
+constexpr int64_t kMaxRowStride = 1 << 22;
 
 // What the kernels get, by value.  Strides count elements; the last dimension is contiguous.
 struct Params {
@@ -258,8 +258,14 @@ __device__ __forceinline__ void column_product(const char* tile, int r0, int d0,
 // Which rows of a tile of up to 128 may be used, one bit each.
 struct RowBits {
   uint64_t lo = 0, hi = 0;
-  __device__ __forceinline__ uint32_t of(int sub) const { return (uint32_t)((sub & 2 ? +hi : +lo) >> (32 * (sub & 1))); }
-  __device__ __forceinline__ bool at(int r) const { return ((r & 64 ? +hi : +lo) >> (r & 63)) & 1; }
+  __device__ __forceinline__ uint32_t of(int sub) const {
+    const uint64_t a = lo, b = hi;
+    return (uint32_t)((sub & 2 ? b : a) >> (32 * (sub & 1)));
+  }
+  __device__ __forceinline__ bool at(int r) const {
+    const uint64_t a = lo, b = hi;
+    return ((r & 64 ? b : a) >> (r & 63)) & 1;
+  }
   template <int ROWS>
   __device__ __forceinline__ bool all() const {
     constexpr uint64_t first = ROWS >= 64 ? ~0ull : (1ull << (ROWS & 63)) - 1;
@@ -275,7 +281,7 @@ struct KeyBits {
   uint32_t out_lo = 0, out_hi = 0;
   __device__ __forceinline__ KeyBits(const uint8_t* mask_, int end_, int lane_) : mask(mask_), end(end_), lane(lane_) {}
   __device__ __forceinline__ void load(int key0) {
-    if (!mask) return;
+    if (!mask || end <= 0) return;  // no key at all: nothing to look at (and mask[end - 1] would lie before it)
     out_lo = mask[min(key0 + lane, end - 1)];
     if (ROWS > 64) out_hi = mask[min(key0 + 64 + lane, end - 1)];
   }
@@ -287,26 +293,45 @@ struct KeyBits {
   }
 };
 
-// Rows of a tensor's [.., T, D] slice on their way to an LDS tile: requested before a tile's arithmetic, written to LDS after it.
-// Rows that may not be used become zero: what lies there (another sequence's values, infinities, NaN) must not reach a
-// product, where 0 * NaN would.
+// Rows of a tensor's [.., T, D] slice on their way to an LDS tile: requested a round before they are written to LDS.  Buffer loads check
+// every lane against the tile's last byte: rows at or past `limit`, and the chunks past D, come back as zero without a branch.
+// Rows inside that a mask leaves out are zeroed too (drop): what lies at keys that are left out (another sequence's values, infinities, NaN) must
+// not reach a product, where 0 * NaN would.
 template <class T, int DP, int ROWS, int NT>
 struct Stage {
   using TL = Tile<T, DP, ROWS>;
-  static constexpr int N = ROWS * TL::NCH / NT, STEP = NT / TL::NCH;
+  static constexpr int N = ROWS * TL::NCH / NT, STEP = NT / TL::NCH, ES = sizeof(T), PER = 8 * ES / 16;  // PER: 16-byte loads of a chunk
   static_assert(N >= 1 && NT % TL::NCH == 0, "whole rows per pass");
+  static constexpr uint32_t kOutside = 0x80000000u;  // past any tile (rows are below 2^22 elements apart)
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
   Raw<T> r[N];
-  __device__ __forceinline__ void load(const T* base, int64_t stride, int row0, int limit, int D, int tid) {
+  const char* base;
+  int64_t row_bytes;
+  uint32_t off[PER];
+  int limit, last;  // rows; bytes of a row that hold data
+  __device__ __forceinline__ void start(const T* b, int64_t stride, int rows, int D, int tid) {
+    base = reinterpret_cast<const char*>(b);
+    row_bytes = stride * ES;
+    limit = rows;
+    last = D * ES;
     const int ch = tid % TL::NCH, mine = tid / TL::NCH;
 #pragma unroll
+    for (int i = 0; i < PER; ++i) off[i] = ch * 8 * ES + 16 * i < last ? (uint32_t)(mine * (int)row_bytes + ch * 8 * ES + 16 * i) : kOutside;
+  }
+  __device__ __forceinline__ void load(int row0) {
+    const int rows = min(limit - row0, ROWS);
+    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base + (int64_t)row0 * row_bytes), 0,
+                                                        rows > 0 ? (rows - 1) * (int)row_bytes + last : 0, 0x00020000);
+#pragma unroll
     for (int n = 0; n < N; ++n) {
-      const T* rows = base + (int64_t)(row0 + n * STEP) * stride;  // the same for all lanes
-      r[n].x = {};
-      if (row0 + n * STEP + mine < limit) r[n] = load_chunk<T>(rows + mine * (int)stride, ch, D);
+      u32x4 x[PER];
+#pragma unroll
+      for (int i = 0; i < PER; ++i) x[i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, off[i] + (uint32_t)(n * STEP * (int)row_bytes), 0, 0);
+      if constexpr (PER == 1) r[n].x = __builtin_bit_cast(typename Raw<T>::vec, x[0]);
+      else r[n].x = __builtin_shufflevector(__builtin_bit_cast(f32x4, x[0]), __builtin_bit_cast(f32x4, x[1]), 0, 1, 2, 3, 4, 5, 6, 7);
     }
   }
   __device__ __forceinline__ void drop(const RowBits& bits, int tid) {
-    if (bits.all<ROWS>()) return;
 #pragma unroll
     for (int n = 0; n < N; ++n)
       if (!bits.at(tid / TL::NCH + n * STEP)) r[n].x = {};
