@@ -13,7 +13,7 @@ namespace attn {
 struct Running {
   float m = -3e38f, l = 0.f;
   template <int NS, int DT>
-  __device__ __forceinline__ void step(float (&s)[NS][16], f32x16 (&acc)[DT]) {
+  __device__ __forceinline__ void move(const float (&s)[NS][16], f32x16 (&acc)[DT]) {
     float mx = s[0][0];
 #pragma unroll
     for (int n = 0; n < NS; ++n)
@@ -27,13 +27,11 @@ struct Running {
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) acc[dt] *= a;
     }
-#pragma unroll
-    for (int n = 0; n < NS; ++n)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        s[n][i] = __builtin_amdgcn_exp2f(s[n][i] - m);
-        l += s[n][i];
-      }
+  }
+  __device__ __forceinline__ float weight(float s) {
+    const float x = __builtin_amdgcn_exp2f(s - m);
+    l += x;
+    return x;
   }
 };
 
@@ -146,13 +144,29 @@ __global__ __launch_bounds__((ForwardShape<T, DP, WIDE>::THREADS), (ForwardShape
     }
     if (key0 < end && !(p.causal && key0 > pos_hi)) {
       f32x16 raw[NS] = {};
+      if constexpr (S::EARLY) {
+        char *kn = kt + ((t + 1) & (BUFS - 1)) * TL::BYTES, *vn = vt + ((t + 1) & (BUFS - 1)) * TL::BYTES;
+        u32x4 w[3];
+        constexpr int PIECES = decltype(sk)::PIECES;
+        const auto piece = [&](int i) {
+          if (i < PIECES) sk.store_piece(kn, tid, i, w);
+          else sv.store_piece(vn, tid, i - PIECES, w);
+        };
+        const Shadow<decltype(piece)> shadow(6 * NC2, 2 * PIECES, piece);
+        Operand<T> a = TL::row_chunk(kk, col, half);
 #pragma unroll
-      for (int c = 0; c < NC2; ++c)
-#pragma unroll
-        for (int s = 0; s < NS; ++s) raw[s] = mma(TL::row_chunk(kk, (sub0 + s) * 32 + col, 2 * c + half), q.get(c), raw[s]);
-      if (S::EARLY) {
-        store(t + 1);
+        for (int c = 0; c < NC2; ++c) {
+          Operand<T> next = a;
+          if (c + 1 < NC2) next = TL::row_chunk(kk, col, 2 * c + 2 + half);
+          raw[0] = mma(a, q.get(c), raw[0], [&](int m) { shadow(6 * c + m); });
+          a = next;
+        }
         load(t + 2);
+      } else {
+#pragma unroll
+        for (int c = 0; c < NC2; ++c)
+#pragma unroll
+          for (int s = 0; s < NS; ++s) raw[s] = mma(TL::row_chunk(kk, (sub0 + s) * 32 + col, 2 * c + half), q.get(c), raw[s]);
       }
       float s[NS][16];
 #pragma unroll
@@ -161,9 +175,17 @@ __global__ __launch_bounds__((ForwardShape<T, DP, WIDE>::THREADS), (ForwardShape
         for (int i = 0; i < 16; ++i) s[x][i] = raw[x][i];
         finish_scores<BIAS>(p, s[x], key0 + 32 * x, pos, pos_lo, pos_hi, use.of(sub0 + x), my_lut, half);
       }
-      run.step(s, acc);
+      run.move(s, acc);
+      if constexpr (S::EARLY) {
+        column_product_shadow<TL>(vv, 0, 0, [&](int i) { return run.weight(s[0][i]); }, acc, lane);
+      } else {
 #pragma unroll
-      for (int x = 0; x < NS; ++x) column_product<T, TL>(vv, (sub0 + x) * 32, 0, Weights<T>(s[x]), acc, lane);
+        for (int x = 0; x < NS; ++x) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[x][i] = run.weight(s[x][i]);
+          column_product<T, TL>(vv, (sub0 + x) * 32, 0, Weights<T>(s[x]), acc, lane);
+        }
+      }
     } else if (S::EARLY) {
       store(t + 1);
       load(t + 2);

@@ -8,10 +8,10 @@
 // registers are already the right-hand operand of the second product  Z(moving)^T * P : its sum runs over the moving rows, whose
 // order is free as long as both operands use the same one.  No score ever goes through shared memory.
 //
-// float32 goes through the same instructions: a value is the sum of three bfloat16 (8 bits of mantissa each, rounded to nearest, so 24 and a
-// sign in each remainder), and a product the six partial products down to 2^-24 of it, added in 32 bits, smallest first.  What is left out
-// is below 2^-25: the result is as exact as the 32-bit matrix instruction's and takes 6 x 32 cycles for 16 columns of a 32 x 32
-// tile where that one takes 8 x 64.
+// float32 goes through the same instructions: a value is the sum of three bfloat16 (8 bits of mantissa each), and a product the six partial
+// products that reach 2^-16 of it, added in 32 bits, smallest first.  What is left out is 2^-23 of a product on average and 2^-20 at
+// most, the result as exact as the 32-bit matrix instruction's (measured: 5e-7 of the norm either way), and 16 columns of a 32 x 32 tile take
+// 6 x 32 cycles where that one takes 8 x 64.
 //
 // Moving tiles lie in LDS row by row in 16-byte chunks of 8 bfloat16 (three planes for float32).  The first product reads chunk 2c + half of
 // a row per lane; the second reads columns with ds_read_b64_tr_b16 (four rows x 16 columns transposed per 16 lanes).
@@ -86,28 +86,31 @@ struct Raw {  // 8 elements as they come from memory
 };
 
 __device__ __forceinline__ Operand<__bf16> operand(const Raw<__bf16>& r) { return {{r.x}}; }
-// Two values at a time: one packed conversion, and the two roundings back as bits (a shift, a mask).
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-  return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)a, (__bf16)b});
-}
-__device__ __forceinline__ void split(f32x8 x, bf16x8 (&p)[3]) {
-  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-  u32x4 w[3];
+// Two values at a time, by cutting: a plane is the upper half of what the planes before it leave (8 bits of mantissa, the subtraction is
+// exact), so the three add up to the value itself.
+__device__ __forceinline__ void split2(float a, float b, uint32_t (&w)[3]) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    float a = x[2 * j], b = x[2 * j + 1];
-#pragma unroll
-    for (int n = 0; n < 3; ++n) {
-      uint32_t u = pack2(a, b);
-      asm("" : "+v"(u));  // keeps it one conversion: without this the low half is converted a second time on its own
-      w[n][j] = u;
-      a -= __uint_as_float(u << 16);  // exact
-      b -= __uint_as_float(u & 0xffff0000u);
+  for (int n = 0; n < 3; ++n) {
+    const uint32_t x = __float_as_uint(a), y = __float_as_uint(b);
+    w[n] = __builtin_amdgcn_perm(y, x, 0x07060302u);  // upper halves of x and y
+    if (n < 2) {
+      a -= __uint_as_float(x & 0xffff0000u);
+      b -= __uint_as_float(y & 0xffff0000u);
     }
   }
+}
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ void split(f32x8 x, bf16x8 (&p)[3]) {
+  u32x4 v[3];
 #pragma unroll
-  for (int n = 0; n < 3; ++n) p[n] = __builtin_bit_cast(bf16x8, w[n]);
+  for (int j = 0; j < 4; ++j) {
+    uint32_t w[3];
+    split2(x[2 * j], x[2 * j + 1], w);
+#pragma unroll
+    for (int n = 0; n < 3; ++n) v[n][j] = w[n];
+  }
+#pragma unroll
+  for (int n = 0; n < 3; ++n) p[n] = __builtin_bit_cast(bf16x8, v[n]);
 }
 __device__ __forceinline__ Operand<float> operand(const Raw<float>& r) {
   Operand<float> o;
@@ -116,15 +119,43 @@ __device__ __forceinline__ Operand<float> operand(const Raw<float>& r) {
 }
 
 __device__ __forceinline__ f32x16 mma1(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
-__device__ __forceinline__ f32x16 mma(const Operand<__bf16>& a, const Operand<__bf16>& b, f32x16 c) { return mma1(a.p[0], b.p[0], c); }
-__device__ __forceinline__ f32x16 mma(const Operand<float>& a, const Operand<float>& b, f32x16 c) {
-  c = mma1(a.p[2], b.p[0], c);
-  c = mma1(a.p[0], b.p[2], c);
-  c = mma1(a.p[1], b.p[1], c);
-  c = mma1(a.p[1], b.p[0], c);
-  c = mma1(a.p[0], b.p[1], c);
-  return mma1(a.p[0], b.p[0], c);
+
+// One product of 16 columns; between(m) runs after its m-th matrix instruction.
+template <class F>
+__device__ __forceinline__ f32x16 mma(const Operand<__bf16>& a, const Operand<__bf16>& b, f32x16 c, F&& between) {
+  c = mma1(a.p[0], b.p[0], c);
+  between(0);
+  return c;
 }
+template <class F>
+__device__ __forceinline__ f32x16 mma(const Operand<float>& a, const Operand<float>& b, f32x16 c, F&& between) {
+  constexpr int pa[6] = {2, 0, 1, 1, 0, 0}, pb[6] = {0, 2, 1, 0, 1, 0};
+#pragma unroll
+  for (int m = 0; m < 6; ++m) {
+    c = mma1(a.p[pa[m]], b.p[pb[m]], c);
+    between(m);
+  }
+  return c;
+}
+template <class T>
+__device__ __forceinline__ f32x16 mma(const Operand<T>& a, const Operand<T>& b, f32x16 c) {
+  return mma(a, b, c, [](int) {});
+}
+
+// Work in the matrix instructions' shadow: a 32 x 32 x 16 product keeps the matrix unit for 32 cycles, a vector instruction its unit for 4, and a
+// wave issues in order, so a wave that is alone on its SIMD has to have vector instructions BETWEEN its products.  The compiler's
+// scheduler moves them behind; Shadow(products, pieces, f) deals f(0) .. f(pieces - 1) out over the products and fences each step.
+template <class F>
+struct Shadow {
+  int products, pieces;
+  F f;
+  __device__ __forceinline__ Shadow(int products_, int pieces_, F f_) : products(products_), pieces(pieces_), f(f_) {}
+  __device__ __forceinline__ void operator()(int m) const {
+#pragma unroll
+    for (int i = m * pieces / products; i < (m + 1) * pieces / products; ++i) f(i);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+};
 
 __device__ __forceinline__ int moving_row(int i, int half) { return 8 * (i >> 2) + 4 * half + (i & 3); }
 
@@ -228,30 +259,69 @@ struct Weights {
   }
 };
 
+// Left-hand operand X^T of 16 moving rows from row r0 of the tile, output rows d0 .. d0 + 31.  Lane l of a 16-lane group hands in row
+// l / 4, columns 4 (l % 4) .. + 3 and gets column l of the four rows.
+template <class T, class TL>
+__device__ __forceinline__ Operand<T> column_chunk(const char* tile, int r0, int d0, int lane) {
+  const int half = lane >> 5, sub = lane & 15, colgrp = (lane >> 4) & 1;
+  const int rr = r0 + 4 * half + (sub >> 2), col = d0 + colgrp * 16 + 4 * (sub & 3);
+  Operand<T> a;
+#pragma unroll
+  for (int n = 0; n < TL::NP; ++n)
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int r = rr + 8 * u;
+      const char* at = tile + n * TL::PLANE + r * TL::ROWB + TL::swizzle(r, col >> 3) * 16 + (col & 7) * 2;
+      const bf16x4 t = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)(uintptr_t)(uint32_t)(uintptr_t)at);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) a.p[n][4 * u + e] = t[e];
+    }
+  return a;
+}
+
 // acc[dt] += X^T W over 32 moving rows from row r0 of the tile, output rows d0 + 32 dt ..
 template <class T, class TL, int DT>
 __device__ __forceinline__ void column_product(const char* tile, int r0, int d0, const Weights<T>& w, f32x16 (&acc)[DT], int lane) {
-  // lane l of a 16-lane group hands in row l / 4, columns 4 (l % 4) .. + 3 and gets column l of the four rows
-  const int half = lane >> 5, sub = lane & 15, colgrp = (lane >> 4) & 1;
-  const int rr = r0 + 4 * half + (sub >> 2);
 #pragma unroll
-  for (int dt = 0; dt < DT; ++dt) {
-    const int col = d0 + dt * 32 + colgrp * 16 + 4 * (sub & 3);
+  for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      Operand<T> a;
+    for (int s = 0; s < 2; ++s) acc[dt] = mma(column_chunk<T, TL>(tile, r0 + 16 * s, d0 + 32 * dt, lane), w.o[s], acc[dt]);
+}
+
+// The same for float32 from weights not made yet: value(i) gives weight i of the lane.  The first 16 moving rows' weights are made
+// ahead, the others' in the shadow of the first products.
+template <class TL, int DT, class V>
+__device__ __forceinline__ void column_product_shadow(const char* tile, int r0, int d0, V&& value, f32x16 (&acc)[DT], int lane) {
+  u32x4 w[2][3];
+  auto make = [&](int i) {
+    uint32_t x[3];
+    split2(value(2 * i), value(2 * i + 1), x);
 #pragma unroll
-      for (int n = 0; n < TL::NP; ++n)
+    for (int k = 0; k < 3; ++k) w[i >> 2][k][i & 3] = x[k];
+  };
+  auto get = [&](int s) {
+    Operand<float> o;
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int r = rr + 16 * s + 8 * u;
-          const char* at = tile + n * TL::PLANE + r * TL::ROWB + TL::swizzle(r, col >> 3) * 16 + (col & 7) * 2;
-          const bf16x4 t = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)(uintptr_t)(uint32_t)(uintptr_t)at);
+    for (int k = 0; k < 3; ++k) o.p[k] = __builtin_bit_cast(bf16x8, w[s][k]);
+    return o;
+  };
+  Operand<float> a = column_chunk<float, TL>(tile, r0, d0, lane);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) a.p[n][4 * u + e] = t[e];
-        }
-      acc[dt] = mma(a, w.o[s], acc[dt]);
-    }
+  for (int i = 0; i < 4; ++i) make(i);
+  Operand<float> b = get(0);
+  const auto later = [&](int i) { make(4 + i); };
+  const Shadow<decltype(later)> shadow(6 * DT, 4, later);
+#pragma unroll
+  for (int n = 0; n < 2 * DT; ++n) {
+    const int s = n / DT, dt = n % DT, ns = (n + 1) / DT, nd = (n + 1) % DT;
+    if (n == DT) b = get(1);
+    Operand<float> next = a;
+    if (n + 1 < 2 * DT) next = column_chunk<float, TL>(tile, r0 + 16 * ns, d0 + 32 * nd, lane);
+    acc[dt] = mma(a, b, acc[dt], [&](int m) {
+      if (s == 0) shadow(6 * dt + m);
+      else __builtin_amdgcn_sched_barrier(0);
+    });
+    a = next;
   }
 }
 
@@ -303,7 +373,6 @@ struct Stage {
   static constexpr int N = ROWS * TL::NCH / NT, STEP = NT / TL::NCH, ES = sizeof(T), PER = 8 * ES / 16;  // PER: 16-byte loads of a chunk
   static_assert(N >= 1 && NT % TL::NCH == 0, "whole rows per pass");
   static constexpr uint32_t kOutside = 0x80000000u;  // past any tile (rows are below 2^22 elements apart)
-  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
   Raw<T> r[N];
   const char* base;
   int64_t row_bytes;
@@ -339,6 +408,21 @@ struct Stage {
   __device__ __forceinline__ void store(char* tile, int tid) {
 #pragma unroll
     for (int n = 0; n < N; ++n) TL::put(tile, tid / TL::NCH + n * STEP, tid % TL::NCH, operand(r[n]));
+  }
+  // The same in PIECES steps (float32), two values each.
+  static constexpr int PIECES = 4 * N;
+  __device__ __forceinline__ void store_piece(char* tile, int tid, int i, u32x4 (&w)[3]) {
+    const int n = i >> 2, j = i & 3;
+    uint32_t x[3];
+    split2(r[n].x[2 * j], r[n].x[2 * j + 1], x);
+#pragma unroll
+    for (int k = 0; k < 3; ++k) w[k][j] = x[k];
+    if (j == 3) {
+      Operand<T> o;
+#pragma unroll
+      for (int k = 0; k < 3; ++k) o.p[k] = __builtin_bit_cast(bf16x8, w[k]);
+      TL::put(tile, tid / TL::NCH + n * STEP, tid % TL::NCH, o);
+    }
   }
 };
 
