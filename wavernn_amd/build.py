@@ -15,14 +15,20 @@ LIB_DIR = os.path.join(HERE, "lib")
 OBJ_DIR = os.path.join(LIB_DIR, "obj")
 LIB_PATH = os.path.join(LIB_DIR, "libwrnn_mi355.so")
 SOURCES = ["taco_decoder.hip", "length_regulator.hip", "bilstm.hip", "bigru.hip", "durations.hip", "wavernn.hip",
-           "aligner.hip", "mol.hip", "relative_bias.hip", "attention.hip", "attention_forward_bf16.hip",
-           "attention_forward_f32.hip", "attention_backward_bf16.hip", "attention_backward_f32.hip"]
+           "aligner.hip", "mol.hip", "relative_bias.hip", "attention.hip"] + [
+               f"attention_{d}_{t}.hip" for d in ("forward", "backward") for t in ("bf16", "bf16_d256", "f32", "f32_d256")]
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function"]
 # The attention kernels are built without packed fp32 instructions: some of their forms have given wrong results on this
 # hardware, with no error.  (The host pass does not know the feature and says so; harmless.)  The older kernels keep the code they were
 # verified with: the teacher-forced loop loses 5.5 % without them (13.7 -> 14.5 us per decoder step at B=64).
 NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-SOURCE_FLAGS = {s: NO_PACKED_FP32 for s in SOURCES if s.startswith(("attention", "relative_bias"))}
+# MFMA_IN_VGPRS: sums stay in the vector registers that the softmax works on; by default every value that passes between
+# matrix and vector instructions is copied (forward, float32, 128 columns: 64 copies a tile, 376 -> 330 us at 2 x 16 x 2048).  The compiler crashes
+# on the forward kernels of float32 with 256 columns that way; those do without.
+MFMA_IN_VGPRS = ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
+SOURCE_FLAGS = {s: NO_PACKED_FP32 + (MFMA_IN_VGPRS if s in ("attention_forward_bf16_d256.hip", "attention_forward_f32.hip",
+                                                            "attention_backward_bf16_d256.hip", "attention_backward_f32.hip") else [])
+                for s in SOURCES if s.startswith(("attention", "relative_bias"))}
 
 
 def _hipcc() -> str:

@@ -1,13 +1,22 @@
-// Entry points of the self-attention (kernels: attention_forward.h, attention_backward.h; one source per type for the build's sake).
+// Entry points of the self-attention (kernels: attention_forward.h, attention_backward.h; several sources for the build's sake).
 #include "attention_tile.h"
 
 namespace wrnn {
 namespace attn {
 
-template <class T>
+template <class T, int DP>
 int forward(const Params& p, hipStream_t st);
-template <class T>
+template <class T, int DP>
 int backward(const Params& p, float* dtable, hipStream_t st);
+
+template <class T>
+static int forward(const Params& p, hipStream_t st) {
+  return p.D <= 64 ? forward<T, 64>(p, st) : p.D <= 128 ? forward<T, 128>(p, st) : forward<T, 256>(p, st);
+}
+template <class T>
+static int backward(const Params& p, float* dtable, hipStream_t st) {
+  return p.D <= 64 ? backward<T, 64>(p, dtable, st) : p.D <= 128 ? backward<T, 128>(p, dtable, st) : backward<T, 256>(p, dtable, st);
+}
 
 constexpr int kComputeUnits = 256;
 

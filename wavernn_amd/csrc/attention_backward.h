@@ -168,17 +168,9 @@ __global__ __launch_bounds__((BackwardShape<T, DP, WIDE>::THREADS), (BackwardSha
   Stage<T, DP, BN, NT> sk, sv;
   sk.start(kb, p.k_t, end, p.D, tid);
   sv.start(vb, p.v_t, end, p.D, tid);
-  KeyBits<BN> keys(mask, end, lane);
-  auto load = [&](int t) {
-    sk.load(t * BN);
-    sv.load(t * BN);
-    keys.load(t * BN);
-  };
-  auto drop = [&](const RowBits& use) {
-    if (mask && !use.template all<BN>()) {
-      sk.drop(use, tid);
-      sv.drop(use, tid);
-    }
+  auto load = [&](int t, const RowBits& use) {
+    sk.load(t * BN, mask ? &use : nullptr, tid);
+    sv.load(t * BN, mask ? &use : nullptr, tid);
   };
   auto store = [&](int t) {
     const int o = t & (BUFS - 1);
@@ -188,21 +180,16 @@ __global__ __launch_bounds__((BackwardShape<T, DP, WIDE>::THREADS), (BackwardSha
 #pragma unroll
   for (int walk = TWICE ? 0 : 1; walk < 2; ++walk) {
     // the order of a round: as in the forward pass
-    RowBits use, next;
-    load(0);
-    use = keys.get(0);
-    drop(use);
+    KeyBits<BN> keys(mask, end, lane, 0);
+    RowBits use = keys.next(0), use1 = keys.next(BN), use2;  // of tiles t, t + 1, t + 2
+    load(0, use);
     store(0);
-    if (S::EARLY) load(1);
+    if (S::EARLY) load(1, use1);
     __syncthreads();
     for (int t = 0; t < tiles; ++t) {
       const char *kk = kt + (t & (BUFS - 1)) * TL::BYTES, *vv = vt + (t & (BUFS - 1)) * TL::BYTES;
-      if (S::EARLY) {
-        next = keys.get((t + 1) * BN);
-        drop(next);
-      } else if (S::AHEAD) {
-        load(t + 1);
-      }
+      use2 = keys.next((t + 2) * BN);
+      if (!S::EARLY && S::AHEAD) load(t + 1, use1);
 #pragma unroll
       for (int x = 0; x < S::NS; ++x) {
         const int sub = S::NS * wm + x, key0 = t * BN + sub * 32;
@@ -210,14 +197,13 @@ __global__ __launch_bounds__((BackwardShape<T, DP, WIDE>::THREADS), (BackwardSha
         f32x16 raw = {}, dp = {};
         if (work) {
 #pragma unroll
-          for (int c = 0; c < NC2; ++c) {
-            raw = mma(TL::row_chunk(kk, sub * 32 + col, 2 * c + half), q.get(c), raw);
-            dp = mma(TL::row_chunk(vv, sub * 32 + col, 2 * c + half), go.get(c), dp);
-          }
+          for (int c = 0; c < NC2; ++c)
+            mma2(TL::row_chunk(kk, sub * 32 + col, 2 * c + half), q.get(c), raw, TL::row_chunk(vv, sub * 32 + col, 2 * c + half), go.get(c), dp,
+                 [](int) {});
         }
         if (x == 0 && S::EARLY) {
           store(t + 1);
-          load(t + 2);
+          load(t + 2, use2);
         }
         if (work) {
           float pr[16];
@@ -240,12 +226,11 @@ __global__ __launch_bounds__((BackwardShape<T, DP, WIDE>::THREADS), (BackwardSha
       }
       if (!S::EARLY) {
         if (BUFS == 1) __syncthreads();
-        if (!S::AHEAD) load(t + 1);
-        next = keys.get((t + 1) * BN);
-        drop(next);
+        if (!S::AHEAD) load(t + 1, use1);
         store(t + 1);
       }
-      use = next;
+      use = use1;
+      use1 = use2;
       __syncthreads();
     }
     if (TWICE && walk == 0) {
@@ -328,8 +313,8 @@ __global__ __launch_bounds__((BackwardShape<T, DP, WIDE>::THREADS), (BackwardSha
     const int h = kvh * p.group + it / per, r0 = (qt_0 + it % per) * BM;
     sq.base = reinterpret_cast<const char*>(reinterpret_cast<const T*>(p.q) + b * p.q_b + h * p.q_h);
     sg.base = reinterpret_cast<const char*>(reinterpret_cast<const T*>(p.dout) + b * p.do_b + h * p.do_h);
-    sq.load(r0);
-    sg.load(r0);
+    sq.load(r0, nullptr, tid);
+    sg.load(r0, nullptr, tid);
     if (tid < BM) {
       const int64_t row = ((int64_t)b * p.H + h) * p.Tq + r0 + tid;
       const float l = r0 + tid < p.Tq ? p.lse[row] : -INFINITY;
@@ -367,10 +352,9 @@ __global__ __launch_bounds__((BackwardShape<T, DP, WIDE>::THREADS), (BackwardSha
       f32x16 raw = {}, dp = {};
       if (work) {
 #pragma unroll
-        for (int c = 0; c < NC2; ++c) {
-          raw = mma(TL::row_chunk(qq, sub * 32 + col, 2 * c + half), k.get(c), raw);
-          dp = mma(TL::row_chunk(gg, sub * 32 + col, 2 * c + half), v.get(c), dp);
-        }
+        for (int c = 0; c < NC2; ++c)
+          mma2(TL::row_chunk(qq, sub * 32 + col, 2 * c + half), k.get(c), raw, TL::row_chunk(gg, sub * 32 + col, 2 * c + half), v.get(c), dp,
+               [](int) {});
       }
       if (x == 0 && S::EARLY) {
         store(it + 1);
@@ -460,13 +444,8 @@ static int launch_backward(const Params& p, float* dtable, hipStream_t st) {
 }
 
 template <class T, int DP>
-static int launch_bias(const Params& p, float* dtable, hipStream_t st) {
-  return !p.table ? launch_backward<T, DP, 0>(p, dtable, st) : dtable ? launch_backward<T, DP, 2>(p, dtable, st) : launch_backward<T, DP, 1>(p, dtable, st);
-}
-
-template <class T>
 int backward(const Params& p, float* dtable, hipStream_t st) {
-  return p.D <= 64 ? launch_bias<T, 64>(p, dtable, st) : p.D <= 128 ? launch_bias<T, 128>(p, dtable, st) : launch_bias<T, 256>(p, dtable, st);
+  return !p.table ? launch_backward<T, DP, 0>(p, dtable, st) : dtable ? launch_backward<T, DP, 2>(p, dtable, st) : launch_backward<T, DP, 1>(p, dtable, st);
 }
 
 }  // namespace attn

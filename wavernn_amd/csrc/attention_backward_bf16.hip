@@ -1,3 +1,8 @@
 #include "attention_backward.h"
 
-template int wrnn::attn::backward<__bf16>(const Params&, float*, hipStream_t);
+namespace wrnn {
+namespace attn {
+template int backward<__bf16, 64>(const Params&, float*, hipStream_t);
+template int backward<__bf16, 128>(const Params&, float*, hipStream_t);
+}  // namespace attn
+}  // namespace wrnn

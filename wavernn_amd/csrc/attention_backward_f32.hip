@@ -1,3 +1,8 @@
 #include "attention_backward.h"
 
-template int wrnn::attn::backward<float>(const Params&, float*, hipStream_t);
+namespace wrnn {
+namespace attn {
+template int backward<float, 64>(const Params&, float*, hipStream_t);
+template int backward<float, 128>(const Params&, float*, hipStream_t);
+}  // namespace attn
+}  // namespace wrnn

@@ -20,7 +20,7 @@ struct Running {
 #pragma unroll
       for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[n][i]);
     mx = both_max(mx);
-    if (__any(mx > m + 8.f)) {
+    if (__builtin_expect(__any(mx > m + 8.f), 0)) {
       const float mn = fmaxf(m, mx), a = exp2f(m - mn);
       m = mn;
       l *= a;
@@ -106,17 +106,10 @@ __global__ __launch_bounds__((ForwardShape<T, DP, WIDE>::THREADS), (ForwardShape
   Stage<T, DP, BN, NT> sk, sv;
   sk.start(kb, p.k_t, end, p.D, tid);
   sv.start(vb, p.v_t, end, p.D, tid);
-  KeyBits<BN> keys(mask, end, lane);
-  auto load = [&](int t) {
-    sk.load(t * BN);
-    sv.load(t * BN);
-    keys.load(t * BN);
-  };
-  auto drop = [&](const RowBits& use) {
-    if (mask && !use.template all<BN>()) {
-      sk.drop(use, tid);
-      sv.drop(use, tid);
-    }
+  KeyBits<BN> keys(mask, end, lane, t0 * BN);
+  auto load = [&](int t, const RowBits& use) {
+    sk.load(t * BN, mask ? &use : nullptr, tid);
+    sv.load(t * BN, mask ? &use : nullptr, tid);
   };
   auto store = [&](int t) {
     const int o = t & (BUFS - 1);
@@ -126,23 +119,18 @@ __global__ __launch_bounds__((ForwardShape<T, DP, WIDE>::THREADS), (ForwardShape
   // float32 (EARLY): tile t is worked on while tile t + 1 goes from registers to LDS (its conversion fills the matrix instructions' shadow)
   // and tile t + 2 is requested.  Otherwise tile t + 1 is requested before tile t's arithmetic and goes to LDS after it; with one buffer
   // that waits for everybody to be done with tile t.
-  RowBits use, next;
-  load(t0);
-  use = keys.get(t0 * BN);
-  drop(use);
+  RowBits use = keys.next(t0 * BN), use1 = keys.next((t0 + 1) * BN), use2;  // of tiles t, t + 1, t + 2
+  load(t0, use);
   store(t0);
-  if (S::EARLY) load(t0 + 1);
+  if (S::EARLY) load(t0 + 1, use1);
   __syncthreads();
   for (int t = t0; t < t1; ++t) {
     const char *kk = kt + (t & (BUFS - 1)) * TL::BYTES, *vv = vt + (t & (BUFS - 1)) * TL::BYTES;
     const int sub0 = NS * wk, key0 = t * BN + 32 * sub0;
-    if (S::EARLY) {
-      next = keys.get((t + 1) * BN);
-      drop(next);
-    } else {
-      load(t + 1);
-    }
-    if (key0 < end && !(p.causal && key0 > pos_hi)) {
+    use2 = keys.next((t + 2) * BN);
+    if (!S::EARLY) load(t + 1, use1);
+    // (EARLY goes without the way round a tile past the wave's reach: joining its two ways costs a copy of every sum in every round)
+    if (S::EARLY || (key0 < end && !(p.causal && key0 > pos_hi))) {
       f32x16 raw[NS] = {};
       if constexpr (S::EARLY) {
         char *kn = kt + ((t + 1) & (BUFS - 1)) * TL::BYTES, *vn = vt + ((t + 1) & (BUFS - 1)) * TL::BYTES;
@@ -153,15 +141,18 @@ __global__ __launch_bounds__((ForwardShape<T, DP, WIDE>::THREADS), (ForwardShape
           else sv.store_piece(vn, tid, i - PIECES, w);
         };
         const Shadow<decltype(piece)> shadow(6 * NC2, 2 * PIECES, piece);
-        Operand<T> a = TL::row_chunk(kk, col, half);
+        auto chunk = [&](int c) { return TL::row_chunk(kk, col, 2 * c + half); };
+        f32x16 odd = {};
+        Operand<T> a0 = chunk(0), a1 = chunk(1);
 #pragma unroll
-        for (int c = 0; c < NC2; ++c) {
-          Operand<T> next = a;
-          if (c + 1 < NC2) next = TL::row_chunk(kk, col, 2 * c + 2 + half);
-          raw[0] = mma(a, q.get(c), raw[0], [&](int m) { shadow(6 * c + m); });
-          a = next;
+        for (int c = 0; c < NC2; c += 2) {
+          Operand<T> n0 = a0, n1 = a1;
+          if (c + 2 < NC2) n0 = chunk(c + 2), n1 = chunk(c + 3);
+          mma2(a0, q.get(c), raw[0], a1, q.get(c + 1), odd, [&](int m) { shadow(6 * c + m); });
+          a0 = n0, a1 = n1;
         }
-        load(t + 2);
+        raw[0] += odd;
+        load(t + 2, use2);
       } else {
 #pragma unroll
         for (int c = 0; c < NC2; ++c)
@@ -186,17 +177,13 @@ __global__ __launch_bounds__((ForwardShape<T, DP, WIDE>::THREADS), (ForwardShape
           column_product<T, TL>(vv, (sub0 + x) * 32, 0, Weights<T>(s[x]), acc, lane);
         }
       }
-    } else if (S::EARLY) {
-      store(t + 1);
-      load(t + 2);
     }
     if (!S::EARLY) {
       if (BUFS == 1) __syncthreads();
-      next = keys.get((t + 1) * BN);
-      drop(next);
       store(t + 1);
     }
-    use = next;
+    use = use1;
+    use1 = use2;
     __syncthreads();
   }
   const float l = both_sum(run.l);
@@ -326,13 +313,8 @@ static int launch_forward(const Params& p, hipStream_t st) {
 }
 
 template <class T, int DP>
-static int launch_bias(const Params& p, hipStream_t st) {
-  return p.table ? launch_forward<T, DP, true>(p, st) : launch_forward<T, DP, false>(p, st);
-}
-
-template <class T>
 int forward(const Params& p, hipStream_t st) {
-  return p.D <= 64 ? launch_bias<T, 64>(p, st) : p.D <= 128 ? launch_bias<T, 128>(p, st) : launch_bias<T, 256>(p, st);
+  return p.table ? launch_forward<T, DP, true>(p, st) : launch_forward<T, DP, false>(p, st);
 }
 
 }  // namespace attn

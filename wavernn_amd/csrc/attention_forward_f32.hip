@@ -1,3 +1,8 @@
 #include "attention_forward.h"
 
-template int wrnn::attn::forward<float>(const Params&, hipStream_t);
+namespace wrnn {
+namespace attn {
+template int forward<float, 64>(const Params&, hipStream_t);
+template int forward<float, 128>(const Params&, hipStream_t);
+}  // namespace attn
+}  // namespace wrnn

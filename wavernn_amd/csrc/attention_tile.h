@@ -142,6 +142,29 @@ __device__ __forceinline__ f32x16 mma(const Operand<T>& a, const Operand<T>& b, 
   return mma(a, b, c, [](int) {});
 }
 
+// Two products, instruction by instruction in turn: a product that adds to the one right before it waits for the whole of that one's
+// latency, twice the time the unit is busy (float32 forward, one wave a SIMD: PAIRGAIN).
+template <class F>
+__device__ __forceinline__ void mma2(const Operand<__bf16>& a0, const Operand<__bf16>& b0, f32x16& c0, const Operand<__bf16>& a1,
+                                     const Operand<__bf16>& b1, f32x16& c1, F&& between) {
+  c0 = mma1(a0.p[0], b0.p[0], c0);
+  between(0);
+  c1 = mma1(a1.p[0], b1.p[0], c1);
+  between(1);
+}
+template <class F>
+__device__ __forceinline__ void mma2(const Operand<float>& a0, const Operand<float>& b0, f32x16& c0, const Operand<float>& a1,
+                                     const Operand<float>& b1, f32x16& c1, F&& between) {
+  constexpr int pa[6] = {2, 0, 1, 1, 0, 0}, pb[6] = {0, 2, 1, 0, 1, 0};
+#pragma unroll
+  for (int m = 0; m < 6; ++m) {
+    c0 = mma1(a0.p[pa[m]], b0.p[pb[m]], c0);
+    between(2 * m);
+    c1 = mma1(a1.p[pa[m]], b1.p[pb[m]], c1);
+    between(2 * m + 1);
+  }
+}
+
 // Work in the matrix instructions' shadow: a 32 x 32 x 16 product keeps the matrix unit for 32 cycles, a vector instruction its unit for 4, and a
 // wave issues in order, so a wave that is alone on its SIMD has to have vector instructions BETWEEN its products.  The compiler's
 // scheduler moves them behind; Shadow(products, pieces, f) deals f(0) .. f(pieces - 1) out over the products and fences each step.
@@ -283,9 +306,11 @@ __device__ __forceinline__ Operand<T> column_chunk(const char* tile, int r0, int
 template <class T, class TL, int DT>
 __device__ __forceinline__ void column_product(const char* tile, int r0, int d0, const Weights<T>& w, f32x16 (&acc)[DT], int lane) {
 #pragma unroll
-  for (int dt = 0; dt < DT; ++dt)
+  for (int s = 0; s < 2; ++s)
 #pragma unroll
-    for (int s = 0; s < 2; ++s) acc[dt] = mma(column_chunk<T, TL>(tile, r0 + 16 * s, d0 + 32 * dt, lane), w.o[s], acc[dt]);
+    for (int dt = 0; dt < DT; dt += 2)
+      mma2(column_chunk<T, TL>(tile, r0 + 16 * s, d0 + 32 * dt, lane), w.o[s], acc[dt],
+           column_chunk<T, TL>(tile, r0 + 16 * s, d0 + 32 * dt + 32, lane), w.o[s], acc[dt + 1], [](int) {});
 }
 
 // The same for float32 from weights not made yet: value(i) gives weight i of the lane.  The first 16 moving rows' weights are made
@@ -305,23 +330,23 @@ __device__ __forceinline__ void column_product_shadow(const char* tile, int r0, 
     for (int k = 0; k < 3; ++k) o.p[k] = __builtin_bit_cast(bf16x8, w[s][k]);
     return o;
   };
-  Operand<float> a = column_chunk<float, TL>(tile, r0, d0, lane);
+  auto chunk = [&](int n) { return column_chunk<float, TL>(tile, r0 + 16 * (n / DT), d0 + 32 * (n % DT), lane); };
+  Operand<float> a0 = chunk(0), a1 = chunk(1);
 #pragma unroll
   for (int i = 0; i < 4; ++i) make(i);
   Operand<float> b = get(0);
   const auto later = [&](int i) { make(4 + i); };
   const Shadow<decltype(later)> shadow(6 * DT, 4, later);
 #pragma unroll
-  for (int n = 0; n < 2 * DT; ++n) {
-    const int s = n / DT, dt = n % DT, ns = (n + 1) / DT, nd = (n + 1) % DT;
+  for (int n = 0; n < 2 * DT; n += 2) {
     if (n == DT) b = get(1);
-    Operand<float> next = a;
-    if (n + 1 < 2 * DT) next = column_chunk<float, TL>(tile, r0 + 16 * ns, d0 + 32 * nd, lane);
-    acc[dt] = mma(a, b, acc[dt], [&](int m) {
-      if (s == 0) shadow(6 * dt + m);
+    Operand<float> n0 = a0, n1 = a1;
+    if (n + 2 < 2 * DT) n0 = chunk(n + 2), n1 = chunk(n + 3);
+    mma2(a0, b, acc[n % DT], a1, b, acc[n % DT + 1], [&](int m) {
+      if (n < DT) shadow(6 * n + m);
       else __builtin_amdgcn_sched_barrier(0);
     });
-    a = next;
+    a0 = n0, a1 = n1;
   }
 }
 
@@ -343,30 +368,32 @@ struct RowBits {
   }
 };
 
-// The keys of a tile that lengths, reach (end) and mask leave: lane l looks at keys l and l + 64.
+// The keys of a tile that lengths, reach (end) and mask leave: lane l looks at keys l and l + 64.  The mask's bytes of the tile after are
+// requested with each answer.
 template <int ROWS>
 struct KeyBits {
   const uint8_t* mask;
   int end, lane;
   uint32_t out_lo = 0, out_hi = 0;
-  __device__ __forceinline__ KeyBits(const uint8_t* mask_, int end_, int lane_) : mask(mask_), end(end_), lane(lane_) {}
-  __device__ __forceinline__ void load(int key0) {
+  __device__ __forceinline__ KeyBits(const uint8_t* mask_, int end_, int lane_, int first) : mask(mask_), end(end_), lane(lane_) { request(first); }
+  __device__ __forceinline__ void request(int key0) {
     if (!mask || end <= 0) return;  // no key at all: nothing to look at (and mask[end - 1] would lie before it)
     out_lo = mask[min(key0 + lane, end - 1)];
     if (ROWS > 64) out_hi = mask[min(key0 + 64 + lane, end - 1)];
   }
-  __device__ __forceinline__ RowBits get(int key0) const {
+  __device__ __forceinline__ RowBits next(int key0) {
     RowBits r;
     r.lo = __ballot(key0 + lane < end && out_lo == 0);
     if (ROWS > 64) r.hi = __ballot(key0 + 64 + lane < end && out_hi == 0);
+    request(key0 + ROWS);
     return r;
   }
 };
 
 // Rows of a tensor's [.., T, D] slice on their way to an LDS tile: requested a round before they are written to LDS.  Buffer loads check
-// every lane against the tile's last byte: rows at or past `limit`, and the chunks past D, come back as zero without a branch.
-// Rows inside that a mask leaves out are zeroed too (drop): what lies at keys that are left out (another sequence's values, infinities, NaN) must
-// not reach a product, where 0 * NaN would.
+// every lane against the tile's last byte: rows at or past `limit`, the chunks past D and, by an offset beyond it, rows that a mask leaves out
+// come back as zero without a branch.  What lies at keys that are left out (another sequence's values, infinities, NaN) must not reach a
+// product, where 0 * NaN would.
 template <class T, int DP, int ROWS, int NT>
 struct Stage {
   using TL = Tile<T, DP, ROWS>;
@@ -387,23 +414,28 @@ struct Stage {
 #pragma unroll
     for (int i = 0; i < PER; ++i) off[i] = ch * 8 * ES + 16 * i < last ? (uint32_t)(mine * (int)row_bytes + ch * 8 * ES + 16 * i) : kOutside;
   }
-  __device__ __forceinline__ void load(int row0) {
+  // use: the rows that a mask leaves, or null
+  __device__ __forceinline__ void load(int row0, const RowBits* use, int tid) {
     const int rows = min(limit - row0, ROWS);
     const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base + (int64_t)row0 * row_bytes), 0,
                                                         rows > 0 ? (rows - 1) * (int)row_bytes + last : 0, 0x00020000);
+    if (use && !use->template all<ROWS>()) {
+      get(rsrc, [&](int n) { return use->at(tid / TL::NCH + n * STEP) ? 0u : kOutside; });
+    } else {
+      get(rsrc, [](int) { return 0u; });
+    }
+  }
+  template <class R, class F>
+  __device__ __forceinline__ void get(R rsrc, F&& out) {
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       u32x4 x[PER];
 #pragma unroll
-      for (int i = 0; i < PER; ++i) x[i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, off[i] + (uint32_t)(n * STEP * (int)row_bytes), 0, 0);
+      for (int i = 0; i < PER; ++i)
+        x[i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, (off[i] + (uint32_t)(n * STEP * (int)row_bytes)) | out(n), 0, 0);
       if constexpr (PER == 1) r[n].x = __builtin_bit_cast(typename Raw<T>::vec, x[0]);
       else r[n].x = __builtin_shufflevector(__builtin_bit_cast(f32x4, x[0]), __builtin_bit_cast(f32x4, x[1]), 0, 1, 2, 3, 4, 5, 6, 7);
     }
-  }
-  __device__ __forceinline__ void drop(const RowBits& bits, int tid) {
-#pragma unroll
-    for (int n = 0; n < N; ++n)
-      if (!bits.at(tid / TL::NCH + n * STEP)) r[n].x = {};
   }
   __device__ __forceinline__ void store(char* tile, int tid) {
 #pragma unroll
