@@ -23,31 +23,43 @@ constexpr int kComputeUnits = 256;
 static int padded_dim(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 static int lut_floats(const Params& p) { return p.table ? 2 * p.max_distance + 1 : 0; }
 
-// How a call runs.  The 128-query kernel shares each key tile among four waves and is the faster one as soon as its workgroups
-// fill the compute units; below that the split kernel has four times the workgroups and can divide the keys too.
-static void plan(Params* p) {
-  const int64_t wide = (int64_t)p->B * p->H * ((p->Tq + 127) / 128);
-  p->splits = 0;
-  p->pack = 0;
-  if (wide >= kComputeUnits && p->Tq > 32) return;
-  p->pack = (int64_t)p->group * p->Tq <= 32 && (size_t)p->group * lut_floats(*p) * 4 <= 16 * 1024;
-  const int64_t base = p->pack ? (int64_t)p->B * p->Hkv : (int64_t)p->B * p->H * ((p->Tq + 31) / 32);
-  const int64_t rounds = (p->Tk + 127) / 128;  // a wave's tiles if the keys are not split
-  int64_t s = (2 * kComputeUnits + base - 1) / base;
-  if (s > (rounds + 1) / 2) s = (rounds + 1) / 2;
-  p->splits = (int)(s < 1 ? 1 : s > 256 ? 256 : s);
+// Workgroups that share one block of stationary rows, each with part of the `tiles` of the other side: as many as fill the compute units,
+// none with fewer than `least` tiles.
+static int shares(int64_t blocks, int64_t tiles, int least) {
+  const int64_t want = kComputeUnits / (blocks > 0 ? blocks : 1), most = tiles / least;
+  const int64_t n = want < most ? want : most;
+  return (int)(n < 1 ? 1 : n > 256 ? 256 : n);
 }
 
+// How a call runs.  The wide shape shares each key tile among four waves; the narrow one is for few queries, which would leave three of
+// them idle.
+static void plan(Params* p) {
+  p->pack = p->group > 1 && (int64_t)p->group * p->Tq <= 32 && (size_t)p->group * lut_floats(*p) * 4 <= 16 * 1024;
+  p->narrow = p->pack || p->Tq <= 32;
+  if (p->narrow) {
+    const int64_t blocks = p->pack ? (int64_t)p->B * p->Hkv : (int64_t)p->B * p->H;
+    p->splits = shares((blocks + 1) / 2, (p->Tk + 127) / 128, 2);
+  } else {
+    p->splits = shares((int64_t)p->B * p->H * ((p->Tq + 127) / 128), (p->Tk + 31) / 32, 4);
+  }
+}
 static size_t split_workspace(const Params& p) {
   return p.splits > 1 ? (size_t)p.B * p.H * p.Tq * p.splits * (padded_dim(p.D) + 4) * sizeof(float) : 0;
 }
 
-// The backward pass likewise: 128 stationary rows per workgroup, or 32.
 static void plan_backward(Params* p) {
-  p->wide_dq = (int64_t)p->B * p->H * ((p->Tq + 127) / 128) >= kComputeUnits;
-  p->wide_dkv = (int64_t)p->B * p->Hkv * ((p->Tk + 127) / 128) >= kComputeUnits;
+  const int parts = p->D > 128 ? 2 : 1;
+  p->dq_splits = shares((int64_t)p->B * p->H * ((p->Tq + 127) / 128) * parts, (p->Tk + 31) / 32, 4);
+  p->dkv_splits = shares((int64_t)p->B * p->Hkv * ((p->Tk + 127) / 128) * parts, (int64_t)((p->Tq + 31) / 32) * p->group, 4);
 }
-static size_t delta_bytes(const Params& p) { return ((size_t)p.B * p.H * p.Tq * sizeof(float) + 255) & ~size_t(255); }
+static size_t aligned(size_t x) { return (x + 255) & ~size_t(255); }
+// the backward workspace: delta, the table's partial sums, the shares
+static size_t delta_bytes(const Params& p) { return aligned((size_t)p.B * p.H * p.Tq * sizeof(float)); }
+static size_t table_bytes(const Params& p) {
+  return p.table ? aligned((size_t)p.B * ((p.Tq + 127) / 128) * p.dq_splits * p.H * p.buckets * sizeof(float)) : 0;
+}
+static size_t dq_bytes(const Params& p) { return p.dq_splits > 1 ? aligned((size_t)p.dq_splits * p.B * p.H * p.Tq * p.D * sizeof(float)) : 0; }
+static size_t dkv_bytes(const Params& p) { return p.dkv_splits > 1 ? (size_t)p.dkv_splits * 2 * p.B * p.Hkv * p.Tk * p.D * sizeof(float) : 0; }
 
 }  // namespace attn
 
@@ -122,7 +134,7 @@ extern "C" size_t wrnn_attention_backward_workspace_bytes(const wrnn_attention_d
   attn::Params p;
   if (attention_params(desc, &p, "wrnn_attention_backward_workspace_bytes") || !p.B || !p.H || !p.Tq) return 0;
   attn::plan_backward(&p);
-  return attn::delta_bytes(p) + (p.table ? (size_t)p.B * attn::dq_tiles(p) * p.H * p.buckets * sizeof(float) : 0);
+  return attn::delta_bytes(p) + attn::table_bytes(p) + attn::dq_bytes(p) + attn::dkv_bytes(p);
 }
 
 extern "C" int wrnn_attention_backward(const wrnn_attention_desc* desc, const wrnn_attention_grads* g, void* workspace, size_t workspace_bytes,
@@ -151,8 +163,11 @@ extern "C" int wrnn_attention_backward(const wrnn_attention_desc* desc, const wr
   p.dv = g->dv, p.dv_b = g->dv_stride[0], p.dv_h = g->dv_stride[1], p.dv_t = g->dv_stride[2];
   attn::plan_backward(&p);
   p.lse = const_cast<float*>(g->lse);
-  p.delta = static_cast<float*>(workspace);
-  p.dtable_part = reinterpret_cast<float*>(static_cast<char*>(workspace) + attn::delta_bytes(p));
+  char* w = static_cast<char*>(workspace);
+  p.delta = reinterpret_cast<float*>(w);
+  p.dtable_part = reinterpret_cast<float*>(w += attn::delta_bytes(p));
+  p.dq_part = reinterpret_cast<float*>(w += attn::table_bytes(p));
+  p.dkv_part = reinterpret_cast<float*>(w + attn::dq_bytes(p));
   const hipStream_t st = static_cast<hipStream_t>(stream);
   return desc->dtype == WRNN_FLOAT32 ? attn::backward<float>(p, g->dtable, st) : attn::backward<__bf16>(p, g->dtable, st);
 }

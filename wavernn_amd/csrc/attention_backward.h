@@ -49,60 +49,53 @@ struct BiasGrad {
   }
 };
 
-// Shapes of a workgroup, as in the forward pass: wide = 4 waves of 32 stationary rows each against every subtile of a tile; narrow = 32
-// stationary rows, the waves on different subtiles, joined at the end.
-template <class T, int DP, bool WIDE>
+// A workgroup: 4 waves of 32 stationary rows each against every subtile of a tile.
+template <class T, int DP>
 struct BackwardShape {
   static constexpr int NP = Type<T>::NP;
-  static constexpr int WS = WIDE ? 4 : 1, WM = WIDE ? 1 : NP == 1 ? (DP == 256 ? 2 : 4) : DP == 64 ? 4 : DP == 128 ? 2 : 1;
-  static constexpr int NS = WIDE && NP == 1 && DP < 256 ? 2 : 1;  // subtiles of a tile per wave
-  static constexpr int WAVES = WS * WM, THREADS = 64 * WAVES, BM = 32 * WM * NS;
-  static constexpr int BUFS = WIDE && !(NP == 3 && DP == 256) ? 2 : 1;  // two where they leave room for the position bias's tables
-  static constexpr bool AHEAD = WIDE || DP * NP <= 256;                 // the next tile is requested before this one's arithmetic
-  static constexpr bool EARLY = NP == 3 && BUFS == 2;                   // it goes to LDS beside the arithmetic (forward pass)
+  static constexpr int THREADS = 256, NS = NP == 1 && DP < 256 ? 2 : 1, BM = 32 * NS;
+  static constexpr int BUFS = NP == 3 && DP == 256 ? 1 : 2;  // two where they leave room for the position bias's tables
+  static constexpr bool EARLY = NP == 3 && BUFS == 2;        // the next tile goes to LDS beside the arithmetic (forward pass)
   static constexpr bool RAW = NP == 3 && DP == 256;
   // output columns of a workgroup: both sums and both stationary operands have to fit the registers
   static constexpr int DA = DP > 128 ? 128 : DP, PARTS = DP / DA, DT = DA / 32;
   using TL = Tile<T, DP, BM>;
-  static constexpr size_t TILES = 2 * BUFS * TL::BYTES, SUMS = WM > 1 ? (size_t)WM * 32 * (DA + 4) * 4 : 0;
-  static constexpr size_t BODY = TILES > SUMS ? TILES : SUMS;
-  static constexpr int DQ_WAVES = DP * NP <= 64 ? 2 : 1, DKV_WAVES = DP * NP <= 64 ? 2 : 1;  // per SIMD
+  static constexpr size_t TILES = 2 * BUFS * TL::BYTES;
+  static constexpr int WAVES = DP * NP <= 64 ? 2 : 1;  // per SIMD
 };
 
-// Sum over the waves of the narrow shape, through LDS in the tiles' place, and out: row of column c = base + c * stride.
+// A lane's sums to its row: of the gradient, or (part) of the workgroup's share in 32 bits, which attention_share_kernel adds up.
 template <class S, class T>
-__device__ __forceinline__ void join_and_store(const f32x16 (&acc)[S::DT], float* sums, T* base, int64_t stride, int rows, int d0, int D,
-                                               float scale, int wave, int lane, int tid) {
-  constexpr int LD = S::DA + 4, TPC = S::THREADS / 32;
-  const int half = lane >> 5, col = lane & 31;
-  __syncthreads();
+__device__ __forceinline__ void store_rows(const f32x16 (&acc)[S::DT], T* row, float* part, int d0, int D, float scale, int half) {
 #pragma unroll
   for (int dt = 0; dt < S::DT; ++dt)
 #pragma unroll
-    for (int g = 0; g < 4; ++g)
-      *reinterpret_cast<f32x4*>(sums + (wave * 32 + col) * LD + dt * 32 + 8 * g + 4 * half) =
-          f32x4{acc[dt][4 * g], acc[dt][4 * g + 1], acc[dt][4 * g + 2], acc[dt][4 * g + 3]};
-  __syncthreads();
-  const int c = tid / TPC;
-  if (c < rows) {
-    T* row = base + c * stride;
-#pragma unroll
-    for (int d = (tid % TPC) * 4; d < S::DA; d += TPC * 4) {
-      f32x4 x = *reinterpret_cast<const f32x4*>(sums + c * LD + d);
-#pragma unroll
-      for (int w = 1; w < S::WM; ++w) x += *reinterpret_cast<const f32x4*>(sums + (w * 32 + c) * LD + d);
-      store4<T>(row, d0 + d, D, x[0] * scale, x[1] * scale, x[2] * scale, x[3] * scale);
+    for (int g = 0; g < 4; ++g) {
+      const int d = d0 + dt * 32 + 8 * g + 4 * half;
+      const float x[4] = {acc[dt][4 * g] * scale, acc[dt][4 * g + 1] * scale, acc[dt][4 * g + 2] * scale, acc[dt][4 * g + 3] * scale};
+      if (part) store4<float>(part, d, D, x[0], x[1], x[2], x[3]);
+      else store4<T>(row, d, D, x[0], x[1], x[2], x[3]);
     }
-  }
 }
-template <class S, class T>
-__device__ __forceinline__ void store_rows(const f32x16 (&acc)[S::DT], T* row, int d0, int D, float scale, int half) {
+
+// The two products of a float32 round (scores, and dP), with the next tiles' conversion in their shadow.
+template <class TL, int NC2, class ST, class STAGE>
+__device__ __forceinline__ void products_shadow(const char* x, const char* y, const ST& u, const ST& v, f32x16& raw, f32x16& dp, STAGE& sx, STAGE& sy,
+                                                char* xn, char* yn, int col, int half, int tid) {
+  Splitter sp;
+  constexpr int PIECES = STAGE::PIECES;
+  const auto piece = [&](int i) {
+    if (i < PIECES) sx.store_piece(xn, tid, i, sp);
+    else sy.store_piece(yn, tid, i - PIECES, sp);
+  };
+  Operand<float> a0 = TL::row_chunk(x, col, half), a1 = TL::row_chunk(y, col, half);
 #pragma unroll
-  for (int dt = 0; dt < S::DT; ++dt)
-#pragma unroll
-    for (int g = 0; g < 4; ++g)
-      store4<T>(row, d0 + dt * 32 + 8 * g + 4 * half, D, acc[dt][4 * g] * scale, acc[dt][4 * g + 1] * scale, acc[dt][4 * g + 2] * scale,
-                acc[dt][4 * g + 3] * scale);
+  for (int c = 0; c < NC2; ++c) {
+    Operand<float> n0 = a0, n1 = a1;
+    if (c + 1 < NC2) n0 = TL::row_chunk(x, col, 2 * c + 2 + half), n1 = TL::row_chunk(y, col, 2 * c + 2 + half);
+    mma2(a0, u.get(c), raw, a1, v.get(c), dp, [&](int m) { shadow<12 * NC2, 2 * PIECES>(12 * c + m, piece); });
+    a0 = n0, a1 = n1;
+  }
 }
 
 // dq (and with BIAS == 2 the table's gradient): queries stationary, key tiles through LDS.
@@ -110,29 +103,30 @@ __device__ __forceinline__ void store_rows(const f32x16 (&acc)[S::DT], T* row, i
 // delta = rowsum(dout * out) serves a softmax gradient well as long as out is exact; in bfloat16 it carries out's rounding, and a bucket that
 // holds most of a row's keys adds that error up over all rows.  There the table's gradient takes delta = sum_j P dP from a first walk over the
 // keys instead.
-template <class T, int DP, int BIAS, bool WIDE>
-__global__ __launch_bounds__((BackwardShape<T, DP, WIDE>::THREADS), (BackwardShape<T, DP, WIDE>::DQ_WAVES)) void attention_dq_kernel(Params p) {
-  using S = BackwardShape<T, DP, WIDE>;
+template <class T, int DP, int BIAS>
+__global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_dq_kernel(Params p) {
+  using S = BackwardShape<T, DP>;
   using TL = typename S::TL;
   constexpr int BN = S::BM, NC2 = DP / 16, BUFS = S::BUFS, NT = S::THREADS;
   constexpr bool TWICE = BIAS == 2 && sizeof(T) == 2;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   char* kt = smem;
   char* vt = smem + BUFS * TL::BYTES;
-  float* wave_delta = reinterpret_cast<float*>(smem + S::BODY);  // [WM][32]
-  int* word = reinterpret_cast<int*>(wave_delta + 4 * 32);
+  int* word = reinterpret_cast<int*>(smem + S::TILES);
   float* lut = reinterpret_cast<float*>(word + 4);
   const int lut_len = BIAS ? 2 * p.max_distance + 1 : 0, lut_pad = (lut_len + 3) & ~3;
-  float* scratch = lut + lut_pad;                        // [WAVES][32 * LD]
-  float* sums = scratch + S::WAVES * 32 * BiasGrad::LD;  // [WAVES][lut_pad]
-  const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31, wave = __builtin_amdgcn_readfirstlane(tid >> 6), ws = WIDE ? wave : 0, wm = WIDE ? 0 : wave;
-  const int nt = (p.Tq + 32 * S::WS - 1) / (32 * S::WS), n = p.B * p.H * nt * S::PARTS;
+  float* scratch = lut + lut_pad;                 // [4][32 * LD]
+  float* sums = scratch + 4 * 32 * BiasGrad::LD;  // [4][lut_pad]
+  const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int nt = (p.Tq + 127) / 128, n = p.B * p.H * nt * S::PARTS * p.dq_splits;
   int item = xcd_item(n);
   if (item >= n) return;
+  const int share = item % p.dq_splits;
+  item /= p.dq_splits;
   const int d0 = (item % S::PARTS) * S::DA;
   item /= S::PARTS;
   const int bh = item / nt, b = bh / p.H, h = bh - b * p.H, qt = p.causal ? nt - 1 - item % nt : item % nt;
-  const int q0 = qt * 32 * S::WS + 32 * ws;
+  const int q0 = qt * 128 + 32 * wave;
   const int off = start_of(p, b), kvh = h / p.group;
   const T* kb = reinterpret_cast<const T*>(p.k) + b * p.k_b + kvh * p.k_h;
   const T* vb = reinterpret_cast<const T*>(p.v) + b * p.v_b + kvh * p.v_h;
@@ -160,9 +154,9 @@ __global__ __launch_bounds__((BackwardShape<T, DP, WIDE>::THREADS), (BackwardSha
   const float lse2 = lse == -INFINITY ? INFINITY : lse * kLog2e;  // a row without keys, or none at all: P = exp2(.. - inf) = 0
   if constexpr (BIAS != 0) fill_lut(p, h, lut, tid, NT);
   if constexpr (BIAS == 2)
-    for (int i = tid; i < S::WAVES * lut_pad; i += NT) sums[i] = 0.f;
-  const int end = key_end(p, b, min(qt * 32 * S::WS + 32 * S::WS - 1, p.Tq - 1) + off, word, tid, NT);
-  const int tiles = (end + BN - 1) / BN;
+    for (int i = tid; i < 4 * lut_pad; i += NT) sums[i] = 0.f;
+  const int end = key_end(p, b, min(qt * 128 + 127, p.Tq - 1) + off, word, tid, NT);
+  const int all = (end + BN - 1) / BN, per = (all + p.dq_splits - 1) / p.dq_splits;
   f32x16 acc[S::DT] = {};
   BiasGrad bias_grad;
   Stage<T, DP, BN, NT> sk, sv;
@@ -180,32 +174,34 @@ __global__ __launch_bounds__((BackwardShape<T, DP, WIDE>::THREADS), (BackwardSha
 #pragma unroll
   for (int walk = TWICE ? 0 : 1; walk < 2; ++walk) {
     // the order of a round: as in the forward pass
-    KeyBits<BN> keys(mask, end, lane, 0);
-    RowBits use = keys.next(0), use1 = keys.next(BN), use2;  // of tiles t, t + 1, t + 2
-    load(0, use);
-    store(0);
-    if (S::EARLY) load(1, use1);
+    // (the first walk is over all keys, whatever the share)
+    const int t0 = TWICE && walk == 0 ? 0 : share * per, t1 = TWICE && walk == 0 ? all : min(all, t0 + per);
+    KeyBits<BN> keys(mask, end, lane, t0 * BN);
+    RowBits use = keys.next(t0 * BN), use1 = keys.next((t0 + 1) * BN), use2;  // of tiles t, t + 1, t + 2
+    load(t0, use);
+    store(t0);
+    if (S::EARLY) load(t0 + 1, use1);
     __syncthreads();
-    for (int t = 0; t < tiles; ++t) {
+    for (int t = t0; t < t1; ++t) {
       const char *kk = kt + (t & (BUFS - 1)) * TL::BYTES, *vv = vt + (t & (BUFS - 1)) * TL::BYTES;
       use2 = keys.next((t + 2) * BN);
-      if (!S::EARLY && S::AHEAD) load(t + 1, use1);
+      if (!S::EARLY) load(t + 1, use1);
 #pragma unroll
       for (int x = 0; x < S::NS; ++x) {
-        const int sub = S::NS * wm + x, key0 = t * BN + sub * 32;
+        const int sub = x, key0 = t * BN + sub * 32;
         const bool work = key0 < end && !(p.causal && key0 > pos_hi);
         f32x16 raw = {}, dp = {};
-        if (work) {
+        if constexpr (S::EARLY) {
+          char *kn = kt + ((t + 1) & (BUFS - 1)) * TL::BYTES, *vn = vt + ((t + 1) & (BUFS - 1)) * TL::BYTES;
+          products_shadow<TL, NC2>(kk, vv, q, go, raw, dp, sk, sv, kn, vn, col, half, tid);
+          load(t + 2, use2);
+        } else if (work) {
 #pragma unroll
           for (int c = 0; c < NC2; ++c)
             mma2(TL::row_chunk(kk, sub * 32 + col, 2 * c + half), q.get(c), raw, TL::row_chunk(vv, sub * 32 + col, 2 * c + half), go.get(c), dp,
                  [](int) {});
         }
-        if (x == 0 && S::EARLY) {
-          store(t + 1);
-          load(t + 2, use2);
-        }
-        if (work) {
+        if (S::EARLY || work) {
           float pr[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) pr[i] = raw[i];
@@ -220,36 +216,27 @@ __global__ __launch_bounds__((BackwardShape<T, DP, WIDE>::THREADS), (BackwardSha
             for (int i = 0; i < 16; ++i) pr[i] *= dp[i] - delta;
             if constexpr (BIAS == 2)
               if (d0 == 0) bias_grad.add(pr, key0 - pos_lo, p.max_distance, scratch + wave * 32 * BiasGrad::LD, sums + wave * lut_pad, lane);
-            column_product<T, TL>(kk, sub * 32, d0, Weights<T>(pr), acc, lane);
+            if constexpr (S::EARLY)
+              column_product_shadow<TL, S::DT, 0>(kk, 0, d0, [&](int i) { return pr[i]; }, acc, lane, nullptr, [](int) {});
+            else
+              column_product<T, TL>(kk, sub * 32, d0, Weights<T>(pr), acc, lane);
           }
         }
       }
       if (!S::EARLY) {
         if (BUFS == 1) __syncthreads();
-        if (!S::AHEAD) load(t + 1, use1);
         store(t + 1);
       }
       use = use1;
       use1 = use2;
       __syncthreads();
     }
-    if (TWICE && walk == 0) {
-      delta = both_sum(delta);
-      if constexpr (S::WM > 1) {
-        if (half == 0) wave_delta[wm * 32 + col] = delta;
-        __syncthreads();
-        delta = 0.f;
-#pragma unroll
-        for (int w = 0; w < S::WM; ++w) delta += wave_delta[w * 32 + col];
-      }
-    }
+    if (TWICE && walk == 0) delta = both_sum(delta);
   }
-  if (half == 0 && wm == 0 && d0 == 0 && qi < p.Tq) p.delta[(int64_t)bh * p.Tq + qi] = delta;
-  T* out = reinterpret_cast<T*>(p.dq) + b * p.dq_b + h * p.dq_h;
-  if constexpr (S::WM > 1)
-    join_and_store<S>(acc, reinterpret_cast<float*>(smem), out + q0 * p.dq_t, p.dq_t, p.Tq - q0, d0, p.D, p.scale, wave, lane, tid);
-  else if (qi < p.Tq)
-    store_rows<S>(acc, out + qi * p.dq_t, d0, p.D, p.scale, half);
+  if (half == 0 && share == 0 && d0 == 0 && qi < p.Tq) p.delta[(int64_t)bh * p.Tq + qi] = delta;
+  if (qi < p.Tq)
+    store_rows<S>(acc, reinterpret_cast<T*>(p.dq) + b * p.dq_b + h * p.dq_h + qi * p.dq_t,
+                  p.dq_splits > 1 ? p.dq_part + (((int64_t)share * p.B * p.H + bh) * p.Tq + qi) * p.D : nullptr, d0, p.D, p.scale, half);
   if constexpr (BIAS == 2) {
     if (d0 != 0) return;
     for (int m = 1; m < 64; m <<= 1) {
@@ -264,32 +251,34 @@ __global__ __launch_bounds__((BackwardShape<T, DP, WIDE>::THREADS), (BackwardSha
     // the waves' sums, then a bucket's distances, each in a fixed order
     for (int i = tid; i < lut_len; i += NT) {
       float x = sums[i];
-      for (int w = 1; w < S::WAVES; ++w) x += sums[w * lut_pad + i];
+      for (int w = 1; w < 4; ++w) x += sums[w * lut_pad + i];
       sums[i] = x;
     }
     __syncthreads();
-    for (int i = tid; i < p.buckets; i += NT) p.dtable_part[((int64_t)(b * nt + qt) * p.H + h) * p.buckets + i] = bucket_sum(p, sums, i);
+    for (int i = tid; i < p.buckets; i += NT) p.dtable_part[((int64_t)((b * nt + qt) * p.dq_splits + share) * p.H + h) * p.buckets + i] = bucket_sum(p, sums, i);
   }
 }
 
 // dk, dv: keys of one key head stationary; tiles of queries and their output gradients through LDS, over all heads of the group.
-template <class T, int DP, bool BIAS, bool WIDE>
-__global__ __launch_bounds__((BackwardShape<T, DP, WIDE>::THREADS), (BackwardShape<T, DP, WIDE>::DKV_WAVES)) void attention_dkv_kernel(Params p) {
-  using S = BackwardShape<T, DP, WIDE>;
+template <class T, int DP, bool BIAS>
+__global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_dkv_kernel(Params p) {
+  using S = BackwardShape<T, DP>;
   using TL = typename S::TL;
   constexpr int BM = S::BM, NC2 = DP / 16, BUFS = S::BUFS, NT = S::THREADS;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   char* qt = smem;
   char* gt = smem + BUFS * TL::BYTES;
-  float* stat = reinterpret_cast<float*>(smem + S::BODY);  // [BUFS][2][BM]: lse in log2 units, delta
+  float* stat = reinterpret_cast<float*>(smem + S::TILES);  // [BUFS][2][BM]: lse in log2 units, delta
   float* lut = stat + BUFS * 2 * BM;
-  const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31, wave = __builtin_amdgcn_readfirstlane(tid >> 6), ws = WIDE ? wave : 0, wm = WIDE ? 0 : wave;
-  const int nt = (p.Tk + 32 * S::WS - 1) / (32 * S::WS), n = p.B * p.Hkv * nt * S::PARTS;
+  const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int nt = (p.Tk + 127) / 128, n = p.B * p.Hkv * nt * S::PARTS * p.dkv_splits;
   int item = xcd_item(n);
   if (item >= n) return;
+  const int share = item % p.dkv_splits;
+  item /= p.dkv_splits;
   const int d0 = (item % S::PARTS) * S::DA;
   item /= S::PARTS;
-  const int bh = item / nt, b = bh / p.Hkv, kvh = bh - b * p.Hkv, k0 = (item % nt) * 32 * S::WS, kw = k0 + 32 * ws;
+  const int bh = item / nt, b = bh / p.Hkv, kvh = bh - b * p.Hkv, k0 = (item % nt) * 128, kw = k0 + 32 * wave;
   const int off = start_of(p, b), key = kw + col, kc = min(key, p.Tk - 1);
   const uint8_t* mask = p.key_mask ? p.key_mask + b * p.mask_b : nullptr;
   int end = p.Tk;
@@ -303,7 +292,8 @@ __global__ __launch_bounds__((BackwardShape<T, DP, WIDE>::THREADS), (BackwardSha
   f32x16 dk[S::DT] = {}, dv[S::DT] = {};
   // under causality queries before key - off see nothing of this block
   const int qt_n = (p.Tq + BM - 1) / BM, qt_0 = p.causal ? min(max(k0 - off, 0) / BM, qt_n) : 0, per = qt_n - qt_0;
-  const int steps = k0 < end ? per * p.group : 0;
+  const int all = k0 < end ? per * p.group : 0, mine = (all + p.dkv_splits - 1) / p.dkv_splits, first_it = share * mine,
+            steps = min(all, first_it + mine);
   Stage<T, DP, BM, NT> sq, sg;
   sq.start(nullptr, p.q_t, p.Tq, p.D, tid);
   sg.start(nullptr, p.do_t, p.Tq, p.D, tid);
@@ -322,45 +312,50 @@ __global__ __launch_bounds__((BackwardShape<T, DP, WIDE>::THREADS), (BackwardSha
       s_delta = r0 + tid < p.Tq ? p.delta[row] : 0.f;
     }
   };
-  auto store = [&](int it) {
+  auto store_stat = [&](int it) {
     const int o = it & (BUFS - 1);
-    sq.store(qt + o * TL::BYTES, tid);
-    sg.store(gt + o * TL::BYTES, tid);
     if (tid < BM) {
       stat[o * 2 * BM + tid] = s_lse;
       stat[(o * 2 + 1) * BM + tid] = s_delta;
     }
   };
-  load(0);
-  store(0);
-  if (S::EARLY) load(1);
+  auto store = [&](int it) {
+    const int o = it & (BUFS - 1);
+    sq.store(qt + o * TL::BYTES, tid);
+    sg.store(gt + o * TL::BYTES, tid);
+    store_stat(it);
+  };
+  load(first_it);
+  store(first_it);
+  if (S::EARLY) load(first_it + 1);
   __syncthreads();
-  for (int it = 0; it < steps; ++it) {
+  for (int it = first_it; it < steps; ++it) {
     if constexpr (BIAS) {
-      if (it % per == 0) {
+      if (it == first_it || it % per == 0) {
         fill_lut(p, kvh * p.group + it / per, lut, tid, NT);
         __syncthreads();
       }
     }
     const int o = it & (BUFS - 1), r0 = (qt_0 + it % per) * BM;
     const char *qq = qt + o * TL::BYTES, *gg = gt + o * TL::BYTES;
-    if (!S::EARLY && S::AHEAD) load(it + 1);
+    if (!S::EARLY) load(it + 1);
 #pragma unroll
     for (int x = 0; x < S::NS; ++x) {
-      const int sub = S::NS * wm + x, i0 = r0 + sub * 32, p0 = i0 + off;  // position of the subtile's first query
+      const int sub = x, i0 = r0 + sub * 32, p0 = i0 + off;  // position of the subtile's first query
       const bool work = kw < end && i0 < p.Tq && !(p.causal && kw > p0 + 31);
       f32x16 raw = {}, dp = {};
-      if (work) {
+      if constexpr (S::EARLY) {
+        char *qn = qt + ((it + 1) & (BUFS - 1)) * TL::BYTES, *gn = gt + ((it + 1) & (BUFS - 1)) * TL::BYTES;
+        products_shadow<TL, NC2>(qq, gg, k, v, raw, dp, sq, sg, qn, gn, col, half, tid);
+        store_stat(it + 1);
+        load(it + 2);
+      } else if (work) {
 #pragma unroll
         for (int c = 0; c < NC2; ++c)
           mma2(TL::row_chunk(qq, sub * 32 + col, 2 * c + half), k.get(c), raw, TL::row_chunk(gg, sub * 32 + col, 2 * c + half), v.get(c), dp,
                [](int) {});
       }
-      if (x == 0 && S::EARLY) {
-        store(it + 1);
-        load(it + 2);
-      }
-      if (work) {
+      if (S::EARLY || work) {
         float s[16];
         if constexpr (BIAS) {
           const int md = p.max_distance;
@@ -393,53 +388,82 @@ __global__ __launch_bounds__((BackwardShape<T, DP, WIDE>::THREADS), (BackwardSha
             ds[i] = s[i] * (dp[i] - de[e]);
           }
         }
-        column_product<T, TL>(gg, sub * 32, d0, Weights<T>(s), dv, lane);
-        column_product<T, TL>(qq, sub * 32, d0, Weights<T>(ds), dk, lane);
+        if constexpr (S::EARLY) {
+          Splitter first;  // of dS, made beside the products with P
+          column_product_shadow<TL, S::DT, 12>(gg, 0, d0, [&](int i) { return s[i]; }, dv, lane, nullptr,
+                                               [&](int i) { first.step(i, [&](int n) { return ds[n]; }); });
+          column_product_shadow<TL, S::DT, 0>(qq, 0, d0, [&](int i) { return ds[i]; }, dk, lane, &first, [](int) {});
+        } else {
+          column_product<T, TL>(gg, sub * 32, d0, Weights<T>(s), dv, lane);
+          column_product<T, TL>(qq, sub * 32, d0, Weights<T>(ds), dk, lane);
+        }
       }
     }
     if (!S::EARLY) {
       if (BUFS == 1) __syncthreads();
-      if (!S::AHEAD) load(it + 1);
       store(it + 1);
     }
     __syncthreads();
   }
   T* kout = reinterpret_cast<T*>(p.dk) + b * p.dk_b + kvh * p.dk_h;
   T* vout = reinterpret_cast<T*>(p.dv) + b * p.dv_b + kvh * p.dv_h;
-  if constexpr (S::WM > 1) {
-    float* sums = reinterpret_cast<float*>(smem);
-    join_and_store<S>(dk, sums, kout + kw * p.dk_t, p.dk_t, p.Tk - kw, d0, p.D, p.scale, wave, lane, tid);
-    join_and_store<S>(dv, sums, vout + kw * p.dv_t, p.dv_t, p.Tk - kw, d0, p.D, 1.f, wave, lane, tid);
-  } else if (key < p.Tk) {
-    store_rows<S>(dk, kout + key * p.dk_t, d0, p.D, p.scale, half);
-    store_rows<S>(dv, vout + key * p.dv_t, d0, p.D, 1.f, half);
+  if (key < p.Tk) {
+    float* part = nullptr;
+    const int64_t rows = (int64_t)p.B * p.Hkv * p.Tk;
+    if (p.dkv_splits > 1) part = p.dkv_part + (share * 2 * rows + (int64_t)bh * p.Tk + key) * p.D;
+    store_rows<S>(dk, kout + key * p.dk_t, part, d0, p.D, p.scale, half);
+    store_rows<S>(dv, vout + key * p.dv_t, part ? part + rows * p.D : nullptr, d0, p.D, 1.f, half);
   }
+}
+
+// The workgroups' shares added up in their order: out[b, h, t, :] = sum over s of part[s][(b H + h) T + t][:].  blockIdx.y: dk, dv.
+template <class T>
+__global__ __launch_bounds__(256) void attention_share_kernel(const float* part, int splits, int64_t step, int64_t pair, int64_t rows, int T_, int H, int D, T* out0,
+                                                              T* out1, int64_t b0, int64_t h0, int64_t t0, int64_t b1, int64_t h1, int64_t t1) {
+  const int quads = D / 4;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, row = i / quads;
+  if (row >= rows) return;
+  const int d = (int)(i - row * quads) * 4;
+  const float* x = part + blockIdx.y * pair + row * D + d;
+  f32x4 s = *reinterpret_cast<const f32x4*>(x);
+  for (int n = 1; n < splits; ++n) s += *reinterpret_cast<const f32x4*>(x + n * step);
+  const int t = row % T_;
+  const int64_t bh = row / T_, b = bh / H, h = bh % H;
+  T* o = blockIdx.y ? out1 + b * b1 + h * h1 + t * t1 : out0 + b * b0 + h * h0 + t * t0;
+  store4<T>(o, d, D, s[0], s[1], s[2], s[3]);
 }
 
 // ------------------------------------------------------------------ host
 
-template <class T, int DP, int BIAS, bool WIDE>
-static int launch_dq(const Params& p, hipStream_t st) {
-  using S = BackwardShape<T, DP, WIDE>;
-  static std::atomic<uint64_t> done{0};
-  const size_t lut = BIAS ? (size_t)(2 * p.max_distance + 4) * 4 : 0;
-  return launch(&attention_dq_kernel<T, DP, BIAS, WIDE>, &done, (int64_t)p.B * p.H * ((p.Tq + 32 * S::WS - 1) / (32 * S::WS)) * S::PARTS, S::THREADS,
-                S::BODY + 4 * 32 * 4 + 16 + lut + (BIAS == 2 ? S::WAVES * (32 * BiasGrad::LD * 4 + lut) : 0), p, st);
-}
-template <class T, int DP, bool BIAS, bool WIDE>
-static int launch_dkv(const Params& p, hipStream_t st) {
-  using S = BackwardShape<T, DP, WIDE>;
-  static std::atomic<uint64_t> done{0};
-  const size_t lut = BIAS ? (size_t)(2 * p.max_distance + 4) * 4 : 0;
-  return launch(&attention_dkv_kernel<T, DP, BIAS, WIDE>, &done, (int64_t)p.B * p.Hkv * ((p.Tk + 32 * S::WS - 1) / (32 * S::WS)) * S::PARTS,
-                S::THREADS, S::BODY + S::BUFS * 2 * S::BM * 4 + lut, p, st);
-}
-
 template <class T, int DP, int BIAS>
 static int launch_backward(const Params& p, float* dtable, hipStream_t st) {
-  if (p.wide_dq ? launch_dq<T, DP, BIAS, true>(p, st) : launch_dq<T, DP, BIAS, false>(p, st)) return 1;
-  if (p.dk && p.Tk && (p.wide_dkv ? launch_dkv<T, DP, BIAS != 0, true>(p, st) : launch_dkv<T, DP, BIAS != 0, false>(p, st))) return 1;
-  if (BIAS == 2) return launch_table_sum<float>(p.dtable_part, p.B * dq_tiles(p), p.H, p.buckets, dtable, st);
+  using S = BackwardShape<T, DP>;
+  static std::atomic<uint64_t> dq_done{0}, dkv_done{0};
+  const size_t lut = BIAS ? (size_t)(2 * p.max_distance + 4) * 4 : 0;
+  const int q_tiles = (p.Tq + 127) / 128;
+  if (launch(&attention_dq_kernel<T, DP, BIAS>, &dq_done, (int64_t)p.B * p.H * q_tiles * S::PARTS * p.dq_splits, S::THREADS,
+             S::TILES + 16 + lut + (BIAS == 2 ? 4 * (32 * BiasGrad::LD * 4 + lut) : 0), p, st))
+    return 1;
+  if (p.dq_splits > 1) {
+    const int64_t rows = (int64_t)p.B * p.H * p.Tq;
+    T* dq = static_cast<T*>(p.dq);
+    hipLaunchKernelGGL((attention_share_kernel<T>), dim3((unsigned)((rows * (p.D / 4) + 255) / 256)), dim3(256), 0, st, p.dq_part, p.dq_splits, rows * p.D,
+                       int64_t(0), rows, p.Tq, p.H, p.D, dq, dq, p.dq_b, p.dq_h, p.dq_t, p.dq_b, p.dq_h, p.dq_t);
+    WRNN_LAUNCH_CHECK();
+  }
+  if (p.dk && p.Tk) {
+    if (launch(&attention_dkv_kernel<T, DP, BIAS != 0>, &dkv_done, (int64_t)p.B * p.Hkv * ((p.Tk + 127) / 128) * S::PARTS * p.dkv_splits, S::THREADS,
+               S::TILES + S::BUFS * 2 * S::BM * 4 + lut, p, st))
+      return 1;
+    if (p.dkv_splits > 1) {
+      const int64_t rows = (int64_t)p.B * p.Hkv * p.Tk;
+      hipLaunchKernelGGL((attention_share_kernel<T>), dim3((unsigned)((rows * (p.D / 4) + 255) / 256), 2), dim3(256), 0, st, p.dkv_part, p.dkv_splits,
+                         2 * rows * p.D, rows * p.D, rows, p.Tk, p.Hkv, p.D, static_cast<T*>(p.dk), static_cast<T*>(p.dv), p.dk_b, p.dk_h, p.dk_t, p.dv_b,
+                         p.dv_h, p.dv_t);
+      WRNN_LAUNCH_CHECK();
+    }
+  }
+  if (BIAS == 2) return launch_table_sum<float>(p.dtable_part, p.B * q_tiles * p.dq_splits, p.H, p.buckets, dtable, st);
   return 0;
 }
 

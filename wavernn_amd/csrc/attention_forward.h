@@ -37,9 +37,9 @@ struct Running {
 
 // Shapes of a workgroup.
 //   wide   4 waves, 32 queries each, all against every 32 keys of a tile: a tile in LDS serves 128 queries.
-//   narrow 32 queries, the waves on different 32 keys of a tile, joined at the end; the keys may further be split over
-//          workgroups, and the 32 columns may hold the queries of all heads that share k and v (p.pack).  For calls with few
-//          queries, or too few workgroups of the wide shape to fill the compute units.
+//   narrow 32 query columns, the waves on different 32 keys of a tile, joined at the end; the columns may hold the queries of all heads that
+//          share k and v (p.pack).  For single tokens and few queries.
+// In either the keys may be divided over workgroups (p.splits), whose sums attention_join_kernel adds up.
 template <class T, int DP, bool WIDE>
 struct ForwardShape {
   static constexpr int NP = Type<T>::NP;
@@ -70,7 +70,7 @@ __global__ __launch_bounds__((ForwardShape<T, DP, WIDE>::THREADS), (ForwardShape
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wq = WIDE ? wave : 0, wk = WIDE ? 0 : wave;
   const bool pack = !WIDE && p.pack;
-  const int heads = pack ? p.Hkv : p.H, splits = WIDE ? 1 : p.splits;
+  const int heads = pack ? p.Hkv : p.H, splits = p.splits;
   const int nt = pack ? 1 : (p.Tq + 32 * S::WQ - 1) / (32 * S::WQ), n = p.B * heads * nt * splits;
   int item = xcd_item(n);
   if (item >= n) return;
@@ -134,13 +134,12 @@ __global__ __launch_bounds__((ForwardShape<T, DP, WIDE>::THREADS), (ForwardShape
       f32x16 raw[NS] = {};
       if constexpr (S::EARLY) {
         char *kn = kt + ((t + 1) & (BUFS - 1)) * TL::BYTES, *vn = vt + ((t + 1) & (BUFS - 1)) * TL::BYTES;
-        u32x4 w[3];
+        Splitter sp;
         constexpr int PIECES = decltype(sk)::PIECES;
         const auto piece = [&](int i) {
-          if (i < PIECES) sk.store_piece(kn, tid, i, w);
-          else sv.store_piece(vn, tid, i - PIECES, w);
+          if (i < PIECES) sk.store_piece(kn, tid, i, sp);
+          else sv.store_piece(vn, tid, i - PIECES, sp);
         };
-        const Shadow<decltype(piece)> shadow(6 * NC2, 2 * PIECES, piece);
         auto chunk = [&](int c) { return TL::row_chunk(kk, col, 2 * c + half); };
         f32x16 odd = {};
         Operand<T> a0 = chunk(0), a1 = chunk(1);
@@ -148,7 +147,7 @@ __global__ __launch_bounds__((ForwardShape<T, DP, WIDE>::THREADS), (ForwardShape
         for (int c = 0; c < NC2; c += 2) {
           Operand<T> n0 = a0, n1 = a1;
           if (c + 2 < NC2) n0 = chunk(c + 2), n1 = chunk(c + 3);
-          mma2(a0, q.get(c), raw[0], a1, q.get(c + 1), odd, [&](int m) { shadow(6 * c + m); });
+          mma2(a0, q.get(c), raw[0], a1, q.get(c + 1), odd, [&](int m) { shadow<6 * NC2, 2 * PIECES>(6 * c + m, piece); });
           a0 = n0, a1 = n1;
         }
         raw[0] += odd;
@@ -168,7 +167,7 @@ __global__ __launch_bounds__((ForwardShape<T, DP, WIDE>::THREADS), (ForwardShape
       }
       run.move(s, acc);
       if constexpr (S::EARLY) {
-        column_product_shadow<TL>(vv, 0, 0, [&](int i) { return run.weight(s[0][i]); }, acc, lane);
+        column_product_shadow<TL, DT, 0>(vv, 0, 0, [&](int i) { return run.weight(s[0][i]); }, acc, lane, nullptr, [](int) {});
       } else {
 #pragma unroll
         for (int x = 0; x < NS; ++x) {
@@ -297,13 +296,15 @@ template <class T, int DP, bool BIAS>
 static int launch_forward(const Params& p, hipStream_t st) {
   static std::atomic<uint64_t> wide_done{0}, narrow_done{0};
   const size_t lut = BIAS ? (2 * p.max_distance + 1) * sizeof(float) : 0;
-  if (p.splits == 0) {
+  if (!p.narrow) {
     using S = ForwardShape<T, DP, true>;
-    return launch(&attention_forward_kernel<T, DP, BIAS, true>, &wide_done, (int64_t)p.B * p.H * ((p.Tq + 127) / 128), S::THREADS, S::LDS + lut, p, st);
+    const int64_t n = (int64_t)p.B * p.H * ((p.Tq + 127) / 128) * p.splits;
+    if (launch(&attention_forward_kernel<T, DP, BIAS, true>, &wide_done, n, S::THREADS, S::LDS + lut, p, st)) return 1;
+  } else {
+    using S = ForwardShape<T, DP, false>;
+    const int64_t n = (p.pack ? (int64_t)p.B * p.Hkv : (int64_t)p.B * p.H * ((p.Tq + 31) / 32)) * p.splits;
+    if (launch(&attention_forward_kernel<T, DP, BIAS, false>, &narrow_done, n, S::THREADS, S::LDS + lut * (p.pack ? p.group : 1), p, st)) return 1;
   }
-  using S = ForwardShape<T, DP, false>;
-  const int64_t n = (p.pack ? (int64_t)p.B * p.Hkv : (int64_t)p.B * p.H * ((p.Tq + 31) / 32)) * p.splits;
-  if (launch(&attention_forward_kernel<T, DP, BIAS, false>, &narrow_done, n, S::THREADS, S::LDS + lut * (p.pack ? p.group : 1), p, st)) return 1;
   if (p.splits > 1) {
     const int64_t rows = (int64_t)p.B * p.H * p.Tq;
     hipLaunchKernelGGL((attention_join_kernel<T, DP>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, p);

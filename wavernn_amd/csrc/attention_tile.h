@@ -57,10 +57,11 @@ struct Params {
   const void *dout, *o_in;
   void *dq, *dk, *dv;
   float *delta, *dtable_part;
-  int wide_dq, wide_dkv;  // 128 stationary rows per workgroup, not 32
+  int dq_splits, dkv_splits;  // workgroups that share a block of rows, each with part of the other side
+  float *dq_part, *dkv_part;  // their sums, where there are several
   int64_t do_b, do_h, do_t, oi_b, oi_h, oi_t, dq_b, dq_h, dq_t, dk_b, dk_h, dk_t, dv_b, dv_h, dv_t;
-  // keys split over workgroups (few queries)
-  int splits, pack;
+  int narrow, pack;  // shape of the forward pass
+  int splits;        // workgroups that share a block of queries, each with part of the keys
   float* part;
 };
 
@@ -86,28 +87,24 @@ struct Raw {  // 8 elements as they come from memory
 };
 
 __device__ __forceinline__ Operand<__bf16> operand(const Raw<__bf16>& r) { return {{r.x}}; }
-// Two values at a time, by cutting: a plane is the upper half of what the planes before it leave (8 bits of mantissa, the subtraction is
-// exact), so the three add up to the value itself.
-__device__ __forceinline__ void split2(float a, float b, uint32_t (&w)[3]) {
-#pragma unroll
-  for (int n = 0; n < 3; ++n) {
-    const uint32_t x = __float_as_uint(a), y = __float_as_uint(b);
-    w[n] = __builtin_amdgcn_perm(y, x, 0x07060302u);  // upper halves of x and y
-    if (n < 2) {
-      a -= __uint_as_float(x & 0xffff0000u);
-      b -= __uint_as_float(y & 0xffff0000u);
-    }
+// One plane of two values, by cutting: the upper half of what the planes before it left (8 bits of mantissa); the subtraction is exact, so
+// the three add up to the value itself.
+__device__ __forceinline__ uint32_t split2(float& a, float& b, bool more) {
+  const uint32_t x = __float_as_uint(a), y = __float_as_uint(b);
+  if (more) {
+    a -= __uint_as_float(x & 0xffff0000u);
+    b -= __uint_as_float(y & 0xffff0000u);
   }
+  return __builtin_amdgcn_perm(y, x, 0x07060302u);  // the upper halves of x and y
 }
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ void split(f32x8 x, bf16x8 (&p)[3]) {
   u32x4 v[3];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    uint32_t w[3];
-    split2(x[2 * j], x[2 * j + 1], w);
+    float a = x[2 * j], b = x[2 * j + 1];
 #pragma unroll
-    for (int n = 0; n < 3; ++n) v[n][j] = w[n];
+    for (int n = 0; n < 3; ++n) v[n][j] = split2(a, b, n < 2);
   }
 #pragma unroll
   for (int n = 0; n < 3; ++n) p[n] = __builtin_bit_cast(bf16x8, v[n]);
@@ -143,7 +140,7 @@ __device__ __forceinline__ f32x16 mma(const Operand<T>& a, const Operand<T>& b, 
 }
 
 // Two products, instruction by instruction in turn: a product that adds to the one right before it waits for the whole of that one's
-// latency, twice the time the unit is busy (float32 forward, one wave a SIMD: PAIRGAIN).
+// latency.
 template <class F>
 __device__ __forceinline__ void mma2(const Operand<__bf16>& a0, const Operand<__bf16>& b0, f32x16& c0, const Operand<__bf16>& a1,
                                      const Operand<__bf16>& b1, f32x16& c1, F&& between) {
@@ -166,17 +163,29 @@ __device__ __forceinline__ void mma2(const Operand<float>& a0, const Operand<flo
 }
 
 // Work in the matrix instructions' shadow: a 32 x 32 x 16 product keeps the matrix unit for 32 cycles, a vector instruction its unit for 4, and a
-// wave issues in order, so a wave that is alone on its SIMD has to have vector instructions BETWEEN its products.  The compiler's
-// scheduler moves them behind; Shadow(products, pieces, f) deals f(0) .. f(pieces - 1) out over the products and fences each step.
-template <class F>
-struct Shadow {
-  int products, pieces;
-  F f;
-  __device__ __forceinline__ Shadow(int products_, int pieces_, F f_) : products(products_), pieces(pieces_), f(f_) {}
-  __device__ __forceinline__ void operator()(int m) const {
+// wave issues in order: one that is alone on its SIMD has to have a few vector instructions behind EVERY product, for behind a second
+// product they wait with it.  The compiler's scheduler gathers them at the end; shadow<PRODUCTS, PIECES>(m, f) deals f(0) .. f(PIECES - 1)
+// out over the products and fences each step.
+template <int PRODUCTS, int PIECES, class F>
+__device__ __forceinline__ void shadow(int m, F&& f) {
 #pragma unroll
-    for (int i = m * pieces / products; i < (m + 1) * pieces / products; ++i) f(i);
-    __builtin_amdgcn_sched_barrier(0);
+  for (int i = m * PIECES / PRODUCTS; i < (m + 1) * PIECES / PRODUCTS; ++i) f(i);
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// float32 values on their way to three planes, in steps of one plane of two values (5 vector instructions or 1).
+struct Splitter {
+  u32x4 w[3];
+  float a, b;
+  // step i of 12 for 8 values; value(k) gives the k-th
+  template <class V>
+  __device__ __forceinline__ void step(int i, V&& value) {
+    const int j = i / 3, n = i % 3;
+    if (n == 0) a = value(2 * j), b = value(2 * j + 1);
+    w[n][j] = split2(a, b, n < 2);
+  }
+  __device__ __forceinline__ Operand<float> get() const {
+    return {{__builtin_bit_cast(bf16x8, w[0]), __builtin_bit_cast(bf16x8, w[1]), __builtin_bit_cast(bf16x8, w[2])}};
   }
 };
 
@@ -306,45 +315,33 @@ __device__ __forceinline__ Operand<T> column_chunk(const char* tile, int r0, int
 template <class T, class TL, int DT>
 __device__ __forceinline__ void column_product(const char* tile, int r0, int d0, const Weights<T>& w, f32x16 (&acc)[DT], int lane) {
 #pragma unroll
-  for (int s = 0; s < 2; ++s)
+  for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-    for (int dt = 0; dt < DT; dt += 2)
-      mma2(column_chunk<T, TL>(tile, r0 + 16 * s, d0 + 32 * dt, lane), w.o[s], acc[dt],
-           column_chunk<T, TL>(tile, r0 + 16 * s, d0 + 32 * dt + 32, lane), w.o[s], acc[dt + 1], [](int) {});
+    for (int s = 0; s < 2; ++s) acc[dt] = mma(column_chunk<T, TL>(tile, r0 + 16 * s, d0 + 32 * dt, lane), w.o[s], acc[dt]);
 }
 
-// The same for float32 from weights not made yet: value(i) gives weight i of the lane.  The first 16 moving rows' weights are made
-// ahead, the others' in the shadow of the first products.
-template <class TL, int DT, class V>
-__device__ __forceinline__ void column_product_shadow(const char* tile, int r0, int d0, V&& value, f32x16 (&acc)[DT], int lane) {
-  u32x4 w[2][3];
-  auto make = [&](int i) {
-    uint32_t x[3];
-    split2(value(2 * i), value(2 * i + 1), x);
-#pragma unroll
-    for (int k = 0; k < 3; ++k) w[i >> 2][k][i & 3] = x[k];
-  };
-  auto get = [&](int s) {
-    Operand<float> o;
-#pragma unroll
-    for (int k = 0; k < 3; ++k) o.p[k] = __builtin_bit_cast(bf16x8, w[s][k]);
-    return o;
-  };
+// The same for float32 from weights not made yet: value(i) gives weight i of the lane, called once for each in their order.  The first 16
+// moving rows' weights are made ahead (or handed in, made in an earlier product's shadow), the others' in the shadow of the first
+// products; after(i), AFTER steps of other work, in the shadow of the others.
+template <class TL, int DT, int AFTER, class V, class F>
+__device__ __forceinline__ void column_product_shadow(const char* tile, int r0, int d0, V&& value, f32x16 (&acc)[DT], int lane, const Splitter* made,
+                                                      F&& after) {
   auto chunk = [&](int n) { return column_chunk<float, TL>(tile, r0 + 16 * (n / DT), d0 + 32 * (n % DT), lane); };
   Operand<float> a0 = chunk(0), a1 = chunk(1);
+  Splitter first, second;
+  if (!made) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) make(i);
-  Operand<float> b = get(0);
-  const auto later = [&](int i) { make(4 + i); };
-  const Shadow<decltype(later)> shadow(6 * DT, 4, later);
+    for (int i = 0; i < 12; ++i) first.step(i, value);
+  }
+  Operand<float> b = made ? made->get() : first.get();
 #pragma unroll
   for (int n = 0; n < 2 * DT; n += 2) {
-    if (n == DT) b = get(1);
+    if (n == DT) b = second.get();
     Operand<float> n0 = a0, n1 = a1;
     if (n + 2 < 2 * DT) n0 = chunk(n + 2), n1 = chunk(n + 3);
     mma2(a0, b, acc[n % DT], a1, b, acc[n % DT + 1], [&](int m) {
-      if (n < DT) shadow(6 * n + m);
-      else __builtin_amdgcn_sched_barrier(0);
+      if (n < DT) shadow<6 * DT, 12>(6 * n + m, [&](int i) { second.step(i, [&](int k) { return value(8 + k); }); });
+      else shadow<6 * DT, AFTER>(6 * (n - DT) + m, after);
     });
     a0 = n0, a1 = n1;
   }
@@ -441,20 +438,12 @@ struct Stage {
 #pragma unroll
     for (int n = 0; n < N; ++n) TL::put(tile, tid / TL::NCH + n * STEP, tid % TL::NCH, operand(r[n]));
   }
-  // The same in PIECES steps (float32), two values each.
-  static constexpr int PIECES = 4 * N;
-  __device__ __forceinline__ void store_piece(char* tile, int tid, int i, u32x4 (&w)[3]) {
-    const int n = i >> 2, j = i & 3;
-    uint32_t x[3];
-    split2(r[n].x[2 * j], r[n].x[2 * j + 1], x);
-#pragma unroll
-    for (int k = 0; k < 3; ++k) w[k][j] = x[k];
-    if (j == 3) {
-      Operand<T> o;
-#pragma unroll
-      for (int k = 0; k < 3; ++k) o.p[k] = __builtin_bit_cast(bf16x8, w[k]);
-      TL::put(tile, tid / TL::NCH + n * STEP, tid % TL::NCH, o);
-    }
+  // The same in PIECES steps (float32).
+  static constexpr int PIECES = 12 * N;
+  __device__ __forceinline__ void store_piece(char* tile, int tid, int i, Splitter& sp) {
+    const int n = i / 12;
+    sp.step(i % 12, [&](int k) { return r[n].x[k]; });
+    if (i % 12 == 11) TL::put(tile, tid / TL::NCH + n * STEP, tid % TL::NCH, sp.get());
   }
 };
 
@@ -607,11 +596,6 @@ static inline bool rows_on_16(const void* ptr, int64_t b, int64_t h, int64_t t, 
   return ((reinterpret_cast<uintptr_t>(ptr) | (uintptr_t)(b * es) | (uintptr_t)(h * es) | (uintptr_t)(t * es)) & 15) == 0;
 }
 
-}  // namespace attn
-
-// Query tiles of a head in the dq kernel: rows of the table gradient's partial sums.
-namespace attn {
-static inline int dq_tiles(const Params& p) { return p.wide_dq ? (p.Tq + 127) / 128 : (p.Tq + 31) / 32; }
 }  // namespace attn
 
 // dtable[n, h] = sum over r of part[r][h][n] (relative_bias.hip).
