@@ -162,12 +162,17 @@ __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_
   Stage<T, DP, BN, NT> sk, sv;
   sk.start(kb, p.k_t, end, p.D, tid);
   sv.start(vb, p.v_t, end, p.D, tid);
+  // rows that the mask leaves out: not requested (EARLY), or zeroed on their way to LDS, which keeps the requests one block of code
   auto load = [&](int t, const RowBits& use) {
-    sk.load(t * BN, mask ? &use : nullptr, tid);
-    sv.load(t * BN, mask ? &use : nullptr, tid);
+    sk.load(t * BN, S::EARLY && mask ? &use : nullptr, tid);
+    sv.load(t * BN, S::EARLY && mask ? &use : nullptr, tid);
   };
-  auto store = [&](int t) {
+  auto store = [&](int t, const RowBits& use) {
     const int o = t & (BUFS - 1);
+    if (!S::EARLY && mask && !use.template all<BN>()) {
+      sk.drop(use, tid);
+      sv.drop(use, tid);
+    }
     sk.store(kt + o * TL::BYTES, tid);
     sv.store(vt + o * TL::BYTES, tid);
   };
@@ -179,7 +184,7 @@ __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_
     KeyBits<BN> keys(mask, end, lane, t0 * BN);
     RowBits use = keys.next(t0 * BN), use1 = keys.next((t0 + 1) * BN), use2;  // of tiles t, t + 1, t + 2
     load(t0, use);
-    store(t0);
+    store(t0, use);
     if (S::EARLY) load(t0 + 1, use1);
     __syncthreads();
     for (int t = t0; t < t1; ++t) {
@@ -225,7 +230,7 @@ __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_
       }
       if (!S::EARLY) {
         if (BUFS == 1) __syncthreads();
-        store(t + 1);
+        store(t + 1, use1);
       }
       use = use1;
       use1 = use2;

@@ -434,6 +434,12 @@ struct Stage {
       else r[n].x = __builtin_shufflevector(__builtin_bit_cast(f32x4, x[0]), __builtin_bit_cast(f32x4, x[1]), 0, 1, 2, 3, 4, 5, 6, 7);
     }
   }
+  // the same for rows that are here already
+  __device__ __forceinline__ void drop(const RowBits& use, int tid) {
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+      if (!use.at(tid / TL::NCH + n * STEP)) r[n].x = {};
+  }
   __device__ __forceinline__ void store(char* tile, int tid) {
 #pragma unroll
     for (int n = 0; n < N; ++n) TL::put(tile, tid / TL::NCH + n * STEP, tid % TL::NCH, operand(r[n]));
