@@ -86,6 +86,16 @@ def test_no_cpu_fallback():
         A.RelativePositionBias(2)(3, 3)
 
 
+def test_packed_structures_are_the_headers():
+    assert A._DESC.size == C.sizeof(_lib.AttentionDesc) and A._GRADS.size == C.sizeof(_lib.AttentionGrads)
+    i3 = _lib.I64x3
+    e = (C.c_int32 * 3)(1, 2, 3)
+    whole = _lib.AttentionDesc(1, 2, 3, 4, 5, 6, 7, 1, 8, 9, 1, 0.5, 11, 12, 13, i3(14, 15, 16), i3(17, 18, 19), i3(20, 21, 22), 23, 24, 25, 26, 27, e)
+    assert bytes(whole) == A._DESC.pack(1, 2, 3, 4, 5, 6, 7, 1, 8, 9, 1, 0.5, *range(11, 28), C.addressof(e))
+    grads = _lib.AttentionGrads(1, 2, 3, 4, 5, 6, 7, i3(8, 9, 10), i3(11, 12, 13), i3(14, 15, 16), i3(17, 18, 19), i3(20, 21, 22))
+    assert bytes(grads) == A._GRADS.pack(*range(1, 23))
+
+
 def desc(**kw):
     i3 = _lib.I64x3(0, 0, 0)
     d = _lib.AttentionDesc(dtype=0, batch=1, heads=2, kv_heads=2, q_len=4, k_len=4, head_dim=8, scale=1.0, q=16, k=16, v=16, q_stride=i3,

@@ -140,10 +140,11 @@ SYMBOLS = {
     "wrnn_bilstm_set_path": (_I, [_P, _I]),
     "wrnn_bigru_create": (_I, [_I, _I, C.POINTER(BiGruWeights), _I, C.POINTER(_P)]),
     "wrnn_bigru_destroy": (_I, [_P]),
-    "wrnn_attention_workspace_bytes": (C.c_size_t, [C.POINTER(AttentionDesc)]),
-    "wrnn_attention_forward": (_I, [C.POINTER(AttentionDesc), _P, I64x3, _P, _P, C.c_size_t, _P]),
-    "wrnn_attention_backward_workspace_bytes": (C.c_size_t, [C.POINTER(AttentionDesc)]),
-    "wrnn_attention_backward": (_I, [C.POINTER(AttentionDesc), C.POINTER(AttentionGrads), _P, C.c_size_t, _P]),
+    # (the two structures by address: wavernn_amd.attention passes them as bytes)
+    "wrnn_attention_workspace_bytes": (C.c_size_t, [_P]),
+    "wrnn_attention_forward": (_I, [_P, _P, I64x3, _P, _P, C.c_size_t, _P]),
+    "wrnn_attention_backward_workspace_bytes": (C.c_size_t, [_P]),
+    "wrnn_attention_backward": (_I, [_P, _P, _P, C.c_size_t, _P]),
     "wrnn_relative_bias_forward": (_I, [_P] + [_I] * 8 + [C.POINTER(C.c_int32), _P, _P]),
     "wrnn_relative_bias_workspace_bytes": (C.c_size_t, [_I] * 5),
     "wrnn_relative_bias_backward": (_I, [_P] + [_I] * 8 + [C.POINTER(C.c_int32), _P, _P, C.c_size_t, _P]),

@@ -14,6 +14,7 @@ from __future__ import annotations
 import ctypes as C
 import functools
 import math
+import struct
 from typing import Optional
 
 import torch
@@ -68,40 +69,70 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return nn.functional.pad(t, (0, pad)) if pad else t.contiguous() if not t.is_contiguous() else t.clone()
 
 
-def _strides(t: torch.Tensor):
-    return t.stride()[:3]
+@functools.lru_cache(maxsize=1024)
+def _dense(shape, stride):
+    """Strides of a dense tensor of that shape whose batch / head / position order in memory is the given strides': the projections
+    around attention then need no copy."""
+    order = sorted(range(3), key=lambda i: (-stride[i], i))
+    out, n = [0, 0, 0, 1], shape[3]
+    for i in reversed(order):
+        out[i] = n
+        n *= max(shape[i], 1)
+    return tuple(out)
 
 
 def _empty_like(t: torch.Tensor) -> torch.Tensor:
-    """Dense, its batch / head / position order in memory as t's: the projections around attention then need no copy."""
-    if t.is_contiguous():
-        return torch.empty_like(t)
-    s = t.stride()
-    order = sorted(range(3), key=lambda i: (-s[i], i)) + [3]
-    return torch.empty([t.shape[i] for i in order], dtype=t.dtype, device=t.device).permute([order.index(i) for i in range(4)])
+    return torch.empty_strided(t.shape, _dense(t.shape, t.stride()), dtype=t.dtype, device=t.device)
+
+
+# wrnn_attention_desc and wrnn_attention_grads as bytes: a call's time on the host is mostly the filling of these
+_DESC = struct.Struct("11i f 3P 9q P q 4P")
+_GRADS = struct.Struct("7P 15q")
+
+
+def _ptr(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 def _desc(q, k, v, table, key_mask, key_lens, q_start, causal, scale, max_distance, bidirectional):
     B, H, Tq, D = q.shape
-    edges = None
+    buckets, edges = 0, 0
     if table is not None:
-        edges = _edges(table.shape[0], max_distance, bidirectional)[1]
-    I3 = _lib.I64x3
-    return _lib.AttentionDesc(_DTYPES[q.dtype], B, H, k.shape[1], Tq, k.shape[2], D, causal, 0 if table is None else table.shape[0],
-                              max_distance, bidirectional, scale, q.data_ptr(), k.data_ptr(), v.data_ptr(), I3(*_strides(q)),
-                              I3(*_strides(k)), I3(*_strides(v)), None if key_mask is None else key_mask.data_ptr(),
-                              0 if key_mask is None else key_mask.stride(0), None if key_lens is None else key_lens.data_ptr(),
-                              None if q_start is None else q_start.data_ptr(), None if table is None else table.data_ptr(), edges)
+        buckets = table.shape[0]
+        edges = C.addressof(_edges(buckets, max_distance, bidirectional)[1])
+    return _DESC.pack(_DTYPES[q.dtype], B, H, k.shape[1], Tq, k.shape[2], D, causal, buckets, max_distance, bidirectional, scale, q.data_ptr(),
+                      k.data_ptr(), v.data_ptr(), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], _ptr(key_mask),
+                      0 if key_mask is None else key_mask.stride(0), _ptr(key_lens), _ptr(q_start), _ptr(table), edges)
+
+
+class _on:
+    """The tensor's device as the current one for a library call; nothing to do where it is already."""
+    __slots__ = ("guard",)
+
+    def __init__(self, device: torch.device):
+        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *e):
+        if self.guard is not None:
+            self.guard.__exit__(*e)
+
+
+def _space(size: int, device: torch.device) -> Optional[torch.Tensor]:
+    return torch.empty(size, dtype=torch.uint8, device=device) if size else None
 
 
 def _forward(desc, q, lse):
     lib = _lib.load()
     out = _empty_like(q)
-    size = lib.wrnn_attention_workspace_bytes(C.byref(desc))
-    space = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
-    _lib.check(lib.wrnn_attention_forward(C.byref(desc), out.data_ptr(), _lib.I64x3(*_strides(out)), None if lse is None else lse.data_ptr(),
-                                          None if space is None else space.data_ptr(), size,
-                                          torch.cuda.current_stream(q.device).cuda_stream), "wrnn_attention_forward")
+    size = lib.wrnn_attention_workspace_bytes(desc)
+    space = _space(size, q.device)
+    if lib.wrnn_attention_forward(desc, out.data_ptr(), _lib.I64x3(*out.stride()[:3]), _ptr(lse), _ptr(space), size,
+                                  torch.cuda.current_stream(q.device).cuda_stream):
+        _lib.check(1, "wrnn_attention_forward")
     return out
 
 
@@ -109,10 +140,11 @@ class _Attention(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, table, key_mask, key_lens, q_start, causal, scale, max_distance, bidirectional):
-        ctx.rule = (causal, scale, max_distance, bidirectional)
-        with torch.cuda.device(q.device):
+        with _on(q.device):
             lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device)
-            out = _forward(_desc(q, k, v, table, key_mask, key_lens, q_start, *ctx.rule), q, lse)
+            desc = _desc(q, k, v, table, key_mask, key_lens, q_start, causal, scale, max_distance, bidirectional)
+            out = _forward(desc, q, lse)
+        ctx.desc = desc      # addresses of the saved tensors, which live as long as the node
         ctx.save_for_backward(q, k, v, table, key_mask, key_lens, q_start, out, lse)
         ctx.mark_non_differentiable(lse)
         return out, lse
@@ -126,23 +158,21 @@ class _Attention(torch.autograd.Function):
         if not (B and H and Tq):
             return (torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v), torch.zeros_like(table) if want_table else None) + (None,) * 7
         lib = _lib.load()
-        want_keys = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
-        with torch.cuda.device(q.device):
+        with _on(q.device):
             dout = _rows(dout)
-            dq = _empty_like(q)
-            dk, dv = (_empty_like(k), _empty_like(v)) if want_keys else (None, None)
-            dtable = torch.empty_like(table) if want_table else None
-            desc = _desc(q, k, v, table, key_mask, key_lens, q_start, *ctx.rule)
-            I3 = _lib.I64x3
-            none = I3(0, 0, 0)
-            grads = _lib.AttentionGrads(out.data_ptr(), lse.data_ptr(), dout.data_ptr(), dq.data_ptr(), dk.data_ptr() if want_keys else None,
-                                        dv.data_ptr() if want_keys else None, dtable.data_ptr() if want_table else None,
-                                        I3(*_strides(out)), I3(*_strides(dout)), I3(*_strides(dq)),
-                                        I3(*_strides(dk)) if want_keys else none, I3(*_strides(dv)) if want_keys else none)
-            size = lib.wrnn_attention_backward_workspace_bytes(C.byref(desc))
-            space = torch.empty(size, dtype=torch.uint8, device=q.device)
-            _lib.check(lib.wrnn_attention_backward(C.byref(desc), C.byref(grads), space.data_ptr(), size,
-                                                   torch.cuda.current_stream(q.device).cuda_stream), "wrnn_attention_backward")
+            dq, dk, dv, dtable = _empty_like(q), None, None, None
+            if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
+                dk, dv = _empty_like(k), _empty_like(v)
+            if want_table:
+                dtable = torch.empty_like(table)
+            zero = (0, 0, 0)
+            grads = _GRADS.pack(out.data_ptr(), lse.data_ptr(), dout.data_ptr(), dq.data_ptr(), _ptr(dk), _ptr(dv), _ptr(dtable), *out.stride()[:3],
+                                *dout.stride()[:3], *dq.stride()[:3], *(zero if dk is None else dk.stride()[:3]),
+                                *(zero if dv is None else dv.stride()[:3]))
+            size = lib.wrnn_attention_backward_workspace_bytes(ctx.desc)
+            space = _space(size, q.device)
+            if lib.wrnn_attention_backward(ctx.desc, grads, space.data_ptr(), size, torch.cuda.current_stream(q.device).cuda_stream):
+                _lib.check(1, "wrnn_attention_backward")
         return (dq, dk, dv, dtable) + (None,) * 7
 
 
@@ -209,7 +239,7 @@ def _run(q, k, v, bias_table, key_mask, key_lens, q_start, causal, scale, max_di
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
                                     or (bias_table is not None and bias_table.requires_grad)):
         return _Attention.apply(q, k, v, bias_table, key_mask, key_lens, q_start, causal, scale, max_distance, bidirectional)
-    with torch.cuda.device(q.device):
+    with _on(q.device):
         lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) if want_lse else None
         out = _forward(_desc(q, k, v, bias_table, key_mask, key_lens, q_start, causal, scale, max_distance, bidirectional), q, lse)
     return out, lse
@@ -221,7 +251,7 @@ class _RelativeBias(torch.autograd.Function):
     def forward(ctx, table, q_len, k_len, start, max_distance, bidirectional):
         ctx.rule = (table.shape[1], q_len, k_len, start, table.shape[0], max_distance, bidirectional)
         lib = _lib.load()
-        with torch.cuda.device(table.device):
+        with _on(table.device):
             out = torch.empty(table.shape[1], q_len, k_len, dtype=table.dtype, device=table.device)
             _lib.check(lib.wrnn_relative_bias_forward(table.data_ptr(), _DTYPES[table.dtype], *ctx.rule, _edges(table.shape[0], max_distance, bidirectional)[1],
                                                       out.data_ptr(), torch.cuda.current_stream(table.device).cuda_stream),
@@ -235,7 +265,7 @@ class _RelativeBias(torch.autograd.Function):
         if not (H and q_len and k_len):
             return (dout.new_zeros(buckets, H),) + (None,) * 5
         lib = _lib.load()
-        with torch.cuda.device(dout.device):
+        with _on(dout.device):
             dout = dout.contiguous()
             dtable = torch.empty(buckets, H, dtype=dout.dtype, device=dout.device)
             size = lib.wrnn_relative_bias_workspace_bytes(H, q_len, k_len, buckets, max_distance)
