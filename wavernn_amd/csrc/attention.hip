@@ -28,7 +28,7 @@ static int lut_floats(const Params& p) { return p.table ? 2 * p.max_distance + 1
 static int shares(int64_t blocks, int64_t tiles, int least) {
   const int64_t want = kComputeUnits / (blocks > 0 ? blocks : 1), most = tiles / least;
   const int64_t n = want < most ? want : most;
-  return (int)(n < 1 ? 1 : n > 256 ? 256 : n);
+  return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
 }
 
 // How a call runs.  The wide shape shares each key tile among four waves; the narrow one is for few queries, which would leave three of
@@ -50,7 +50,9 @@ static size_t split_workspace(const Params& p) {
 static void plan_backward(Params* p) {
   const int parts = p->D > 128 ? 2 : 1;
   p->dq_splits = shares((int64_t)p->B * p->H * ((p->Tq + 127) / 128) * parts, (p->Tk + 31) / 32, 4);
-  p->dkv_splits = shares((int64_t)p->B * p->Hkv * ((p->Tk + 127) / 128) * parts, (int64_t)((p->Tq + 31) / 32) * p->group, 4);
+  // (causality: the first keys' blocks are the longest by far; half as long they leave the others time to fill up)
+  const int64_t blocks = (int64_t)p->B * p->Hkv * ((p->Tk + 127) / 128) * parts;
+  p->dkv_splits = shares(p->causal ? (blocks + 1) / 2 : blocks, (int64_t)((p->Tq + 31) / 32) * p->group, 4);
 }
 static size_t aligned(size_t x) { return (x + 255) & ~size_t(255); }
 // the backward workspace: delta, the table's partial sums, the shares

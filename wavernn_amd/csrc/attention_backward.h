@@ -118,14 +118,11 @@ __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_
   float* scratch = lut + lut_pad;                 // [4][32 * LD]
   float* sums = scratch + 4 * 32 * BiasGrad::LD;  // [4][lut_pad]
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int nt = (p.Tq + 127) / 128, n = p.B * p.H * nt * S::PARTS * p.dq_splits;
-  int item = xcd_item(n);
-  if (item >= n) return;
-  const int share = item % p.dq_splits;
-  item /= p.dq_splits;
-  const int d0 = (item % S::PARTS) * S::DA;
-  item /= S::PARTS;
-  const int bh = item / nt, b = bh / p.H, h = bh - b * p.H, qt = p.causal ? nt - 1 - item % nt : item % nt;
+  const int nt = (p.Tq + 127) / 128;
+  const Item item(p.B * p.H, nt, S::PARTS * p.dq_splits, p.causal);
+  if (item.share < 0) return;
+  const int share = item.share / S::PARTS, d0 = (item.share % S::PARTS) * S::DA;
+  const int bh = item.head, b = bh / p.H, h = bh - b * p.H, qt = p.causal ? nt - 1 - item.tile : item.tile;
   const int q0 = qt * 128 + 32 * wave;
   const int off = start_of(p, b), kvh = h / p.group;
   const T* kb = reinterpret_cast<const T*>(p.k) + b * p.k_b + kvh * p.k_h;
@@ -276,14 +273,11 @@ __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_
   float* stat = reinterpret_cast<float*>(smem + S::TILES);  // [BUFS][2][BM]: lse in log2 units, delta
   float* lut = stat + BUFS * 2 * BM;
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int nt = (p.Tk + 127) / 128, n = p.B * p.Hkv * nt * S::PARTS * p.dkv_splits;
-  int item = xcd_item(n);
-  if (item >= n) return;
-  const int share = item % p.dkv_splits;
-  item /= p.dkv_splits;
-  const int d0 = (item % S::PARTS) * S::DA;
-  item /= S::PARTS;
-  const int bh = item / nt, b = bh / p.Hkv, kvh = bh - b * p.Hkv, k0 = (item % nt) * 128, kw = k0 + 32 * wave;
+  const int nt = (p.Tk + 127) / 128;
+  const Item item(p.B * p.Hkv, nt, S::PARTS * p.dkv_splits, p.causal);
+  if (item.share < 0) return;
+  const int share = item.share / S::PARTS, d0 = (item.share % S::PARTS) * S::DA;
+  const int bh = item.head, b = bh / p.Hkv, kvh = bh - b * p.Hkv, k0 = item.tile * 128, kw = k0 + 32 * wave;
   const int off = start_of(p, b), key = kw + col, kc = min(key, p.Tk - 1);
   const uint8_t* mask = p.key_mask ? p.key_mask + b * p.mask_b : nullptr;
   int end = p.Tk;

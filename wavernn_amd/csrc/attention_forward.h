@@ -71,13 +71,11 @@ __global__ __launch_bounds__((ForwardShape<T, DP, WIDE>::THREADS), (ForwardShape
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wq = WIDE ? wave : 0, wk = WIDE ? 0 : wave;
   const bool pack = !WIDE && p.pack;
   const int heads = pack ? p.Hkv : p.H, splits = p.splits;
-  const int nt = pack ? 1 : (p.Tq + 32 * S::WQ - 1) / (32 * S::WQ), n = p.B * heads * nt * splits;
-  int item = xcd_item(n);
-  if (item >= n) return;
-  const int part = item % splits;
-  item /= splits;
-  const int bh = item / nt, b = bh / heads, hh = bh - b * heads;
-  const int q0 = (p.causal ? nt - 1 - item % nt : item % nt) * 32 * S::WQ + 32 * wq;  // under causality the long rows start first
+  const int nt = pack ? 1 : (p.Tq + 32 * S::WQ - 1) / (32 * S::WQ);
+  const Item item(p.B * heads, nt, splits, p.causal);
+  if (item.share < 0) return;
+  const int part = item.share, bh = item.head, b = bh / heads, hh = bh - b * heads;
+  const int q0 = (p.causal ? nt - 1 - item.tile : item.tile) * 32 * S::WQ + 32 * wq;  // under causality the last queries have the longest rows
   const int lh = pack ? col / p.Tq : 0;                                              // the column's head within the group
   const int h = pack ? hh * p.group + min(lh, p.group - 1) : hh, kvh = pack ? hh : hh / p.group;
   const int qi = pack ? col - lh * p.Tq : q0 + col;
@@ -270,30 +268,36 @@ __global__ __launch_bounds__((ForwardShape<T, DP, WIDE>::THREADS), (ForwardShape
   }
 }
 
-// Joins the splits of a query: one wave per query, splits in their order.
+// Joins the splits of a query: one wave per query.  Lane s weighs split s, then the lanes take the columns, splits in their order.
 template <class T, int DP>
 __global__ __launch_bounds__(256) void attention_join_kernel(Params p) {
   const int lane = threadIdx.x & 63;
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (row >= (int64_t)p.B * p.H * p.Tq) return;
   const float* part = p.part + row * p.splits * (DP + 4);
-  float m = -3e38f, l = 0.f;
-  for (int s = 0; s < p.splits; ++s) m = fmaxf(m, part[s * (DP + 4)]);
-  constexpr int E = DP / 64;
-  float x[E] = {};
-  for (int s = 0; s < p.splits; ++s) {
-    const float* ps = part + s * (DP + 4);
-    const float a = exp2f(ps[0] - m);
-    l += ps[1] * a;
-#pragma unroll
-    for (int e = 0; e < E; ++e) x[e] += ps[4 + e * 64 + lane] * a;
+  float ms = -3e38f, ls = 0.f;
+  if (lane < p.splits) {
+    ms = part[lane * (DP + 4)];
+    ls = part[lane * (DP + 4) + 1];
   }
+  float m = ms;
+#pragma unroll
+  for (int i = 1; i < 64; i <<= 1) m = fmaxf(m, __shfl_xor(m, i));
+  const float w = exp2f(ms - m);
+  float l = ls * w;
+#pragma unroll
+  for (int i = 1; i < 64; i <<= 1) l += __shfl_xor(l, i);
+  constexpr int E = DP / 64;
+  typedef float vec __attribute__((ext_vector_type(E)));
+  vec x = vec(0.f);
+#pragma unroll 8
+  for (int s = 0; s < p.splits; ++s) x += *reinterpret_cast<const vec*>(part + s * (DP + 4) + 4 + lane * E) * __shfl(w, s);
   const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
   const int qi = row % p.Tq, h = (row / p.Tq) % p.H, b = row / p.Tq / p.H;
   T* orow = reinterpret_cast<T*>(p.out) + b * p.o_b + h * p.o_h + qi * p.o_t;
 #pragma unroll
   for (int e = 0; e < E; ++e)
-    if (e * 64 + lane < p.D) orow[e * 64 + lane] = (T)(x[e] * inv);
+    if (lane * E + e < p.D) orow[lane * E + e] = (T)(x[e] * inv);
   if (lane == 0 && p.lse) p.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 

@@ -538,12 +538,27 @@ __device__ __forceinline__ float bucket_sum(const Params& p, const float* sums, 
   return x;
 }
 
-// Work item of a workgroup: consecutive items go to one XCD (workgroups are dealt to the eight XCDs in turn), so that the tiles of
-// one head share an L2.  Launch 8 * ceil(n / 8) workgroups; a result >= n has nothing to do.
-__device__ __forceinline__ int xcd_item(int n) {
-  const int per = (n + 7) >> 3;
-  return (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
-}
+// What a workgroup works on: one of `inner` shares of a tile of a head.  Consecutive items go to one XCD (workgroups are dealt to the eight XCDs in
+// turn), so that the tiles of one head share an L2.  Tiles come in the order 0, 1, ..; with `sorted`, where they get shorter in that order
+// (causality), an XCD takes tile 0 of all its heads first, then tile 1: the long ones start first and the short ones fill the gaps.
+// Launch 8 * ceil(heads * tiles * inner / 8) workgroups.
+struct Item {
+  int head, tile, share;  // share < 0: nothing to do
+  __device__ __forceinline__ Item(int heads, int tiles, int inner, bool sorted) {
+    const int x = blockIdx.x & 7, l = blockIdx.x >> 3, n = heads * tiles * inner;
+    if (sorted && (heads & 7) == 0) {
+      const int per = heads >> 3, u = l / inner;
+      share = l - u * inner;
+      tile = u / per;
+      head = x * per + u - tile * per;
+    } else {
+      const int per = (n + 7) >> 3, i = x * per + l, u = i / inner;
+      share = l < per && i < n ? i - u * inner : -1;
+      head = u / tiles;
+      tile = u - head * tiles;
+    }
+  }
+};
 
 // One past the last key that some query of row b in [.., last_pos] may use, over lengths, causality and the key mask (a workgroup
 // scans the mask's tail once).  `word` is one int of LDS.  All threads of the workgroup call it.
