@@ -290,8 +290,13 @@ __global__ __launch_bounds__(256) void attention_join_kernel(Params p) {
   constexpr int E = DP / 64;
   typedef float vec __attribute__((ext_vector_type(E)));
   vec x = vec(0.f);
-#pragma unroll 8
-  for (int s = 0; s < p.splits; ++s) x += *reinterpret_cast<const vec*>(part + s * (DP + 4) + 4 + lane * E) * __shfl(w, s);
+  for (int s0 = 0; s0 < p.splits; s0 += 8) {  // eight loads in flight; past the last split its own again, weighed zero
+    vec y[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) y[u] = *reinterpret_cast<const vec*>(part + min(s0 + u, p.splits - 1) * (DP + 4) + 4 + lane * E);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) x += y[u] * (s0 + u < p.splits ? __shfl(w, s0 + u) : 0.f);
+  }
   const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
   const int qi = row % p.Tq, h = (row / p.Tq) % p.H, b = row / p.Tq / p.H;
   T* orow = reinterpret_cast<T*>(p.out) + b * p.o_b + h * p.o_h + qi * p.o_t;

@@ -47,50 +47,65 @@ __global__ __launch_bounds__(256) void relative_bias_kernel(Params p, DenseBias 
   }
 }
 
-// Sum of row[lo .. hi) by the wave's lanes: 16 bytes a load where the row allows it.
-template <class T>
-__device__ __forceinline__ float segment_sum(const T* row, int lo, int hi, int lane) {
-  constexpr int V = 16 / sizeof(T);
-  typedef T vec __attribute__((ext_vector_type(V)));
-  if (hi <= lo) return 0.f;
-  const T* s = row + lo;
-  const int n = hi - lo, head = min((int)((16 - (reinterpret_cast<uintptr_t>(s) & 15)) & 15) / (int)sizeof(T), n), full = (n - head) / V;
-  float x[V] = {};
-#pragma unroll 4
-  for (int c = lane; c < full; c += 64) {
-    const vec v = *reinterpret_cast<const vec*>(s + head + c * V);
-#pragma unroll
-    for (int e = 0; e < V; ++e) x[e] += (float)v[e];
-  }
-  float y = lane < head ? (float)s[lane] : 0.f;
-  const int tail = head + full * V + lane;
-  if (lane < V && tail < n) y += (float)s[tail];
-#pragma unroll
-  for (int e = 0; e < V; ++e) y += x[e];
-  return y;
-}
-
-// A workgroup's rows -> one partial sum per bucket.  Near the diagonal a thread owns a distance and walks the rows; further out a wave sums
-// the two ends of a row.
+// A workgroup's rows -> one partial sum per bucket.  Near the diagonal a thread owns a distance and walks the rows; what lies further out a wave
+// reads row by row, four rows at a time to have enough loads in flight, 16 bytes a load from each row's first aligned element on (the
+// vectors that lie wholly near the diagonal are left to the walk).
 template <class T>
 __global__ __launch_bounds__(256) void relative_bias_grad_kernel(Params p, DenseBias a) {
+  constexpr int V = 16 / sizeof(T), R = 4;
+  typedef T vec __attribute__((ext_vector_type(V)));
   extern __shared__ __attribute__((aligned(16))) char smem[];
   float* sums = reinterpret_cast<float*>(smem);  // [2 * max_distance + 1]
   float* ends = sums + 2 * p.max_distance + 1;   // [4][2]
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, md = p.max_distance;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), md = p.max_distance;
   const int chunks = (p.Tq + a.rows - 1) / a.rows, h = blockIdx.x / chunks, i0 = (blockIdx.x - h * chunks) * a.rows,
             i1 = min(i0 + a.rows, p.Tq);
   const T* base = reinterpret_cast<const T*>(a.in) + (int64_t)h * p.Tq * p.Tk;
-  float below = 0.f, above = 0.f;
-  for (int i = i0 + wave; i < i1; i += 4) {
-    const T* row = base + (int64_t)i * p.Tk;
-    const int pos = i + a.start;
-    below += segment_sum(row, 0, min(max(pos - md + 1, 0), p.Tk), lane);
-    above += segment_sum(row, min(max(pos + md, 0), p.Tk), p.Tk, lane);
+  float below[R] = {}, above[R] = {};
+  for (int i = i0 + wave * R; i < i1; i += 4 * R) {
+    const T* row[R];
+    int head[R], full[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      row[r] = base + (int64_t)min(i + r, i1 - 1) * p.Tk;
+      head[r] = min((int)((16 - (reinterpret_cast<uintptr_t>(row[r]) & 15)) & 15) / (int)sizeof(T), p.Tk);
+      full[r] = i + r < i1 ? (p.Tk - head[r]) / V : 0;
+    }
+    auto put = [&](int r, int rel, float x) {
+      below[r] += rel <= -md ? x : 0.f;
+      above[r] += rel >= md ? x : 0.f;
+    };
+    const int most = (p.Tk + V - 1) / V;
+#pragma unroll 2
+    for (int c = lane; c < most; c += 64) {
+      vec v[R];
+      int rel[R];
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const int j = head[r] + c * V;
+        rel[r] = j - (i + r + a.start);
+        v[r] = vec(T(0));
+        if (c < full[r] && !(rel[r] > -md && rel[r] + V - 1 < md)) v[r] = *reinterpret_cast<const vec*>(row[r] + j);
+      }
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int e = 0; e < V; ++e) put(r, rel[r] + e, (float)v[r][e]);
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if (i + r >= i1) break;
+      const int pos = i + r + a.start, tail = head[r] + full[r] * V + lane;
+      if (lane < head[r]) put(r, lane - pos, (float)row[r][lane]);
+      if (lane < V && tail < p.Tk) put(r, tail - pos, (float)row[r][tail]);
+    }
   }
+  float lo = below[0], hi = above[0];
+#pragma unroll
+  for (int r = 1; r < R; ++r) lo += below[r], hi += above[r];
   for (int r = 1 - md + tid; r < md; r += 256) {
     float x = 0.f;
-#pragma unroll 8
+#pragma unroll 16
     for (int i = i0; i < i1; ++i) {
       const int j = i + a.start + r;
       if (j >= 0 && j < p.Tk) x += (float)base[(int64_t)i * p.Tk + j];
@@ -98,12 +113,12 @@ __global__ __launch_bounds__(256) void relative_bias_grad_kernel(Params p, Dense
     sums[r + md] = x;
   }
   for (int m = 1; m < 64; m <<= 1) {
-    below += __shfl_xor(below, m);
-    above += __shfl_xor(above, m);
+    lo += __shfl_xor(lo, m);
+    hi += __shfl_xor(hi, m);
   }
   if (lane == 0) {
-    ends[2 * wave] = below;
-    ends[2 * wave + 1] = above;
+    ends[2 * wave] = lo;
+    ends[2 * wave + 1] = hi;
   }
   __syncthreads();
   if (tid < 2) sums[tid * 2 * md] = ends[tid] + ends[2 + tid] + ends[4 + tid] + ends[6 + tid];
