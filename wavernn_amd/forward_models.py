@@ -9,7 +9,12 @@ Same constructors, state_dict keys (so reference checkpoints load), ``forward(ba
 signatures.  The transformer blocks, predictors and projections are per-utterance work on stock PyTorch-ROCm
 ops, written here from the reference's behaviour (models/common_layers.py:127-240); the expand runs in
 libwrnn_mi355.so (``LengthRegulator``), and so do the frame-recurrent ``lstm`` of the multispeaker
-ForwardTacotron (``BiLSTM``) and every CBHG / predictor GRU (``BiGRU``).  Forward/inference only.
+ForwardTacotron (``BiLSTM``) and every CBHG / predictor GRU (``BiGRU``).  Those are forward/inference only; the transformer blocks
+can be trained.
+
+The blocks' self-attention runs on ``nn.MultiheadAttention`` ('stock', the default) or in libwrnn_mi355.so, forward and backward
+(``set_attention_path``).  Build extension, not in the reference: ``rel_buckets`` > 0 gives each transformer a learned relative
+position bias (``RelativePositionBias``, shared by its layers), on either path.
 
 Reference quirks kept on purpose: the multispeaker ForwardTacotron builds its predictors with their default
 ``speaker_emb_dims=256`` whatever the model's own value is (multi_forward_tacotron.py:135-157); both multispeaker
@@ -25,6 +30,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 from torch.nn.utils.rnn import pack_padded_sequence, pad_packed_sequence
 
+from .attention import MAX_HEAD_DIM, RelativePositionBias, attention
 from .bigru import BiGRU
 from .bilstm import BiLSTM
 from .length_regulator import LengthRegulator
@@ -49,6 +55,9 @@ class PositionalEncoding(nn.Module):  # common_layers.py:127-145
         return self.dropout(x + self.scale * self.pe[:x.size(0)])
 
 
+ATTENTION_PATHS = ('stock', 'fused', 'auto')
+
+
 class FFTBlock(nn.Module):  # common_layers.py:148-185: post-norm self-attention, then a two-conv feed-forward over time
     def __init__(self, d_model: int, nhead: int, conv1_kernel: int, conv2_kernel: int, d_fft: int, dropout: float = 0.1):
         super().__init__()
@@ -59,29 +68,79 @@ class FFTBlock(nn.Module):  # common_layers.py:148-185: post-norm self-attention
         self.norm1, self.norm2 = nn.LayerNorm(d_model), nn.LayerNorm(d_model)
         self.dropout1, self.dropout2 = nn.Dropout(dropout), nn.Dropout(dropout)
         self.activation = nn.ReLU()
+        self.attention_path = 'stock'
 
-    def forward(self, src, src_pad_mask=None):                   # [T, N, d_model]
-        att = self.self_attn(src, src, src, attn_mask=None, key_padding_mask=src_pad_mask)[0]
+    def _why_not_fused(self, src) -> Optional[str]:
+        if src.device.type != 'cuda':
+            return "it runs only on an MI355X (HIP) device"
+        if self.training and self.self_attn.dropout > 0:
+            return "it has no dropout on the probabilities (train with dropout=0, or on the stock path)"
+        if self.self_attn.head_dim > MAX_HEAD_DIM:
+            return f"head dimension {self.self_attn.head_dim} is over {MAX_HEAD_DIM}"
+        return None
+
+    def _attend(self, src, src_pad_mask, position_bias):
+        why = self._why_not_fused(src) if self.attention_path != 'stock' else ''
+        if why and self.attention_path == 'fused':
+            raise RuntimeError(f"FFTBlock: the fused attention path does not apply: {why}")
+        if why is not None:
+            bias = None
+            if position_bias is not None:
+                bias = position_bias(src.size(0), src.size(0)).to(src.dtype)     # [H, T, T], for every row of the batch
+                bias = bias.expand(src.size(1), -1, -1, -1).reshape(-1, *bias.shape[1:])
+                if src_pad_mask is not None:
+                    src_pad_mask = torch.zeros_like(src_pad_mask, dtype=src.dtype).masked_fill(src_pad_mask, -math.inf)
+            return self.self_attn(src, src, src, attn_mask=bias, key_padding_mask=src_pad_mask)[0]
+        # the packed projection's q, k, v as views [N, H, T, head_dim]; the result lies in memory as [T, N, d_model]
+        a = self.self_attn
+        T, N, E = src.shape
+        q, k, v = F.linear(src, a.in_proj_weight, a.in_proj_bias).view(T, N, 3, a.num_heads, a.head_dim).permute(2, 1, 3, 0, 4).unbind(0)
+        rule = {} if position_bias is None else dict(bias_table=position_bias.weight, max_distance=position_bias.max_distance,
+                                                     bidirectional=position_bias.bidirectional)
+        y = attention(q, k, v, key_mask=src_pad_mask, **rule)
+        return F.linear(y.permute(2, 0, 1, 3).reshape(T, N, E), a.out_proj.weight, a.out_proj.bias)
+
+    def forward(self, src, src_pad_mask=None, position_bias=None):  # [T, N, d_model]
+        att = self._attend(src, src_pad_mask, position_bias)
         src = self.norm1(src + self.dropout1(att))
         y = src.permute(1, 2, 0)                                 # [N, d_model, T] for the convs
         y = self.conv2(self.activation(self.conv1(y))).permute(2, 0, 1)
         return self.norm2(src + self.dropout2(y))
 
 
+def set_attention_path(module: nn.Module, path: str) -> nn.Module:
+    """How every FFTBlock under ``module`` runs its self-attention (no counterpart in the reference):
+    'stock'  nn.MultiheadAttention (the default);
+    'fused'  wavernn_amd.attention, forward and backward: the scores never reach memory; an error where it does not apply (training with
+             dropout > 0, which it has none of; head dimensions over 256);
+    'auto'   'fused' where it applies, 'stock' elsewhere.
+    They agree to rounding, but for batch rows whose every position is masked: 'stock' gives NaN there, 'fused' attends to nothing."""
+    if path not in ATTENTION_PATHS:
+        raise ValueError(f"attention path must be one of {ATTENTION_PATHS}, got {path!r}")
+    for m in module.modules():
+        if isinstance(m, FFTBlock):
+            m.attention_path = path
+    return module
+
+
 class ForwardTransformer(nn.Module):  # common_layers.py:188-223
     def __init__(self, d_model: int, d_fft: int, layers: int, heads: int, conv1_kernel: int, conv2_kernel: int,
-                 dropout: float = 0.1) -> None:
+                 dropout: float = 0.1, rel_buckets: int = 0, rel_max_distance: int = 128) -> None:
         super().__init__()
         self.d_model = d_model
         self.pos_encoder = PositionalEncoding(d_model, dropout)
         self.layers = nn.ModuleList(FFTBlock(d_model=d_model, nhead=heads, d_fft=d_fft, conv1_kernel=conv1_kernel,
                                              conv2_kernel=conv2_kernel, dropout=dropout) for _ in range(layers))
         self.norm = nn.LayerNorm(d_model)
+        self.position_bias = RelativePositionBias(heads, rel_buckets, rel_max_distance) if rel_buckets else None
+
+    def set_attention_path(self, path: str) -> 'ForwardTransformer':
+        return set_attention_path(self, path)
 
     def forward(self, x, src_pad_mask=None):                     # [N, T, d_model]
         x = self.pos_encoder(x.transpose(0, 1))
         for layer in self.layers:
-            x = layer(x, src_pad_mask=src_pad_mask)
+            x = layer(x, src_pad_mask=src_pad_mask, position_bias=self.position_bias)
         return self.norm(x).transpose(0, 1)
 
 
@@ -111,14 +170,15 @@ class TransformerPredictor(nn.Module):
     categorical condition): embedding [++ condition embedding ++ speaker embedding] -> transformer -> linear."""
 
     def __init__(self, num_chars, d_model, n_heads, d_fft, layers, conv1_kernel, conv2_kernel, dropout=0.1,
-                 speaker_emb_dims=0, cond_emb_size=0, cond_emb_dims=0, out_dim=1):
+                 speaker_emb_dims=0, cond_emb_size=0, cond_emb_dims=0, out_dim=1, rel_buckets=0, rel_max_distance=128):
         super().__init__()
         self.embedding = nn.Embedding(num_chars, d_model)
         if cond_emb_size:
             self.conditional_embedding = nn.Embedding(cond_emb_size, cond_emb_dims)
         width = d_model + speaker_emb_dims + (cond_emb_dims if cond_emb_size else 0)
         self.transformer = ForwardTransformer(heads=n_heads, dropout=dropout, d_model=width, d_fft=d_fft,
-                                              conv1_kernel=conv1_kernel, conv2_kernel=conv2_kernel, layers=layers)
+                                              conv1_kernel=conv1_kernel, conv2_kernel=conv2_kernel, layers=layers,
+                                              rel_buckets=rel_buckets, rel_max_distance=rel_max_distance)
         self.lin = nn.Linear(width, out_dim)
         self._cond, self._spk = bool(cond_emb_size), speaker_emb_dims > 0
 
@@ -170,11 +230,12 @@ class FastPitch(nn.Module):
                  energy_layers: int, energy_d_fft: int, pitch_strength: float, energy_strength: float, d_model: int,
                  conv1_kernel: int, conv2_kernel: int, prenet_layers: int, prenet_heads: int, prenet_fft: int,
                  prenet_dropout: float, postnet_layers: int, postnet_heads: int, postnet_fft: int,
-                 postnet_dropout: float, n_mels: int, padding_value=-11.5129):
+                 postnet_dropout: float, n_mels: int, padding_value=-11.5129, rel_buckets: int = 0,
+                 rel_max_distance: int = 128):
         super().__init__()
         self.padding_value = padding_value
         self.lr = LengthRegulator()
-        kern = dict(conv1_kernel=conv1_kernel, conv2_kernel=conv2_kernel)
+        kern = dict(conv1_kernel=conv1_kernel, conv2_kernel=conv2_kernel, rel_buckets=rel_buckets, rel_max_distance=rel_max_distance)
         self.dur_pred = TransformerPredictor(num_chars, durpred_d_model, durpred_n_heads, durpred_d_fft, durpred_layers,
                                              dropout=durpred_dropout, **kern)
         self.pitch_pred = TransformerPredictor(num_chars, pitch_d_model, pitch_n_heads, pitch_d_fft, pitch_layers,
@@ -232,6 +293,9 @@ class FastPitch(nn.Module):
 
     def pad(self, x: torch.Tensor, max_len: int) -> torch.Tensor:
         return pad_frames(x, max_len, self.padding_value)
+
+    def set_attention_path(self, path: str) -> 'FastPitch':
+        return set_attention_path(self, path)
 
     def get_step(self) -> int:
         return self.step.data.item()
