@@ -56,9 +56,9 @@ static void plan_backward(Params* p) {
 }
 static size_t aligned(size_t x) { return (x + 255) & ~size_t(255); }
 // the backward workspace: delta, the table's partial sums, the shares
-static size_t delta_bytes(const Params& p) { return aligned((size_t)p.B * p.H * p.Tq * sizeof(float)); }
+static size_t delta_bytes(const Params& p) { return aligned((size_t)(p.table ? p.dq_splits : 1) * p.B * p.H * p.Tq * sizeof(float)); }
 static size_t table_bytes(const Params& p) {
-  return p.table ? aligned((size_t)p.B * ((p.Tq + 127) / 128) * p.dq_splits * p.H * p.buckets * sizeof(float)) : 0;
+  return p.table ? aligned((size_t)p.B * ((p.Tk + 127) / 128) * p.dkv_splits * p.H * p.buckets * sizeof(float)) : 0;
 }
 static size_t dq_bytes(const Params& p) { return p.dq_splits > 1 ? aligned((size_t)p.dq_splits * p.B * p.H * p.Tq * p.D * sizeof(float)) : 0; }
 static size_t dkv_bytes(const Params& p) { return p.dkv_splits > 1 ? (size_t)p.dkv_splits * 2 * p.B * p.Hkv * p.Tk * p.D * sizeof(float) : 0; }

@@ -11,12 +11,19 @@
 namespace wrnn {
 namespace attn {
 
-// rel = key - position for the 63 diagonals of a 32 x 32 tile: sums dS over each (one lane a diagonal) and adds them to `sums`.
-// Distances at or past max_distance share a bucket with everything further and go to the lane's two registers.
+// The position table's share of a 32 x 32 tile of dS (column: key, the lane's 16 rows: queries), added to the wave's `sums` by distance.  The
+// tile goes through LDS 16 keys at a time, skewed: a row of `skew` is a diagonal, its 16 words the keys; words off the tile stay zero, so one
+// lane adds one diagonal up in wide reads without a condition.  (Adding each element to `sums` by an LDS add took twice as long as everything else
+// of the kernel.)  Distances past max_distance share its bucket: whole tiles of them go to the lane's two registers, the others' to PAD words beside
+// the table, which the end folds in.
 struct BiasGrad {
-  static constexpr int LD = 36;  // floats: keeps the four-word writes aligned, neighbouring lanes of a diagonal read stay apart
+  static constexpr int PAD = 64;  // a tile that reaches past max_distance does so by at most 62
+  static constexpr int LD = 20, SKEW = 48 * LD;  // 47 diagonals of 16 keys, and one that stays zero
   float below = 0.f, above = 0.f;
-  __device__ __forceinline__ void add(const float (&ds)[16], int rel0 /* key0 - pos0 */, int md, float* scratch, float* sums, int lane) {
+  static __host__ __device__ int words(int md) { return (2 * md + 1 + 2 * PAD + 3) & ~3; }
+  static __host__ __device__ int all_words(int md) { return 4 * (words(md) + SKEW); }  // of a workgroup, `skew` first
+  // rel0: first key - position of the first query
+  __device__ __forceinline__ void add(const float (&ds)[16], int rel0, int md, float* skew, float* sums, int lane) {
     const int half = lane >> 5, col = lane & 31;
     if (rel0 + 31 <= -md || rel0 - 31 >= md) {
       float x = 0.f;
@@ -26,26 +33,38 @@ struct BiasGrad {
       else above += x;
       return;
     }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
+    float* to = skew + (15 - (col & 15) + 4 * half) * LD + (col & 15);
+    f32x4 x[8];
 #pragma unroll
-    for (int g = 0; g < 4; ++g)
-      *reinterpret_cast<f32x4*>(scratch + col * LD + 8 * g + 4 * half) = f32x4{ds[4 * g], ds[4 * g + 1], ds[4 * g + 2], ds[4 * g + 3]};
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    float x = 0.f;
-    const int d = lane - 31;  // key - query within the tile; lane 63 has none
+    for (int n = 0; n < 2; ++n) {  // keys 16 n ..; a wave's LDS instructions keep their order
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      if (col >> 4 == n)
 #pragma unroll
-    for (int qq = 0; qq < 32; ++qq) {
-      const int kk = d + qq;
-      const float v = scratch[qq * LD + (kk & 31)];
-      x += (kk >= 0 && kk < 32) ? v : 0.f;
+        for (int i = 0; i < 16; ++i) to[moving_row(i, 0) * LD] = ds[i];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      const int d = n ? lane : lane - 16;  // of distance rel0 + 31 - lane
+      const f32x4* row = reinterpret_cast<const f32x4*>(skew + (d >= 0 && d < 47 ? d : 47) * LD);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) x[4 * n + c] = row[c];
     }
-    if (lane == 63) return;
-    const int rel = rel0 + d;
-    if (rel <= -md) below += x;
-    else if (rel >= md) above += x;
-    else sums[rel + md] += x;
+    const f32x4 y = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+    if (lane < 63) sums[PAD + md + rel0 + 31 - lane] += (y[0] + y[1]) + (y[2] + y[3]);
+  }
+  // the wave's sums at distances -md .. md, from sums[PAD] on
+  __device__ __forceinline__ void fold(int md, float* sums, int lane) {
+    below += sums[lane];
+    above += sums[PAD + 2 * md + 1 + lane];
+    for (int m = 1; m < 64; m <<= 1) {
+      below += __shfl_xor(below, m);
+      above += __shfl_xor(above, m);
+    }
+    if (lane == 0) {
+      sums[PAD] += below;
+      sums[PAD + 2 * md] += above;
+    }
+    below = above = 0.f;
   }
 };
 
@@ -98,25 +117,20 @@ __device__ __forceinline__ void products_shadow(const char* x, const char* y, co
   }
 }
 
-// dq (and with BIAS == 2 the table's gradient): queries stationary, key tiles through LDS.
-//
-// delta = rowsum(dout * out) serves a softmax gradient well as long as out is exact; in bfloat16 it carries out's rounding, and a bucket that
-// holds most of a row's keys adds that error up over all rows.  There the table's gradient takes delta = sum_j P dP from a first walk over the
-// keys instead.
+// dq: queries stationary, key tiles through LDS.  delta = rowsum(dout * out) carries the rounding of out and of the probabilities behind it.  That is
+// less than the rounding of dq itself, but the table's gradient adds it up over all rows in the buckets that hold most of a row's keys.
+// With BIAS == 2 the kernel therefore also sums dS over each row - what delta is off by, as the probabilities add up to one - and hands the
+// corrected delta to the next kernel, which makes the table's gradient: the adds are hidden, a second walk over the keys for it took twice the time.
 template <class T, int DP, int BIAS>
 __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_dq_kernel(Params p) {
   using S = BackwardShape<T, DP>;
   using TL = typename S::TL;
   constexpr int BN = S::BM, NC2 = DP / 16, BUFS = S::BUFS, NT = S::THREADS;
-  constexpr bool TWICE = BIAS == 2 && sizeof(T) == 2;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   char* kt = smem;
   char* vt = smem + BUFS * TL::BYTES;
   int* word = reinterpret_cast<int*>(smem + S::TILES);
   float* lut = reinterpret_cast<float*>(word + 4);
-  const int lut_len = BIAS ? 2 * p.max_distance + 1 : 0, lut_pad = (lut_len + 3) & ~3;
-  float* scratch = lut + lut_pad;                 // [4][32 * LD]
-  float* sums = scratch + 4 * 32 * BiasGrad::LD;  // [4][lut_pad]
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int nt = (p.Tq + 127) / 128;
   const Item item(p.B * p.H, nt, S::PARTS * p.dq_splits, p.causal);
@@ -136,26 +150,22 @@ __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_
     const T* gr = reinterpret_cast<const T*>(p.dout) + b * p.do_b + h * p.do_h + qc * p.do_t;
     q.load(reinterpret_cast<const T*>(p.q) + b * p.q_b + h * p.q_h + qc * p.q_t, half, p.D, true);
     go.load(gr, half, p.D, true);
-    if (!TWICE) {
-      const T* orow = reinterpret_cast<const T*>(p.o_in) + b * p.oi_b + h * p.oi_h + qc * p.oi_t;
+    const T* orow = reinterpret_cast<const T*>(p.o_in) + b * p.oi_b + h * p.oi_h + qc * p.oi_t;
 #pragma unroll
-      for (int c = 0; c < NC2; ++c) {
-        const Raw<T> g = load_chunk<T>(gr, 2 * c + half, p.D), o = load_chunk<T>(orow, 2 * c + half, p.D);
+    for (int c = 0; c < NC2; ++c) {
+      const Raw<T> g = load_chunk<T>(gr, 2 * c + half, p.D), o = load_chunk<T>(orow, 2 * c + half, p.D);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) delta += (float)g.x[e] * (float)o.x[e];
-      }
-      delta = both_sum(delta);
+      for (int e = 0; e < 8; ++e) delta += (float)g.x[e] * (float)o.x[e];
     }
+    delta = both_sum(delta);
   }
   const float lse = qi < p.Tq ? p.lse[(int64_t)bh * p.Tq + qi] : -INFINITY;
   const float lse2 = lse == -INFINITY ? INFINITY : lse * kLog2e;  // a row without keys, or none at all: P = exp2(.. - inf) = 0
   if constexpr (BIAS != 0) fill_lut(p, h, lut, tid, NT);
-  if constexpr (BIAS == 2)
-    for (int i = tid; i < 4 * lut_pad; i += NT) sums[i] = 0.f;
   const int end = key_end(p, b, min(qt * 128 + 127, p.Tq - 1) + off, word, tid, NT);
   const int all = (end + BN - 1) / BN, per = (all + p.dq_splits - 1) / p.dq_splits;
   f32x16 acc[S::DT] = {};
-  BiasGrad bias_grad;
+  float off_by = 0.f;
   Stage<T, DP, BN, NT> sk, sv;
   sk.start(kb, p.k_t, end, p.D, tid);
   sv.start(vb, p.v_t, end, p.D, tid);
@@ -173,96 +183,73 @@ __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_
     sk.store(kt + o * TL::BYTES, tid);
     sv.store(vt + o * TL::BYTES, tid);
   };
+  // the order of a round: as in the forward pass
+  const int t0 = share * per, t1 = min(all, t0 + per);
+  KeyBits<BN> keys(mask, end, lane, t0 * BN);
+  RowBits use = keys.next(t0 * BN), use1 = keys.next((t0 + 1) * BN), use2;  // of tiles t, t + 1, t + 2
+  load(t0, use);
+  store(t0, use);
+  if (S::EARLY) load(t0 + 1, use1);
+  __syncthreads();
+  for (int t = t0; t < t1; ++t) {
+    const char *kk = kt + (t & (BUFS - 1)) * TL::BYTES, *vv = vt + (t & (BUFS - 1)) * TL::BYTES;
+    use2 = keys.next((t + 2) * BN);
+    if (!S::EARLY) load(t + 1, use1);
 #pragma unroll
-  for (int walk = TWICE ? 0 : 1; walk < 2; ++walk) {
-    // the order of a round: as in the forward pass
-    // (the first walk is over all keys, whatever the share)
-    const int t0 = TWICE && walk == 0 ? 0 : share * per, t1 = TWICE && walk == 0 ? all : min(all, t0 + per);
-    KeyBits<BN> keys(mask, end, lane, t0 * BN);
-    RowBits use = keys.next(t0 * BN), use1 = keys.next((t0 + 1) * BN), use2;  // of tiles t, t + 1, t + 2
-    load(t0, use);
-    store(t0, use);
-    if (S::EARLY) load(t0 + 1, use1);
-    __syncthreads();
-    for (int t = t0; t < t1; ++t) {
-      const char *kk = kt + (t & (BUFS - 1)) * TL::BYTES, *vv = vt + (t & (BUFS - 1)) * TL::BYTES;
-      use2 = keys.next((t + 2) * BN);
-      if (!S::EARLY) load(t + 1, use1);
+    for (int x = 0; x < S::NS; ++x) {
+      const int sub = x, key0 = t * BN + sub * 32;
+      const bool work = key0 < end && !(p.causal && key0 > pos_hi);
+      f32x16 raw = {}, dp = {};
+      if constexpr (S::EARLY) {
+        char *kn = kt + ((t + 1) & (BUFS - 1)) * TL::BYTES, *vn = vt + ((t + 1) & (BUFS - 1)) * TL::BYTES;
+        products_shadow<TL, NC2>(kk, vv, q, go, raw, dp, sk, sv, kn, vn, col, half, tid);
+        load(t + 2, use2);
+      } else if (work) {
 #pragma unroll
-      for (int x = 0; x < S::NS; ++x) {
-        const int sub = x, key0 = t * BN + sub * 32;
-        const bool work = key0 < end && !(p.causal && key0 > pos_hi);
-        f32x16 raw = {}, dp = {};
-        if constexpr (S::EARLY) {
-          char *kn = kt + ((t + 1) & (BUFS - 1)) * TL::BYTES, *vn = vt + ((t + 1) & (BUFS - 1)) * TL::BYTES;
-          products_shadow<TL, NC2>(kk, vv, q, go, raw, dp, sk, sv, kn, vn, col, half, tid);
-          load(t + 2, use2);
-        } else if (work) {
-#pragma unroll
-          for (int c = 0; c < NC2; ++c)
-            mma2(TL::row_chunk(kk, sub * 32 + col, 2 * c + half), q.get(c), raw, TL::row_chunk(vv, sub * 32 + col, 2 * c + half), go.get(c), dp,
-                 [](int) {});
-        }
-        if (S::EARLY || work) {
-          float pr[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) pr[i] = raw[i];
-          finish_scores<BIAS != 0>(p, pr, key0, pos, pos_lo, pos_hi, use.of(sub), lut, half);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) pr[i] = __builtin_amdgcn_exp2f(pr[i] - lse2);
-          if (TWICE && walk == 0) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) delta += pr[i] * dp[i];
-          } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) pr[i] *= dp[i] - delta;
-            if constexpr (BIAS == 2)
-              if (d0 == 0) bias_grad.add(pr, key0 - pos_lo, p.max_distance, scratch + wave * 32 * BiasGrad::LD, sums + wave * lut_pad, lane);
-            if constexpr (S::EARLY)
-              column_product_shadow<TL, S::DT, 0>(kk, 0, d0, [&](int i) { return pr[i]; }, acc, lane, nullptr, [](int) {});
-            else
-              column_product<T, TL>(kk, sub * 32, d0, Weights<T>(pr), acc, lane);
-          }
-        }
+        for (int c = 0; c < NC2; ++c)
+          mma2(TL::row_chunk(kk, sub * 32 + col, 2 * c + half), q.get(c), raw, TL::row_chunk(vv, sub * 32 + col, 2 * c + half), go.get(c), dp,
+               [](int) {});
       }
-      if (!S::EARLY) {
-        if (BUFS == 1) __syncthreads();
-        store(t + 1, use1);
+      if (S::EARLY || work) {
+        float pr[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) pr[i] = raw[i];
+        finish_scores<BIAS != 0>(p, pr, key0, pos, pos_lo, pos_hi, use.of(sub), lut, half);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) pr[i] = __builtin_amdgcn_exp2f(pr[i] - lse2);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          pr[i] *= dp[i] - delta;
+          if (BIAS == 2) off_by += pr[i];
+        }
+        if constexpr (S::EARLY)
+          column_product_shadow<TL, S::DT, 0>(kk, 0, d0, [&](int i) { return pr[i]; }, acc, lane, nullptr, [](int) {});
+        else
+          column_product<T, TL>(kk, sub * 32, d0, Weights<T>(pr), acc, lane);
       }
-      use = use1;
-      use1 = use2;
-      __syncthreads();
     }
-    if (TWICE && walk == 0) delta = both_sum(delta);
+    if (!S::EARLY) {
+      if (BUFS == 1) __syncthreads();
+      store(t + 1, use1);
+    }
+    use = use1;
+    use1 = use2;
+    __syncthreads();
   }
-  if (half == 0 && share == 0 && d0 == 0 && qi < p.Tq) p.delta[(int64_t)bh * p.Tq + qi] = delta;
+  const float off_by_sum = both_sum(off_by);
+  if (half == 0 && d0 == 0 && qi < p.Tq && (BIAS == 2 || share == 0)) {
+    float x = share == 0 ? delta : 0.f;
+    if (BIAS == 2) x += off_by_sum;
+    p.delta[((int64_t)(BIAS == 2 ? share : 0) * p.B * p.H + bh) * p.Tq + qi] = x;
+  }
   if (qi < p.Tq)
     store_rows<S>(acc, reinterpret_cast<T*>(p.dq) + b * p.dq_b + h * p.dq_h + qi * p.dq_t,
                   p.dq_splits > 1 ? p.dq_part + (((int64_t)share * p.B * p.H + bh) * p.Tq + qi) * p.D : nullptr, d0, p.D, p.scale, half);
-  if constexpr (BIAS == 2) {
-    if (d0 != 0) return;
-    for (int m = 1; m < 64; m <<= 1) {
-      bias_grad.below += __shfl_xor(bias_grad.below, m);
-      bias_grad.above += __shfl_xor(bias_grad.above, m);
-    }
-    if (lane == 0) {
-      sums[wave * lut_pad] = bias_grad.below;
-      sums[wave * lut_pad + 2 * p.max_distance] = bias_grad.above;
-    }
-    __syncthreads();
-    // the waves' sums, then a bucket's distances, each in a fixed order
-    for (int i = tid; i < lut_len; i += NT) {
-      float x = sums[i];
-      for (int w = 1; w < 4; ++w) x += sums[w * lut_pad + i];
-      sums[i] = x;
-    }
-    __syncthreads();
-    for (int i = tid; i < p.buckets; i += NT) p.dtable_part[((int64_t)((b * nt + qt) * p.dq_splits + share) * p.H + h) * p.buckets + i] = bucket_sum(p, sums, i);
-  }
 }
 
-// dk, dv: keys of one key head stationary; tiles of queries and their output gradients through LDS, over all heads of the group.
-template <class T, int DP, bool BIAS>
+// dk, dv and, with BIAS == 2, the position table's gradient: keys of one key head stationary; tiles of queries and their output gradients through
+// LDS, over all heads of the group.
+template <class T, int DP, int BIAS>
 __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_dkv_kernel(Params p) {
   using S = BackwardShape<T, DP>;
   using TL = typename S::TL;
@@ -272,6 +259,10 @@ __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_
   char* gt = smem + BUFS * TL::BYTES;
   float* stat = reinterpret_cast<float*>(smem + S::TILES);  // [BUFS][2][BM]: lse in log2 units, delta
   float* lut = stat + BUFS * 2 * BM;
+  const int words = BiasGrad::words(p.max_distance);
+  float* skew = lut + ((2 * p.max_distance + 4) & ~3);
+  float* sums = skew + 4 * BiasGrad::SKEW;  // [4][words]
+  BiasGrad bias_grad;
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int nt = (p.Tk + 127) / 128;
   const Item item(p.B * p.Hkv, nt, S::PARTS * p.dkv_splits, p.causal);
@@ -308,7 +299,9 @@ __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_
       const int64_t row = ((int64_t)b * p.H + h) * p.Tq + r0 + tid;
       const float l = r0 + tid < p.Tq ? p.lse[row] : -INFINITY;
       s_lse = l == -INFINITY ? INFINITY : l * kLog2e;
-      s_delta = r0 + tid < p.Tq ? p.delta[row] : 0.f;
+      s_delta = 0.f;
+      if (r0 + tid < p.Tq)
+        for (int n = 0; n < (BIAS == 2 ? p.dq_splits : 1); ++n) s_delta += p.delta[(int64_t)n * p.B * p.H * p.Tq + row];
     }
   };
   auto store_stat = [&](int it) {
@@ -324,6 +317,8 @@ __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_
     sg.store(gt + o * TL::BYTES, tid);
     store_stat(it);
   };
+  if (BIAS == 2)
+    for (int i = tid; i < 4 * BiasGrad::SKEW; i += NT) skew[i] = 0.f;
   load(first_it);
   store(first_it);
   if (S::EARLY) load(first_it + 1);
@@ -332,6 +327,8 @@ __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_
     if constexpr (BIAS) {
       if (it == first_it || it % per == 0) {
         fill_lut(p, kvh * p.group + it / per, lut, tid, NT);
+        if (BIAS == 2)
+          for (int i = tid; i < 4 * words; i += NT) sums[i] = 0.f;
         __syncthreads();
       }
     }
@@ -387,6 +384,8 @@ __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_
             ds[i] = s[i] * (dp[i] - de[e]);
           }
         }
+        if constexpr (BIAS == 2)
+          if (d0 == 0) bias_grad.add(ds, kw - p0, p.max_distance, skew + wave * BiasGrad::SKEW, sums + wave * words, lane);
         if constexpr (S::EARLY) {
           Splitter first;  // of dS, made beside the products with P
           column_product_shadow<TL, S::DT, 12>(gg, 0, d0, [&](int i) { return s[i]; }, dv, lane, nullptr,
@@ -403,6 +402,30 @@ __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_
       store(it + 1);
     }
     __syncthreads();
+    if constexpr (BIAS == 2) {
+      if (d0 == 0 && (it + 1 == steps || (it + 1) % per == 0)) {  // the end of a head: the waves' sums, then a bucket's distances, in a fixed order
+        bias_grad.fold(p.max_distance, sums + wave * words, lane);
+        __syncthreads();
+        for (int i = tid; i < words; i += NT) {
+          float x = sums[i];
+          for (int w = 1; w < 4; ++w) x += sums[w * words + i];
+          sums[i] = x;
+        }
+        __syncthreads();
+        const int64_t row = (int64_t)(b * nt + item.tile) * p.dkv_splits + share;
+        for (int i = tid; i < p.buckets; i += NT) p.dtable_part[(row * p.H + kvh * p.group + it / per) * p.buckets + i] = bucket_sum(p, sums + BiasGrad::PAD, i);
+        __syncthreads();
+      }
+    }
+  }
+  if constexpr (BIAS == 2) {
+    if (d0 == 0)  // heads that this share has nothing of
+      for (int g = 0; g < p.group; ++g)
+        if (first_it >= steps || g < first_it / per || g > (steps - 1) / per) {
+          const int64_t row = (int64_t)(b * nt + item.tile) * p.dkv_splits + share;
+          for (int i = tid; i < p.buckets; i += NT) p.dtable_part[(row * p.H + kvh * p.group + g) * p.buckets + i] = 0.f;
+        }
+    if (!p.dk) return;
   }
   T* kout = reinterpret_cast<T*>(p.dk) + b * p.dk_b + kvh * p.dk_h;
   T* vout = reinterpret_cast<T*>(p.dv) + b * p.dv_b + kvh * p.dv_h;
@@ -439,9 +462,9 @@ static int launch_backward(const Params& p, float* dtable, hipStream_t st) {
   using S = BackwardShape<T, DP>;
   static std::atomic<uint64_t> dq_done{0}, dkv_done{0};
   const size_t lut = BIAS ? (size_t)(2 * p.max_distance + 4) * 4 : 0;
-  const int q_tiles = (p.Tq + 127) / 128;
-  if (launch(&attention_dq_kernel<T, DP, BIAS>, &dq_done, (int64_t)p.B * p.H * q_tiles * S::PARTS * p.dq_splits, S::THREADS,
-             S::TILES + 16 + lut + (BIAS == 2 ? 4 * (32 * BiasGrad::LD * 4 + lut) : 0), p, st))
+  const int k_tiles = (p.Tk + 127) / 128;
+  if (launch(&attention_dq_kernel<T, DP, BIAS>, &dq_done, (int64_t)p.B * p.H * ((p.Tq + 127) / 128) * S::PARTS * p.dq_splits, S::THREADS,
+             S::TILES + 16 + lut, p, st))
     return 1;
   if (p.dq_splits > 1) {
     const int64_t rows = (int64_t)p.B * p.H * p.Tq;
@@ -450,11 +473,11 @@ static int launch_backward(const Params& p, float* dtable, hipStream_t st) {
                        int64_t(0), rows, p.Tq, p.H, p.D, dq, dq, p.dq_b, p.dq_h, p.dq_t, p.dq_b, p.dq_h, p.dq_t);
     WRNN_LAUNCH_CHECK();
   }
-  if (p.dk && p.Tk) {
-    if (launch(&attention_dkv_kernel<T, DP, BIAS != 0>, &dkv_done, (int64_t)p.B * p.Hkv * ((p.Tk + 127) / 128) * S::PARTS * p.dkv_splits, S::THREADS,
-               S::TILES + S::BUFS * 2 * S::BM * 4 + lut, p, st))
+  if ((p.dk || BIAS == 2) && p.Tk) {
+    if (launch(&attention_dkv_kernel<T, DP, BIAS>, &dkv_done, (int64_t)p.B * p.Hkv * k_tiles * S::PARTS * p.dkv_splits, S::THREADS,
+               S::TILES + S::BUFS * 2 * S::BM * 4 + lut + (BIAS == 2 ? (size_t)BiasGrad::all_words(p.max_distance) * 4 : 0), p, st))
       return 1;
-    if (p.dkv_splits > 1) {
+    if (p.dk && p.dkv_splits > 1) {
       const int64_t rows = (int64_t)p.B * p.Hkv * p.Tk;
       hipLaunchKernelGGL((attention_share_kernel<T>), dim3((unsigned)((rows * (p.D / 4) + 255) / 256), 2), dim3(256), 0, st, p.dkv_part, p.dkv_splits,
                          2 * rows * p.D, rows * p.D, rows, p.Tk, p.Hkv, p.D, static_cast<T*>(p.dk), static_cast<T*>(p.dv), p.dk_b, p.dk_h, p.dk_t, p.dv_b,
@@ -462,7 +485,7 @@ static int launch_backward(const Params& p, float* dtable, hipStream_t st) {
       WRNN_LAUNCH_CHECK();
     }
   }
-  if (BIAS == 2) return launch_table_sum<float>(p.dtable_part, p.B * q_tiles * p.dq_splits, p.H, p.buckets, dtable, st);
+  if (BIAS == 2) return launch_table_sum<float>(p.dtable_part, p.B * k_tiles * p.dkv_splits, p.H, p.buckets, dtable, st);
   return 0;
 }
 
