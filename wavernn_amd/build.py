@@ -23,11 +23,12 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-u
 # verified with: the teacher-forced loop loses 5.5 % without them (13.7 -> 14.5 us per decoder step at B=64).
 NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # MFMA_IN_VGPRS: sums stay in the vector registers that the softmax works on; by default every value that passes between
-# matrix and vector instructions is copied (forward, float32, 128 columns: 64 copies a tile, 376 -> 330 us at 2 x 16 x 2048).  The compiler crashes
-# on the forward kernels of float32 with 256 columns that way; those do without.
+# matrix and vector instructions is copied.  2 x 16 heads, 2048 x 2048 in float32 at 128 columns: 376 -> 366 us; bfloat16 at 256
+# columns, 2 x 8 heads, 4096 x 4096: 796 -> 419 us.  The bfloat16 backward pass at 64 and 128 columns is the slower for it (551 -> 467 TFLOP/s).
 MFMA_IN_VGPRS = ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
 SOURCE_FLAGS = {s: NO_PACKED_FP32 + (MFMA_IN_VGPRS if s in ("attention_forward_bf16_d256.hip", "attention_forward_f32.hip",
-                                                            "attention_backward_bf16_d256.hip", "attention_backward_f32.hip") else [])
+                                                            "attention_forward_f32_d256.hip", "attention_backward_bf16_d256.hip",
+                                                            "attention_backward_f32.hip", "attention_backward_f32_d256.hip") else [])
                 for s in SOURCES if s.startswith(("attention", "relative_bias"))}
 
 

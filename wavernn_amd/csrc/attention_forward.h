@@ -46,10 +46,13 @@ struct ForwardShape {
   // narrow: as many waves as tiles of 32 keys fit the LDS beside each other (three planes of float32 are 6 bytes an element)
   static constexpr int WQ = WIDE ? 4 : 1, WK = WIDE ? 1 : NP == 1 ? 4 : DP == 64 ? 4 : DP == 128 ? 2 : 1;
   static constexpr int NS = WIDE && NP == 1 ? 2 : 1;  // 32-key subtiles of a tile per wave
-  static constexpr int THREADS = 64 * WQ * WK, BN = 32 * WK * NS;
+  // one tile of 32 keys is all that fits: four waves fetch and convert it, of which the last three do the first one's arithmetic for nothing
+  static constexpr int COPIES = WQ * WK == 1 ? 4 : 1;
+  static constexpr int THREADS = 64 * WQ * WK * COPIES, BN = 32 * WK * NS;
   static constexpr int BUFS = WIDE && !(NP == 3 && DP == 256) ? 2 : 1;  // two where they fit
   static constexpr int WAVES = WIDE ? (DP * NP <= 192 ? 2 : 1) : (DP * NP <= 128 ? 2 : 1);  // per SIMD
   static constexpr bool EARLY = NP == 3 && BUFS == 2;
+  static constexpr bool RAW = NP == 3 && DP == 256;
   using TL = Tile<T, DP, BN>;
   static constexpr size_t TILES = 2 * BUFS * TL::BYTES, SUMS = WK > 1 ? (size_t)WK * 32 * (DP + 4) * 4 : 0;
   static constexpr size_t BODY = TILES > SUMS ? TILES : SUMS;
@@ -68,7 +71,7 @@ __global__ __launch_bounds__((ForwardShape<T, DP, WIDE>::THREADS), (ForwardShape
   int* word = reinterpret_cast<int*>(ml + 4 * 2 * 32);
   float* lut = reinterpret_cast<float*>(word + 4);
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wq = WIDE ? wave : 0, wk = WIDE ? 0 : wave;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wq = WIDE ? wave : 0, wk = WIDE || S::WK == 1 ? 0 : wave;
   const bool pack = !WIDE && p.pack;
   const int heads = pack ? p.Hkv : p.H, splits = p.splits;
   const int nt = pack ? 1 : (p.Tq + 32 * S::WQ - 1) / (32 * S::WQ);
@@ -84,7 +87,7 @@ __global__ __launch_bounds__((ForwardShape<T, DP, WIDE>::THREADS), (ForwardShape
   const T* kb = reinterpret_cast<const T*>(p.k) + b * p.k_b + kvh * p.k_h;
   const T* vb = reinterpret_cast<const T*>(p.v) + b * p.v_b + kvh * p.v_h;
   const uint8_t* mask = p.key_mask ? p.key_mask + b * p.mask_b : nullptr;
-  Stationary<T, DP, false> q;
+  Stationary<T, DP, S::RAW> q;
   q.load(reinterpret_cast<const T*>(p.q) + b * p.q_b + h * p.q_h + min(qi, p.Tq - 1) * p.q_t, half, p.D, true);
   const int lut_len = 2 * p.max_distance + 1;
   const float* my_lut = lut;
@@ -190,7 +193,7 @@ __global__ __launch_bounds__((ForwardShape<T, DP, WIDE>::THREADS), (ForwardShape
   }
   const float l = both_sum(run.l);
   if constexpr (S::WK == 1) {
-    if (qi >= p.Tq || (pack && lh >= p.group)) return;
+    if (qi >= p.Tq || (pack && lh >= p.group) || (S::COPIES > 1 && wave)) return;
     const int64_t row = ((int64_t)b * p.H + h) * p.Tq + qi;
     if (splits == 1) {
       const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);

@@ -89,22 +89,22 @@ struct Raw {  // 8 elements as they come from memory
 __device__ __forceinline__ Operand<__bf16> operand(const Raw<__bf16>& r) { return {{r.x}}; }
 // One plane of two values, by cutting: the upper half of what the planes before it left (8 bits of mantissa); the subtraction is exact, so
 // the three add up to the value itself.
-__device__ __forceinline__ uint32_t split2(float& a, float& b, bool more) {
+__device__ __forceinline__ uint32_t split2(float& a, float& b, bool more, uint32_t upper = 0xffff0000u, uint32_t uppers = 0x07060302u) {
   const uint32_t x = __float_as_uint(a), y = __float_as_uint(b);
   if (more) {
-    a -= __uint_as_float(x & 0xffff0000u);
-    b -= __uint_as_float(y & 0xffff0000u);
+    a -= __uint_as_float(x & upper);
+    b -= __uint_as_float(y & upper);
   }
-  return __builtin_amdgcn_perm(y, x, 0x07060302u);  // the upper halves of x and y
+  return __builtin_amdgcn_perm(y, x, uppers);  // the upper halves of x and y
 }
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-__device__ __forceinline__ void split(f32x8 x, bf16x8 (&p)[3]) {
+__device__ __forceinline__ void split(f32x8 x, bf16x8 (&p)[3], uint32_t upper = 0xffff0000u, uint32_t uppers = 0x07060302u) {
   u32x4 v[3];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     float a = x[2 * j], b = x[2 * j + 1];
 #pragma unroll
-    for (int n = 0; n < 3; ++n) v[n][j] = split2(a, b, n < 2);
+    for (int n = 0; n < 3; ++n) v[n][j] = split2(a, b, n < 2, upper, uppers);
   }
 #pragma unroll
   for (int n = 0; n < 3; ++n) p[n] = __builtin_bit_cast(bf16x8, v[n]);
@@ -244,7 +244,14 @@ struct Stationary<T, DP, true> {
       if (!ok) o[c].x = {};
     }
   }
-  __device__ __forceinline__ Operand<T> get(int c) const { return operand(o[c]); }
+  // the constants are hidden from the compiler, or it moves the conversion out of the loop and its results to memory
+  __device__ __forceinline__ Operand<T> get(int c) const {
+    uint32_t upper = 0xffff0000u, uppers = 0x07060302u;
+    asm volatile("" : "+s"(upper), "+s"(uppers));
+    Operand<T> x;
+    split(o[c].x, x.p, upper, uppers);
+    return x;
+  }
 };
 
 // A tile of ROWS rows of DP elements in LDS, plane after plane.
