@@ -47,18 +47,19 @@ static size_t split_workspace(const Params& p) {
   return p.splits > 1 ? (size_t)p.B * p.H * p.Tq * p.splits * (padded_dim(p.D) + 4) * sizeof(float) : 0;
 }
 
+// blocks of a workgroup's rows: two waves share a row past 128 columns (BackwardShape)
+static int row_blocks(const Params& p, int rows) { return p.D > 128 ? (rows + 63) / 64 : (rows + 127) / 128; }
 static void plan_backward(Params* p) {
-  const int parts = p->D > 128 ? 2 : 1;
-  p->dq_splits = shares((int64_t)p->B * p->H * ((p->Tq + 127) / 128) * parts, (p->Tk + 31) / 32, 4);
+  p->dq_splits = shares((int64_t)p->B * p->H * row_blocks(*p, p->Tq), (p->Tk + 31) / 32, 4);
   // (causality: the first keys' blocks are the longest by far; half as long they leave the others time to fill up)
-  const int64_t blocks = (int64_t)p->B * p->Hkv * ((p->Tk + 127) / 128) * parts;
+  const int64_t blocks = (int64_t)p->B * p->Hkv * row_blocks(*p, p->Tk);
   p->dkv_splits = shares(p->causal ? (blocks + 1) / 2 : blocks, (int64_t)((p->Tq + 31) / 32) * p->group, 4);
 }
 static size_t aligned(size_t x) { return (x + 255) & ~size_t(255); }
 // the backward workspace: delta, the table's partial sums, the shares
 static size_t delta_bytes(const Params& p) { return aligned((size_t)(p.table ? p.dq_splits : 1) * p.B * p.H * p.Tq * sizeof(float)); }
 static size_t table_bytes(const Params& p) {
-  return p.table ? aligned((size_t)p.B * ((p.Tk + 127) / 128) * p.dkv_splits * p.H * p.buckets * sizeof(float)) : 0;
+  return p.table ? aligned((size_t)p.B * row_blocks(p, p.Tk) * p.dkv_splits * p.H * p.buckets * sizeof(float)) : 0;
 }
 static size_t dq_bytes(const Params& p) { return p.dq_splits > 1 ? aligned((size_t)p.dq_splits * p.B * p.H * p.Tq * p.D * sizeof(float)) : 0; }
 static size_t dkv_bytes(const Params& p) { return p.dkv_splits > 1 ? (size_t)p.dkv_splits * 2 * p.B * p.Hkv * p.Tk * p.D * sizeof(float) : 0; }

@@ -21,7 +21,6 @@ struct BiasGrad {
   static constexpr int LD = 20, SKEW = 48 * LD;  // 47 diagonals of 16 keys, and one that stays zero
   float below = 0.f, above = 0.f;
   static __host__ __device__ int words(int md) { return (2 * md + 1 + 2 * PAD + 3) & ~3; }
-  static __host__ __device__ int all_words(int md) { return 4 * (words(md) + SKEW); }  // of a workgroup, `skew` first
   // rel0: first key - position of the first query
   __device__ __forceinline__ void add(const float (&ds)[16], int rel0, int md, float* skew, float* sums, int lane) {
     const int half = lane >> 5, col = lane & 31;
@@ -68,20 +67,36 @@ struct BiasGrad {
   }
 };
 
-// A workgroup: 4 waves of 32 stationary rows each against every subtile of a tile.
+// A workgroup: 4 waves against every subtile of a tile.  Up to 128 columns each has 32 stationary rows of its own; with more, both sums and both
+// stationary operands of a wave would not fit its registers, and two waves share 32 rows, each with half of the columns: of the scores' and dP's
+// sums they exchange their parts through LDS.
 template <class T, int DP>
 struct BackwardShape {
   static constexpr int NP = Type<T>::NP;
   static constexpr int THREADS = 256, NS = NP == 1 && DP < 256 ? 2 : 1, BM = 32 * NS;
   static constexpr int BUFS = NP == 3 && DP == 256 ? 1 : 2;  // two where they leave room for the position bias's tables
   static constexpr bool EARLY = NP == 3 && BUFS == 2;        // the next tile goes to LDS beside the arithmetic (forward pass)
-  static constexpr bool RAW = NP == 3 && DP == 256;
-  // output columns of a workgroup: both sums and both stationary operands have to fit the registers
-  static constexpr int DA = DP > 128 ? 128 : DP, PARTS = DP / DA, DT = DA / 32;
+  static constexpr int SLICES = DP > 128 ? 2 : 1, RG = 4 / SLICES, ROWS = 32 * RG;  // waves of a row; groups of 32 rows
+  static constexpr int DA = DP / SLICES, DT = DA / 32, NC2 = DA / 16;               // a wave's columns
+  static constexpr bool RAW = NP == 3 && SLICES > 1;  // of dk, dv: their two sums leave no room for the planes
   using TL = Tile<T, DP, BM>;
-  static constexpr size_t TILES = 2 * BUFS * TL::BYTES;
+  static constexpr size_t EXCHANGE = SLICES > 1 ? 4 * 16 * 64 * 4 : 0, TILES = 2 * BUFS * TL::BYTES + EXCHANGE;
   static constexpr int WAVES = DP * NP <= 64 ? 2 : 1;  // per SIMD
 };
+
+// Both waves' parts of a sum added up.  `mine` and `other` are the waves' places; what a wave hands in stays until the other has read it, so the
+// next sum goes the other way round, into the place that only this wave reads from.
+__device__ __forceinline__ void exchange(f32x16& x, float* mine, const float* other, int lane) {
+#pragma unroll
+  for (int g = 0; g < 4; ++g) *reinterpret_cast<f32x4*>(mine + (g * 64 + lane) * 4) = f32x4{x[4 * g], x[4 * g + 1], x[4 * g + 2], x[4 * g + 3]};
+  __syncthreads();
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const f32x4 y = *reinterpret_cast<const f32x4*>(other + (g * 64 + lane) * 4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[4 * g + e] += y[e];
+  }
+}
 
 // A lane's sums to its row: of the gradient, or (part) of the workgroup's share in 32 bits, which attention_share_kernel adds up.
 template <class S, class T>
@@ -125,34 +140,36 @@ template <class T, int DP, int BIAS>
 __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_dq_kernel(Params p) {
   using S = BackwardShape<T, DP>;
   using TL = typename S::TL;
-  constexpr int BN = S::BM, NC2 = DP / 16, BUFS = S::BUFS, NT = S::THREADS;
+  constexpr int BN = S::BM, NC2 = S::NC2, BUFS = S::BUFS, NT = S::THREADS;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   char* kt = smem;
   char* vt = smem + BUFS * TL::BYTES;
   int* word = reinterpret_cast<int*>(smem + S::TILES);
   float* lut = reinterpret_cast<float*>(word + 4);
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int nt = (p.Tq + 127) / 128;
-  const Item item(p.B * p.H, nt, S::PARTS * p.dq_splits, p.causal);
+  const int nt = (p.Tq + S::ROWS - 1) / S::ROWS;
+  const Item item(p.B * p.H, nt, p.dq_splits, p.causal);
   if (item.share < 0) return;
-  const int share = item.share / S::PARTS, d0 = (item.share % S::PARTS) * S::DA;
+  const int share = item.share, d0 = wave % S::SLICES * S::DA, ch0 = d0 / 8;  // the wave's first column, and its chunk
+  float* place = reinterpret_cast<float*>(smem + S::TILES - S::EXCHANGE);
+  float *mine = place + wave * 1024, *other = place + (wave ^ 1) * 1024;
   const int bh = item.head, b = bh / p.H, h = bh - b * p.H, qt = p.causal ? nt - 1 - item.tile : item.tile;
-  const int q0 = qt * 128 + 32 * wave;
+  const int q0 = qt * S::ROWS + 32 * (wave / S::SLICES);
   const int off = start_of(p, b), kvh = h / p.group;
   const T* kb = reinterpret_cast<const T*>(p.k) + b * p.k_b + kvh * p.k_h;
   const T* vb = reinterpret_cast<const T*>(p.v) + b * p.v_b + kvh * p.v_h;
   const uint8_t* mask = p.key_mask ? p.key_mask + b * p.mask_b : nullptr;
   const int qi = q0 + col, qc = min(qi, p.Tq - 1), pos = qi + off;
   const int pos_lo = q0 + off, pos_hi = pos_lo + 31;
-  Stationary<T, DP, S::RAW> q, go;
+  Stationary<T, S::DA, false> q, go;
   float delta = 0.f;
   {
     const T* gr = reinterpret_cast<const T*>(p.dout) + b * p.do_b + h * p.do_h + qc * p.do_t;
-    q.load(reinterpret_cast<const T*>(p.q) + b * p.q_b + h * p.q_h + qc * p.q_t, half, p.D, true);
-    go.load(gr, half, p.D, true);
+    q.load(reinterpret_cast<const T*>(p.q) + b * p.q_b + h * p.q_h + qc * p.q_t + d0, half, p.D - d0, true);
+    go.load(gr + d0, half, p.D - d0, true);
     const T* orow = reinterpret_cast<const T*>(p.o_in) + b * p.oi_b + h * p.oi_h + qc * p.oi_t;
 #pragma unroll
-    for (int c = 0; c < NC2; ++c) {
+    for (int c = 0; c < DP / 16; ++c) {
       const Raw<T> g = load_chunk<T>(gr, 2 * c + half, p.D), o = load_chunk<T>(orow, 2 * c + half, p.D);
 #pragma unroll
       for (int e = 0; e < 8; ++e) delta += (float)g.x[e] * (float)o.x[e];
@@ -162,7 +179,7 @@ __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_
   const float lse = qi < p.Tq ? p.lse[(int64_t)bh * p.Tq + qi] : -INFINITY;
   const float lse2 = lse == -INFINITY ? INFINITY : lse * kLog2e;  // a row without keys, or none at all: P = exp2(.. - inf) = 0
   if constexpr (BIAS != 0) fill_lut(p, h, lut, tid, NT);
-  const int end = key_end(p, b, min(qt * 128 + 127, p.Tq - 1) + off, word, tid, NT);
+  const int end = key_end(p, b, min(qt * S::ROWS + S::ROWS - 1, p.Tq - 1) + off, word, tid, NT);
   const int all = (end + BN - 1) / BN, per = (all + p.dq_splits - 1) / p.dq_splits;
   f32x16 acc[S::DT] = {};
   float off_by = 0.f;
@@ -207,8 +224,12 @@ __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_
       } else if (work) {
 #pragma unroll
         for (int c = 0; c < NC2; ++c)
-          mma2(TL::row_chunk(kk, sub * 32 + col, 2 * c + half), q.get(c), raw, TL::row_chunk(vv, sub * 32 + col, 2 * c + half), go.get(c), dp,
-               [](int) {});
+          mma2(TL::row_chunk(kk, sub * 32 + col, ch0 + 2 * c + half), q.get(c), raw, TL::row_chunk(vv, sub * 32 + col, ch0 + 2 * c + half), go.get(c),
+               dp, [](int) {});
+      }
+      if constexpr (S::SLICES > 1) {
+        exchange(raw, mine, other, lane);
+        exchange(dp, other, mine, lane);
       }
       if (S::EARLY || work) {
         float pr[16];
@@ -253,7 +274,7 @@ template <class T, int DP, int BIAS>
 __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_dkv_kernel(Params p) {
   using S = BackwardShape<T, DP>;
   using TL = typename S::TL;
-  constexpr int BM = S::BM, NC2 = DP / 16, BUFS = S::BUFS, NT = S::THREADS;
+  constexpr int BM = S::BM, NC2 = S::NC2, BUFS = S::BUFS, NT = S::THREADS;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   char* qt = smem;
   char* gt = smem + BUFS * TL::BYTES;
@@ -261,29 +282,31 @@ __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_
   float* lut = stat + BUFS * 2 * BM;
   const int words = BiasGrad::words(p.max_distance);
   float* skew = lut + ((2 * p.max_distance + 4) & ~3);
-  float* sums = skew + 4 * BiasGrad::SKEW;  // [4][words]
+  float* sums = skew + S::RG * BiasGrad::SKEW;  // [RG][words]
   BiasGrad bias_grad;
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int nt = (p.Tk + 127) / 128;
-  const Item item(p.B * p.Hkv, nt, S::PARTS * p.dkv_splits, p.causal);
+  const int nt = (p.Tk + S::ROWS - 1) / S::ROWS;
+  const Item item(p.B * p.Hkv, nt, p.dkv_splits, p.causal);
   if (item.share < 0) return;
-  const int share = item.share / S::PARTS, d0 = (item.share % S::PARTS) * S::DA;
-  const int bh = item.head, b = bh / p.Hkv, kvh = bh - b * p.Hkv, k0 = item.tile * 128, kw = k0 + 32 * wave;
+  const int share = item.share, d0 = wave % S::SLICES * S::DA, ch0 = d0 / 8, rg = wave / S::SLICES;
+  float* place = reinterpret_cast<float*>(smem + S::TILES - S::EXCHANGE);
+  float *mine = place + wave * 1024, *other = place + (wave ^ 1) * 1024;
+  const int bh = item.head, b = bh / p.Hkv, kvh = bh - b * p.Hkv, k0 = item.tile * S::ROWS, kw = k0 + 32 * rg;
   const int off = start_of(p, b), key = kw + col, kc = min(key, p.Tk - 1);
   const uint8_t* mask = p.key_mask ? p.key_mask + b * p.mask_b : nullptr;
   int end = p.Tk;
   if (p.key_lens) end = min(end, max(p.key_lens[b], 0));
   if (p.causal) end = min(end, max(p.Tq + off, 0));  // past the last query's reach
   const bool ok = key < end && !(mask && mask[kc]);
-  Stationary<T, DP, S::RAW> k, v;
-  k.load(reinterpret_cast<const T*>(p.k) + b * p.k_b + kvh * p.k_h + kc * p.k_t, half, p.D, ok);
-  v.load(reinterpret_cast<const T*>(p.v) + b * p.v_b + kvh * p.v_h + kc * p.v_t, half, p.D, ok);
+  Stationary<T, S::DA, S::RAW> k, v;
+  k.load(reinterpret_cast<const T*>(p.k) + b * p.k_b + kvh * p.k_h + kc * p.k_t + d0, half, p.D - d0, ok);
+  v.load(reinterpret_cast<const T*>(p.v) + b * p.v_b + kvh * p.v_h + kc * p.v_t + d0, half, p.D - d0, ok);
   const float add = ok ? 0.f : -INFINITY;
   f32x16 dk[S::DT] = {}, dv[S::DT] = {};
   // under causality queries before key - off see nothing of this block
   const int qt_n = (p.Tq + BM - 1) / BM, qt_0 = p.causal ? min(max(k0 - off, 0) / BM, qt_n) : 0, per = qt_n - qt_0;
-  const int all = k0 < end ? per * p.group : 0, mine = (all + p.dkv_splits - 1) / p.dkv_splits, first_it = share * mine,
-            steps = min(all, first_it + mine);
+  const int all = k0 < end ? per * p.group : 0, part = (all + p.dkv_splits - 1) / p.dkv_splits, first_it = share * part,
+            steps = min(all, first_it + part);
   Stage<T, DP, BM, NT> sq, sg;
   sq.start(nullptr, p.q_t, p.Tq, p.D, tid);
   sg.start(nullptr, p.do_t, p.Tq, p.D, tid);
@@ -318,7 +341,7 @@ __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_
     store_stat(it);
   };
   if (BIAS == 2)
-    for (int i = tid; i < 4 * BiasGrad::SKEW; i += NT) skew[i] = 0.f;
+    for (int i = tid; i < S::RG * BiasGrad::SKEW; i += NT) skew[i] = 0.f;
   load(first_it);
   store(first_it);
   if (S::EARLY) load(first_it + 1);
@@ -328,7 +351,7 @@ __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_
       if (it == first_it || it % per == 0) {
         fill_lut(p, kvh * p.group + it / per, lut, tid, NT);
         if (BIAS == 2)
-          for (int i = tid; i < 4 * words; i += NT) sums[i] = 0.f;
+          for (int i = tid; i < S::RG * words; i += NT) sums[i] = 0.f;
         __syncthreads();
       }
     }
@@ -348,8 +371,12 @@ __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_
       } else if (work) {
 #pragma unroll
         for (int c = 0; c < NC2; ++c)
-          mma2(TL::row_chunk(qq, sub * 32 + col, 2 * c + half), k.get(c), raw, TL::row_chunk(gg, sub * 32 + col, 2 * c + half), v.get(c), dp,
+          mma2(TL::row_chunk(qq, sub * 32 + col, ch0 + 2 * c + half), k.get(c), raw, TL::row_chunk(gg, sub * 32 + col, ch0 + 2 * c + half), v.get(c), dp,
                [](int) {});
+      }
+      if constexpr (S::SLICES > 1) {
+        exchange(raw, mine, other, lane);
+        exchange(dp, other, mine, lane);
       }
       if (S::EARLY || work) {
         float s[16];
@@ -385,7 +412,7 @@ __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_
           }
         }
         if constexpr (BIAS == 2)
-          if (d0 == 0) bias_grad.add(ds, kw - p0, p.max_distance, skew + wave * BiasGrad::SKEW, sums + wave * words, lane);
+          if (d0 == 0) bias_grad.add(ds, kw - p0, p.max_distance, skew + rg * BiasGrad::SKEW, sums + rg * words, lane);
         if constexpr (S::EARLY) {
           Splitter first;  // of dS, made beside the products with P
           column_product_shadow<TL, S::DT, 12>(gg, 0, d0, [&](int i) { return s[i]; }, dv, lane, nullptr,
@@ -403,12 +430,12 @@ __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_
     }
     __syncthreads();
     if constexpr (BIAS == 2) {
-      if (d0 == 0 && (it + 1 == steps || (it + 1) % per == 0)) {  // the end of a head: the waves' sums, then a bucket's distances, in a fixed order
-        bias_grad.fold(p.max_distance, sums + wave * words, lane);
+      if (it + 1 == steps || (it + 1) % per == 0) {  // the end of a head: the waves' sums, then a bucket's distances, in a fixed order
+        if (d0 == 0) bias_grad.fold(p.max_distance, sums + rg * words, lane);
         __syncthreads();
         for (int i = tid; i < words; i += NT) {
           float x = sums[i];
-          for (int w = 1; w < 4; ++w) x += sums[w * words + i];
+          for (int w = 1; w < S::RG; ++w) x += sums[w * words + i];
           sums[i] = x;
         }
         __syncthreads();
@@ -419,22 +446,21 @@ __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_
     }
   }
   if constexpr (BIAS == 2) {
-    if (d0 == 0)  // heads that this share has nothing of
-      for (int g = 0; g < p.group; ++g)
-        if (first_it >= steps || g < first_it / per || g > (steps - 1) / per) {
-          const int64_t row = (int64_t)(b * nt + item.tile) * p.dkv_splits + share;
-          for (int i = tid; i < p.buckets; i += NT) p.dtable_part[(row * p.H + kvh * p.group + g) * p.buckets + i] = 0.f;
-        }
+    for (int g = 0; g < p.group; ++g)  // heads that this share has nothing of
+      if (first_it >= steps || g < first_it / per || g > (steps - 1) / per) {
+        const int64_t row = (int64_t)(b * nt + item.tile) * p.dkv_splits + share;
+        for (int i = tid; i < p.buckets; i += NT) p.dtable_part[(row * p.H + kvh * p.group + g) * p.buckets + i] = 0.f;
+      }
     if (!p.dk) return;
   }
   T* kout = reinterpret_cast<T*>(p.dk) + b * p.dk_b + kvh * p.dk_h;
   T* vout = reinterpret_cast<T*>(p.dv) + b * p.dv_b + kvh * p.dv_h;
   if (key < p.Tk) {
-    float* part = nullptr;
+    float* to = nullptr;
     const int64_t rows = (int64_t)p.B * p.Hkv * p.Tk;
-    if (p.dkv_splits > 1) part = p.dkv_part + (share * 2 * rows + (int64_t)bh * p.Tk + key) * p.D;
-    store_rows<S>(dk, kout + key * p.dk_t, part, d0, p.D, p.scale, half);
-    store_rows<S>(dv, vout + key * p.dv_t, part ? part + rows * p.D : nullptr, d0, p.D, 1.f, half);
+    if (p.dkv_splits > 1) to = p.dkv_part + (share * 2 * rows + (int64_t)bh * p.Tk + key) * p.D;
+    store_rows<S>(dk, kout + key * p.dk_t, to, d0, p.D, p.scale, half);
+    store_rows<S>(dv, vout + key * p.dv_t, to ? to + rows * p.D : nullptr, d0, p.D, 1.f, half);
   }
 }
 
@@ -462,8 +488,8 @@ static int launch_backward(const Params& p, float* dtable, hipStream_t st) {
   using S = BackwardShape<T, DP>;
   static std::atomic<uint64_t> dq_done{0}, dkv_done{0};
   const size_t lut = BIAS ? (size_t)(2 * p.max_distance + 4) * 4 : 0;
-  const int k_tiles = (p.Tk + 127) / 128;
-  if (launch(&attention_dq_kernel<T, DP, BIAS>, &dq_done, (int64_t)p.B * p.H * ((p.Tq + 127) / 128) * S::PARTS * p.dq_splits, S::THREADS,
+  const int k_tiles = (p.Tk + S::ROWS - 1) / S::ROWS;
+  if (launch(&attention_dq_kernel<T, DP, BIAS>, &dq_done, (int64_t)p.B * p.H * ((p.Tq + S::ROWS - 1) / S::ROWS) * p.dq_splits, S::THREADS,
              S::TILES + 16 + lut, p, st))
     return 1;
   if (p.dq_splits > 1) {
@@ -474,8 +500,8 @@ static int launch_backward(const Params& p, float* dtable, hipStream_t st) {
     WRNN_LAUNCH_CHECK();
   }
   if ((p.dk || BIAS == 2) && p.Tk) {
-    if (launch(&attention_dkv_kernel<T, DP, BIAS>, &dkv_done, (int64_t)p.B * p.Hkv * k_tiles * S::PARTS * p.dkv_splits, S::THREADS,
-               S::TILES + S::BUFS * 2 * S::BM * 4 + lut + (BIAS == 2 ? (size_t)BiasGrad::all_words(p.max_distance) * 4 : 0), p, st))
+    if (launch(&attention_dkv_kernel<T, DP, BIAS>, &dkv_done, (int64_t)p.B * p.Hkv * k_tiles * p.dkv_splits, S::THREADS,
+               S::TILES + S::BUFS * 2 * S::BM * 4 + lut + (BIAS == 2 ? (size_t)S::RG * (BiasGrad::SKEW + BiasGrad::words(p.max_distance)) * 4 : 0), p, st))
       return 1;
     if (p.dk && p.dkv_splits > 1) {
       const int64_t rows = (int64_t)p.B * p.Hkv * p.Tk;
