@@ -82,6 +82,10 @@ struct BackwardShape {
   using TL = Tile<T, DP, BM>;
   static constexpr size_t EXCHANGE = SLICES > 1 ? 4 * 16 * 64 * 4 : 0, TILES = 2 * BUFS * TL::BYTES + EXCHANGE;
   static constexpr int WAVES = DP * NP <= 64 ? 2 : 1;  // per SIMD
+  // dS of the dq kernel.  A query's keys share the shift along it that its softmax gives them, and the errors of dS add up along it, the more so
+  // the fewer columns there are (dq off by 2.5e-3 .. 3.3e-3 of its norm up to 64): there it keeps 16 bits (1.8e-3 .. 2.1e-3; the backward pass at
+  // 2 x 16 heads, 4096 x 4096 x 64 takes 611 us instead of 541).  At 128 columns one rounding gives 2.4e-3.
+  using QueryWeights = std::conditional_t<(NP == 1 && DP == 64), Weights2, Weights<T>>;
 };
 
 // Both waves' parts of a sum added up.  `mine` and `other` are the waves' places; what a wave hands in stays until the other has read it, so the
@@ -141,6 +145,7 @@ __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_
   using S = BackwardShape<T, DP>;
   using TL = typename S::TL;
   constexpr int BN = S::BM, NC2 = S::NC2, BUFS = S::BUFS, NT = S::THREADS;
+  using DS = typename S::QueryWeights;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   char* kt = smem;
   char* vt = smem + BUFS * TL::BYTES;
@@ -246,7 +251,7 @@ __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_
         if constexpr (S::EARLY)
           column_product_shadow<TL, S::DT, 0>(kk, 0, d0, [&](int i) { return pr[i]; }, acc, lane, nullptr, [](int) {});
         else
-          column_product<T, TL>(kk, sub * 32, d0, Weights<T>(pr), acc, lane);
+          column_product<T, TL>(kk, sub * 32, d0, DS(pr), acc, lane);
       }
     }
     if (!S::EARLY) {
