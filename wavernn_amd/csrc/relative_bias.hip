@@ -1,6 +1,7 @@
 // The learned relative position bias as a dense tensor, and its table's gradient.
-//   out[h, i, j] = table[bucket(j - (i + start)), h]          bound by the writes of H * Tq * Tk values
-//   dtable[n, h] = sum over the pairs of bucket n of dout      bound by the reads of them
+//   out[h, i, j] = table[bucket(j - (i + start)), h]          bound by the writes of H * Tq * Tk values: 16 x 2048 x 2048 in float32 in 41 us,
+//                                                              6.5 TB/s (filling as much memory 6.9)
+//   dtable[n, h] = sum over the pairs of bucket n of dout      bound by the reads of them: the same 75 us, 3.6 TB/s (a plain sum 4.0)
 // A bucket depends on the distance alone and is constant from max_distance on, so both work on one value per distance in
 // [-max_distance, max_distance] (LDS) and never look at a bucket inside the loops.
 #include "attention_tile.h"
@@ -49,7 +50,8 @@ __global__ __launch_bounds__(256) void relative_bias_kernel(Params p, DenseBias 
 
 // A workgroup's rows -> one partial sum per bucket.  Near the diagonal a thread owns a distance and walks the rows; what lies further out a wave
 // reads row by row, four rows at a time to have enough loads in flight, 16 bytes a load from each row's first aligned element on (the
-// vectors that lie wholly near the diagonal are left to the walk).
+// vectors that lie wholly near the diagonal are left to the walk).  Nothing is read twice: loads that leave the caches alone are the faster
+// (16 x 2048 x 2048 and 2047 x 2047 with the forward pass 140 and 150 -> 122 and 119 us).
 template <class T>
 __global__ __launch_bounds__(256) void relative_bias_grad_kernel(Params p, DenseBias a) {
   constexpr int V = 16 / sizeof(T), R = 4;
@@ -85,7 +87,7 @@ __global__ __launch_bounds__(256) void relative_bias_grad_kernel(Params p, Dense
         const int j = head[r] + c * V;
         rel[r] = j - (i + r + a.start);
         v[r] = vec(T(0));
-        if (c < full[r] && !(rel[r] > -md && rel[r] + V - 1 < md)) v[r] = *reinterpret_cast<const vec*>(row[r] + j);
+        if (c < full[r] && !(rel[r] > -md && rel[r] + V - 1 < md)) v[r] = __builtin_nontemporal_load(reinterpret_cast<const vec*>(row[r] + j));
       }
 #pragma unroll
       for (int r = 0; r < R; ++r)
