@@ -445,3 +445,60 @@ def test_other_stream_and_graph():
         got = [x.clone() for x in static]
         want = work()
         assert all(torch.equal(a, b) for a, b in zip(got, want)), n
+
+
+def test_c_entry_refuses_unaligned_workspaces():
+    lib = _lib.load()
+    one, i3 = desc(batch=1, q_len=1, k_len=100000), _lib.I64x3(0, 0, 0)
+    assert lib.wrnn_attention_forward(C.byref(one), 16, i3, None, 8, 1 << 30, None) != 0 and b"on 16 bytes" in lib.wrnn_last_error()
+    g = _lib.AttentionGrads(out=16, lse=16, dout=16, dq=16, dk=16, dv=16)
+    assert lib.wrnn_attention_backward(C.byref(one), C.byref(g), 8, 1 << 30, None) != 0 and b"on 16 bytes" in lib.wrnn_last_error()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("move", ["clone", "host", "contiguous"])
+def test_saved_tensors_that_come_back_elsewhere(dtype, move):
+    """Offloading and checkpointing keep copies of what a node saves: the backward pass works on those, in whatever place and strides."""
+    pack, unpack = {"clone": (lambda t: t.clone(), lambda t: t), "host": (lambda t: t.cpu(), lambda t: t.cuda()),
+                    "contiguous": (lambda t: t.contiguous().clone(), lambda t: t)}[move]
+    def inputs():
+        q, k, v = normal(0, 70, 2, 3, 4, 24, dtype=dtype).permute(2, 1, 3, 0, 4).unbind(0)
+        return [q, k, v, normal(1, 16, 4)]
+    mask = (torch.arange(70) >= torch.tensor([[70], [41]])).t().contiguous().t().cuda()
+    lens, start = torch.tensor([66, 50]).cuda(), torch.tensor([3, -2]).cuda()
+    dout = normal(2, 2, 4, 70, 24, dtype=dtype)
+    def run(leaves, **kw):
+        leaves = [x.detach().requires_grad_() for x in leaves]
+        out = A.attention(*(x.clone() for x in leaves[:3]), bias_table=leaves[3].clone(), max_distance=40, key_mask=mask, key_lens=lens, q_start=start)
+        return out, leaves
+    out, leaves = run(inputs())
+    want = torch.autograd.grad(out, leaves, dout)
+    with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+        out, leaves = run(inputs())
+    torch.cuda.synchronize()
+    fill = [torch.full((1 << 20,), math.nan, device="cuda") for _ in range(4)]    # takes what was freed
+    got = torch.autograd.grad(out, leaves, dout)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    del fill
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("Tq,Tk,D", [(300, 70, 64), (70, 300, 128), (150, 150, 200)])
+def test_bias_gradient_of_shared_key_heads(dtype, Tq, Tk, D):
+    """The table's gradient where a workgroup's share begins or ends inside a head's queries."""
+    table = normal(9, 32, 6)
+    run_case(dtype, 1, 6, 2, Tq, Tk, D, table=table, lens=torch.tensor([Tk - 3]).cuda())
+    run_case(dtype, 2, 6, 1, Tq, Tk, D, table=table, causal=True, bidirectional=False, max_distance=1024)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("D", [64, 128, 200])
+def test_table_gradient_alone(dtype, D):
+    q, k, v, dout = (normal(i, 2, 4, 200, D, dtype=dtype) for i in range(4))
+    leaves = [x.detach().requires_grad_() for x in (q, k, v, normal(4, 32, 4))]
+    want = torch.autograd.grad(A.attention(*leaves[:3], bias_table=leaves[3]), leaves, dout)[3]
+    got = torch.autograd.grad(A.attention(q, k, v, bias_table=leaves[3]), leaves[3], dout)[0]
+    assert torch.equal(got, want)

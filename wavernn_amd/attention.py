@@ -148,7 +148,7 @@ class _Attention(torch.autograd.Function):
             lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device)
             desc = _desc(q, k, v, table, key_mask, key_lens, q_start, causal, scale, max_distance, bidirectional)
             out = _forward(desc, q, lse)
-        ctx.desc = desc      # addresses of the saved tensors, which live as long as the node
+        ctx.rule = (causal, scale, max_distance, bidirectional)
         ctx.save_for_backward(q, k, v, table, key_mask, key_lens, q_start, out, lse)
         ctx.mark_non_differentiable(lse)
         ctx.set_materialize_grads(False)    # lse gets none: no tensor of zeros for it
@@ -164,7 +164,12 @@ class _Attention(torch.autograd.Function):
             return (torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v), torch.zeros_like(table) if want_table else None) + (None,) * 7
         lib = _lib.load()
         with _on(q.device):
-            dout = _rows(dout)
+            # saved-tensor hooks (offloading, checkpointing) hand other tensors back than were saved, in other places and strides
+            q, k, v, out, dout = _rows(q), _rows(k), _rows(v), _rows(out), _rows(dout)
+            if key_mask is not None and key_mask.stride(1) != 1:
+                key_mask = key_mask.contiguous()
+            lse, table, key_lens, q_start = (None if t is None else t.contiguous() for t in (lse, table, key_lens, q_start))
+            desc = _desc(q, k, v, table, key_mask, key_lens, q_start, *ctx.rule)
             dq, dk, dv, dtable = _empty_like(q), None, None, None
             if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
                 dk, dv = _empty_like(k), _empty_like(v)
@@ -174,9 +179,9 @@ class _Attention(torch.autograd.Function):
             grads = _GRADS.pack(out.data_ptr(), lse.data_ptr(), dout.data_ptr(), dq.data_ptr(), _ptr(dk), _ptr(dv), _ptr(dtable), *out.stride()[:3],
                                 *dout.stride()[:3], *dq.stride()[:3], *(zero if dk is None else dk.stride()[:3]),
                                 *(zero if dv is None else dv.stride()[:3]))
-            size = lib.wrnn_attention_backward_workspace_bytes(ctx.desc)
+            size = lib.wrnn_attention_backward_workspace_bytes(desc)
             space = _space(size, q.device)
-            if lib.wrnn_attention_backward(ctx.desc, grads, space.data_ptr(), size, _stream(q.device)):
+            if lib.wrnn_attention_backward(desc, grads, space.data_ptr(), size, _stream(q.device)):
                 _lib.check(1, "wrnn_attention_backward")
         return (dq, dk, dv, dtable) + (None,) * 7
 
@@ -201,7 +206,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, key_mask: Op
     key_mask [B, Tk] bool: True leaves a key out (``key_padding_mask`` of nn.MultiheadAttention).  key_lens [B]: keys at or past a
     row's length are left out.  causal: query i of row b sees keys up to position i + q_start[b]; q_start [B] defaults to Tk - Tq, the
     queries being the last positions.  A query that is left no key gives zeros and takes part in no gradient.  What lies at keys that are left
-    out for a whole row is never used, NaN and infinities included.
+    out for a whole row is never used, NaN and infinities included.  (An infinity at a key in use gives NaN where the formula in
+    float32 would keep it.)
     scale: 1 / sqrt(D) by default.
     bias_table [num_buckets, H] (``RelativePositionBias.weight``) adds table[bucket(j - (i + q_start[b])), h]; max_distance and
     bidirectional are its rule.  -inf in a table leaves its distances out.

@@ -124,8 +124,8 @@ extern "C" int wrnn_attention_forward(const wrnn_attention_desc* desc, void* out
   WRNN_REQUIRE(out && out_stride, "wrnn_attention_forward: null pointer");
   attn::plan(&p);
   const size_t need = attn::split_workspace(p);
-  WRNN_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "wrnn_attention_forward: workspace of %zu bytes, %zu are needed",
-               workspace_bytes, need);
+  WRNN_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && !((uintptr_t)workspace & 15)),
+               "wrnn_attention_forward: workspace of %zu bytes, %zu are needed, on 16 bytes", workspace_bytes, need);
   p.out = out, p.o_b = out_stride[0], p.o_h = out_stride[1], p.o_t = out_stride[2], p.lse = lse;
   p.part = static_cast<float*>(workspace);
   WRNN_REQUIRE(attn::rows_on_16(out, p.o_b, p.o_h, p.o_t, desc->dtype == WRNN_FLOAT32 ? 4 : 2), "wrnn_attention_forward: rows of out have to start on 16 bytes");
@@ -152,7 +152,8 @@ extern "C" int wrnn_attention_backward(const wrnn_attention_desc* desc, const wr
   WRNN_REQUIRE(g->out && g->lse && g->dout && g->dq && !g->dk == !g->dv, "wrnn_attention_backward: null pointer");
   WRNN_REQUIRE(!g->dtable || p.table, "wrnn_attention_backward: a table's gradient without a table");
   const size_t need = wrnn_attention_backward_workspace_bytes(desc);
-  WRNN_REQUIRE(workspace && workspace_bytes >= need, "wrnn_attention_backward: workspace of %zu bytes, %zu are needed", workspace_bytes, need);
+  WRNN_REQUIRE(workspace && workspace_bytes >= need && !((uintptr_t)workspace & 15),
+               "wrnn_attention_backward: workspace of %zu bytes, %zu are needed, on 16 bytes", workspace_bytes, need);
   const int es = desc->dtype == WRNN_FLOAT32 ? 4 : 2;
   auto on16 = [&](const void* x, const int64_t* st) { return attn::rows_on_16(x, st[0], st[1], st[2], es); };
   WRNN_REQUIRE(on16(g->out, g->out_stride) && on16(g->dout, g->dout_stride) && on16(g->dq, g->dq_stride) && on16(g->dk, g->dk_stride) && on16(g->dv, g->dv_stride),
