@@ -146,3 +146,35 @@ def test_models_take_the_position_bias():
     for k in gen["stock"]:
         assert gen["stock"][k].shape == gen["fused"][k].shape
         assert G.rel_err(gen["fused"][k].cpu().numpy(), gen["stock"][k].cpu().numpy()) < 1e-4, k
+
+
+@gpu
+def test_auto_path_leaves_what_does_not_fit_to_the_stock_path():
+    """Types that the operators do not take, in the weights or by autocast, and masks that are added rather than leaving keys out."""
+    torch.manual_seed(0)
+    block = FM.FFTBlock(32, 2, 3, 1, 64, dropout=0.).cuda()
+    x, mask = torch.randn(20, 3, 32, device="cuda"), torch.zeros(3, 20, device="cuda")
+    mask[1, 11:] = -np.inf
+
+    def both(*args):
+        out = []
+        for path in ("stock", "auto"):
+            FM.set_attention_path(block, path)
+            out.append(block(*args))
+        return out
+
+    with torch.autocast("cuda", torch.float16):
+        a, b = both(x)
+        assert torch.equal(a, b)
+        with pytest.raises(RuntimeError, match="float32 or bfloat16"):
+            FM.set_attention_path(block, "fused")(x)
+    a, b = both(x, mask)
+    assert torch.equal(a, b)
+    with pytest.raises(RuntimeError, match="bool"):
+        FM.set_attention_path(block, "fused")(x, mask)
+    block.half()
+    a, b = both(x.half())
+    assert torch.equal(a, b)
+    block.double()
+    a, b = both(x.double())
+    assert torch.equal(a, b)

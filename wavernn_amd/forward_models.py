@@ -70,9 +70,14 @@ class FFTBlock(nn.Module):  # common_layers.py:148-185: post-norm self-attention
         self.activation = nn.ReLU()
         self.attention_path = 'stock'
 
-    def _why_not_fused(self, src) -> Optional[str]:
+    def _why_not_fused(self, src, src_pad_mask) -> Optional[str]:
         if src.device.type != 'cuda':
             return "it runs only on an MI355X (HIP) device"
+        dtype = torch.get_autocast_dtype('cuda') if torch.is_autocast_enabled('cuda') else src.dtype
+        if dtype not in (torch.float32, torch.bfloat16):
+            return f"it takes float32 or bfloat16, not {dtype}"
+        if src_pad_mask is not None and src_pad_mask.dtype != torch.bool:
+            return f"it takes a bool mask, not {src_pad_mask.dtype}"
         if self.training and self.self_attn.dropout > 0:
             return "it has no dropout on the probabilities (train with dropout=0, or on the stock path)"
         if self.self_attn.head_dim > MAX_HEAD_DIM:
@@ -80,7 +85,7 @@ class FFTBlock(nn.Module):  # common_layers.py:148-185: post-norm self-attention
         return None
 
     def _attend(self, src, src_pad_mask, position_bias):
-        why = self._why_not_fused(src) if self.attention_path != 'stock' else ''
+        why = self._why_not_fused(src, src_pad_mask) if self.attention_path != 'stock' else ''
         if why and self.attention_path == 'fused':
             raise RuntimeError(f"FFTBlock: the fused attention path does not apply: {why}")
         if why is not None:
@@ -112,7 +117,7 @@ def set_attention_path(module: nn.Module, path: str) -> nn.Module:
     """How every FFTBlock under ``module`` runs its self-attention (no counterpart in the reference):
     'stock'  nn.MultiheadAttention (the default);
     'fused'  wavernn_amd.attention, forward and backward: the scores never reach memory; an error where it does not apply (training with
-             dropout > 0, which it has none of; head dimensions over 256);
+             dropout > 0, which it has none of; head dimensions over 256; types other than float32 and bfloat16; masks that are not bool);
     'auto'   'fused' where it applies, 'stock' elsewhere.
     They agree to rounding, but for batch rows whose every position is masked: 'stock' gives NaN there, 'fused' attends to nothing."""
     if path not in ATTENTION_PATHS:
