@@ -84,7 +84,8 @@ struct BackwardShape {
   static constexpr int WAVES = DP * NP <= 64 ? 2 : 1;  // per SIMD
   // dS of the dq kernel.  A query's keys share the shift along it that its softmax gives them, and the errors of dS add up along it, the more so
   // the fewer columns there are (dq off by 2.5e-3 .. 3.3e-3 of its norm up to 64): there it keeps 16 bits (1.8e-3 .. 2.1e-3; the backward pass at
-  // 2 x 16 heads, 4096 x 4096 x 64 takes 611 us instead of 541).  At 128 columns one rounding gives 2.4e-3.
+  // 2 x 16 heads, 4096 x 4096 x 64 takes 611 us instead of 541).  At 128 columns, where the matrix instructions bound the kernel, one rounding
+  // stays: 2.4e-3, up to 2.9e-3 where a query has some ten keys and delta's error weighs the most.
   using QueryWeights = std::conditional_t<(NP == 1 && DP == 64), Weights2, Weights<T>>;
 };
 
