@@ -5,6 +5,15 @@
 // Two kernels, each with its own output rows stationary, so that every sum has one owner and one order (no atomics: the same
 // inputs give the same bits): dq walks the keys, dk / dv walk the queries of all heads that share them.  Seven tile products
 // in place of the five of a form that adds dq up in memory.
+//
+// Bound by the matrix instructions (the rates count all seven products):
+//   bfloat16  2 x 16 heads, 4096 x 4096 x 128  1247 us  771 TFLOP/s (a library product of 8192 x 8192 x 8192: 1173)
+//                                     x 64      623 us  772, and the eighth product of dS's second plane
+//             2 x 8 heads,  4096 x 4096 x 256  2300 us  420
+//   float32   2 x 16 heads, 2048 x 2048 x 128  1295 us  186 (six partial products: 195 is the library product's sixth)
+//                                     x 64      664 us  181
+//             2 x 8 heads,  2048 x 2048 x 256  1780 us  135
+// Past 128 columns one tile buffer is all that fits in float32, so its conversion is not hidden, and the two waves of a row meet twice a round.
 #pragma once
 #include "attention_tile.h"
 

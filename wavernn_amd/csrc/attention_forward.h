@@ -2,6 +2,17 @@
 //
 // One pass over the keys with a running maximum and sum per query (kept in 32 bits, in units of log2 so that the exponential is
 // one v_exp_f32).  The [Tq, Tk] scores only ever exist as 32 x 32 tiles in registers (attention_tile.h).
+//
+// Long sequences are bound by the matrix instructions and, the fewer columns the more, by the softmax's vector instructions between them (bfloat16
+// at 128 columns: 120 of those to 16 products a subtile).  Measured, forward only:
+//   bfloat16  2 x 16 heads, 4096 x 4096 x 128   302 us  910 TFLOP/s (a library product of 8192 x 8192 x 8192: 1173)
+//                                     x 64      183 us  750
+//             2 x 8 heads,  4096 x 4096 x 256   410 us  670
+//   float32   2 x 16 heads, 2048 x 2048 x 128   368 us  187 (six partial products: 195 is the library product's sixth)
+//                                     x 64      186 us  185
+//             2 x 8 heads,  2048 x 2048 x 256   457 us  150
+// Single tokens over a cache are bound by the reading of it: 8 rows, 16 heads on 4, 8191 keys of 128 columns in bfloat16 32 us, the joining kernel's 4
+// included (134 MB at 4.2 TB/s; a large copy moves 4.8).
 #pragma once
 #include "attention_tile.h"
 
@@ -38,7 +49,8 @@ struct Running {
 // Shapes of a workgroup.
 //   wide   4 waves, 32 queries each, all against every 32 keys of a tile: a tile in LDS serves 128 queries.
 //   narrow 32 query columns, the waves on different 32 keys of a tile, joined at the end; the columns may hold the queries of all heads that
-//          share k and v (p.pack).  For single tokens and few queries.
+//          share k and v (p.pack).  For single tokens and few queries.  (For more than 32 queries the wide one is the faster also where only a few
+//          workgroups run: 32 x 2 heads, 150 x 150 x 64 in float32 17 against 28 us.)
 // In either the keys may be divided over workgroups (p.splits), whose sums attention_join_kernel adds up.
 template <class T, int DP, bool WIDE>
 struct ForwardShape {

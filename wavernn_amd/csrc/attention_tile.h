@@ -1,4 +1,4 @@
-// Shared device pieces of the attention kernels (attention.hip, attention_backward.hip).
+// Shared pieces of the attention kernels (attention_forward.h, attention_backward.h) and of the dense position bias (relative_bias.hip).
 //
 // Everything is built on one wave tile: 32 "stationary" rows (queries in the forward pass and for dq, keys for dk / dv), one per
 // lane column, against 32 "moving" rows.  With v_mfma_f32_32x32x16_bf16 the product  X(moving) * Y(stationary)^T  leaves a lane with
@@ -10,7 +10,7 @@
 //
 // float32 goes through the same instructions: a value is the sum of three bfloat16 (8 bits of mantissa each), and a product the six partial
 // products that reach 2^-16 of it, added in 32 bits, smallest first.  What is left out is 2^-23 of a product on average and 2^-20 at
-// most, the result as exact as the 32-bit matrix instruction's (measured: 5e-7 of the norm either way), and 16 columns of a 32 x 32 tile take
+// most, the result as exact as the 32-bit matrix instruction's (out at 4096 x 4096 x 128: 8e-7 of the norm, plain float32 products 1.2e-6), and 16 columns of a 32 x 32 tile take
 // 6 x 32 cycles where that one takes 8 x 64.
 //
 // Moving tiles lie in LDS row by row in 16-byte chunks of 8 bfloat16 (three planes for float32).  The first product reads chunk 2c + half of
