@@ -53,8 +53,9 @@ static size_t split_workspace(const Params& p) {
 
 // blocks of a workgroup's rows: two waves share a row past 128 columns (BackwardShape)
 static int row_blocks(const Params& p, int rows) { return p.D > 128 ? (rows + 63) / 64 : (rows + 127) / 128; }
-static void plan_backward(Params* p) {
-  p->dq_splits = shares((int64_t)p->B * p->H * row_blocks(*p, p->Tq), (p->Tk + 31) / 32, 4);
+static void plan_backward(Params* p, int dtype) {
+  // (bfloat16 with few keys: a query's row sum of dS has to lie in one workgroup, BackwardShape; the joining launch costs what shares would save)
+  p->dq_splits = dtype == WRNN_BFLOAT16 && p->Tk <= kFewKeys ? 1 : shares((int64_t)p->B * p->H * row_blocks(*p, p->Tq), (p->Tk + 31) / 32, 4);
   // (causality: the first keys' blocks are the longest by far; half as long they leave the others time to fill up)
   const int64_t blocks = (int64_t)p->B * p->Hkv * row_blocks(*p, p->Tk);
   p->dkv_splits = shares(p->causal ? (blocks + 1) / 2 : blocks, (int64_t)((p->Tq + 31) / 32) * p->group, 4);
@@ -140,7 +141,7 @@ extern "C" int wrnn_attention_forward(const wrnn_attention_desc* desc, void* out
 extern "C" size_t wrnn_attention_backward_workspace_bytes(const wrnn_attention_desc* desc) {
   attn::Params p;
   if (attention_params(desc, &p, "wrnn_attention_backward_workspace_bytes") || !p.B || !p.H || !p.Tq) return 0;
-  attn::plan_backward(&p);
+  attn::plan_backward(&p, desc->dtype);
   return attn::delta_bytes(p) + attn::table_bytes(p) + attn::dq_bytes(p) + attn::dkv_bytes(p);
 }
 
@@ -169,7 +170,7 @@ extern "C" int wrnn_attention_backward(const wrnn_attention_desc* desc, const wr
   p.dq = g->dq, p.dq_b = g->dq_stride[0], p.dq_h = g->dq_stride[1], p.dq_t = g->dq_stride[2];
   p.dk = g->dk, p.dk_b = g->dk_stride[0], p.dk_h = g->dk_stride[1], p.dk_t = g->dk_stride[2];
   p.dv = g->dv, p.dv_b = g->dv_stride[0], p.dv_h = g->dv_stride[1], p.dv_t = g->dv_stride[2];
-  attn::plan_backward(&p);
+  attn::plan_backward(&p, desc->dtype);
   p.lse = const_cast<float*>(g->lse);
   char* w = static_cast<char*>(workspace);
   p.delta = reinterpret_cast<float*>(w);

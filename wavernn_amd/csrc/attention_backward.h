@@ -91,11 +91,12 @@ struct BackwardShape {
   using TL = Tile<T, DP, BM>;
   static constexpr size_t EXCHANGE = SLICES > 1 ? 4 * 16 * 64 * 4 : 0, TILES = 2 * BUFS * TL::BYTES + EXCHANGE;
   static constexpr int WAVES = DP * NP <= 64 ? 2 : 1;  // per SIMD
-  // dS of the dq kernel.  A query's keys share the shift along it that its softmax gives them, and the errors of dS add up along it, the more so
-  // the fewer columns there are (dq off by 2.5e-3 .. 3.3e-3 of its norm up to 64): there it keeps 16 bits (1.8e-3 .. 2.1e-3; the backward pass at
-  // 2 x 16 heads, 4096 x 4096 x 64 takes 611 us instead of 541).  At 128 columns, where the matrix instructions bound the kernel, one rounding
-  // stays: 2.4e-3, up to 2.9e-3 where a query has some ten keys and delta's error weighs the most.
-  using QueryWeights = std::conditional_t<(NP == 1 && DP == 64), Weights2, Weights<T>>;
+  // dS of the dq kernel in bfloat16.  A query's keys share the shift along it that its softmax gives them, and the errors of dS add up along it,
+  // the more so the fewer columns there are: with one plane dq is off by 2.5e-3 .. 3.3e-3 of its norm up to 64 columns, by 2.4e-3 .. 2.9e-3 above,
+  // the most where a query has few keys (rounding dq itself: 1.7e-3).  With two, 1.7e-3 .. 2.1e-3: always up to 64 columns (2 x 16 heads,
+  // 4096 x 4096: 541 -> 611 us), above that, where the matrix instructions bound the kernel (1253 -> 1407 us), only for blocks of queries that
+  // reach at most kFewKeys keys.  Those hand on the corrected delta, too.
+  static constexpr bool FINE = NP == 1 && DP == 64;
 };
 
 // Both waves' parts of a sum added up.  `mine` and `other` are the waves' places; what a wave hands in stays until the other has read it, so the
@@ -147,15 +148,15 @@ __device__ __forceinline__ void products_shadow(const char* x, const char* y, co
 }
 
 // dq: queries stationary, key tiles through LDS.  delta = rowsum(dout * out) carries the rounding of out and of the probabilities behind it.  That is
-// less than the rounding of dq itself, but the table's gradient adds it up over all rows in the buckets that hold most of a row's keys.
-// With BIAS == 2 the kernel therefore also sums dS over each row - what delta is off by, as the probabilities add up to one - and hands the
-// corrected delta to the next kernel, which makes the table's gradient: the adds are hidden, a second walk over the keys for it took twice the time.
+// less than the rounding of dq itself, but the table's gradient adds it up over all rows in the buckets that hold most of a row's keys, and in
+// bfloat16 with few keys dk shows it (2.8e-3 of its norm, without 2.4e-3).  There the kernel also sums dS over each row - what delta is off by, as the
+// probabilities add up to one - and the next kernel, which makes dk, dv and the table's gradient, works with the corrected delta: the adds are hidden
+// or few, a second walk over the keys for it took twice the time.
 template <class T, int DP, int BIAS>
 __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_dq_kernel(Params p) {
   using S = BackwardShape<T, DP>;
   using TL = typename S::TL;
   constexpr int BN = S::BM, NC2 = S::NC2, BUFS = S::BUFS, NT = S::THREADS;
-  using DS = typename S::QueryWeights;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   char* kt = smem;
   char* vt = smem + BUFS * TL::BYTES;
@@ -223,60 +224,70 @@ __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_
   store(t0, use);
   if (S::EARLY) load(t0 + 1, use1);
   __syncthreads();
-  for (int t = t0; t < t1; ++t) {
-    const char *kk = kt + (t & (BUFS - 1)) * TL::BYTES, *vv = vt + (t & (BUFS - 1)) * TL::BYTES;
-    use2 = keys.next((t + 2) * BN);
-    if (!S::EARLY) load(t + 1, use1);
+  auto walk = [&](auto few) {
+    constexpr bool exact = decltype(few)::value;
+    for (int t = t0; t < t1; ++t) {
+      const char *kk = kt + (t & (BUFS - 1)) * TL::BYTES, *vv = vt + (t & (BUFS - 1)) * TL::BYTES;
+      use2 = keys.next((t + 2) * BN);
+      if (!S::EARLY) load(t + 1, use1);
 #pragma unroll
-    for (int x = 0; x < S::NS; ++x) {
-      const int sub = x, key0 = t * BN + sub * 32;
-      const bool work = key0 < end && !(p.causal && key0 > pos_hi);
-      f32x16 raw = {}, dp = {};
-      if constexpr (S::EARLY) {
-        char *kn = kt + ((t + 1) & (BUFS - 1)) * TL::BYTES, *vn = vt + ((t + 1) & (BUFS - 1)) * TL::BYTES;
-        products_shadow<TL, NC2>(kk, vv, q, go, raw, dp, sk, sv, kn, vn, col, half, tid);
-        load(t + 2, use2);
-      } else if (work) {
+      for (int x = 0; x < S::NS; ++x) {
+        const int sub = x, key0 = t * BN + sub * 32;
+        const bool work = key0 < end && !(p.causal && key0 > pos_hi);
+        f32x16 raw = {}, dp = {};
+        if constexpr (S::EARLY) {
+          char *kn = kt + ((t + 1) & (BUFS - 1)) * TL::BYTES, *vn = vt + ((t + 1) & (BUFS - 1)) * TL::BYTES;
+          products_shadow<TL, NC2>(kk, vv, q, go, raw, dp, sk, sv, kn, vn, col, half, tid);
+          load(t + 2, use2);
+        } else if (work) {
 #pragma unroll
-        for (int c = 0; c < NC2; ++c)
-          mma2(TL::row_chunk(kk, sub * 32 + col, ch0 + 2 * c + half), q.get(c), raw, TL::row_chunk(vv, sub * 32 + col, ch0 + 2 * c + half), go.get(c),
-               dp, [](int) {});
-      }
-      if constexpr (S::SLICES > 1) {
-        exchange(raw, mine, other, lane);
-        exchange(dp, other, mine, lane);
-      }
-      if (S::EARLY || work) {
-        float pr[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) pr[i] = raw[i];
-        finish_scores<BIAS != 0>(p, pr, key0, pos, pos_lo, pos_hi, use.of(sub), lut, half);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) pr[i] = __builtin_amdgcn_exp2f(pr[i] - lse2);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          pr[i] *= dp[i] - delta;
-          if (BIAS == 2) off_by += pr[i];
+          for (int c = 0; c < NC2; ++c)
+            mma2(TL::row_chunk(kk, sub * 32 + col, ch0 + 2 * c + half), q.get(c), raw, TL::row_chunk(vv, sub * 32 + col, ch0 + 2 * c + half), go.get(c),
+                 dp, [](int) {});
         }
-        if constexpr (S::EARLY)
-          column_product_shadow<TL, S::DT, 0>(kk, 0, d0, [&](int i) { return pr[i]; }, acc, lane, nullptr, [](int) {});
-        else
-          column_product<T, TL>(kk, sub * 32, d0, DS(pr), acc, lane);
+        if constexpr (S::SLICES > 1) {
+          exchange(raw, mine, other, lane);
+          exchange(dp, other, mine, lane);
+        }
+        if (S::EARLY || work) {
+          float pr[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) pr[i] = raw[i];
+          finish_scores<BIAS != 0>(p, pr, key0, pos, pos_lo, pos_hi, use.of(sub), lut, half);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) pr[i] = __builtin_amdgcn_exp2f(pr[i] - lse2);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) pr[i] *= dp[i] - delta;
+          if constexpr (BIAS == 2 || exact)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) off_by += pr[i];
+          if constexpr (S::EARLY)
+            column_product_shadow<TL, S::DT, 0>(kk, 0, d0, [&](int i) { return pr[i]; }, acc, lane, nullptr, [](int) {});
+          else
+            column_product<T, TL>(kk, sub * 32, d0, std::conditional_t<S::FINE || exact, Weights2, Weights<T>>(pr), acc, lane);
+        }
       }
+      if (!S::EARLY) {
+        if (BUFS == 1) __syncthreads();
+        store(t + 1, use1);
+      }
+      use = use1;
+      use1 = use2;
+      __syncthreads();
     }
-    if (!S::EARLY) {
-      if (BUFS == 1) __syncthreads();
-      store(t + 1, use1);
-    }
-    use = use1;
-    use1 = use2;
-    __syncthreads();
+  };
+  // (two loops: a choice inside would have both its ways' sums copied in every round)
+  if constexpr (S::NP == 1) {
+    if (end <= kFewKeys) walk(std::true_type());
+    else walk(std::false_type());
+  } else {
+    walk(std::false_type());
   }
-  const float off_by_sum = both_sum(off_by);
+  off_by = both_sum(off_by);
+  // (a share's sum is only part of a row's: with BIAS == 2 the next kernel adds them up, otherwise such rows do without)
   if (half == 0 && d0 == 0 && qi < p.Tq && (BIAS == 2 || share == 0)) {
-    float x = share == 0 ? delta : 0.f;
-    if (BIAS == 2) x += off_by_sum;
-    p.delta[((int64_t)(BIAS == 2 ? share : 0) * p.B * p.H + bh) * p.Tq + qi] = x;
+    const float whole = BIAS == 2 || p.dq_splits == 1 ? off_by : 0.f;
+    p.delta[((int64_t)(BIAS == 2 ? share : 0) * p.B * p.H + bh) * p.Tq + qi] = share == 0 ? delta + whole : whole;
   }
   if (qi < p.Tq)
     store_rows<S>(acc, reinterpret_cast<T*>(p.dq) + b * p.dq_b + h * p.dq_h + qi * p.dq_t,
