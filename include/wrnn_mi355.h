@@ -469,9 +469,10 @@ int wrnn_mol_sample(const float* y, const float* u_mix, const float* u_logistic,
  * every query of the row) causality leave out are never used, whatever they hold.
  *
  * All pointers are device pointers of `dtype` unless stated; strides count elements for [batch, head, position], the head
- * dimension is contiguous, rows start on 16 bytes and are whole in them (head_dim a multiple of 8 bfloat16 or 4 float32; a
- * caller with other rows pads them with zeros, which changes no score).  Sums, maxima and exponentials are held in 32 bits; with WRNN_BFLOAT16 the probabilities and the
- * scores' gradients are rounded to bfloat16 where they enter a matrix product.
+ * dimension is contiguous, rows start on the bytes of four elements (16 in float32, 8 in bfloat16); head_dim is a multiple of 4,
+ * in bfloat16 8 at least (a caller with other rows pads them with zeros, which changes no score).  Sums, maxima and exponentials
+ * are held in 32 bits; with WRNN_BFLOAT16 the probabilities and the scores' gradients are rounded to bfloat16 where they
+ * enter a matrix product.
  *
  * Buckets: a distance d = |j - (i + start_b)| below E = side / 2 has a bucket of its own, above it a bucket E + (number of
  * bucket_edges <= d); side = num_buckets, or num_buckets / 2 with `bidirectional`, where keys behind the query (positive

@@ -502,3 +502,26 @@ def test_table_gradient_alone(dtype, D):
     want = torch.autograd.grad(A.attention(*leaves[:3], bias_table=leaves[3]), leaves, dout)[3]
     got = torch.autograd.grad(A.attention(q, k, v, bias_table=leaves[3]), leaves[3], dout)[0]
     assert torch.equal(got, want)
+
+
+@gpu
+@pytest.mark.parametrize("D", [8, 12, 36, 60, 64, 100, 132, 196, 252])
+@pytest.mark.parametrize("Tq,Tk", [(1, 300), (70, 41), (200, 600)])
+def test_rows_that_start_on_eight_bytes(D, Tq, Tk):
+    """bfloat16 rows between 16-byte borders, with NaN before and behind each and at masked keys; whole fours of elements, so nothing is copied."""
+    def rows(seed, heads, T):
+        t = torch.full((2, T, heads, D + 8), math.nan, dtype=BF16, device="cuda")
+        t[..., 4:4 + D] = normal(seed, 2, T, heads, D, dtype=BF16)
+        return t[..., 4:4 + D].permute(0, 2, 1, 3)
+    q, k, v, dout = rows(0, 6, Tq), rows(1, 3, Tk), rows(2, 3, Tk), rows(3, 6, Tq)
+    assert A._rows(q) is q and A._rows(k) is k
+    mask = torch.zeros(2, Tk, dtype=torch.bool, device="cuda")
+    mask[0, 5:7] = mask[1, -3:] = True
+    k, v = (x.masked_fill(mask[:, None, :, None], math.nan) for x in (k, v))
+    clean = [x.detach().masked_fill(mask[:, None, :, None], 0.) for x in (k, v)]
+    q, k, v = (x.detach().requires_grad_() for x in (q, k, v))
+    out = A.attention(q, k, v, key_mask=mask)
+    want = reference(q, clean[0].requires_grad_(), clean[1].requires_grad_(), dout, key_mask=mask)
+    check("out", out, want["out"])
+    for name, g in zip(("dq", "dk", "dv"), torch.autograd.grad(out, (q, k, v), dout)):
+        check(name, g, want[name])

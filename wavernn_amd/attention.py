@@ -58,14 +58,13 @@ def _on_gpu(t: torch.Tensor, what: str) -> None:
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
-    """The kernels take any strides of batch, head and position; rows are contiguous, start on 16 bytes and are whole in them.  A
-    copy, padded with zeros, where that does not hold."""
-    e = t.element_size()
+    """The kernels take any strides of batch, head and position; rows are contiguous, hold whole fours of elements (16 bytes at
+    least) and start on the bytes of four.  A copy, padded with zeros, where that does not hold."""
     s, n = t.stride(), t.shape
-    if ((s[3] == 1 or n[3] == 1) and n[3] * e % 16 == 0 and t.data_ptr() % 16 == 0 and s[2] < 1 << 22
-            and all(s[i] * e % 16 == 0 or n[i] == 1 for i in range(3))):
+    if (s[3] == 1 and not n[3] % 4 and (n[3] > 4 or t.element_size() == 4) and not t.data_ptr() % (4 * t.element_size()) and s[2] < 1 << 22
+            and not ((s[0] % 4 and n[0] != 1) or (s[1] % 4 and n[1] != 1) or (s[2] % 4 and n[2] != 1))):
         return t
-    pad = -n[3] % (16 // e)
+    pad = max(-n[3] % 4, 16 // t.element_size() - n[3])
     return nn.functional.pad(t, (0, pad)) if pad else t.contiguous() if not t.is_contiguous() else t.clone()
 
 

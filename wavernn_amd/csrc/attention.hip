@@ -100,9 +100,9 @@ int attention_params(const wrnn_attention_desc* d, attn::Params* p, const char* 
   p->scale = d->scale, p->scale2 = d->scale * kLog2e;
   p->key_mask = d->key_mask, p->mask_b = d->key_mask_stride, p->key_lens = d->key_lens, p->q_start = d->q_start;
   const int es = d->dtype == WRNN_FLOAT32 ? 4 : 2;
-  WRNN_REQUIRE(d->head_dim * es % 16 == 0 && rows_on_16(p->q, p->q_b, p->q_h, p->q_t, es) && rows_on_16(p->k, p->k_b, p->k_h, p->k_t, es) &&
-                   rows_on_16(p->v, p->v_b, p->v_h, p->v_t, es),
-               "%s: rows have to start on 16 bytes and be whole in them", who);
+  WRNN_REQUIRE(d->head_dim % 4 == 0 && d->head_dim * es >= 16 && rows_on_four(p->q, p->q_b, p->q_h, p->q_t, es) &&
+                   rows_on_four(p->k, p->k_b, p->k_h, p->k_t, es) && rows_on_four(p->v, p->v_b, p->v_h, p->v_t, es),
+               "%s: rows have to hold whole fours of elements, 16 bytes at least, and start on the bytes of four", who);
   if (d->bias_table) {
     if (bias_params(p, d->num_buckets, d->max_distance, d->bidirectional, d->bucket_edges, who)) return 1;
     p->table = d->bias_table;
@@ -133,7 +133,7 @@ extern "C" int wrnn_attention_forward(const wrnn_attention_desc* desc, void* out
                "wrnn_attention_forward: workspace of %zu bytes, %zu are needed, on 16 bytes", workspace_bytes, need);
   p.out = out, p.o_b = out_stride[0], p.o_h = out_stride[1], p.o_t = out_stride[2], p.lse = lse;
   p.part = static_cast<float*>(workspace);
-  WRNN_REQUIRE(attn::rows_on_16(out, p.o_b, p.o_h, p.o_t, desc->dtype == WRNN_FLOAT32 ? 4 : 2), "wrnn_attention_forward: rows of out have to start on 16 bytes");
+  WRNN_REQUIRE(attn::rows_on_four(out, p.o_b, p.o_h, p.o_t, desc->dtype == WRNN_FLOAT32 ? 4 : 2), "wrnn_attention_forward: rows of out have to start on the bytes of four elements");
   const hipStream_t st = static_cast<hipStream_t>(stream);
   return desc->dtype == WRNN_FLOAT32 ? attn::forward<float>(p, st) : attn::forward<__bf16>(p, st);
 }
@@ -160,9 +160,9 @@ extern "C" int wrnn_attention_backward(const wrnn_attention_desc* desc, const wr
   WRNN_REQUIRE(workspace && workspace_bytes >= need && !((uintptr_t)workspace & 15),
                "wrnn_attention_backward: workspace of %zu bytes, %zu are needed, on 16 bytes", workspace_bytes, need);
   const int es = desc->dtype == WRNN_FLOAT32 ? 4 : 2;
-  auto on16 = [&](const void* x, const int64_t* st) { return attn::rows_on_16(x, st[0], st[1], st[2], es); };
-  WRNN_REQUIRE(on16(g->out, g->out_stride) && on16(g->dout, g->dout_stride) && on16(g->dq, g->dq_stride) && on16(g->dk, g->dk_stride) && on16(g->dv, g->dv_stride),
-               "wrnn_attention_backward: rows have to start on 16 bytes");
+  auto whole = [&](const void* x, const int64_t* st) { return attn::rows_on_four(x, st[0], st[1], st[2], es); };
+  WRNN_REQUIRE(whole(g->out, g->out_stride) && whole(g->dout, g->dout_stride) && whole(g->dq, g->dq_stride) && whole(g->dk, g->dk_stride) && whole(g->dv, g->dv_stride),
+               "wrnn_attention_backward: rows have to start on the bytes of four elements");
   for (const int64_t* x : {g->out_stride, g->dout_stride, g->dq_stride, g->dk_stride, g->dv_stride})
     WRNN_REQUIRE(x[2] >= 0 && x[2] < attn::kMaxRowStride, "wrnn_attention_backward: position strides are in 0 .. 2^22 - 1 elements");
   p.o_in = g->out, p.oi_b = g->out_stride[0], p.oi_h = g->out_stride[1], p.oi_t = g->out_stride[2];

@@ -95,8 +95,9 @@ struct BackwardShape {
   // the more so the fewer columns there are: with one plane dq is off by 2.5e-3 .. 3.3e-3 of its norm up to 64 columns, by 2.4e-3 .. 2.9e-3 above,
   // the most where a query has few keys (rounding dq itself: 1.7e-3).  With two, 1.7e-3 .. 2.1e-3: always up to 64 columns (2 x 16 heads,
   // 4096 x 4096: 541 -> 611 us), above that, where the matrix instructions bound the kernel (1253 -> 1407 us), only for blocks of queries that
-  // reach at most kFewKeys keys.  Those hand on the corrected delta, too.
+  // reach at most FEW keys.  Those hand on the corrected delta, too.
   static constexpr bool FINE = NP == 1 && DP == 64;
+  static constexpr int FEW = FINE ? kFewKeys : 2 * kFewKeys;
 };
 
 // Both waves' parts of a sum added up.  `mine` and `other` are the waves' places; what a wave hands in stays until the other has read it, so the
@@ -120,7 +121,7 @@ __device__ __forceinline__ void store_rows(const f32x16 (&acc)[S::DT], T* row, f
   for (int dt = 0; dt < S::DT; ++dt)
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      const int d = d0 + dt * 32 + 8 * g + 4 * half;
+      const int d = column_of<T>(d0 + dt * 32 + 8 * g + 4 * half, D);
       const float x[4] = {acc[dt][4 * g] * scale, acc[dt][4 * g + 1] * scale, acc[dt][4 * g + 2] * scale, acc[dt][4 * g + 3] * scale};
       if (part) store4<float>(part, d, D, x[0], x[1], x[2], x[3]);
       else store4<T>(row, d, D, x[0], x[1], x[2], x[3]);
@@ -278,7 +279,7 @@ __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_
   };
   // (two loops: a choice inside would have both its ways' sums copied in every round)
   if constexpr (S::NP == 1) {
-    if (end <= kFewKeys) walk(std::true_type());
+    if (end <= S::FEW) walk(std::true_type());
     else walk(std::false_type());
   } else {
     walk(std::false_type());

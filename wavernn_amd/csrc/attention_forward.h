@@ -214,7 +214,7 @@ __global__ __launch_bounds__((ForwardShape<T, DP, WIDE>::THREADS), (ForwardShape
       for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
         for (int g = 0; g < 4; ++g)
-          store4<T>(orow, dt * 32 + 8 * g + 4 * half, p.D, acc[dt][4 * g] * inv, acc[dt][4 * g + 1] * inv, acc[dt][4 * g + 2] * inv,
+          store4<T>(orow, column_of<T>(dt * 32 + 8 * g + 4 * half, p.D), p.D, acc[dt][4 * g] * inv, acc[dt][4 * g + 1] * inv, acc[dt][4 * g + 2] * inv,
                     acc[dt][4 * g + 3] * inv);
       if (half == 0 && p.lse) p.lse[row] = l == 0.f ? -INFINITY : (run.m + log2f(l)) * kLn2;
     } else {
@@ -268,7 +268,7 @@ __global__ __launch_bounds__((ForwardShape<T, DP, WIDE>::THREADS), (ForwardShape
 #pragma unroll
       for (int w = 1; w < S::WK; ++w) x += *reinterpret_cast<const f32x4*>(sums + (w * 32 + c2) * LD + d);
       if (splits == 1)
-        store4<T>(orow, d, p.D, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+        store4<T>(orow, column_of<T>(d, p.D), p.D, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
       else
         *reinterpret_cast<f32x4*>(to + 4 + d) = x;
     }
@@ -316,8 +316,10 @@ __global__ __launch_bounds__(256) void attention_join_kernel(Params p) {
   const int qi = row % p.Tq, h = (row / p.Tq) % p.H, b = row / p.Tq / p.H;
   T* orow = reinterpret_cast<T*>(p.out) + b * p.o_b + h * p.o_h + qi * p.o_t;
 #pragma unroll
-  for (int e = 0; e < E; ++e)
-    if (lane * E + e < p.D) orow[lane * E + e] = (T)(x[e] * inv);
+  for (int e = 0; e < E; ++e) {
+    const int c = lane * E + e, d = column_of<T>(c & ~3, p.D);
+    if (d >= 0) orow[d + (c & 3)] = (T)(x[e] * inv);
+  }
   if (lane == 0 && p.lse) p.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 

@@ -202,13 +202,18 @@ __device__ __forceinline__ float both_sum(float x) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// Chunk ch (8 elements) of a row of D; what lies past D is zero and not read.  Rows start on 16 bytes and D is whole in them.
+// Chunk ch (8 elements) of a stationary row of D; what lies past D is zero and not read.  Rows are whole in four elements and start on the bytes of
+// four.  Half a chunk at the end of a bfloat16 row: a moving row's is requested as the row's last 16 bytes, so its four elements come second, behind
+// four that are in the chunk before, too.  A stationary row has its own in the same place and zeros first, which leaves products over columns right;
+// output columns D .. D + 3 then hold what belongs into D - 4 .. D - 1 (column_of).
 template <class T>
 __device__ __forceinline__ Raw<T> load_chunk(const T* row, int ch, int D) {
   Raw<T> r;
   r.x = {};
   if constexpr (sizeof(T) == 2) {
-    if (ch * 8 < D) r.x = *reinterpret_cast<const bf16x8*>(row + ch * 8);
+    typedef __bf16 chunk __attribute__((ext_vector_type(8), aligned(8)));
+    if ((D & 4) && ch == D / 8) r.x = __builtin_shufflevector(bf16x4{}, *reinterpret_cast<const bf16x4*>(row + ch * 8), 0, 1, 2, 3, 4, 5, 6, 7);
+    else if (ch * 8 < D) r.x = *reinterpret_cast<const chunk*>(row + ch * 8);
   } else {
     f32x4 a = {}, b = {};
     if (ch * 8 < D) a = *reinterpret_cast<const f32x4*>(row + ch * 8);
@@ -455,8 +460,10 @@ struct Stage {
     limit = rows;
     last = D * ES;
     const int ch = tid % TL::NCH, mine = tid / TL::NCH;
+    const int back = ES == 2 && (D & 4) && ch == D / 8 ? 8 : 0;  // load_chunk
 #pragma unroll
-    for (int i = 0; i < PER; ++i) off[i] = ch * 8 * ES + 16 * i < last ? (uint32_t)(mine * (int)row_bytes + ch * 8 * ES + 16 * i) : kOutside;
+    for (int i = 0; i < PER; ++i)
+      off[i] = ch * 8 * ES + 16 * i < last ? (uint32_t)(mine * (int)row_bytes + ch * 8 * ES + 16 * i - back) : kOutside;
   }
   // use: the rows that a mask leaves, or null
   __device__ __forceinline__ void load(int row0, const RowBits* use, int tid) {
@@ -500,10 +507,17 @@ struct Stage {
   }
 };
 
+// The column of a row of D that four output columns from d on belong to, or -1: d itself but for rows that end in half a chunk (load_chunk).
+template <class T>
+__device__ __forceinline__ int column_of(int d, int D) {
+  if (sizeof(T) == 2 && (D & 4) && d >= D - 4) return d == D ? D - 4 : -1;
+  return d < D ? d : -1;
+}
+
 // A lane's 32 columns x 4 rows of an accumulator as output: column = stationary row, 4 neighbouring d per register group.
 template <class T>
 __device__ __forceinline__ void store4(T* row, int d, int D, float a, float b, float c, float e) {
-  if (d >= D) return;  // D is a whole number of fours
+  if (d < 0 || d >= D) return;  // D is a whole number of fours
   if constexpr (sizeof(T) == 4) {
     *reinterpret_cast<f32x4*>(row + d) = f32x4{a, b, c, e};
   } else {
@@ -659,9 +673,9 @@ static int launch(K kernel, std::atomic<uint64_t>* done, int64_t items, int thre
   return 0;
 }
 
-// Whether every row of a [B, H, T, D] tensor starts on 16 bytes.
-static inline bool rows_on_16(const void* ptr, int64_t b, int64_t h, int64_t t, int es) {
-  return ((reinterpret_cast<uintptr_t>(ptr) | (uintptr_t)(b * es) | (uintptr_t)(h * es) | (uintptr_t)(t * es)) & 15) == 0;
+// Whether every row of a [B, H, T, D] tensor starts on the bytes of four elements.
+static inline bool rows_on_four(const void* ptr, int64_t b, int64_t h, int64_t t, int es) {
+  return ((reinterpret_cast<uintptr_t>(ptr) | (uintptr_t)(b * es) | (uintptr_t)(h * es) | (uintptr_t)(t * es)) & (4 * es - 1)) == 0;
 }
 
 }  // namespace attn
