@@ -525,3 +525,13 @@ def test_rows_that_start_on_eight_bytes(D, Tq, Tk):
     check("out", out, want["out"])
     for name, g in zip(("dq", "dk", "dv"), torch.autograd.grad(out, (q, k, v), dout)):
         check(name, g, want[name])
+
+
+@pytest.mark.parametrize("change", [dict(head_dim=6), dict(dtype=1, head_dim=4), dict(dtype=1, head_dim=12, q=20), dict(head_dim=12, k=24),
+                                    dict(dtype=1, head_dim=12, v_stride=(0, 0, 14))])
+def test_c_entry_refuses_rows_it_cannot_read(change):
+    lib = _lib.load()
+    if "v_stride" in change:
+        change = dict(change, v_stride=_lib.I64x3(*change["v_stride"]))
+    assert lib.wrnn_attention_forward(C.byref(desc(**change)), 16, _lib.I64x3(0, 0, 0), None, None, 0, None) != 0
+    assert b"fours" in lib.wrnn_last_error()
