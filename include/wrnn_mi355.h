@@ -504,12 +504,18 @@ typedef struct wrnn_attention_desc {
 size_t wrnn_attention_workspace_bytes(const wrnn_attention_desc* desc);
 int wrnn_attention_forward(const wrnn_attention_desc* desc, void* out, const int64_t out_stride[3], float* lse, void* workspace,
                            size_t workspace_bytes, void* stream);
+/* The same, with what the backward pass needs of each row: stats [2, batch, heads, q_len] fp32, a reference m near the row's highest score
+ * (of S * log2 e) and the sum of exp2(S * log2 e - m) over its allowed keys, 0 without any.  (lse alone does not do: where the scores of a row
+ * share a large level, as biases like -1e9 give it, the sum's logarithm is lost beside it.) */
+int wrnn_attention_forward_stats(const wrnn_attention_desc* desc, void* out, const int64_t out_stride[3], float* lse, float* stats,
+                                 void* workspace, size_t workspace_bytes, void* stream);
 
-/* The backward pass; recomputes the probabilities from lse, so nothing of size q_len x k_len is kept or written.  All
- * sums have a fixed order: the same inputs give the same bits. */
+/* The backward pass; recomputes the probabilities from the rows' statistics, so nothing of size q_len x k_len is kept or written.  All
+ * sums have a fixed order: the same inputs give the same bits.  wrnn_attention_backward makes the statistics anew, at the cost of another
+ * forward pass; wrnn_attention_backward_stats takes them from wrnn_attention_forward_stats.  One workspace size serves both. */
 typedef struct wrnn_attention_grads {
   const void* out;   /* of the forward pass */
-  const float* lse;  /* of the forward pass */
+  const float* lse;  /* not read; may be NULL */
   const void* dout;  /* [batch, heads, q_len, head_dim] */
   void* dq;
   void* dk;          /* [batch, kv_heads, k_len, head_dim], summed over the heads that share them; dk and dv may both be NULL */
@@ -520,6 +526,8 @@ typedef struct wrnn_attention_grads {
 size_t wrnn_attention_backward_workspace_bytes(const wrnn_attention_desc* desc);
 int wrnn_attention_backward(const wrnn_attention_desc* desc, const wrnn_attention_grads* grads, void* workspace, size_t workspace_bytes,
                             void* stream);
+int wrnn_attention_backward_stats(const wrnn_attention_desc* desc, const wrnn_attention_grads* grads, const float* stats, void* workspace,
+                                  size_t workspace_bytes, void* stream);
 
 /* The same bias as a dense [heads, q_len, k_len] tensor, as the additive attn_mask of nn.MultiheadAttention takes it, and its
  * table's gradient: out[h,i,j] = table[bucket(j - (i + start)), h];  dtable[n,h] = sum of dout[h,i,j] over the pairs of bucket n.

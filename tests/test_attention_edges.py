@@ -1,0 +1,103 @@
+"""Self-attention where rows are extreme: scores whose common level hides the sum of their exponentials, queries without keys that hold NaN,
+tables with low values of different size, roundings that add up."""
+import math
+
+import pytest
+import torch
+
+from attention_ref import check, reference
+from test_attention import BF16, F32, normal, run_case
+from wavernn_amd import _lib
+from wavernn_amd import attention as A
+
+gpu = pytest.mark.gpu
+LOWEST = torch.finfo(F32).min
+
+
+def gradients(leaves, dout, **rule):
+    leaves = [x.detach().requires_grad_() for x in leaves]
+    out = A.attention(*leaves[:3], bias_table=leaves[3] if len(leaves) > 3 else None, **rule)
+    return [out.detach(), *torch.autograd.grad(out, leaves, dout)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("H,G,Tq,Tk,D", [(2, 2, 40, 40, 16), (4, 2, 20, 700, 64), (2, 1, 150, 130, 128), (2, 2, 70, 300, 200)])
+@pytest.mark.parametrize("low", [-1e5, -1e6, -1e8, -1e9, -1e30, LOWEST, 1e9])
+def test_gradients_where_all_biases_of_a_query_lie_far_from_zero(dtype, H, G, Tq, Tk, D, low):
+    """A common shift of a row's scores changes neither its softmax nor a gradient, however large it is beside the logarithm of the row's sum.
+    Queries are zero, so that the scores are the biases themselves and no bit of them is lost beside the shift: the values and bounds are those
+    of the same table without the shift (head 0), or, where a few near distances keep zero (the other heads), with -60 in place of the
+    low values: exp(-60) is 1e-26."""
+    k, v, dout = normal(1, 2, G, Tk, D, dtype=dtype), normal(2, 2, G, Tk, D, dtype=dtype), normal(3, 2, H, Tq, D, dtype=dtype)
+    q = torch.zeros(2, H, Tq, D, device="cuda", dtype=dtype)
+    mask = (torch.rand(2, Tk, generator=torch.Generator().manual_seed(4)) < 0.3).cuda()
+    mask[1, Tk // 2:] = True                      # queries that are left distant keys alone
+    table = torch.full((8, H), low)
+    same = torch.zeros(8, H)
+    if low < 0:
+        table[:2, 1:], same[2:, 1:] = 0.0, -60.0
+    rule = dict(key_mask=mask, max_distance=20)
+    got = gradients([q, k, v, table.cuda()], dout, **rule)
+    want = reference(q, k, v, dout, table=same, **rule)
+    # what -60 adds in the reference and the low values do not: less than exp(-60) = 8.8e-27 a pair of P, times |dP| + |delta| < 1e4 (sums of 200
+    # products of normal values), over at most 2 x 150 x 700 pairs
+    for name, x in zip(("out", "dq", "dk", "dv", "dtable"), got):
+        check(name, x, (want[name][0], want[name][1] + 8.8e-27 * 1e4 * 2.1e5))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("D", [16, 128, 200])
+def test_gradients_where_all_scores_of_a_query_lie_far_from_zero(dtype, D):
+    """The same by the scores: all keys of a head are one vector, whose products with a query are a common shift of some 1e7; the softmax is even
+    and dk = dS^T q is all that the queries enter.  Queries and keys are small whole numbers (times 16), so that every product and sum is
+    exact in 32 bits in whatever order a pass takes them, and a score the same number in each."""
+    g = torch.Generator().manual_seed(0)
+    q = (torch.randint(-255, 256, (2, 2, 90, D), generator=g) * 16).to(dtype).cuda()
+    k = torch.randint(-7, 8, (2, 2, 1, D), generator=g).to(dtype).cuda().expand(2, 2, 150, D)
+    v, dout = normal(2, 2, 2, 150, D, dtype=dtype), normal(3, 2, 2, 90, D, dtype=dtype)
+    out, dq, dk, dv = gradients([q, k, v], dout, scale=64.0)
+    even = reference(torch.zeros_like(q), k, v, dout, scale=64.0)
+    check("out", out, even["out"])
+    check("dv", dv, even["dv"])
+    # dq: a sum of dS over the keys, zero but for roundings, times the key; dk from the even softmax's dS
+    check("dq", dq, even["dq"])
+    go, vd = dout.double().cpu(), v.double().cpu()
+    ds = ((go @ vd.transpose(-1, -2)) - (go * vd.mean(2, keepdim=True)).sum(-1, keepdim=True)) / 150
+    qd, ub, u = q.double().cpu(), torch.finfo(dtype).eps / 2, 2.0 ** -24
+    # dS: rounded where it enters the product (bfloat16), made of 32-bit sums of dP and of delta, delta of the rounded output
+    size = (go.abs() @ vd.abs().transpose(-1, -2) + (go.abs() * vd.abs().mean(2, keepdim=True)).sum(-1, keepdim=True)) / 150
+    off = 2 * ub * ds.abs() + (2 * D + 400) * u * size + (2 * ub * (go.abs() * vd.abs().mean(2, keepdim=True)).sum(-1, keepdim=True) / 150)
+    dkx = ds.transpose(-1, -2) @ qd * 64
+    check("dk", dk, (dkx, off.transpose(-1, -2) @ qd.abs() * 64 * (1 + 1e-3) + ub * dkx.abs()))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("Tq,Tk", [(3, 900), (150, 90), (40, 1500)])
+def test_backward_entry_that_makes_the_statistics_anew(dtype, Tq, Tk):
+    """The C entry without statistics against the one that is handed them: the same bits."""
+    q, k, v, dout = (normal(i, 2, 4 if i in (0, 3) else 2, Tq if i in (0, 3) else Tk, 64, dtype=dtype) for i in range(4))
+    lens = torch.tensor([Tk, 5], dtype=torch.int32, device="cuda")
+    want = gradients([q, k, v], dout, key_lens=lens)
+    lib = _lib.load()
+    desc = A._desc(q, k, v, None, None, lens, None, False, 0.125, 128, True)
+    got = [want[0], *(torch.full_like(x, math.nan) for x in (q, k, v))]
+    strides = [x.stride()[:3] for x in (want[0], dout, *got[1:])]
+    grads = A._GRADS.pack(want[0].data_ptr(), 0, dout.data_ptr(), *(x.data_ptr() for x in got[1:]), 0, *(s for x in strides for s in x))
+    size = lib.wrnn_attention_backward_workspace_bytes(desc)
+    space = torch.empty(size, dtype=torch.uint8, device="cuda")
+    assert lib.wrnn_attention_backward(desc, grads, space.data_ptr(), size, torch.cuda.current_stream().cuda_stream) == 0
+    for x, y in zip(got, want):
+        assert torch.equal(x, y)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("scale", [-0.3, 0.0, 1e-6])
+@pytest.mark.parametrize("D,Tq,Tk", [(64, 70, 90), (200, 70, 90), (36, 3, 200), (128, 50, 700)])
+def test_scales_of_any_sign(dtype, scale, D, Tq, Tk):
+    mask = (torch.rand(2, Tk, generator=torch.Generator().manual_seed(2)) < 0.3).cuda()
+    run_case(dtype, 2, 4, 2, Tq, Tk, D, scale=scale, mask=mask, causal=True)
+    run_case(dtype, 2, 4, 2, Tq, Tk, D, scale=scale, mask=mask, table=normal(3, 16, 4))

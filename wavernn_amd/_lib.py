@@ -143,8 +143,10 @@ SYMBOLS = {
     # (the two structures by address: wavernn_amd.attention passes them as bytes)
     "wrnn_attention_workspace_bytes": (C.c_size_t, [_P]),
     "wrnn_attention_forward": (_I, [_P, _P, I64x3, _P, _P, C.c_size_t, _P]),
+    "wrnn_attention_forward_stats": (_I, [_P, _P, I64x3, _P, _P, _P, C.c_size_t, _P]),
     "wrnn_attention_backward_workspace_bytes": (C.c_size_t, [_P]),
     "wrnn_attention_backward": (_I, [_P, _P, _P, C.c_size_t, _P]),
+    "wrnn_attention_backward_stats": (_I, [_P, _P, _P, _P, C.c_size_t, _P]),
     "wrnn_relative_bias_forward": (_I, [_P] + [_I] * 8 + [C.POINTER(C.c_int32), _P, _P]),
     "wrnn_relative_bias_workspace_bytes": (C.c_size_t, [_I] * 5),
     "wrnn_relative_bias_backward": (_I, [_P] + [_I] * 8 + [C.POINTER(C.c_int32), _P, _P, C.c_size_t, _P]),

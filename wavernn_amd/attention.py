@@ -128,46 +128,48 @@ def _space(size: int, device: torch.device) -> Optional[torch.Tensor]:
     return torch.empty(size, dtype=torch.uint8, device=device) if size else None
 
 
-def _forward(desc, q, lse):
+def _forward(desc, q, lse, stats):
     lib = _lib.load()
     out = _empty_like(q)
     size = lib.wrnn_attention_workspace_bytes(desc)
     space = _space(size, q.device)
-    if lib.wrnn_attention_forward(desc, out.data_ptr(), _lib.I64x3(*out.stride()[:3]), _ptr(lse), _ptr(space), size,
-                                  _stream(q.device)):
-        _lib.check(1, "wrnn_attention_forward")
+    if lib.wrnn_attention_forward_stats(desc, out.data_ptr(), _lib.I64x3(*out.stride()[:3]), _ptr(lse), _ptr(stats), _ptr(space), size,
+                                        _stream(q.device)):
+        _lib.check(1, "wrnn_attention_forward_stats")
     return out
 
 
 class _Attention(torch.autograd.Function):
 
     @staticmethod
-    def forward(ctx, q, k, v, table, key_mask, key_lens, q_start, causal, scale, max_distance, bidirectional):
+    def forward(ctx, q, k, v, table, key_mask, key_lens, q_start, causal, scale, max_distance, bidirectional, want_lse):
         with _on(q.device):
-            lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device)
+            lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) if want_lse else None
+            stats = torch.empty(2, *q.shape[:3], dtype=torch.float32, device=q.device)
             desc = _desc(q, k, v, table, key_mask, key_lens, q_start, causal, scale, max_distance, bidirectional)
-            out = _forward(desc, q, lse)
+            out = _forward(desc, q, lse, stats)
         ctx.rule = (causal, scale, max_distance, bidirectional)
-        ctx.save_for_backward(q, k, v, table, key_mask, key_lens, q_start, out, lse)
-        ctx.mark_non_differentiable(lse)
+        ctx.save_for_backward(q, k, v, table, key_mask, key_lens, q_start, out, stats)
+        if want_lse:
+            ctx.mark_non_differentiable(lse)
         ctx.set_materialize_grads(False)    # lse gets none: no tensor of zeros for it
         return out, lse
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout, _):
-        q, k, v, table, key_mask, key_lens, q_start, out, lse = ctx.saved_tensors
+        q, k, v, table, key_mask, key_lens, q_start, out, stats = ctx.saved_tensors
         want_table = table is not None and ctx.needs_input_grad[3]
         B, H, Tq, _ = q.shape
         if not (B and H and Tq):
-            return (torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v), torch.zeros_like(table) if want_table else None) + (None,) * 7
+            return (torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v), torch.zeros_like(table) if want_table else None) + (None,) * 8
         lib = _lib.load()
         with _on(q.device):
             # saved-tensor hooks (offloading, checkpointing) hand other tensors back than were saved, in other places and strides
             q, k, v, out, dout = _rows(q), _rows(k), _rows(v), _rows(out), _rows(dout)
             if key_mask is not None and key_mask.stride(1) != 1:
                 key_mask = key_mask.contiguous()
-            lse, table, key_lens, q_start = (None if t is None else t.contiguous() for t in (lse, table, key_lens, q_start))
+            stats, table, key_lens, q_start = (None if t is None else t.contiguous() for t in (stats, table, key_lens, q_start))
             desc = _desc(q, k, v, table, key_mask, key_lens, q_start, *ctx.rule)
             dq, dk, dv, dtable = _empty_like(q), None, None, None
             if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
@@ -175,14 +177,14 @@ class _Attention(torch.autograd.Function):
             if want_table:
                 dtable = torch.empty_like(table)
             zero = (0, 0, 0)
-            grads = _GRADS.pack(out.data_ptr(), lse.data_ptr(), dout.data_ptr(), dq.data_ptr(), _ptr(dk), _ptr(dv), _ptr(dtable), *out.stride()[:3],
+            grads = _GRADS.pack(out.data_ptr(), 0, dout.data_ptr(), dq.data_ptr(), _ptr(dk), _ptr(dv), _ptr(dtable), *out.stride()[:3],
                                 *dout.stride()[:3], *dq.stride()[:3], *(zero if dk is None else dk.stride()[:3]),
                                 *(zero if dv is None else dv.stride()[:3]))
             size = lib.wrnn_attention_backward_workspace_bytes(desc)
             space = _space(size, q.device)
-            if lib.wrnn_attention_backward(desc, grads, space.data_ptr(), size, _stream(q.device)):
-                _lib.check(1, "wrnn_attention_backward")
-        return (dq, dk, dv, dtable) + (None,) * 7
+            if lib.wrnn_attention_backward_stats(desc, grads, stats.data_ptr(), space.data_ptr(), size, _stream(q.device)):
+                _lib.check(1, "wrnn_attention_backward_stats")
+        return (dq, dk, dv, dtable) + (None,) * 8
 
 
 def _whole(t: Optional[torch.Tensor], B: int, q: torch.Tensor, name: str) -> Optional[torch.Tensor]:
@@ -248,10 +250,10 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, key_mask: Op
 def _run(q, k, v, bias_table, key_mask, key_lens, q_start, causal, scale, max_distance, bidirectional, want_lse):
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
                                     or (bias_table is not None and bias_table.requires_grad)):
-        return _Attention.apply(q, k, v, bias_table, key_mask, key_lens, q_start, causal, scale, max_distance, bidirectional)
+        return _Attention.apply(q, k, v, bias_table, key_mask, key_lens, q_start, causal, scale, max_distance, bidirectional, want_lse)
     with _on(q.device):
         lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) if want_lse else None
-        out = _forward(_desc(q, k, v, bias_table, key_mask, key_lens, q_start, causal, scale, max_distance, bidirectional), q, lse)
+        out = _forward(_desc(q, k, v, bias_table, key_mask, key_lens, q_start, causal, scale, max_distance, bidirectional), q, lse, None)
     return out, lse
 
 

@@ -1,4 +1,6 @@
 // Entry points of the self-attention (kernels: attention_forward.h, attention_backward.h; several sources for the build's sake).
+#include <cmath>
+
 #include "attention_tile.h"
 
 namespace wrnn {
@@ -61,7 +63,8 @@ static void plan_backward(Params* p, int dtype) {
   p->dkv_splits = shares(p->causal ? (blocks + 1) / 2 : blocks, (int64_t)((p->Tq + 31) / 32) * p->group, 4);
 }
 static size_t aligned(size_t x) { return (x + 255) & ~size_t(255); }
-// the backward workspace: delta, the table's partial sums, the shares
+// the backward workspace: the rows' statistics, delta, the table's partial sums, the shares
+static size_t stats_bytes(const Params& p) { return aligned((size_t)2 * p.B * p.H * p.Tq * sizeof(float)); }
 static size_t delta_bytes(const Params& p) { return aligned((size_t)(p.table ? p.dq_splits : 1) * p.B * p.H * p.Tq * sizeof(float)); }
 static size_t table_bytes(const Params& p) {
   return p.table ? aligned((size_t)p.B * row_blocks(p, p.Tk) * p.dkv_splits * p.H * p.buckets * sizeof(float)) : 0;
@@ -97,7 +100,9 @@ int attention_params(const wrnn_attention_desc* d, attn::Params* p, const char* 
   p->B = d->batch, p->H = d->heads, p->Hkv = d->kv_heads, p->group = d->heads ? d->heads / d->kv_heads : 1;
   p->Tq = d->q_len, p->Tk = d->k_len, p->D = d->head_dim;
   p->causal = d->causal != 0;
-  p->scale = d->scale, p->scale2 = d->scale * kLog2e;
+  // the kernels take the scale as positive (the highest product is the highest score) and not zero, which a left out pair's -inf would not survive
+  p->scale = d->scale, p->flip = d->scale < 0.f ? 0x80000000u : 0u;
+  p->scale2 = d->scale == 0.f ? 1.17549435e-38f : std::fabs(d->scale) * kLog2e;
   p->key_mask = d->key_mask, p->mask_b = d->key_mask_stride, p->key_lens = d->key_lens, p->q_start = d->q_start;
   const int es = d->dtype == WRNN_FLOAT32 ? 4 : 2;
   WRNN_REQUIRE(d->head_dim % 4 == 0 && d->head_dim * es >= 16 && rows_on_four(p->q, p->q_b, p->q_h, p->q_t, es) &&
@@ -123,6 +128,11 @@ extern "C" size_t wrnn_attention_workspace_bytes(const wrnn_attention_desc* desc
 
 extern "C" int wrnn_attention_forward(const wrnn_attention_desc* desc, void* out, const int64_t out_stride[3], float* lse, void* workspace,
                                       size_t workspace_bytes, void* stream) {
+  return wrnn_attention_forward_stats(desc, out, out_stride, lse, nullptr, workspace, workspace_bytes, stream);
+}
+
+extern "C" int wrnn_attention_forward_stats(const wrnn_attention_desc* desc, void* out, const int64_t out_stride[3], float* lse, float* stats,
+                                            void* workspace, size_t workspace_bytes, void* stream) {
   attn::Params p;
   if (attention_params(desc, &p, "wrnn_attention_forward")) return 1;
   if (!p.B || !p.H || !p.Tq) return 0;
@@ -131,7 +141,7 @@ extern "C" int wrnn_attention_forward(const wrnn_attention_desc* desc, void* out
   const size_t need = attn::split_workspace(p);
   WRNN_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && !((uintptr_t)workspace & 15)),
                "wrnn_attention_forward: workspace of %zu bytes, %zu are needed, on 16 bytes", workspace_bytes, need);
-  p.out = out, p.o_b = out_stride[0], p.o_h = out_stride[1], p.o_t = out_stride[2], p.lse = lse;
+  p.out = out, p.o_b = out_stride[0], p.o_h = out_stride[1], p.o_t = out_stride[2], p.lse = lse, p.stats = stats;
   p.part = static_cast<float*>(workspace);
   WRNN_REQUIRE(attn::rows_on_four(out, p.o_b, p.o_h, p.o_t, desc->dtype == WRNN_FLOAT32 ? 4 : 2), "wrnn_attention_forward: rows of out have to start on the bytes of four elements");
   const hipStream_t st = static_cast<hipStream_t>(stream);
@@ -141,12 +151,19 @@ extern "C" int wrnn_attention_forward(const wrnn_attention_desc* desc, void* out
 extern "C" size_t wrnn_attention_backward_workspace_bytes(const wrnn_attention_desc* desc) {
   attn::Params p;
   if (attention_params(desc, &p, "wrnn_attention_backward_workspace_bytes") || !p.B || !p.H || !p.Tq) return 0;
+  attn::plan(&p);
   attn::plan_backward(&p, desc->dtype);
-  return attn::delta_bytes(p) + attn::table_bytes(p) + attn::dq_bytes(p) + attn::dkv_bytes(p);
+  const size_t rest = attn::delta_bytes(p) + attn::table_bytes(p) + attn::dq_bytes(p) + attn::dkv_bytes(p), forward = attn::split_workspace(p);
+  return attn::stats_bytes(p) + (rest > forward ? rest : forward);
 }
 
 extern "C" int wrnn_attention_backward(const wrnn_attention_desc* desc, const wrnn_attention_grads* g, void* workspace, size_t workspace_bytes,
                                        void* stream) {
+  return wrnn_attention_backward_stats(desc, g, nullptr, workspace, workspace_bytes, stream);
+}
+
+extern "C" int wrnn_attention_backward_stats(const wrnn_attention_desc* desc, const wrnn_attention_grads* g, const float* stats, void* workspace,
+                                             size_t workspace_bytes, void* stream) {
   attn::Params p;
   if (attention_params(desc, &p, "wrnn_attention_backward")) return 1;
   WRNN_REQUIRE(g, "wrnn_attention_backward: null gradients");
@@ -154,7 +171,7 @@ extern "C" int wrnn_attention_backward(const wrnn_attention_desc* desc, const wr
     WRNN_REQUIRE(!p.B || !p.H || !p.Tk, "wrnn_attention_backward: no queries; dk, dv and the table's gradient are zero and left to the caller");
     return 0;
   }
-  WRNN_REQUIRE(g->out && g->lse && g->dout && g->dq && !g->dk == !g->dv, "wrnn_attention_backward: null pointer");
+  WRNN_REQUIRE(g->out && g->dout && g->dq && !g->dk == !g->dv, "wrnn_attention_backward: null pointer");
   WRNN_REQUIRE(!g->dtable || p.table, "wrnn_attention_backward: a table's gradient without a table");
   const size_t need = wrnn_attention_backward_workspace_bytes(desc);
   WRNN_REQUIRE(workspace && workspace_bytes >= need && !((uintptr_t)workspace & 15),
@@ -170,13 +187,20 @@ extern "C" int wrnn_attention_backward(const wrnn_attention_desc* desc, const wr
   p.dq = g->dq, p.dq_b = g->dq_stride[0], p.dq_h = g->dq_stride[1], p.dq_t = g->dq_stride[2];
   p.dk = g->dk, p.dk_b = g->dk_stride[0], p.dk_h = g->dk_stride[1], p.dk_t = g->dk_stride[2];
   p.dv = g->dv, p.dv_b = g->dv_stride[0], p.dv_h = g->dv_stride[1], p.dv_t = g->dv_stride[2];
-  attn::plan_backward(&p, desc->dtype);
-  p.lse = const_cast<float*>(g->lse);
+  const hipStream_t st = static_cast<hipStream_t>(stream);
   char* w = static_cast<char*>(workspace);
-  p.delta = reinterpret_cast<float*>(w);
+  if (!stats) {  // made anew: the forward kernel without an output
+    attn::plan(&p);
+    p.stats = reinterpret_cast<float*>(w);
+    p.part = reinterpret_cast<float*>(w + attn::stats_bytes(p));
+    if (desc->dtype == WRNN_FLOAT32 ? attn::forward<float>(p, st) : attn::forward<__bf16>(p, st)) return 1;
+  } else {
+    p.stats = const_cast<float*>(stats);
+  }
+  attn::plan_backward(&p, desc->dtype);
+  p.delta = reinterpret_cast<float*>(w += attn::stats_bytes(p));
   p.dtable_part = reinterpret_cast<float*>(w += attn::delta_bytes(p));
   p.dq_part = reinterpret_cast<float*>(w += attn::table_bytes(p));
   p.dkv_part = reinterpret_cast<float*>(w + attn::dq_bytes(p));
-  const hipStream_t st = static_cast<hipStream_t>(stream);
   return desc->dtype == WRNN_FLOAT32 ? attn::backward<float>(p, g->dtable, st) : attn::backward<__bf16>(p, g->dtable, st);
 }

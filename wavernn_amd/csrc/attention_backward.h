@@ -1,4 +1,4 @@
-// Self-attention, backward.  With P recomputed from the forward pass's log-sum-exp:
+// Self-attention, backward.  With P recomputed from the forward pass's row statistics, P = exp2(score - m) / l:
 //   dv = P^T dout,  dP = dout v^T,  delta = rowsum(dout * out),  dS = P * (dP - delta),  dq = scale * dS k,  dk = scale * dS^T q,
 //   dtable[n, h] = sum of dS over the pairs whose distance falls in bucket n.
 //
@@ -183,6 +183,7 @@ __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_
   {
     const T* gr = reinterpret_cast<const T*>(p.dout) + b * p.do_b + h * p.do_h + qc * p.do_t;
     q.load(reinterpret_cast<const T*>(p.q) + b * p.q_b + h * p.q_h + qc * p.q_t + d0, half, p.D - d0, true);
+    q.flip(p.flip);
     go.load(gr + d0, half, p.D - d0, true);
     const T* orow = reinterpret_cast<const T*>(p.o_in) + b * p.oi_b + h * p.oi_h + qc * p.oi_t;
 #pragma unroll
@@ -193,8 +194,9 @@ __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_
     }
     delta = both_sum(delta);
   }
-  const float lse = qi < p.Tq ? p.lse[(int64_t)bh * p.Tq + qi] : -INFINITY;
-  const float lse2 = lse == -INFINITY ? INFINITY : lse * kLog2e;  // a row without keys, or none at all: P = exp2(.. - inf) = 0
+  RowStats row;
+  row.load(p, (int64_t)bh * p.Tq + qi, qi < p.Tq);
+  const float m = row.m(), inv = row.inv();  // 1 / l enters where the sums over the keys are stored
   if constexpr (BIAS != 0) fill_lut(p, h, lut, tid, NT);
   const int end = key_end(p, b, min(qt * S::ROWS + S::ROWS - 1, p.Tq - 1) + off, word, tid, NT);
   const int all = (end + BN - 1) / BN, per = (all + p.dq_splits - 1) / p.dq_splits;
@@ -256,7 +258,7 @@ __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_
           for (int i = 0; i < 16; ++i) pr[i] = raw[i];
           finish_scores<BIAS != 0>(p, pr, key0, pos, pos_lo, pos_hi, use.of(sub), lut, half);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) pr[i] = __builtin_amdgcn_exp2f(pr[i] - lse2);
+          for (int i = 0; i < 16; ++i) pr[i] = __builtin_amdgcn_exp2f(exponent<BIAS != 0>(p, pr[i], m));
 #pragma unroll
           for (int i = 0; i < 16; ++i) pr[i] *= dp[i] - delta;
           if constexpr (BIAS == 2 || exact)
@@ -284,7 +286,7 @@ __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_
   } else {
     walk(std::false_type());
   }
-  off_by = both_sum(off_by);
+  off_by = both_sum(off_by) * inv;
   // (a share's sum is only part of a row's: with BIAS == 2 the next kernel adds them up, otherwise such rows do without)
   if (half == 0 && d0 == 0 && qi < p.Tq && (BIAS == 2 || share == 0)) {
     const float whole = BIAS == 2 || p.dq_splits == 1 ? off_by : 0.f;
@@ -292,7 +294,7 @@ __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_
   }
   if (qi < p.Tq)
     store_rows<S>(acc, reinterpret_cast<T*>(p.dq) + b * p.dq_b + h * p.dq_h + qi * p.dq_t,
-                  p.dq_splits > 1 ? p.dq_part + (((int64_t)share * p.B * p.H + bh) * p.Tq + qi) * p.D : nullptr, d0, p.D, p.scale, half);
+                  p.dq_splits > 1 ? p.dq_part + (((int64_t)share * p.B * p.H + bh) * p.Tq + qi) * p.D : nullptr, d0, p.D, p.scale * inv, half);
 }
 
 // dk, dv and, with BIAS == 2, the position table's gradient: keys of one key head stationary; tiles of queries and their output gradients through
@@ -305,8 +307,8 @@ __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_
   extern __shared__ __attribute__((aligned(16))) char smem[];
   char* qt = smem;
   char* gt = smem + BUFS * TL::BYTES;
-  float* stat = reinterpret_cast<float*>(smem + S::TILES);  // [BUFS][2][BM]: lse in log2 units, delta
-  float* lut = stat + BUFS * 2 * BM;
+  float* stat = reinterpret_cast<float*>(smem + S::TILES);  // [BUFS][3][BM]: m, 1 / l, delta
+  float* lut = stat + BUFS * 3 * BM;
   const int words = BiasGrad::words(p.max_distance);
   float* skew = lut + ((2 * p.max_distance + 4) & ~3);
   float* sums = skew + S::RG * BiasGrad::SKEW;  // [RG][words]
@@ -327,8 +329,9 @@ __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_
   const bool ok = key < end && !(mask && mask[kc]);
   Stationary<T, S::DA, S::RAW> k, v;
   k.load(reinterpret_cast<const T*>(p.k) + b * p.k_b + kvh * p.k_h + kc * p.k_t + d0, half, p.D - d0, ok);
+  k.flip(p.flip);
   v.load(reinterpret_cast<const T*>(p.v) + b * p.v_b + kvh * p.v_h + kc * p.v_t + d0, half, p.D - d0, ok);
-  const float add = ok ? 0.f : -INFINITY;
+  [[maybe_unused]] const float add = ok ? 0.f : -INFINITY;
   f32x16 dk[S::DT] = {}, dv[S::DT] = {};
   // under causality queries before key - off see nothing of this block
   const int qt_n = (p.Tq + BM - 1) / BM, qt_0 = p.causal ? min(max(k0 - off, 0) / BM, qt_n) : 0, per = qt_n - qt_0;
@@ -337,7 +340,8 @@ __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_
   Stage<T, DP, BM, NT> sq, sg;
   sq.start(nullptr, p.q_t, p.Tq, p.D, tid);
   sg.start(nullptr, p.do_t, p.Tq, p.D, tid);
-  float s_lse = 0.f, s_delta = 0.f;
+  RowStats s_row = {};
+  float s_delta = 0.f;
   auto load = [&](int it) {
     if (it >= steps) return;
     const int h = kvh * p.group + it / per, r0 = (qt_0 + it % per) * BM;
@@ -347,8 +351,7 @@ __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_
     sg.load(r0, nullptr, tid);
     if (tid < BM) {
       const int64_t row = ((int64_t)b * p.H + h) * p.Tq + r0 + tid;
-      const float l = r0 + tid < p.Tq ? p.lse[row] : -INFINITY;
-      s_lse = l == -INFINITY ? INFINITY : l * kLog2e;
+      s_row.load(p, row, r0 + tid < p.Tq);
       s_delta = 0.f;
       if (r0 + tid < p.Tq)
         for (int n = 0; n < (BIAS == 2 ? p.dq_splits : 1); ++n) s_delta += p.delta[(int64_t)n * p.B * p.H * p.Tq + row];
@@ -357,8 +360,9 @@ __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_
   auto store_stat = [&](int it) {
     const int o = it & (BUFS - 1);
     if (tid < BM) {
-      stat[o * 2 * BM + tid] = s_lse;
-      stat[(o * 2 + 1) * BM + tid] = s_delta;
+      stat[o * 3 * BM + tid] = s_row.m();
+      stat[(o * 3 + 1) * BM + tid] = s_row.inv();
+      stat[(o * 3 + 2) * BM + tid] = s_delta;
     }
   };
   auto store = [&](int it) {
@@ -419,24 +423,26 @@ __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_
           }
         } else {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) s[i] = fmaf(raw[i], p.scale2, add);
+          for (int i = 0; i < 16; ++i) s[i] = raw[i];
+        }
+        const float* of = stat + o * 3 * BM + sub * 32 + 4 * half;
+        float ds[16];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const f32x4 m = *reinterpret_cast<const f32x4*>(of + 8 * g), inv = *reinterpret_cast<const f32x4*>(of + BM + 8 * g);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[4 * g + e] = __builtin_amdgcn_exp2f(exponent<BIAS != 0>(p, s[4 * g + e], m[e])) * inv[e];
         }
         if (p.causal && kw + 31 > p0) {
           const int first = key - p0 - 4 * half;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) s[i] = first > moving_row(i, 0) ? -INFINITY : s[i];
+          for (int i = 0; i < 16; ++i) s[i] = first > moving_row(i, 0) ? 0.f : s[i];
         }
-        const float* l2 = stat + o * 2 * BM + sub * 32 + 4 * half;
-        float ds[16];
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          const f32x4 l = *reinterpret_cast<const f32x4*>(l2 + 8 * g), de = *reinterpret_cast<const f32x4*>(l2 + BM + 8 * g);
+          const f32x4 de = *reinterpret_cast<const f32x4*>(of + 2 * BM + 8 * g);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int i = 4 * g + e;
-            s[i] = __builtin_amdgcn_exp2f(s[i] - l[e]);
-            ds[i] = s[i] * (dp[i] - de[e]);
-          }
+          for (int e = 0; e < 4; ++e) ds[4 * g + e] = s[4 * g + e] * (dp[4 * g + e] - de[e]);
         }
         if constexpr (BIAS == 2)
           if (d0 == 0) bias_grad.add(ds, kw - p0, p.max_distance, skew + rg * BiasGrad::SKEW, sums + rg * words, lane);
@@ -482,6 +488,10 @@ __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_
   }
   T* kout = reinterpret_cast<T*>(p.dk) + b * p.dk_b + kvh * p.dk_h;
   T* vout = reinterpret_cast<T*>(p.dv) + b * p.dv_b + kvh * p.dv_h;
+  if (!ok) {  // left out: what the loop added up there is no probability
+#pragma unroll
+    for (int dt = 0; dt < S::DT; ++dt) dk[dt] = f32x16{}, dv[dt] = f32x16{};
+  }
   if (key < p.Tk) {
     float* to = nullptr;
     const int64_t rows = (int64_t)p.B * p.Hkv * p.Tk;
@@ -528,7 +538,7 @@ static int launch_backward(const Params& p, float* dtable, hipStream_t st) {
   }
   if ((p.dk || BIAS == 2) && p.Tk) {
     if (launch(&attention_dkv_kernel<T, DP, BIAS>, &dkv_done, (int64_t)p.B * p.Hkv * k_tiles * p.dkv_splits, S::THREADS,
-               S::TILES + S::BUFS * 2 * S::BM * 4 + lut + (BIAS == 2 ? (size_t)S::RG * (BiasGrad::SKEW + BiasGrad::words(p.max_distance)) * 4 : 0), p, st))
+               S::TILES + S::BUFS * 3 * S::BM * 4 + lut + (BIAS == 2 ? (size_t)S::RG * (BiasGrad::SKEW + BiasGrad::words(p.max_distance)) * 4 : 0), p, st))
       return 1;
     if (p.dk && p.dkv_splits > 1) {
       const int64_t rows = (int64_t)p.B * p.Hkv * p.Tk;

@@ -21,16 +21,18 @@ namespace attn {
 
 // Running softmax of one query per lane: maximum, sum (this half-wave's share), and the accumulators it scales.
 // The maximum only moves when a score exceeds it by more than 8 (a factor 256, far inside float's range): most tiles rescale nothing.
+template <bool BIAS>
 struct Running {
   float m = -3e38f, l = 0.f;
   template <int NS, int DT>
-  __device__ __forceinline__ void move(const float (&s)[NS][16], f32x16 (&acc)[DT]) {
+  __device__ __forceinline__ void move(const Params& p, const float (&s)[NS][16], f32x16 (&acc)[DT]) {
     float mx = s[0][0];
 #pragma unroll
     for (int n = 0; n < NS; ++n)
 #pragma unroll
       for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[n][i]);
     mx = both_max(mx);
+    if (!BIAS) mx *= p.scale2;
     if (__builtin_expect(__any(mx > m + 8.f), 0)) {
       const float mn = fmaxf(m, mx), a = exp2f(m - mn);
       m = mn;
@@ -39,8 +41,8 @@ struct Running {
       for (int dt = 0; dt < DT; ++dt) acc[dt] *= a;
     }
   }
-  __device__ __forceinline__ float weight(float s) {
-    const float x = __builtin_amdgcn_exp2f(s - m);
+  __device__ __forceinline__ float weight(const Params& p, float s) {
+    const float x = __builtin_amdgcn_exp2f(exponent<BIAS>(p, s, m));
     l += x;
     return x;
   }
@@ -101,6 +103,7 @@ __global__ __launch_bounds__((ForwardShape<T, DP, WIDE>::THREADS), (ForwardShape
   const uint8_t* mask = p.key_mask ? p.key_mask + b * p.mask_b : nullptr;
   Stationary<T, DP, S::RAW> q;
   q.load(reinterpret_cast<const T*>(p.q) + b * p.q_b + h * p.q_h + min(qi, p.Tq - 1) * p.q_t, half, p.D, true);
+  q.flip(p.flip);
   const int lut_len = 2 * p.max_distance + 1;
   const float* my_lut = lut;
   if constexpr (BIAS) {
@@ -115,7 +118,7 @@ __global__ __launch_bounds__((ForwardShape<T, DP, WIDE>::THREADS), (ForwardShape
   const int end = key_end(p, b, last_pos, word, tid, NT);
   const int all = (end + BN - 1) / BN, per = (all + splits - 1) / splits, t0 = part * per, t1 = min(all, t0 + per);
   f32x16 acc[DT] = {};
-  Running run;
+  Running<BIAS> run;
   Stage<T, DP, BN, NT> sk, sv;
   sk.start(kb, p.k_t, end, p.D, tid);
   sv.start(vb, p.v_t, end, p.D, tid);
@@ -183,14 +186,14 @@ __global__ __launch_bounds__((ForwardShape<T, DP, WIDE>::THREADS), (ForwardShape
         for (int i = 0; i < 16; ++i) s[x][i] = raw[x][i];
         finish_scores<BIAS>(p, s[x], key0 + 32 * x, pos, pos_lo, pos_hi, use.of(sub0 + x), my_lut, half);
       }
-      run.move(s, acc);
+      run.move(p, s, acc);
       if constexpr (S::EARLY) {
-        column_product_shadow<TL, DT, 0>(vv, 0, 0, [&](int i) { return run.weight(s[0][i]); }, acc, lane, nullptr, [](int) {});
+        column_product_shadow<TL, DT, 0>(vv, 0, 0, [&](int i) { return run.weight(p, s[0][i]); }, acc, lane, nullptr, [](int) {});
       } else {
 #pragma unroll
         for (int x = 0; x < NS; ++x) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) s[x][i] = run.weight(s[x][i]);
+          for (int i = 0; i < 16; ++i) s[x][i] = run.weight(p, s[x][i]);
           column_product<T, TL>(vv, (sub0 + x) * 32, 0, Weights<T>(s[x]), acc, lane);
         }
       }
@@ -208,6 +211,8 @@ __global__ __launch_bounds__((ForwardShape<T, DP, WIDE>::THREADS), (ForwardShape
     if (qi >= p.Tq || (pack && lh >= p.group) || (S::COPIES > 1 && wave)) return;
     const int64_t row = ((int64_t)b * p.H + h) * p.Tq + qi;
     if (splits == 1) {
+      if (half == 0) store_stats(p, row, run.m, l);
+      if (!p.out) return;
       const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
       T* orow = reinterpret_cast<T*>(p.out) + b * p.o_b + h * p.o_h + qi * p.o_t;
 #pragma unroll
@@ -216,7 +221,6 @@ __global__ __launch_bounds__((ForwardShape<T, DP, WIDE>::THREADS), (ForwardShape
         for (int g = 0; g < 4; ++g)
           store4<T>(orow, column_of<T>(dt * 32 + 8 * g + 4 * half, p.D), p.D, acc[dt][4 * g] * inv, acc[dt][4 * g + 1] * inv, acc[dt][4 * g + 2] * inv,
                     acc[dt][4 * g + 3] * inv);
-      if (half == 0 && p.lse) p.lse[row] = l == 0.f ? -INFINITY : (run.m + log2f(l)) * kLn2;
     } else {
       float* to = p.part + (row * splits + part) * (DP + 4);
 #pragma unroll
@@ -267,17 +271,17 @@ __global__ __launch_bounds__((ForwardShape<T, DP, WIDE>::THREADS), (ForwardShape
       f32x4 x = *reinterpret_cast<const f32x4*>(sums + c2 * LD + d);
 #pragma unroll
       for (int w = 1; w < S::WK; ++w) x += *reinterpret_cast<const f32x4*>(sums + (w * 32 + c2) * LD + d);
-      if (splits == 1)
-        store4<T>(orow, column_of<T>(d, p.D), p.D, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
-      else
+      if (splits > 1)
         *reinterpret_cast<f32x4*>(to + 4 + d) = x;
+      else if (p.out)
+        store4<T>(orow, column_of<T>(d, p.D), p.D, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
     }
     if (d_first == 0) {
       if (splits > 1) {
         to[0] = m2;
         to[1] = l2;
-      } else if (p.lse) {
-        p.lse[row] = l2 == 0.f ? -INFINITY : (m2 + log2f(l2)) * kLn2;
+      } else {
+        store_stats(p, row, m2, l2);
       }
     }
   }
@@ -312,6 +316,8 @@ __global__ __launch_bounds__(256) void attention_join_kernel(Params p) {
 #pragma unroll
     for (int u = 0; u < 8; ++u) x += y[u] * (s0 + u < p.splits ? __shfl(w, s0 + u) : 0.f);
   }
+  if (lane == 0) store_stats(p, row, m, l);
+  if (!p.out) return;
   const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
   const int qi = row % p.Tq, h = (row / p.Tq) % p.H, b = row / p.Tq / p.H;
   T* orow = reinterpret_cast<T*>(p.out) + b * p.o_b + h * p.o_h + qi * p.o_t;
@@ -320,7 +326,6 @@ __global__ __launch_bounds__(256) void attention_join_kernel(Params p) {
     const int c = lane * E + e, d = column_of<T>(c & ~3, p.D);
     if (d >= 0) orow[d + (c & 3)] = (T)(x[e] * inv);
   }
-  if (lane == 0 && p.lse) p.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
 template <class T, int DP, bool BIAS>

@@ -43,11 +43,13 @@ constexpr int64_t kMaxRowStride = 1 << 22;
 struct Params {
   const void *q, *k, *v;
   void* out;
-  float* lse;  // [B, H, Tq], natural logarithm; -inf where a row has no key
+  float* lse;    // [B, H, Tq], natural logarithm; -inf where a row has no key
+  float* stats;  // [2][B, H, Tq]: a row's reference m (log2 units) and l, the sum of exp2(score - m) over its keys; l = 0 where it has none
   int64_t q_b, q_h, q_t, k_b, k_h, k_t, v_b, v_h, v_t, o_b, o_h, o_t;
   int B, H, Hkv, group, Tq, Tk, D;
   int causal;
-  float scale, scale2;      // scale, scale * log2(e)
+  float scale, scale2;      // scale, |scale| * log2(e), above zero
+  uint32_t flip;            // sign bit for the stationary operand of the scores where the scale is negative
   const uint8_t* key_mask;  // [B, Tk], non-zero = left out
   int64_t mask_b;
   const int32_t *key_lens, *q_start;
@@ -238,6 +240,12 @@ struct Stationary {
     }
   }
   __device__ __forceinline__ const Operand<T>& get(int c) const { return o[c]; }
+  __device__ __forceinline__ void flip(uint32_t sign) {
+#pragma unroll
+    for (int c = 0; c < NC2; ++c)
+#pragma unroll
+      for (int n = 0; n < Type<T>::NP; ++n) o[c].p[n] = __builtin_bit_cast(bf16x8, __builtin_bit_cast(u32x4, o[c].p[n]) ^ (sign | sign >> 16));
+  }
 };
 template <class T, int DP>
 struct Stationary<T, DP, true> {
@@ -249,6 +257,12 @@ struct Stationary<T, DP, true> {
       o[c] = load_chunk<T>(row, 2 * c + half, D);
       if (!ok) o[c].x = {};
     }
+  }
+  __device__ __forceinline__ void flip(uint32_t sign) {
+#pragma unroll
+    for (int c = 0; c < NC2; ++c)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[c].x[e] = __uint_as_float(__float_as_uint(o[c].x[e]) ^ sign);
   }
   // the constants are hidden from the compiler, or it moves the conversion out of the loop and its results to memory
   __device__ __forceinline__ Operand<T> get(int c) const {
@@ -525,6 +539,27 @@ __device__ __forceinline__ void store4(T* row, int d, int D, float a, float b, f
   }
 }
 
+// A row's statistics.  The backward pass works with m and l apart: in the logarithm of their sum, one float, a large m leaves no bit of log2(l) (at
+// |m| > 2^24 every key of a row would count whole instead of 1 / l).
+__device__ __forceinline__ void store_stats(const Params& p, int64_t row, float m, float l) {
+  if (p.lse) p.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+  if (p.stats) {
+    p.stats[row] = m;
+    p.stats[(int64_t)p.B * p.H * p.Tq + row] = l;
+  }
+}
+// They as the backward pass takes them: P = exp2(score - m()) * inv().  A row without keys, or none at all: P = exp2(.. - inf) * 0.  Two loads that do
+// not wait for each other; the rest where the values are used.
+struct RowStats {
+  float ref, l;
+  __device__ __forceinline__ void load(const Params& p, int64_t row, bool there) {
+    ref = l = 0.f;
+    if (there) ref = p.stats[row], l = p.stats[(int64_t)p.B * p.H * p.Tq + row];
+  }
+  __device__ __forceinline__ float m() const { return l == 0.f ? INFINITY : ref; }
+  __device__ __forceinline__ float inv() const { return l == 0.f ? 0.f : 1.f / l; }
+};
+
 // Position of row b's query 0 among the keys.  Clamped so that differences of positions stay in 32 bits.
 __device__ __forceinline__ int start_of(const Params& p, int b) {
   if (!p.q_start) return p.Tk - p.Tq;
@@ -551,7 +586,7 @@ __device__ __forceinline__ void fill_lut(const Params& p, int h, float* lut, int
   }
 }
 
-// s = raw products of one 32-key subtile -> scores in log2 units with the bias; -inf where a pair is left out.
+// s = raw products of one 32-key subtile -> scores in log2 units with the bias, or the products as they are; -inf where a pair is left out.
 // key0: first key of the subtile; pos: the lane's query position, pos_lo .. pos_hi the wave's; use: bit r = key key0 + r may be used.
 template <bool BIAS>
 __device__ __forceinline__ void finish_scores(const Params& p, float (&s)[16], int key0, int pos, int pos_lo, int pos_hi, uint32_t use,
@@ -566,9 +601,6 @@ __device__ __forceinline__ void finish_scores(const Params& p, float (&s)[16], i
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[i] = fmaf(s[i], p.scale2, lut[min(max(key0 + moving_row(i, half) - pos, -md), md) + md]);
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) s[i] *= p.scale2;
   }
   if (p.causal && key0 + 31 > pos_lo) {
     const int last = pos - key0 - 4 * half;
@@ -580,6 +612,14 @@ __device__ __forceinline__ void finish_scores(const Params& p, float (&s)[16], i
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[i] = (mine >> moving_row(i, 0)) & 1 ? s[i] : -INFINITY;
   }
+}
+
+// What finish_scores gives, less the row's reference m in log2 units.  Scores without a bias are scaled here, by the one fma that takes m off: no
+// rounding in between, the same expression in every kernel (beside a large common level half a step of a score would be as much as the scores
+// differ), and an instruction less, which is what the factor 1 / l of P costs in the kernel of dk and dv.
+template <bool BIAS>
+__device__ __forceinline__ float exponent(const Params& p, float s, float m) {
+  return BIAS ? s - m : fmaf(s, p.scale2, -m);
 }
 
 // The sum over bucket n's distances of sums[rel + max_distance], in their order.
