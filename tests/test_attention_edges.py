@@ -101,3 +101,65 @@ def test_scales_of_any_sign(dtype, scale, D, Tq, Tk):
     mask = (torch.rand(2, Tk, generator=torch.Generator().manual_seed(2)) < 0.3).cuda()
     run_case(dtype, 2, 4, 2, Tq, Tk, D, scale=scale, mask=mask, causal=True)
     run_case(dtype, 2, 4, 2, Tq, Tk, D, scale=scale, mask=mask, table=normal(3, 16, 4))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("B,H,G,Tq,Tk,D", [(2, 2, 2, 50, 40, 64), (2, 4, 2, 300, 130, 128), (2, 2, 1, 90, 70, 200), (40, 4, 4, 160, 160, 32),
+                                           (2, 2, 2, 7, 300, 64)])
+@pytest.mark.parametrize("with_table", [False, True])
+def test_what_lies_at_queries_without_keys_is_never_used(dtype, bad, B, H, G, Tq, Tk, D, with_table):
+    """Queries that causality or a row's mask leaves no key, with NaN or infinities in q and in the output's gradient: no bit of the other rows'
+    results changes, and their own are zero."""
+    q, k, v, dout = (normal(i, B, H if i in (0, 3) else G, Tq if i in (0, 3) else Tk, D, dtype=dtype) for i in range(4))
+    table = [normal(5, 16, H)] if with_table else []
+    start = torch.full((B,), -(Tq // 3), dtype=torch.int32, device="cuda")
+    mask = torch.zeros(B, Tk, dtype=torch.bool, device="cuda")
+    mask[1], mask[0, 2] = True, True
+    lens = torch.full((B,), Tk - 2, dtype=torch.int32, device="cuda")
+    lens[1] = 0
+    for rule, first in ((dict(causal=True, q_start=start), True), (dict(key_mask=mask), False), (dict(key_lens=lens), False),
+                        (dict(key_mask=mask, causal=True, q_start=start), True)):
+        empty = torch.zeros(B, Tq, dtype=torch.bool, device="cuda")
+        if first:
+            empty[:, :Tq // 3] = True
+        if "key_mask" in rule or "key_lens" in rule:
+            empty[1] = True
+        empty = empty[:, None, :, None]
+        want = gradients([q, k, v] + table, dout, **rule)
+        got = gradients([q.masked_fill(empty, bad), k, v] + table, dout.masked_fill(empty, bad), **rule)
+        for name, x, y in zip(("out", "dq", "dk", "dv", "dtable"), got, want):
+            assert torch.equal(x, y), (name, rule.keys())
+        assert not got[0].masked_select(empty).any() and not got[1].masked_select(empty).any()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("D", [64, 128, 200])
+def test_left_out_keys_get_no_gradient(dtype, D):
+    """Keys that a mask leaves out have zero gradients whatever a query in use holds, and table entries of distances that only left-out pairs
+    have take no part, NaN included."""
+    q, k, v, dout = (normal(i, 2, 2, 80, D, dtype=dtype) for i in range(4))
+    mask = torch.zeros(2, 80, dtype=torch.bool, device="cuda")
+    mask[:, 60:] = True
+    spoiled = q.clone()
+    spoiled[:, :, 33] = math.nan
+    got = gradients([spoiled, k, v], dout, key_mask=mask)
+    assert not got[2][:, :, 60:].any() and not got[3][:, :, 60:].any()
+    table = normal(5, 16, 2)
+    rule = dict(causal=True, max_distance=20)           # distances ahead (the second half of the table) are never allowed
+    want = gradients([q, k, v, table], dout, **rule)
+    table[9:] = math.nan
+    got = gradients([q, k, v, table], dout, **rule)
+    for x, y in zip(got, want):
+        assert torch.equal(x, y)
+    start = torch.zeros(2, dtype=torch.int32, device="cuda")      # queries 0 .. 3 against keys 0 .. 9 of 80: no distance above 9 is allowed
+    mask = torch.arange(80, device="cuda").expand(2, 80) >= 10
+    table = normal(5, 64, 2)
+    rule = dict(q_start=start, key_mask=mask, max_distance=128)
+    want = gradients([q[:, :, :4], k, v, table], dout[:, :, :4], **rule)
+    table[32 + 14:] = math.nan
+    got = gradients([q[:, :, :4], k, v, table], dout[:, :, :4], **rule)
+    for x, y in zip(got, want):
+        assert torch.equal(x, y)

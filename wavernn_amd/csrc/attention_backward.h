@@ -178,13 +178,17 @@ __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_
   const uint8_t* mask = p.key_mask ? p.key_mask + b * p.mask_b : nullptr;
   const int qi = q0 + col, qc = min(qi, p.Tq - 1), pos = qi + off;
   const int pos_lo = q0 + off, pos_hi = pos_lo + 31;
+  // a query without keys (or past the last one) takes part in nothing, whatever its q and dout hold
+  RowStats row;
+  row.load(p, (int64_t)bh * p.Tq + qi, qi < p.Tq);
+  const float m = row.m(), inv = row.inv();  // 1 / l enters where the sums over the keys are stored
   Stationary<T, S::DA, false> q, go;
   float delta = 0.f;
   {
     const T* gr = reinterpret_cast<const T*>(p.dout) + b * p.do_b + h * p.do_h + qc * p.do_t;
-    q.load(reinterpret_cast<const T*>(p.q) + b * p.q_b + h * p.q_h + qc * p.q_t + d0, half, p.D - d0, true);
+    q.load(reinterpret_cast<const T*>(p.q) + b * p.q_b + h * p.q_h + qc * p.q_t + d0, half, p.D - d0, row.some());
     q.flip(p.flip);
-    go.load(gr + d0, half, p.D - d0, true);
+    go.load(gr + d0, half, p.D - d0, row.some());
     const T* orow = reinterpret_cast<const T*>(p.o_in) + b * p.oi_b + h * p.oi_h + qc * p.oi_t;
 #pragma unroll
     for (int c = 0; c < DP / 16; ++c) {
@@ -192,11 +196,8 @@ __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_
 #pragma unroll
       for (int e = 0; e < 8; ++e) delta += (float)g.x[e] * (float)o.x[e];
     }
-    delta = both_sum(delta);
+    delta = row.some() ? both_sum(delta) : 0.f;
   }
-  RowStats row;
-  row.load(p, (int64_t)bh * p.Tq + qi, qi < p.Tq);
-  const float m = row.m(), inv = row.inv();  // 1 / l enters where the sums over the keys are stored
   if constexpr (BIAS != 0) fill_lut(p, h, lut, tid, NT);
   const int end = key_end(p, b, min(qt * S::ROWS + S::ROWS - 1, p.Tq - 1) + off, word, tid, NT);
   const int all = (end + BN - 1) / BN, per = (all + p.dq_splits - 1) / p.dq_splits;
@@ -331,7 +332,6 @@ __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_
   k.load(reinterpret_cast<const T*>(p.k) + b * p.k_b + kvh * p.k_h + kc * p.k_t + d0, half, p.D - d0, ok);
   k.flip(p.flip);
   v.load(reinterpret_cast<const T*>(p.v) + b * p.v_b + kvh * p.v_h + kc * p.v_t + d0, half, p.D - d0, ok);
-  [[maybe_unused]] const float add = ok ? 0.f : -INFINITY;
   f32x16 dk[S::DT] = {}, dv[S::DT] = {};
   // under causality queries before key - off see nothing of this block
   const int qt_n = (p.Tq + BM - 1) / BM, qt_0 = p.causal ? min(max(k0 - off, 0) / BM, qt_n) : 0, per = qt_n - qt_0;
@@ -340,20 +340,22 @@ __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_
   Stage<T, DP, BM, NT> sq, sg;
   sq.start(nullptr, p.q_t, p.Tq, p.D, tid);
   sg.start(nullptr, p.do_t, p.Tq, p.D, tid);
-  RowStats s_row = {};
+  RowStats s_row = {};  // lane's row of the tile on its way
   float s_delta = 0.f;
+  bool there = false;
   auto load = [&](int it) {
     if (it >= steps) return;
     const int h = kvh * p.group + it / per, r0 = (qt_0 + it % per) * BM;
+    there = lane < BM && r0 + lane < p.Tq;
+    const int64_t row = ((int64_t)b * p.H + h) * p.Tq + r0 + lane;
+    s_row.load(p, row, there);
     sq.base = reinterpret_cast<const char*>(reinterpret_cast<const T*>(p.q) + b * p.q_b + h * p.q_h);
     sg.base = reinterpret_cast<const char*>(reinterpret_cast<const T*>(p.dout) + b * p.do_b + h * p.do_h);
     sq.load(r0, nullptr, tid);
     sg.load(r0, nullptr, tid);
     if (tid < BM) {
-      const int64_t row = ((int64_t)b * p.H + h) * p.Tq + r0 + tid;
-      s_row.load(p, row, r0 + tid < p.Tq);
       s_delta = 0.f;
-      if (r0 + tid < p.Tq)
+      if (there)
         for (int n = 0; n < (BIAS == 2 ? p.dq_splits : 1); ++n) s_delta += p.delta[(int64_t)n * p.B * p.H * p.Tq + row];
     }
   };
@@ -362,11 +364,22 @@ __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_
     if (tid < BM) {
       stat[o * 3 * BM + tid] = s_row.m();
       stat[(o * 3 + 1) * BM + tid] = s_row.inv();
-      stat[(o * 3 + 2) * BM + tid] = s_delta;
+      stat[(o * 3 + 2) * BM + tid] = s_row.some() ? s_delta : 0.f;
+    }
+  };
+  // Queries without keys: their rows become zero on their way to LDS.  P = 0 alone would not keep out what they hold, 0 * NaN being NaN.
+  auto drop = [&]() {
+    const uint64_t none = __ballot(there && !s_row.some());
+    if (none) {
+      RowBits use;
+      use.lo = ~none;
+      sq.drop(use, tid);
+      sg.drop(use, tid);
     }
   };
   auto store = [&](int it) {
     const int o = it & (BUFS - 1);
+    drop();
     sq.store(qt + o * TL::BYTES, tid);
     sg.store(gt + o * TL::BYTES, tid);
     store_stat(it);
@@ -396,6 +409,7 @@ __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_
       f32x16 raw = {}, dp = {};
       if constexpr (S::EARLY) {
         char *qn = qt + ((it + 1) & (BUFS - 1)) * TL::BYTES, *gn = gt + ((it + 1) & (BUFS - 1)) * TL::BYTES;
+        drop();
         products_shadow<TL, NC2>(qq, gg, k, v, raw, dp, sq, sg, qn, gn, col, half, tid);
         store_stat(it + 1);
         load(it + 2);
@@ -414,12 +428,12 @@ __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_
         if constexpr (BIAS) {
           const int md = p.max_distance;
           if (kw + 31 - p0 <= -md || kw - (p0 + 31) >= md) {
-            const float far = lut[kw > p0 ? 2 * md : 0] + add;
+            const float far = ok ? lut[kw > p0 ? 2 * md : 0] : -INFINITY;
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[i] = fmaf(raw[i], p.scale2, far);
           } else {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] = fmaf(raw[i], p.scale2, lut[min(max(key - p0 - moving_row(i, half), -md), md) + md] + add);
+            for (int i = 0; i < 16; ++i) s[i] = fmaf(raw[i], p.scale2, ok ? lut[min(max(key - p0 - moving_row(i, half), -md), md) + md] : -INFINITY);
           }
         } else {
 #pragma unroll

@@ -556,6 +556,7 @@ struct RowStats {
     ref = l = 0.f;
     if (there) ref = p.stats[row], l = p.stats[(int64_t)p.B * p.H * p.Tq + row];
   }
+  __device__ __forceinline__ bool some() const { return l != 0.f; }  // whether the row has a key
   __device__ __forceinline__ float m() const { return l == 0.f ? INFINITY : ref; }
   __device__ __forceinline__ float inv() const { return l == 0.f ? 0.f : 1.f / l; }
 };
