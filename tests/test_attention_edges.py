@@ -163,3 +163,23 @@ def test_left_out_keys_get_no_gradient(dtype, D):
     got = gradients([q[:, :, :4], k, v, table], dout[:, :, :4], **rule)
     for x, y in zip(got, want):
         assert torch.equal(x, y)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("Tq,D", [(60, 16), (60, 200), (3, 64)])
+@pytest.mark.parametrize("low,lower", [(-1e30, LOWEST), (-1e31, -1e35), (-2e38, LOWEST), (-3e38, LOWEST)])
+def test_low_values_of_a_table_keep_their_order(dtype, Tq, D, low, lower):
+    """A key whose bias is `lower` gets no weight beside one of `low`, as finite as both are."""
+    q, k, v, dout = (normal(i, 1, 2, Tq if i in (0, 3) else 60, D, dtype=dtype) for i in range(4))
+    table, same = torch.full((8, 2), lower), torch.full((8, 2), -math.inf)
+    table[1::2] = low
+    same[1::2] = 0.0
+    q = torch.zeros_like(q)               # any score vanishes beside such a bias
+    rule = dict(max_distance=20)
+    got = gradients([q, k, v, table.cuda()], dout, **rule)
+    want = reference(q, k, v, dout, table=same, **rule)
+    for name, x in zip(("out", "dq", "dk", "dv", "dtable"), got):
+        check(name, x, want[name])
+    lse = A.attention(q, k, v, bias_table=table.cuda(), return_lse=True, **rule)[1]
+    assert bool(((lse / low - 1).abs() < 1e-5).all())

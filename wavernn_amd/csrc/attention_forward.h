@@ -23,7 +23,7 @@ namespace attn {
 // The maximum only moves when a score exceeds it by more than 8 (a factor 256, far inside float's range): most tiles rescale nothing.
 template <bool BIAS>
 struct Running {
-  float m = -3e38f, l = 0.f;
+  float m = kLowest, l = 0.f;
   template <int NS, int DT>
   __device__ __forceinline__ void move(const Params& p, const float (&s)[NS][16], f32x16 (&acc)[DT]) {
     float mx = s[0][0];
@@ -294,7 +294,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(Params p) {
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (row >= (int64_t)p.B * p.H * p.Tq) return;
   const float* part = p.part + row * p.splits * (DP + 4);
-  float ms = -3e38f, ls = 0.f;
+  float ms = kLowest, ls = 0.f;
   if (lane < p.splits) {
     ms = part[lane * (DP + 4)];
     ls = part[lane * (DP + 4) + 1];

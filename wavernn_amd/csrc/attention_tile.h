@@ -33,7 +33,8 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f, kLowest = -3.4028235e38f;
+constexpr float kFarBias = 2.3e38f, kFarSlope = 0.05f;  // bias_log2
 constexpr int kMaxEdges = 128;
 constexpr int kMaxDistance = 1024;
 constexpr int kFewKeys = 512;  // up to here the bfloat16 backward pass takes more care over roundings (BackwardShape)
@@ -539,10 +540,40 @@ __device__ __forceinline__ void store4(T* row, int d, int D, float a, float b, f
   }
 }
 
+// Position of row b's query 0 among the keys.  Clamped so that differences of positions stay in 32 bits.
+__device__ __forceinline__ int start_of(const Params& p, int b) {
+  if (!p.q_start) return p.Tk - p.Tq;
+  return min(max(p.q_start[b], -(1 << 29)), 1 << 29);
+}
+
+__device__ __forceinline__ int bucket_of(const Params& p, int rel) {
+  const int far = p.two_sided ? abs(rel) : max(-rel, 0);
+  int n = far;
+  if (far >= p.exact_side) {
+    n = p.exact_side;
+    for (int i = 0; i < p.n_edges; ++i) n += far >= p.edges[i] ? 1 : 0;
+  }
+  return n + (p.two_sided && rel > 0 ? p.side : 0);
+}
+
+// A bias in log2 units.  Past kFarBias in size the change of unit would overflow: from there on it goes with a gentler slope, which keeps
+// finite values finite and their order (any two of that size are so far apart that the lower gets no weight), and infinite ones infinite.
+__device__ __forceinline__ float bias_log2(float x) {
+  const float a = fabsf(x);
+  return a <= kFarBias ? x * kLog2e : copysignf(kFarBias * kLog2e + (a - kFarBias) * kFarSlope, x);
+}
+// The logarithm of a row's sum of exponentials, natural.
+__device__ __forceinline__ float row_lse(const Params& p, float m, float l) {
+  if (l == 0.f) return -INFINITY;
+  const float far = fabsf(m) - kFarBias * kLog2e;
+  if (p.table && far > 0.f) return copysignf(fminf(kFarBias + far / kFarSlope, -kLowest), m);
+  return (m + log2f(l)) * kLn2;
+}
+
 // A row's statistics.  The backward pass works with m and l apart: in the logarithm of their sum, one float, a large m leaves no bit of log2(l) (at
 // |m| > 2^24 every key of a row would count whole instead of 1 / l).
 __device__ __forceinline__ void store_stats(const Params& p, int64_t row, float m, float l) {
-  if (p.lse) p.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+  if (p.lse) p.lse[row] = row_lse(p, m, l);
   if (p.stats) {
     p.stats[row] = m;
     p.stats[(int64_t)p.B * p.H * p.Tq + row] = l;
@@ -561,29 +592,10 @@ struct RowStats {
   __device__ __forceinline__ float inv() const { return l == 0.f ? 0.f : 1.f / l; }
 };
 
-// Position of row b's query 0 among the keys.  Clamped so that differences of positions stay in 32 bits.
-__device__ __forceinline__ int start_of(const Params& p, int b) {
-  if (!p.q_start) return p.Tk - p.Tq;
-  return min(max(p.q_start[b], -(1 << 29)), 1 << 29);
-}
-
-__device__ __forceinline__ int bucket_of(const Params& p, int rel) {
-  const int far = p.two_sided ? abs(rel) : max(-rel, 0);
-  int n = far;
-  if (far >= p.exact_side) {
-    n = p.exact_side;
-    for (int i = 0; i < p.n_edges; ++i) n += far >= p.edges[i] ? 1 : 0;
-  }
-  return n + (p.two_sided && rel > 0 ? p.side : 0);
-}
-
-// The bias of head h by clamped distance, in log2 units: lut[rel + max_distance].  Finite values below -1e30 become -1e30: the
-// same softmax in 32 bits (nothing a score can add is left at either size), without overflow in the change of unit.
+// The bias of head h by clamped distance, in log2 units: lut[rel + max_distance].
 __device__ __forceinline__ void fill_lut(const Params& p, int h, float* lut, int tid, int threads) {
   for (int i = tid; i <= 2 * p.max_distance; i += threads) {
-    float x = p.table[(int64_t)bucket_of(p, i - p.max_distance) * p.H + h];
-    if (x < -1e30f && x >= -3.4028235e38f) x = -1e30f;
-    lut[i] = x * kLog2e;
+    lut[i] = bias_log2(p.table[(int64_t)bucket_of(p, i - p.max_distance) * p.H + h]);
   }
 }
 
