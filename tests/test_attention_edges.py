@@ -183,3 +183,24 @@ def test_low_values_of_a_table_keep_their_order(dtype, Tq, D, low, lower):
         check(name, x, want[name])
     lse = A.attention(q, k, v, bias_table=table.cuda(), return_lse=True, **rule)[1]
     assert bool(((lse / low - 1).abs() < 1e-5).all())
+
+
+@gpu
+@pytest.mark.parametrize("D", [64, 128, 200])
+@pytest.mark.parametrize("Tk", [60, 300, 700, 1000, 1500])
+@pytest.mark.parametrize("H", [2, 256])
+def test_rounded_outputs_do_not_reach_the_keys_gradients(D, Tk, H):
+    """bfloat16, values far from zero: delta = rowsum(dout * out) carries the rounding of out, here some 4 % of the spread of dS, and dk must not,
+    in however many shares the keys are worked on.  What may be left: dS is rounded where it enters its product (independent roundings, a
+    half step over sqrt 3 each) and dk where it is stored (half a step); all queries are one vector, so neither is magnified."""
+    Tq = 100 if H == 2 else 40
+    q, k, dout = normal(0, 1, H, 1, D, dtype=BF16).expand(1, H, Tq, D), normal(1, 1, H, Tk, D, dtype=BF16), normal(3, 1, H, Tq, D, dtype=BF16)
+    v = (normal(2, 1, H, Tk, D) + 30).to(BF16)
+    dk = gradients([q, k, v], dout)[2].double()
+    qd, kd, vd, go = (x.double() for x in (q.contiguous(), k, v, dout))
+    p = torch.softmax(qd @ kd.transpose(-1, -2).contiguous() / D ** 0.5, -1)
+    dp = go @ vd.transpose(-1, -2).contiguous()
+    ds = p * (dp - (p * dp).sum(-1, keepdim=True))
+    want = ds.transpose(-1, -2).contiguous() @ qd / D ** 0.5
+    half_step = torch.finfo(BF16).eps / 2
+    assert float((dk - want).norm() / want.norm()) < (1 + 1 / 3 ** 0.5) * half_step

@@ -56,8 +56,8 @@ static size_t split_workspace(const Params& p) {
 // blocks of a workgroup's rows: two waves share a row past 128 columns (BackwardShape)
 static int row_blocks(const Params& p, int rows) { return p.D > 128 ? (rows + 63) / 64 : (rows + 127) / 128; }
 static void plan_backward(Params* p, int dtype) {
-  // (bfloat16 with few keys: a query's row sum of dS has to lie in one workgroup, BackwardShape; the joining launch costs what shares would save)
-  p->dq_splits = dtype == WRNN_BFLOAT16 && p->Tk <= kFewKeys ? 1 : shares((int64_t)p->B * p->H * row_blocks(*p, p->Tq), (p->Tk + 31) / 32, 4);
+  // (bfloat16 with few keys: the joining launch costs what shares would save)
+  p->dq_splits = dtype == WRNN_BFLOAT16 && p->Tk <= 512 ? 1 : shares((int64_t)p->B * p->H * row_blocks(*p, p->Tq), (p->Tk + 31) / 32, 4);
   // (causality: the first keys' blocks are the longest by far; half as long they leave the others time to fill up)
   const int64_t blocks = (int64_t)p->B * p->Hkv * row_blocks(*p, p->Tk);
   p->dkv_splits = shares(p->causal ? (blocks + 1) / 2 : blocks, (int64_t)((p->Tq + 31) / 32) * p->group, 4);
@@ -65,7 +65,9 @@ static void plan_backward(Params* p, int dtype) {
 static size_t aligned(size_t x) { return (x + 255) & ~size_t(255); }
 // the backward workspace: the rows' statistics, delta, the table's partial sums, the shares
 static size_t stats_bytes(const Params& p) { return aligned((size_t)2 * p.B * p.H * p.Tq * sizeof(float)); }
-static size_t delta_bytes(const Params& p) { return aligned((size_t)(p.table ? p.dq_splits : 1) * p.B * p.H * p.Tq * sizeof(float)); }
+static size_t delta_bytes(const Params& p, int dtype) {
+  return aligned((size_t)(p.table || dtype == WRNN_BFLOAT16 ? p.dq_splits : 1) * p.B * p.H * p.Tq * sizeof(float));
+}
 static size_t table_bytes(const Params& p) {
   return p.table ? aligned((size_t)p.B * row_blocks(p, p.Tk) * p.dkv_splits * p.H * p.buckets * sizeof(float)) : 0;
 }
@@ -153,7 +155,7 @@ extern "C" size_t wrnn_attention_backward_workspace_bytes(const wrnn_attention_d
   if (attention_params(desc, &p, "wrnn_attention_backward_workspace_bytes") || !p.B || !p.H || !p.Tq) return 0;
   attn::plan(&p);
   attn::plan_backward(&p, desc->dtype);
-  const size_t rest = attn::delta_bytes(p) + attn::table_bytes(p) + attn::dq_bytes(p) + attn::dkv_bytes(p), forward = attn::split_workspace(p);
+  const size_t rest = attn::delta_bytes(p, desc->dtype) + attn::table_bytes(p) + attn::dq_bytes(p) + attn::dkv_bytes(p), forward = attn::split_workspace(p);
   return attn::stats_bytes(p) + (rest > forward ? rest : forward);
 }
 
@@ -199,7 +201,7 @@ extern "C" int wrnn_attention_backward_stats(const wrnn_attention_desc* desc, co
   }
   attn::plan_backward(&p, desc->dtype);
   p.delta = reinterpret_cast<float*>(w += attn::stats_bytes(p));
-  p.dtable_part = reinterpret_cast<float*>(w += attn::delta_bytes(p));
+  p.dtable_part = reinterpret_cast<float*>(w += attn::delta_bytes(p, desc->dtype));
   p.dq_part = reinterpret_cast<float*>(w += attn::table_bytes(p));
   p.dkv_part = reinterpret_cast<float*>(w + attn::dq_bytes(p));
   return desc->dtype == WRNN_FLOAT32 ? attn::backward<float>(p, g->dtable, st) : attn::backward<__bf16>(p, g->dtable, st);

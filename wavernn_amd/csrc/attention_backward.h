@@ -95,9 +95,11 @@ struct BackwardShape {
   // the more so the fewer columns there are: with one plane dq is off by 2.5e-3 .. 3.3e-3 of its norm up to 64 columns, by 2.4e-3 .. 2.9e-3 above,
   // the most where a query has few keys (rounding dq itself: 1.7e-3).  With two, 1.7e-3 .. 2.1e-3: always up to 64 columns (2 x 16 heads,
   // 4096 x 4096: 541 -> 611 us), above that, where the matrix instructions bound the kernel (1253 -> 1407 us), only for blocks of queries that
-  // reach at most FEW keys.  Those hand on the corrected delta, too.
+  // reach at most FEW keys.
   static constexpr bool FINE = NP == 1 && DP == 64;
-  static constexpr int FEW = FINE ? kFewKeys : 2 * kFewKeys;
+  template <int BIAS>
+  static constexpr bool CORRECTED = BIAS == 2 || NP == 1;  // of delta (attention_dq_kernel)
+  static constexpr int FEW = 1024;
 };
 
 // Both waves' parts of a sum added up.  `mine` and `other` are the waves' places; what a wave hands in stays until the other has read it, so the
@@ -148,11 +150,12 @@ __device__ __forceinline__ void products_shadow(const char* x, const char* y, co
   }
 }
 
-// dq: queries stationary, key tiles through LDS.  delta = rowsum(dout * out) carries the rounding of out and of the probabilities behind it.  That is
-// less than the rounding of dq itself, but the table's gradient adds it up over all rows in the buckets that hold most of a row's keys, and in
-// bfloat16 with few keys dk shows it (2.8e-3 of its norm, without 2.4e-3).  There the kernel also sums dS over each row - what delta is off by, as the
-// probabilities add up to one - and the next kernel, which makes dk, dv and the table's gradient, works with the corrected delta: the adds are hidden
-// or few, a second walk over the keys for it took twice the time.
+// dq: queries stationary, key tiles through LDS.  delta = rowsum(dout * out) carries the rounding of out and of the probabilities behind it.  The table's
+// gradient adds it up over all rows in the buckets that hold most of a row's keys, and in bfloat16 dk shows it: with few keys (2.8e-3 of its
+// norm, without 2.4e-3), and at any length where the values lie far from zero beside their spread (30 +- 1: 3 .. 6e-2, without 2.3e-3).
+// There the kernel also sums dS over each row - what delta is off by, as the probabilities add up to one - and the next kernel, which makes dk, dv and the
+// table's gradient, works with the corrected delta, the sum of the shares' planes: a second walk over the keys for it took twice the
+// time.  dq itself keeps the uncorrected delta.
 template <class T, int DP, int BIAS>
 __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_dq_kernel(Params p) {
   using S = BackwardShape<T, DP>;
@@ -262,7 +265,7 @@ __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_
           for (int i = 0; i < 16; ++i) pr[i] = __builtin_amdgcn_exp2f(exponent<BIAS != 0>(p, pr[i], m));
 #pragma unroll
           for (int i = 0; i < 16; ++i) pr[i] *= dp[i] - delta;
-          if constexpr (BIAS == 2 || exact)
+          if constexpr (S::template CORRECTED<BIAS>)
 #pragma unroll
             for (int i = 0; i < 16; ++i) off_by += pr[i];
           if constexpr (S::EARLY)
@@ -281,18 +284,15 @@ __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_
     }
   };
   // (two loops: a choice inside would have both its ways' sums copied in every round)
-  if constexpr (S::NP == 1) {
+  if constexpr (S::NP == 1 && !S::FINE) {
     if (end <= S::FEW) walk(std::true_type());
     else walk(std::false_type());
   } else {
     walk(std::false_type());
   }
   off_by = both_sum(off_by) * inv;
-  // (a share's sum is only part of a row's: with BIAS == 2 the next kernel adds them up, otherwise such rows do without)
-  if (half == 0 && d0 == 0 && qi < p.Tq && (BIAS == 2 || share == 0)) {
-    const float whole = BIAS == 2 || p.dq_splits == 1 ? off_by : 0.f;
-    p.delta[((int64_t)(BIAS == 2 ? share : 0) * p.B * p.H + bh) * p.Tq + qi] = share == 0 ? delta + whole : whole;
-  }
+  if (half == 0 && d0 == 0 && qi < p.Tq && (S::template CORRECTED<BIAS> || share == 0))
+    p.delta[((int64_t)share * p.B * p.H + bh) * p.Tq + qi] = share == 0 ? delta + off_by : off_by;
   if (qi < p.Tq)
     store_rows<S>(acc, reinterpret_cast<T*>(p.dq) + b * p.dq_b + h * p.dq_h + qi * p.dq_t,
                   p.dq_splits > 1 ? p.dq_part + (((int64_t)share * p.B * p.H + bh) * p.Tq + qi) * p.D : nullptr, d0, p.D, p.scale * inv, half);
@@ -356,7 +356,7 @@ __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_
     if (tid < BM) {
       s_delta = 0.f;
       if (there)
-        for (int n = 0; n < (BIAS == 2 ? p.dq_splits : 1); ++n) s_delta += p.delta[(int64_t)n * p.B * p.H * p.Tq + row];
+        for (int n = 0; n < (S::template CORRECTED<BIAS> ? p.dq_splits : 1); ++n) s_delta += p.delta[(int64_t)n * p.B * p.H * p.Tq + row];
     }
   };
   auto store_stat = [&](int it) {

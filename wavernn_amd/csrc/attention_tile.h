@@ -37,7 +37,6 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f, kLowes
 constexpr float kFarBias = 2.3e38f, kFarSlope = 0.05f;  // bias_log2
 constexpr int kMaxEdges = 128;
 constexpr int kMaxDistance = 1024;
-constexpr int kFewKeys = 512;  // up to here the bfloat16 backward pass takes more care over roundings (BackwardShape)
 constexpr int64_t kMaxRowStride = 1 << 22;
 
 // What the kernels get, by value.  Strides count elements; the last dimension is contiguous.
