@@ -1,0 +1,44 @@
+"""Self-attention as it may be called: strides of every kind, other kinds of differentiation, gradients that are not there, lengths and positions
+past what the kernels count in, rules made at the same time."""
+
+import pytest
+import torch
+
+from attention_ref import check, reference
+from test_attention import BF16, F32, normal
+from wavernn_amd import attention as A
+
+gpu = pytest.mark.gpu
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_strides_over_dimensions_of_one(dtype):
+    """What a stride over a single row or position says does not matter, in gradients as in inputs."""
+    q, k, v = (normal(i, 1, 2, 5, 16, dtype=dtype).requires_grad_() for i in range(3))
+    dout = normal(3, 1, 2, 5, 16, dtype=dtype)
+    odd = dout.as_strided(dout.shape, (161, *dout.stride()[1:]))
+    want, got = (torch.autograd.grad(A.attention(q, k, v), (q, k, v), d) for d in (dout, odd))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    q1 = normal(0, 2, 2, 1, 16, dtype=dtype).requires_grad_()
+    k, v = (normal(i, 2, 2, 5, 16, dtype=dtype).requires_grad_() for i in (1, 2))
+    dout = normal(3, 2, 2, 1, 16, dtype=dtype)
+    far = dout.as_strided(dout.shape, (*dout.stride()[:2], 1 << 23, 1))
+    want, got = (torch.autograd.grad(A.attention(q1, k, v), (q1, k, v), d) for d in (dout, far))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_broadcast_batch_with_far_positions(dtype):
+    """Inputs of one row for a large batch: their gradients' positions lie further apart than the kernels read rows, and are only written."""
+    B, H, D = 4096, 4, 256
+    q, k, v = (normal(i, 2, H, D, dtype=dtype).requires_grad_() for i in range(3))
+    many = [x[None].expand(B, 2, H, D).permute(0, 2, 1, 3) for x in (q, k, v)]
+    dout = normal(3, 1, H, 2, D, dtype=dtype)
+    got = torch.autograd.grad(A.attention(*many), (q, k, v), dout.expand(B, H, 2, D))
+    want = reference(*(x[:1] for x in many), dout)
+    for name, g in zip(("dq", "dk", "dv"), got):
+        value, bound = want[name]
+        # autograd adds the rows' gradients up: B equal values, each addition half a step of the inputs' type or of 32 bits
+        check(name, g.double().permute(1, 0, 2)[None] / B, (value, bound + (torch.finfo(dtype).eps + B * 2.0 ** -24) * value.abs()))

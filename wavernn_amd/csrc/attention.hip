@@ -74,6 +74,9 @@ static size_t table_bytes(const Params& p) {
 static size_t dq_bytes(const Params& p) { return p.dq_splits > 1 ? aligned((size_t)p.dq_splits * p.B * p.H * p.Tq * p.D * sizeof(float)) : 0; }
 static size_t dkv_bytes(const Params& p) { return p.dkv_splits > 1 ? (size_t)p.dkv_splits * 2 * p.B * p.Hkv * p.Tk * p.D * sizeof(float) : 0; }
 
+// a stride over a dimension of one is never taken: whatever it says, it does not decide about alignment
+static int64_t stride_of(int n, int64_t s) { return n > 1 ? s : 0; }
+
 }  // namespace attn
 
 int attention_params(const wrnn_attention_desc* d, attn::Params* p, const char* who) {
@@ -90,12 +93,10 @@ int attention_params(const wrnn_attention_desc* d, attn::Params* p, const char* 
   const bool some = d->batch && d->heads && d->q_len;
   WRNN_REQUIRE(!some || (d->q && (d->k_len == 0 || (d->k && d->v))), "%s: null pointer", who);
   *p = Params{};
-  // a stride over a dimension of one is never taken: whatever it says, it does not decide about alignment
-  auto st = [](int n, int64_t s) { return n > 1 ? s : 0; };
   p->q = d->q, p->k = d->k, p->v = d->v;
-  p->q_b = st(d->batch, d->q_stride[0]), p->q_h = st(d->heads, d->q_stride[1]), p->q_t = st(d->q_len, d->q_stride[2]);
-  p->k_b = st(d->batch, d->k_stride[0]), p->k_h = st(d->kv_heads, d->k_stride[1]), p->k_t = st(d->k_len, d->k_stride[2]);
-  p->v_b = st(d->batch, d->v_stride[0]), p->v_h = st(d->kv_heads, d->v_stride[1]), p->v_t = st(d->k_len, d->v_stride[2]);
+  p->q_b = stride_of(d->batch, d->q_stride[0]), p->q_h = stride_of(d->heads, d->q_stride[1]), p->q_t = stride_of(d->q_len, d->q_stride[2]);
+  p->k_b = stride_of(d->batch, d->k_stride[0]), p->k_h = stride_of(d->kv_heads, d->k_stride[1]), p->k_t = stride_of(d->k_len, d->k_stride[2]);
+  p->v_b = stride_of(d->batch, d->v_stride[0]), p->v_h = stride_of(d->kv_heads, d->v_stride[1]), p->v_t = stride_of(d->k_len, d->v_stride[2]);
   // a lane's rows inside a tile are found with 32-bit offsets
   for (int64_t s : {p->q_t, p->k_t, p->v_t})
     WRNN_REQUIRE(s >= 0 && s < kMaxRowStride, "%s: position strides are in 0 .. 2^22 - 1 elements", who);
@@ -143,7 +144,8 @@ extern "C" int wrnn_attention_forward_stats(const wrnn_attention_desc* desc, voi
   const size_t need = attn::split_workspace(p);
   WRNN_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && !((uintptr_t)workspace & 15)),
                "wrnn_attention_forward: workspace of %zu bytes, %zu are needed, on 16 bytes", workspace_bytes, need);
-  p.out = out, p.o_b = out_stride[0], p.o_h = out_stride[1], p.o_t = out_stride[2], p.lse = lse, p.stats = stats;
+  p.out = out, p.lse = lse, p.stats = stats;
+  p.o_b = attn::stride_of(p.B, out_stride[0]), p.o_h = attn::stride_of(p.H, out_stride[1]), p.o_t = attn::stride_of(p.Tq, out_stride[2]);
   p.part = static_cast<float*>(workspace);
   WRNN_REQUIRE(attn::rows_on_four(out, p.o_b, p.o_h, p.o_t, desc->dtype == WRNN_FLOAT32 ? 4 : 2), "wrnn_attention_forward: rows of out have to start on the bytes of four elements");
   const hipStream_t st = static_cast<hipStream_t>(stream);
@@ -179,16 +181,22 @@ extern "C" int wrnn_attention_backward_stats(const wrnn_attention_desc* desc, co
   WRNN_REQUIRE(workspace && workspace_bytes >= need && !((uintptr_t)workspace & 15),
                "wrnn_attention_backward: workspace of %zu bytes, %zu are needed, on 16 bytes", workspace_bytes, need);
   const int es = desc->dtype == WRNN_FLOAT32 ? 4 : 2;
-  auto whole = [&](const void* x, const int64_t* st) { return attn::rows_on_four(x, st[0], st[1], st[2], es); };
-  WRNN_REQUIRE(whole(g->out, g->out_stride) && whole(g->dout, g->dout_stride) && whole(g->dq, g->dq_stride) && whole(g->dk, g->dk_stride) && whole(g->dv, g->dv_stride),
-               "wrnn_attention_backward: rows have to start on the bytes of four elements");
-  for (const int64_t* x : {g->out_stride, g->dout_stride, g->dq_stride, g->dk_stride, g->dv_stride})
-    WRNN_REQUIRE(x[2] >= 0 && x[2] < attn::kMaxRowStride, "wrnn_attention_backward: position strides are in 0 .. 2^22 - 1 elements");
-  p.o_in = g->out, p.oi_b = g->out_stride[0], p.oi_h = g->out_stride[1], p.oi_t = g->out_stride[2];
-  p.dout = g->dout, p.do_b = g->dout_stride[0], p.do_h = g->dout_stride[1], p.do_t = g->dout_stride[2];
-  p.dq = g->dq, p.dq_b = g->dq_stride[0], p.dq_h = g->dq_stride[1], p.dq_t = g->dq_stride[2];
-  p.dk = g->dk, p.dk_b = g->dk_stride[0], p.dk_h = g->dk_stride[1], p.dk_t = g->dk_stride[2];
-  p.dv = g->dv, p.dv_b = g->dv_stride[0], p.dv_h = g->dv_stride[1], p.dv_t = g->dv_stride[2];
+  struct Rows {
+    const void* at;
+    const int64_t* stride;
+    int64_t *b, *h, *t;
+    int heads, len;
+  };
+  for (const Rows& x : {Rows{p.o_in = g->out, g->out_stride, &p.oi_b, &p.oi_h, &p.oi_t, p.H, p.Tq},
+                        Rows{p.dout = g->dout, g->dout_stride, &p.do_b, &p.do_h, &p.do_t, p.H, p.Tq},
+                        Rows{p.dq = g->dq, g->dq_stride, &p.dq_b, &p.dq_h, &p.dq_t, p.H, p.Tq},
+                        Rows{p.dk = g->dk, g->dk_stride, &p.dk_b, &p.dk_h, &p.dk_t, p.Hkv, p.Tk},
+                        Rows{p.dv = g->dv, g->dv_stride, &p.dv_b, &p.dv_h, &p.dv_t, p.Hkv, p.Tk}}) {
+    *x.b = attn::stride_of(p.B, x.stride[0]), *x.h = attn::stride_of(x.heads, x.stride[1]), *x.t = attn::stride_of(x.len, x.stride[2]);
+    WRNN_REQUIRE(attn::rows_on_four(x.at, *x.b, *x.h, *x.t, es), "wrnn_attention_backward: rows have to start on the bytes of four elements");
+  }
+  // (of these only dout's rows go through tiles)
+  WRNN_REQUIRE(p.do_t >= 0 && p.do_t < attn::kMaxRowStride, "wrnn_attention_backward: position strides of dout are in 0 .. 2^22 - 1 elements");
   const hipStream_t st = static_cast<hipStream_t>(stream);
   char* w = static_cast<char*>(workspace);
   if (!stats) {  // made anew: the forward kernel without an output
