@@ -42,3 +42,27 @@ def test_broadcast_batch_with_far_positions(dtype):
         value, bound = want[name]
         # autograd adds the rows' gradients up: B equal values, each addition half a step of the inputs' type or of 32 bits
         check(name, g.double().permute(1, 0, 2)[None] / B, (value, bound + (torch.finfo(dtype).eps + B * 2.0 ** -24) * value.abs()))
+
+
+class NoGradient(torch.autograd.Function):
+    """Passes no gradient on."""
+
+    @staticmethod
+    def forward(ctx, x):
+        return x.clone()
+
+    @staticmethod
+    def backward(ctx, d):
+        return None
+
+
+@gpu
+def test_no_gradient_of_the_output():
+    q, k, v = (normal(i, 1, 2, 5, 16).requires_grad_() for i in range(3))
+    out = NoGradient.apply(A.attention(q, k, v))
+    (out.sum() + 2 * q.sum()).backward()
+    assert bool((q.grad == 2).all()) and k.grad is None and v.grad is None
+    q, k, v = (normal(i, 1, 2, 5, 16).requires_grad_() for i in range(3))
+    table = normal(3, 16, 2).requires_grad_()
+    (NoGradient.apply(A.relative_position_bias(table, 5, 5)).sum() + 2 * table.sum()).backward()
+    assert bool((table.grad == 2).all())

@@ -158,6 +158,8 @@ class _Attention(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dout, _):
+        if dout is None:    # nothing that was computed from out passed a gradient on
+            return (None,) * 12
         q, k, v, table, key_mask, key_lens, q_start, out, stats = ctx.saved_tensors
         want_table = table is not None and ctx.needs_input_grad[3]
         B, H, Tq, _ = q.shape
