@@ -1,5 +1,8 @@
 """Self-attention as it may be called: strides of every kind, other kinds of differentiation, gradients that are not there, lengths and positions
 past what the kernels count in, rules made at the same time."""
+import ctypes as C
+import gc
+import weakref
 
 import pytest
 import torch
@@ -66,3 +69,18 @@ def test_no_gradient_of_the_output():
     table = normal(3, 16, 2).requires_grad_()
     (NoGradient.apply(A.relative_position_bias(table, 5, 5)).sum() + 2 * table.sum()).backward()
     assert bool((table.grad == 2).all())
+
+
+def test_a_description_keeps_its_bucket_edges():
+    """The edges whose address a description holds live as long as it, whatever other rules are made meanwhile (the cache holds some dozens)."""
+    q = torch.zeros(1, 2, 4, 8)
+    table = torch.zeros(14, 2)
+    A._edges.cache_clear()
+    desc = A._desc(q, q, q, table, None, None, None, False, 1.0, 77, True)
+    edges = weakref.ref(A._edges(14, 77, True)[1])
+    A._edges.cache_clear()
+    gc.collect()
+    assert edges() is not None and bytes(desc).endswith(C.addressof(edges()).to_bytes(8, "little"))
+    del desc
+    gc.collect()
+    assert edges() is None

@@ -93,15 +93,23 @@ def _ptr(t: Optional[torch.Tensor]) -> int:
     return 0 if t is None else t.data_ptr()
 
 
+class _Desc(bytes):
+    """A wrnn_attention_desc, with the array of bucket edges whose address it holds: the cache of rules may drop its own reference at any time."""
+    edges = None
+
+
 def _desc(q, k, v, table, key_mask, key_lens, q_start, causal, scale, max_distance, bidirectional):
     B, H, Tq, D = q.shape
-    buckets, edges = 0, 0
+    buckets, edges = 0, None
     if table is not None:
         buckets = table.shape[0]
-        edges = C.addressof(_edges(buckets, max_distance, bidirectional)[1])
-    return _DESC.pack(_DTYPES[q.dtype], B, H, k.shape[1], Tq, k.shape[2], D, causal, buckets, max_distance, bidirectional, scale, q.data_ptr(),
-                      k.data_ptr(), v.data_ptr(), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], _ptr(key_mask),
-                      0 if key_mask is None else key_mask.stride(0), _ptr(key_lens), _ptr(q_start), _ptr(table), edges)
+        edges = _edges(buckets, max_distance, bidirectional)[1]
+    desc = _Desc(_DESC.pack(_DTYPES[q.dtype], B, H, k.shape[1], Tq, k.shape[2], D, causal, buckets, max_distance, bidirectional, scale,
+                            q.data_ptr(), k.data_ptr(), v.data_ptr(), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], _ptr(key_mask),
+                            0 if key_mask is None else key_mask.stride(0), _ptr(key_lens), _ptr(q_start), _ptr(table),
+                            0 if edges is None else C.addressof(edges)))
+    desc.edges = edges
+    return desc
 
 
 class _on:
