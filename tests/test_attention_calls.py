@@ -84,3 +84,10 @@ def test_a_description_keeps_its_bucket_edges():
     del desc
     gc.collect()
     assert edges() is None
+
+
+@pytest.mark.parametrize("q_len,k_len,start", [(4, 4, 1 << 32), (4, 4, -(1 << 32)), (4, 4, (1 << 29) + 1), (1 << 32, 0, 0), (0, (1 << 32) + 1, 0),
+                                               ((1 << 28) + 1, 1, 0), (4, (1 << 28) + 1, None)])
+def test_lengths_and_positions_past_the_kernels_count_are_refused(q_len, k_len, start):
+    with pytest.raises(ValueError, match="2\\^"):
+        A.relative_position_bias(torch.zeros(32, 2), q_len, k_len, q_start=start)

@@ -302,14 +302,17 @@ def relative_position_bias(table: torch.Tensor, q_len: int, k_len: int, *, q_sta
                            bidirectional: bool = True) -> torch.Tensor:
     """table [num_buckets, H] -> [H, q_len, k_len] of the table's type: table[bucket(j - (i + q_start)), h]; q_start defaults to
     k_len - q_len.  Differentiable in the table."""
+    q_len, k_len = int(q_len), int(k_len)
+    start = k_len - q_len if q_start is None else int(q_start)
+    if q_len < 0 or k_len < 0:
+        raise ValueError(f"negative length ({q_len}, {k_len})")
+    if max(q_len, k_len) > 1 << 28 or abs(start) > 1 << 29:
+        raise ValueError(f"lengths are at most 2^28 and q_start is within +-2^29, got {q_len}, {k_len} and {start}")
     _on_gpu(table, "relative_position_bias")
     if table.dim() != 2 or table.dtype not in _DTYPES:
         raise TypeError(f"expected a float32 or bfloat16 table [num_buckets, heads], got {table.dtype} {tuple(table.shape)}")
-    if q_len < 0 or k_len < 0:
-        raise ValueError(f"negative length ({q_len}, {k_len})")
     _edges(table.shape[0], max_distance, bidirectional)
-    return _RelativeBias.apply(table.contiguous(), int(q_len), int(k_len), int(k_len - q_len if q_start is None else q_start),
-                               max_distance, bool(bidirectional))
+    return _RelativeBias.apply(table.contiguous(), q_len, k_len, start, max_distance, bool(bidirectional))
 
 
 class RelativePositionBias(nn.Module):
