@@ -8,7 +8,8 @@ import pytest
 import torch
 
 from attention_ref import check, reference
-from test_attention import BF16, F32, normal
+from test_attention import BF16, F32, desc, normal
+from wavernn_amd import _lib
 from wavernn_amd import attention as A
 
 gpu = pytest.mark.gpu
@@ -91,3 +92,16 @@ def test_a_description_keeps_its_bucket_edges():
 def test_lengths_and_positions_past_the_kernels_count_are_refused(q_len, k_len, start):
     with pytest.raises(ValueError, match="2\\^"):
         A.relative_position_bias(torch.zeros(32, 2), q_len, k_len, q_start=start)
+
+
+
+def test_c_entry_of_the_dense_bias_refuses_more_workgroups_than_a_launch_takes():
+    lib = _lib.load()
+    e = (C.c_int32 * 3)(8, 16, 32)
+    for heads, q_len in ((1 << 22, 300), (1 << 25, 32)):
+        assert lib.wrnn_relative_bias_forward(16, 0, heads, q_len, 1, 0, 8, 64, 0, e, 16, None) != 0 and b"too large" in lib.wrnn_last_error()
+        size = lib.wrnn_relative_bias_workspace_bytes(heads, q_len, 1, 8, 64)
+        assert lib.wrnn_relative_bias_backward(16, 0, heads, q_len, 1, 0, 8, 64, 0, e, 16, 16, size, None) != 0 and b"too large" in lib.wrnn_last_error()
+    many = desc(heads=1 << 20, kv_heads=1 << 20, q_len=1, k_len=1, bias_table=16, num_buckets=256, max_distance=1024,
+                bucket_edges=(C.c_int32 * 127)(*A.bucket_edges(256, 1024, False)))
+    assert lib.wrnn_attention_forward(C.byref(many), 16, _lib.I64x3(0, 0, 0), None, None, 0, None) != 0 and b"too large" in lib.wrnn_last_error()

@@ -152,6 +152,7 @@ int bias_params(Params* p, int num_buckets, int max_distance, int bidirectional,
   const int side = bidirectional ? num_buckets / 2 : num_buckets, n = side - side / 2 - 1;
   WRNN_REQUIRE(num_buckets >= 2 && num_buckets <= 256 && (!bidirectional || (num_buckets % 2 == 0 && side >= 2)),
                "%s: %d buckets: 2 .. 256 are served, 4 .. 256 and an even number with two sides", who, num_buckets);
+  WRNN_REQUIRE((int64_t)p->H * num_buckets < (1LL << 26), "%s: heads x buckets is too large for one launch", who);
   WRNN_REQUIRE(max_distance > side / 2 && max_distance <= kMaxDistance, "%s: max_distance %d is outside %d .. %d", who, max_distance,
                side / 2 + 1, kMaxDistance);
   WRNN_REQUIRE(n <= kMaxEdges && (n == 0 || edges), "%s: null bucket edges", who);
@@ -165,6 +166,13 @@ int bias_params(Params* p, int num_buckets, int max_distance, int bidirectional,
   return 0;
 }
 
+// Rows of a workgroup: enough that its table of distances is small beside them, few enough that the compute units are filled.
+static int bias_rows(int heads, int q_len, int k_len) {
+  const int64_t want = (int64_t)heads * q_len / 1024;
+  const int64_t most = k_len >= 512 ? 32 : 64;
+  return (int)(want < 4 ? 4 : want > most ? most : (want + 3) / 4 * 4);
+}
+
 static int dense_params(Params* p, int dtype, int heads, int q_len, int k_len, int start, int num_buckets, int max_distance, int bidirectional,
                         const int32_t* edges, const char* who) {
   *p = Params{};
@@ -172,16 +180,10 @@ static int dense_params(Params* p, int dtype, int heads, int q_len, int k_len, i
   WRNN_REQUIRE(heads >= 0 && q_len >= 0 && k_len >= 0, "%s: negative size", who);
   WRNN_REQUIRE(q_len <= (1 << 28) && k_len <= (1 << 28) && start >= -(1 << 29) && start <= (1 << 29), "%s: lengths are at most 2^28, start 2^29",
                who);
-  WRNN_REQUIRE((int64_t)heads * q_len < (1LL << 31), "%s: heads x q_len is too large for one launch", who);
+  const int64_t rows = bias_rows(heads, q_len, k_len);
+  WRNN_REQUIRE(heads * ((q_len + rows - 1) / rows) * 256 < (1LL << 32), "%s: heads x q_len is too large for one launch", who);
   p->H = heads, p->Tq = q_len, p->Tk = k_len;
   return bias_params(p, num_buckets, max_distance, bidirectional, edges, who);
-}
-
-// Rows of a workgroup: enough that its table of distances is small beside them, few enough that the compute units are filled.
-static int bias_rows(int heads, int q_len, int k_len) {
-  const int64_t want = (int64_t)heads * q_len / 1024;
-  const int64_t most = k_len >= 512 ? 32 : 64;
-  return (int)(want < 4 ? 4 : want > most ? most : (want + 3) / 4 * 4);
 }
 
 }  // namespace attn
