@@ -6,6 +6,7 @@ import weakref
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from attention_ref import check, reference
 from test_attention import BF16, F32, desc, normal
@@ -105,3 +106,34 @@ def test_c_entry_of_the_dense_bias_refuses_more_workgroups_than_a_launch_takes()
     many = desc(heads=1 << 20, kv_heads=1 << 20, q_len=1, k_len=1, bias_table=16, num_buckets=256, max_distance=1024,
                 bucket_edges=(C.c_int32 * 127)(*A.bucket_edges(256, 1024, False)))
     assert lib.wrnn_attention_forward(C.byref(many), 16, _lib.I64x3(0, 0, 0), None, None, 0, None) != 0 and b"too large" in lib.wrnn_last_error()
+
+
+@gpu
+def test_forward_mode_derivatives_and_transforms_are_refused():
+    """An error, not a result without them."""
+    q, k, v = (normal(i, 1, 2, 5, 16) for i in range(3))
+    table = normal(3, 16, 2)
+    with forward_ad.dual_level():
+        for i in range(4):
+            args = [q, k, v, table]
+            args[i] = forward_ad.make_dual(args[i], torch.ones_like(args[i]))
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="forward-mode"):
+                    A.attention(*args[:3], bias_table=args[3])
+        assert torch.isfinite(A.attention(q, k, v, bias_table=table)).all()     # no dual tensor among them
+        with pytest.raises(RuntimeError):
+            A.relative_position_bias(forward_ad.make_dual(table, torch.ones_like(table)), 5, 5)
+    for transformed in (lambda: torch.func.jvp(lambda x: A.attention(x, k, v), (q,), (torch.ones_like(q),)),
+                        lambda: torch.func.vmap(lambda x: A.attention(x, k, v))(q[None]), lambda: torch.func.grad(lambda x: A.attention(x, k, v).sum())(q)):
+        with pytest.raises(RuntimeError):
+            transformed()
+
+
+def test_dual_tensors_are_seen():
+    x = torch.ones(3)
+    A._no_tangents(x, None)
+    with forward_ad.dual_level():
+        d = forward_ad.make_dual(x, x)
+        A._no_tangents(x, None)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            A._no_tangents(x, d)

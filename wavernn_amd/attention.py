@@ -19,6 +19,7 @@ from typing import Optional
 
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -55,6 +56,12 @@ def bucket_edges(num_buckets: int = 32, max_distance: int = 128, bidirectional: 
 def _on_gpu(t: torch.Tensor, what: str) -> None:
     if t.device.type != 'cuda':
         raise RuntimeError(f"wavernn_amd.{what} runs only on an MI355X (HIP) device; there is no CPU fallback")
+
+
+def _no_tangents(*tensors: Optional[torch.Tensor]) -> None:
+    """A dual tensor asks for no gradient and would come through without its tangent."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError("wavernn_amd.attention has no forward-mode derivatives")
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -222,8 +229,10 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, key_mask: Op
     scale: 1 / sqrt(D) by default.
     bias_table [num_buckets, H] (``RelativePositionBias.weight``) adds table[bucket(j - (i + q_start[b])), h]; max_distance and
     bidirectional are its rule.  -inf in a table leaves its distances out.
+    Differentiable backward, once; forward-mode derivatives and the transforms of torch.func are refused.
     return_lse: also the log of each query's sum of exponentials, [B, H, Tq] float32, -inf for a query without keys (no gradient)."""
     _on_gpu(q, "attention")
+    _no_tangents(q, k, v, bias_table)
     if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
         raise ValueError(f"expected q [B,H,Tq,D] and k, v [B,Hkv,Tk,D], got {tuple(q.shape)}, {tuple(k.shape)} and {tuple(v.shape)}")
     if q.dtype not in _DTYPES or k.dtype != q.dtype or v.dtype != q.dtype:
