@@ -137,3 +137,16 @@ def test_dual_tensors_are_seen():
         A._no_tangents(x, None)
         with pytest.raises(RuntimeError, match="forward-mode"):
             A._no_tangents(x, d)
+
+
+@gpu
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning")
+@pytest.mark.parametrize("grad", [True, False])
+@pytest.mark.parametrize("D", [12, 13, 16])
+def test_traces_compute_on_their_inputs(grad, D):
+    k, v = normal(1, 1, 2, 5, D), normal(2, 1, 2, 5, D)
+    table = normal(3, 16, 2)
+    with torch.set_grad_enabled(grad):
+        traced = torch.jit.trace(lambda x: A.attention(x, k, v, bias_table=table) * 2, (normal(0, 1, 2, 5, D).requires_grad_(grad),), check_trace=False)
+        x = normal(4, 1, 2, 5, D)
+        assert torch.equal(traced(x), A.attention(x, k, v, bias_table=table) * 2)

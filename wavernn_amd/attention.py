@@ -267,8 +267,9 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, key_mask: Op
 
 
 def _run(q, k, v, bias_table, key_mask, key_lens, q_start, causal, scale, max_distance, bidirectional, want_lse):
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
-                                    or (bias_table is not None and bias_table.requires_grad)):
+    # (a trace records the function, not what the library does inside)
+    if torch.jit.is_tracing() or torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
+                                                              or (bias_table is not None and bias_table.requires_grad)):
         return _Attention.apply(q, k, v, bias_table, key_mask, key_lens, q_start, causal, scale, max_distance, bidirectional, want_lse)
     with _on(q.device):
         lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) if want_lse else None
