@@ -1,0 +1,22 @@
+"""FFTBlock's attention paths beside what the block could do before: masks, subclasses, pickles, hooks, modes of the module itself."""
+import pytest
+import torch
+
+from wavernn_amd import forward_models as FM
+
+
+def block(**kw):
+    torch.manual_seed(0)
+    return FM.FFTBlock(**dict(dict(d_model=32, nhead=2, conv1_kernel=3, conv2_kernel=1, d_fft=48, dropout=0.0), **kw))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64])
+def test_additive_masks_beside_a_position_bias(dtype):
+    """On the stock path a mask that is added does what the bool mask does, also where the scores get a bias."""
+    b = block()
+    x = torch.randn(9, 3, 32)
+    leave = torch.arange(9)[None] >= torch.tensor([[9], [5], [1]])
+    added = torch.zeros(3, 9, dtype=dtype).masked_fill(leave, -torch.inf)
+    bias = torch.randn(2, 9, 9)
+    for kw in ({}, dict(position_bias=lambda q_len, k_len: bias)):
+        assert torch.equal(b(x, added.float() if not kw else added, **kw), b(x, leave, **kw))

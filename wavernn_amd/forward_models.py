@@ -93,8 +93,10 @@ class FFTBlock(nn.Module):  # common_layers.py:148-185: post-norm self-attention
             if position_bias is not None:
                 bias = position_bias(src.size(0), src.size(0)).to(src.dtype)     # [H, T, T], for every row of the batch
                 bias = bias.expand(src.size(1), -1, -1, -1).reshape(-1, *bias.shape[1:])
-                if src_pad_mask is not None:
+                if src_pad_mask is not None and src_pad_mask.dtype == torch.bool:
                     src_pad_mask = torch.zeros_like(src_pad_mask, dtype=src.dtype).masked_fill(src_pad_mask, -math.inf)
+                elif src_pad_mask is not None:                                   # one that is added already
+                    src_pad_mask = src_pad_mask.to(src.dtype)
             return self.self_attn(src, src, src, attn_mask=bias, key_padding_mask=src_pad_mask)[0]
         # the packed projection's q, k, v as views [N, H, T, head_dim]; the result lies in memory as [T, N, d_model]
         a = self.self_attn
