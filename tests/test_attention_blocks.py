@@ -20,3 +20,23 @@ def test_additive_masks_beside_a_position_bias(dtype):
     bias = torch.randn(2, 9, 9)
     for kw in ({}, dict(position_bias=lambda q_len, k_len: bias)):
         assert torch.equal(b(x, added.float() if not kw else added, **kw), b(x, leave, **kw))
+
+
+class FormerBlock(FM.FFTBlock):
+
+    def forward(self, src, src_pad_mask=None):
+        return super().forward(src, src_pad_mask=src_pad_mask)
+
+
+def transformer(**kw):
+    torch.manual_seed(0)
+    return FM.ForwardTransformer(**dict(dict(d_model=32, d_fft=48, layers=2, heads=2, conv1_kernel=3, conv2_kernel=1, dropout=0.0), **kw)).eval()
+
+
+def test_layers_without_a_position_bias_are_called_as_before():
+    """A layer, or a subclass of the block, that takes a source and its mask alone."""
+    t, x = transformer(), torch.randn(2, 7, 32)
+    want = t(x)
+    for layer in t.layers:
+        layer.__class__ = FormerBlock
+    assert torch.equal(t(x), want)

@@ -146,8 +146,9 @@ class ForwardTransformer(nn.Module):  # common_layers.py:188-223
 
     def forward(self, x, src_pad_mask=None):                     # [N, T, d_model]
         x = self.pos_encoder(x.transpose(0, 1))
+        bias = {} if self.position_bias is None else dict(position_bias=self.position_bias)
         for layer in self.layers:
-            x = layer(x, src_pad_mask=src_pad_mask, position_bias=self.position_bias)
+            x = layer(x, src_pad_mask=src_pad_mask, **bias)
         return self.norm(x).transpose(0, 1)
 
 
