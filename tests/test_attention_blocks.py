@@ -1,4 +1,7 @@
 """FFTBlock's attention paths beside what the block could do before: masks, subclasses, pickles, hooks, modes of the module itself."""
+import copy
+import pickle
+
 import pytest
 import torch
 
@@ -40,3 +43,17 @@ def test_layers_without_a_position_bias_are_called_as_before():
     for layer in t.layers:
         layer.__class__ = FormerBlock
     assert torch.equal(t(x), want)
+
+
+def test_modules_pickled_before_the_paths_and_the_bias():
+    t, x = transformer(), torch.randn(2, 7, 32)
+    want = t(x)
+    del t.__dict__["position_bias"]
+    for layer in t.layers:
+        layer.__dict__.pop("attention_path", None)
+    old = pickle.loads(pickle.dumps(t))
+    assert torch.equal(old(x), want)
+    assert all(b.attention_path == 'stock' for b in old.layers) and old.position_bias is None
+    new = transformer(rel_buckets=8).set_attention_path('auto')
+    for t in (pickle.loads(pickle.dumps(new)), copy.deepcopy(new)):
+        assert all(b.attention_path == 'auto' for b in t.layers) and torch.equal(t.position_bias.weight, new.position_bias.weight)

@@ -59,6 +59,8 @@ ATTENTION_PATHS = ('stock', 'fused', 'auto')
 
 
 class FFTBlock(nn.Module):  # common_layers.py:148-185: post-norm self-attention, then a two-conv feed-forward over time
+    attention_path = 'stock'
+
     def __init__(self, d_model: int, nhead: int, conv1_kernel: int, conv2_kernel: int, d_fft: int, dropout: float = 0.1):
         super().__init__()
         self.self_attn = nn.MultiheadAttention(d_model, nhead, dropout=dropout)
@@ -68,7 +70,6 @@ class FFTBlock(nn.Module):  # common_layers.py:148-185: post-norm self-attention
         self.norm1, self.norm2 = nn.LayerNorm(d_model), nn.LayerNorm(d_model)
         self.dropout1, self.dropout2 = nn.Dropout(dropout), nn.Dropout(dropout)
         self.activation = nn.ReLU()
-        self.attention_path = 'stock'
 
     def _why_not_fused(self, src, src_pad_mask) -> Optional[str]:
         if src.device.type != 'cuda':
@@ -140,6 +141,11 @@ class ForwardTransformer(nn.Module):  # common_layers.py:188-223
                                              conv2_kernel=conv2_kernel, dropout=dropout) for _ in range(layers))
         self.norm = nn.LayerNorm(d_model)
         self.position_bias = RelativePositionBias(heads, rel_buckets, rel_max_distance) if rel_buckets else None
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        if 'position_bias' not in self._modules:      # none, or pickled before there were any
+            self.position_bias = None
 
     def set_attention_path(self, path: str) -> 'ForwardTransformer':
         return set_attention_path(self, path)
