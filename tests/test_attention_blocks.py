@@ -1,6 +1,7 @@
 """FFTBlock's attention paths beside what the block could do before: masks, subclasses, pickles, hooks, modes of the module itself."""
 import copy
 import pickle
+import types
 
 import pytest
 import torch
@@ -57,3 +58,19 @@ def test_modules_pickled_before_the_paths_and_the_bias():
     new = transformer(rel_buckets=8).set_attention_path('auto')
     for t in (pickle.loads(pickle.dumps(new)), copy.deepcopy(new)):
         assert all(b.attention_path == 'auto' for b in t.layers) and torch.equal(t.position_bias.weight, new.position_bias.weight)
+
+
+def on_the_gpu(dtype=torch.float32):
+    """Stands for a source tensor in the question whether the fused path applies."""
+    return types.SimpleNamespace(device=torch.device("cuda"), dtype=dtype)
+
+
+def test_dropout_of_the_attention_itself_decides():
+    """The probabilities' dropout is nn.MultiheadAttention's, which may be in another mode than the block around it."""
+    b = block(dropout=0.1).train()
+    assert "dropout" in b._why_not_fused(on_the_gpu(), None)
+    b.self_attn.eval()
+    assert b._why_not_fused(on_the_gpu(), None) is None
+    b.eval()
+    b.self_attn.train()
+    assert "dropout" in b._why_not_fused(on_the_gpu(), None)

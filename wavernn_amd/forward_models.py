@@ -79,7 +79,7 @@ class FFTBlock(nn.Module):  # common_layers.py:148-185: post-norm self-attention
             return f"it takes float32 or bfloat16, not {dtype}"
         if src_pad_mask is not None and src_pad_mask.dtype != torch.bool:
             return f"it takes a bool mask, not {src_pad_mask.dtype}"
-        if self.training and self.self_attn.dropout > 0:
+        if self.self_attn.training and self.self_attn.dropout > 0:
             return "it has no dropout on the probabilities (train with dropout=0, or on the stock path)"
         if self.self_attn.head_dim > MAX_HEAD_DIM:
             return f"head dimension {self.self_attn.head_dim} is over {MAX_HEAD_DIM}"
