@@ -74,3 +74,13 @@ def test_dropout_of_the_attention_itself_decides():
     b.eval()
     b.self_attn.train()
     assert "dropout" in b._why_not_fused(on_the_gpu(), None)
+
+
+@pytest.mark.parametrize("register", ["register_forward_hook", "register_forward_pre_hook", "register_full_backward_hook", "register_full_backward_pre_hook"])
+def test_hooks_on_the_attention_keep_the_stock_path(register):
+    """'fused' does not call nn.MultiheadAttention: it says so where somebody listens to that call, and 'auto' makes it."""
+    b = block().eval()
+    handle = getattr(b.self_attn, register)(lambda *a: None)
+    assert "hooks" in b._why_not_fused(on_the_gpu(), None)
+    handle.remove()
+    assert b._why_not_fused(on_the_gpu(), None) is None

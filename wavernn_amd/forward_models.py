@@ -81,6 +81,9 @@ class FFTBlock(nn.Module):  # common_layers.py:148-185: post-norm self-attention
             return f"it takes a bool mask, not {src_pad_mask.dtype}"
         if self.self_attn.training and self.self_attn.dropout > 0:
             return "it has no dropout on the probabilities (train with dropout=0, or on the stock path)"
+        a = self.self_attn
+        if a._forward_hooks or a._forward_pre_hooks or a._backward_hooks or a._backward_pre_hooks:
+            return "it would not call the hooks on self_attn"
         if self.self_attn.head_dim > MAX_HEAD_DIM:
             return f"head dimension {self.self_attn.head_dim} is over {MAX_HEAD_DIM}"
         return None
@@ -120,7 +123,8 @@ def set_attention_path(module: nn.Module, path: str) -> nn.Module:
     """How every FFTBlock under ``module`` runs its self-attention (no counterpart in the reference):
     'stock'  nn.MultiheadAttention (the default);
     'fused'  wavernn_amd.attention, forward and backward: the scores never reach memory; an error where it does not apply (training with
-             dropout > 0, which it has none of; head dimensions over 256; types other than float32 and bfloat16; masks that are not bool);
+             dropout > 0, which it has none of; head dimensions over 256; types other than float32 and bfloat16; masks that are not bool;
+             hooks on self_attn, which is not called);
     'auto'   'fused' where it applies, 'stock' elsewhere.
     They agree to rounding, but for batch rows whose every position is masked: 'stock' gives NaN there, 'fused' attends to nothing."""
     if path not in ATTENTION_PATHS:
