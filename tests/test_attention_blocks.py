@@ -5,6 +5,7 @@ import types
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from wavernn_amd import forward_models as FM
 
@@ -84,3 +85,28 @@ def test_hooks_on_the_attention_keep_the_stock_path(register):
     assert "hooks" in b._why_not_fused(on_the_gpu(), None)
     handle.remove()
     assert b._why_not_fused(on_the_gpu(), None) is None
+
+
+@pytest.mark.gpu
+def test_other_kinds_of_differentiation_keep_the_stock_path():
+    """Forward-mode derivatives and the transforms of torch.func, which the operators refuse."""
+    b = block().eval().cuda()
+    x, tangent = torch.randn(5, 2, 32, device="cuda"), torch.randn(5, 2, 32, device="cuda")
+    w = b.self_attn.in_proj_weight.detach()
+    got = {}
+    for path in ("stock", "auto"):
+        FM.set_attention_path(b, path)
+        with forward_ad.dual_level():
+            by_source = forward_ad.unpack_dual(b(forward_ad.make_dual(x, tangent))).tangent
+            dual = {"self_attn.in_proj_weight": forward_ad.make_dual(w, torch.ones_like(w))}
+            by_weight = forward_ad.unpack_dual(torch.func.functional_call(b, dual, (x,))).tangent
+        got[path] = [by_source, by_weight, *torch.func.jvp(b, (x,), (tangent,)), torch.func.grad(lambda y: b(y).square().sum())(x)]
+    for a, c in zip(*got.values()):
+        assert torch.equal(a, c) and bool(a.any())
+    FM.set_attention_path(b, "fused")
+    with forward_ad.dual_level():
+        assert torch.isfinite(b(x)).all()
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            b(forward_ad.make_dual(x, tangent))
+    with pytest.raises(RuntimeError, match="torch.func"):
+        torch.func.grad(lambda y: b(y).sum())(x)

@@ -58,9 +58,14 @@ def _on_gpu(t: torch.Tensor, what: str) -> None:
         raise RuntimeError(f"wavernn_amd.{what} runs only on an MI355X (HIP) device; there is no CPU fallback")
 
 
+def has_tangents(*tensors: Optional[torch.Tensor]) -> bool:
+    """Whether there is a dual tensor of forward-mode differentiation among them."""
+    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def _no_tangents(*tensors: Optional[torch.Tensor]) -> None:
     """A dual tensor asks for no gradient and would come through without its tangent."""
-    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+    if has_tangents(*tensors):
         raise RuntimeError("wavernn_amd.attention has no forward-mode derivatives")
 
 

@@ -30,7 +30,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 from torch.nn.utils.rnn import pack_padded_sequence, pad_packed_sequence
 
-from .attention import MAX_HEAD_DIM, RelativePositionBias, attention
+from .attention import MAX_HEAD_DIM, RelativePositionBias, attention, has_tangents
 from .bigru import BiGRU
 from .bilstm import BiLSTM
 from .length_regulator import LengthRegulator
@@ -71,7 +71,7 @@ class FFTBlock(nn.Module):  # common_layers.py:148-185: post-norm self-attention
         self.dropout1, self.dropout2 = nn.Dropout(dropout), nn.Dropout(dropout)
         self.activation = nn.ReLU()
 
-    def _why_not_fused(self, src, src_pad_mask) -> Optional[str]:
+    def _why_not_fused(self, src, src_pad_mask, position_bias=None) -> Optional[str]:
         if src.device.type != 'cuda':
             return "it runs only on an MI355X (HIP) device"
         dtype = torch.get_autocast_dtype('cuda') if torch.is_autocast_enabled('cuda') else src.dtype
@@ -84,12 +84,16 @@ class FFTBlock(nn.Module):  # common_layers.py:148-185: post-norm self-attention
         a = self.self_attn
         if a._forward_hooks or a._forward_pre_hooks or a._backward_hooks or a._backward_pre_hooks:
             return "it would not call the hooks on self_attn"
-        if self.self_attn.head_dim > MAX_HEAD_DIM:
-            return f"head dimension {self.self_attn.head_dim} is over {MAX_HEAD_DIM}"
+        if a.head_dim > MAX_HEAD_DIM:
+            return f"head dimension {a.head_dim} is over {MAX_HEAD_DIM}"
+        if torch._C._are_functorch_transforms_active():
+            return "it does not go through the transforms of torch.func"
+        if has_tangents(src, a.in_proj_weight, a.in_proj_bias, None if position_bias is None else position_bias.weight):
+            return "it has no forward-mode derivatives"
         return None
 
     def _attend(self, src, src_pad_mask, position_bias):
-        why = self._why_not_fused(src, src_pad_mask) if self.attention_path != 'stock' else ''
+        why = self._why_not_fused(src, src_pad_mask, position_bias) if self.attention_path != 'stock' else ''
         if why and self.attention_path == 'fused':
             raise RuntimeError(f"FFTBlock: the fused attention path does not apply: {why}")
         if why is not None:
@@ -124,7 +128,7 @@ def set_attention_path(module: nn.Module, path: str) -> nn.Module:
     'stock'  nn.MultiheadAttention (the default);
     'fused'  wavernn_amd.attention, forward and backward: the scores never reach memory; an error where it does not apply (training with
              dropout > 0, which it has none of; head dimensions over 256; types other than float32 and bfloat16; masks that are not bool;
-             hooks on self_attn, which is not called);
+             hooks on self_attn, which is not called; forward-mode derivatives and the transforms of torch.func);
     'auto'   'fused' where it applies, 'stock' elsewhere.
     They agree to rounding, but for batch rows whose every position is masked: 'stock' gives NaN there, 'fused' attends to nothing."""
     if path not in ATTENTION_PATHS:
