@@ -7,6 +7,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
+import golden_util as G
 from wavernn_amd import forward_models as FM
 
 
@@ -110,3 +111,32 @@ def test_other_kinds_of_differentiation_keep_the_stock_path():
             b(forward_ad.make_dual(x, tangent))
     with pytest.raises(RuntimeError, match="torch.func"):
         torch.func.grad(lambda y: b(y).sum())(x)
+
+
+@pytest.mark.parametrize("name", [n for n in G.names("fwdmodel_") if "fastpitch" in n])
+def test_every_transformer_of_the_models_takes_the_position_bias(name):
+    rec, _ = G.load(name)
+    multi = rec["kind"] != "fast_pitch"
+    model = (FM.MultiFastPitch if multi else FM.FastPitch)(**dict(rec["cfg"], rel_buckets=16, rel_max_distance=40))
+    transformers = [m for m in model.modules() if isinstance(m, FM.ForwardTransformer)]
+    assert len(transformers) == (6 if multi else 5)
+    for t in transformers:
+        heads = t.layers[0].self_attn.num_heads
+        assert tuple(t.position_bias.weight.shape) == (16, heads) and t.position_bias.max_distance == 40
+    plain = (FM.MultiFastPitch if multi else FM.FastPitch)(**rec["cfg"])
+    assert not any("position_bias" in k for k in plain.state_dict())
+
+
+@pytest.mark.gpu
+def test_multi_speaker_model_with_the_position_bias_on_either_path():
+    rec, _ = G.load([n for n in G.names("fwdmodel_") if "multifastpitch" in n][0])
+    torch.manual_seed(0)
+    model = FM.MultiFastPitch(**dict(rec["cfg"], rel_buckets=16, rel_max_distance=40))
+    for t in (m for m in model.modules() if isinstance(m, FM.ForwardTransformer)):
+        torch.nn.init.normal_(t.position_bias.weight)
+    model = model.cuda().eval()
+    args = torch.randint(1, 20, (1, 15), device="cuda"), torch.randn(1, rec["cfg"]["speaker_emb_dims"], device="cuda")
+    gen = {p: model.set_attention_path(p).generate(*args) for p in ("stock", "fused")}
+    for k in gen["stock"]:
+        assert gen["stock"][k].shape == gen["fused"][k].shape
+        assert G.rel_err(gen["fused"][k].cpu().numpy(), gen["stock"][k].cpu().numpy()) < 1e-4, k

@@ -343,11 +343,11 @@ class MultiFastPitch(FastPitch):
                  pitch_strength: float, energy_strength: float, d_model: int, conv1_kernel: int, conv2_kernel: int,
                  prenet_layers: int, prenet_heads: int, prenet_fft: int, prenet_dropout: float, postnet_layers: int,
                  postnet_heads: int, postnet_fft: int, postnet_dropout: float, n_mels: int, speaker_emb_dims: int,
-                 padding_value=-11.5129):
+                 padding_value=-11.5129, rel_buckets: int = 0, rel_max_distance: int = 128):
         nn.Module.__init__(self)
         self.padding_value = padding_value
         self.lr = LengthRegulator()
-        kern = dict(conv1_kernel=conv1_kernel, conv2_kernel=conv2_kernel)
+        kern = dict(conv1_kernel=conv1_kernel, conv2_kernel=conv2_kernel, rel_buckets=rel_buckets, rel_max_distance=rel_max_distance)
         spk = dict(speaker_emb_dims=speaker_emb_dims, **kern)
         self.dur_pred = TransformerPredictor(num_chars, durpred_d_model, durpred_n_heads, durpred_d_fft, durpred_layers,
                                              dropout=durpred_dropout, cond_emb_size=4, cond_emb_dims=8, **spk)
