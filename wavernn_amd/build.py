@@ -1,6 +1,6 @@
 """Build libwrnn_mi355.so in-tree with hipcc for gfx950 (cross-compiles without a GPU).
 
-One object per source under lib/obj/ (recompiled only when the source or a header changed, several at a
+One object per source under lib/obj/ (recompiled only when the source, a header or this file changed, several at a
 time), then one link: editing one kernel file costs one file's compile."""
 from __future__ import annotations
 
@@ -39,9 +39,10 @@ def _hipcc() -> str:
     return "hipcc"
 
 
-def _headers():
+def _shared():
     hs = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".h")]
     hs.append(os.path.join(HERE, "..", "include", "wrnn_mi355.h"))
+    hs.append(__file__)     # the flags
     return hs
 
 
@@ -53,7 +54,7 @@ def _stale(target: str, deps) -> bool:
 
 
 def needs_build() -> bool:
-    deps = [os.path.join(CSRC, s) for s in SOURCES] + _headers()
+    deps = [os.path.join(CSRC, s) for s in SOURCES] + _shared()
     return _stale(LIB_PATH, deps)
 
 
@@ -61,11 +62,11 @@ def build(force: bool = False, verbose: bool = True) -> str:
     if not force and not needs_build():
         return LIB_PATH
     os.makedirs(OBJ_DIR, exist_ok=True)
-    hdrs = _headers()
+    shared = _shared()
     jobs = []
     for s in SOURCES:
         src, obj = os.path.join(CSRC, s), os.path.join(OBJ_DIR, s[:-4] + ".o")
-        if force or _stale(obj, [src] + hdrs):
+        if force or _stale(obj, [src] + shared):
             jobs.append([_hipcc()] + FLAGS + SOURCE_FLAGS.get(s, []) + ["-c", src, "-o", obj])
 
     def run(cmd):
