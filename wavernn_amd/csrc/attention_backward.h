@@ -189,8 +189,7 @@ __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_
   float delta = 0.f;
   {
     const T* gr = reinterpret_cast<const T*>(p.dout) + b * p.do_b + h * p.do_h + qc * p.do_t;
-    q.load(reinterpret_cast<const T*>(p.q) + b * p.q_b + h * p.q_h + qc * p.q_t + d0, half, p.D - d0, row.some());
-    q.flip(p.flip);
+    q.load(reinterpret_cast<const T*>(p.q) + b * p.q_b + h * p.q_h + qc * p.q_t + d0, half, p.D - d0, row.some(), p.flip);
     go.load(gr + d0, half, p.D - d0, row.some());
     const T* orow = reinterpret_cast<const T*>(p.o_in) + b * p.oi_b + h * p.oi_h + qc * p.oi_t;
 #pragma unroll
@@ -329,8 +328,7 @@ __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_
   if (p.causal) end = min(end, max(p.Tq + off, 0));  // past the last query's reach
   const bool ok = key < end && !(mask && mask[kc]);
   Stationary<T, S::DA, S::RAW> k, v;
-  k.load(reinterpret_cast<const T*>(p.k) + b * p.k_b + kvh * p.k_h + kc * p.k_t + d0, half, p.D - d0, ok);
-  k.flip(p.flip);
+  k.load(reinterpret_cast<const T*>(p.k) + b * p.k_b + kvh * p.k_h + kc * p.k_t + d0, half, p.D - d0, ok, p.flip);
   v.load(reinterpret_cast<const T*>(p.v) + b * p.v_b + kvh * p.v_h + kc * p.v_t + d0, half, p.D - d0, ok);
   f32x16 dk[S::DT] = {}, dv[S::DT] = {};
   // under causality queries before key - off see nothing of this block

@@ -102,8 +102,7 @@ __global__ __launch_bounds__((ForwardShape<T, DP, WIDE>::THREADS), (ForwardShape
   const T* vb = reinterpret_cast<const T*>(p.v) + b * p.v_b + kvh * p.v_h;
   const uint8_t* mask = p.key_mask ? p.key_mask + b * p.mask_b : nullptr;
   Stationary<T, DP, S::RAW> q;
-  q.load(reinterpret_cast<const T*>(p.q) + b * p.q_b + h * p.q_h + min(qi, p.Tq - 1) * p.q_t, half, p.D, true);
-  q.flip(p.flip);
+  q.load(reinterpret_cast<const T*>(p.q) + b * p.q_b + h * p.q_h + min(qi, p.Tq - 1) * p.q_t, half, p.D, true, p.flip);
   const int lut_len = 2 * p.max_distance + 1;
   const float* my_lut = lut;
   if constexpr (BIAS) {

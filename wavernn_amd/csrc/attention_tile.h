@@ -87,6 +87,16 @@ template <class T>
 struct Raw {  // 8 elements as they come from memory
   typedef T vec __attribute__((ext_vector_type(8)));
   vec x;
+  // the values' signs changed where `sign` is the sign bit.  (Here and not in the planes of a float32 operand: there it costs the forward pass 7 %.)
+  __device__ __forceinline__ void flip(uint32_t sign) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(__float_as_uint(x[e]) ^ sign);
+    } else {
+      typedef uint32_t bits __attribute__((ext_vector_type(4)));
+      x = __builtin_bit_cast(vec, __builtin_bit_cast(bits, x) ^ (sign | sign >> 16));
+    }
+  }
 };
 
 __device__ __forceinline__ Operand<__bf16> operand(const Raw<__bf16>& r) { return {{r.x}}; }
@@ -231,38 +241,28 @@ template <class T, int DP, bool RAW>
 struct Stationary {
   static constexpr int NC2 = DP / 16;
   Operand<T> o[NC2];
-  __device__ __forceinline__ void load(const T* row, int half, int D, bool ok) {
+  __device__ __forceinline__ void load(const T* row, int half, int D, bool ok, uint32_t flip = 0) {
 #pragma unroll
     for (int c = 0; c < NC2; ++c) {
       Raw<T> r = load_chunk<T>(row, 2 * c + half, D);
       if (!ok) r.x = {};
+      r.flip(flip);
       o[c] = operand(r);
     }
   }
   __device__ __forceinline__ const Operand<T>& get(int c) const { return o[c]; }
-  __device__ __forceinline__ void flip(uint32_t sign) {
-#pragma unroll
-    for (int c = 0; c < NC2; ++c)
-#pragma unroll
-      for (int n = 0; n < Type<T>::NP; ++n) o[c].p[n] = __builtin_bit_cast(bf16x8, __builtin_bit_cast(u32x4, o[c].p[n]) ^ (sign | sign >> 16));
-  }
 };
 template <class T, int DP>
 struct Stationary<T, DP, true> {
   static constexpr int NC2 = DP / 16;
   Raw<T> o[NC2];
-  __device__ __forceinline__ void load(const T* row, int half, int D, bool ok) {
+  __device__ __forceinline__ void load(const T* row, int half, int D, bool ok, uint32_t flip = 0) {
 #pragma unroll
     for (int c = 0; c < NC2; ++c) {
       o[c] = load_chunk<T>(row, 2 * c + half, D);
       if (!ok) o[c].x = {};
+      o[c].flip(flip);
     }
-  }
-  __device__ __forceinline__ void flip(uint32_t sign) {
-#pragma unroll
-    for (int c = 0; c < NC2; ++c)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) o[c].x[e] = __uint_as_float(__float_as_uint(o[c].x[e]) ^ sign);
   }
   // the constants are hidden from the compiler, or it moves the conversion out of the loop and its results to memory
   __device__ __forceinline__ Operand<T> get(int c) const {
