@@ -140,3 +140,15 @@ def test_multi_speaker_model_with_the_position_bias_on_either_path():
     for k in gen["stock"]:
         assert gen["stock"][k].shape == gen["fused"][k].shape
         assert G.rel_err(gen["fused"][k].cpu().numpy(), gen["stock"][k].cpu().numpy()) < 1e-4, k
+
+
+def test_autocast_leaves_float64_alone():
+    """It casts no float64, so the projections' results are not of autocast's type."""
+    b = block()
+    torch.set_autocast_enabled("cuda", True)
+    torch.set_autocast_dtype("cuda", torch.bfloat16)
+    try:
+        assert b._why_not_fused(on_the_gpu(), None) is None
+        assert "float64" in b._why_not_fused(on_the_gpu(torch.float64), None)
+    finally:
+        torch.set_autocast_enabled("cuda", False)

@@ -74,7 +74,7 @@ class FFTBlock(nn.Module):  # common_layers.py:148-185: post-norm self-attention
     def _why_not_fused(self, src, src_pad_mask, position_bias=None) -> Optional[str]:
         if src.device.type != 'cuda':
             return "it runs only on an MI355X (HIP) device"
-        dtype = torch.get_autocast_dtype('cuda') if torch.is_autocast_enabled('cuda') else src.dtype
+        dtype = torch.get_autocast_dtype('cuda') if torch.is_autocast_enabled('cuda') and src.dtype != torch.float64 else src.dtype
         if dtype not in (torch.float32, torch.bfloat16):
             return f"it takes float32 or bfloat16, not {dtype}"
         if src_pad_mask is not None and src_pad_mask.dtype != torch.bool:
