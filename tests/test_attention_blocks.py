@@ -152,3 +152,19 @@ def test_autocast_leaves_float64_alone():
         assert "float64" in b._why_not_fused(on_the_gpu(torch.float64), None)
     finally:
         torch.set_autocast_enabled("cuda", False)
+
+
+def test_a_position_bias_of_ones_own_survives_copies():
+    """One that is no module: copies and pickles keep it."""
+    t, x = transformer(), torch.randn(2, 7, 32)
+    t.position_bias = Slope()
+    want = t(x)
+    for c in (copy.deepcopy(t), pickle.loads(pickle.dumps(t))):
+        assert torch.equal(c(x), want)
+    assert not torch.equal(transformer()(x), want)
+
+
+class Slope:
+
+    def __call__(self, q_len, k_len):
+        return -0.3 * (torch.arange(k_len) - torch.arange(q_len)[:, None]).abs().expand(2, q_len, k_len)

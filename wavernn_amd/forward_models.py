@@ -153,7 +153,7 @@ class ForwardTransformer(nn.Module):  # common_layers.py:188-223
     def __setstate__(self, state):
         super().__setstate__(state)
         if 'position_bias' not in self._modules:      # none, or pickled before there were any
-            self.position_bias = None
+            self.__dict__.setdefault('position_bias', None)
 
     def set_attention_path(self, path: str) -> 'ForwardTransformer':
         return set_attention_path(self, path)
