@@ -168,3 +168,9 @@ class Slope:
 
     def __call__(self, q_len, k_len):
         return -0.3 * (torch.arange(k_len) - torch.arange(q_len)[:, None]).abs().expand(2, q_len, k_len)
+
+
+def test_the_fused_path_takes_the_library_s_position_bias_alone():
+    b = block()
+    assert b._why_not_fused(on_the_gpu(), None, FM.RelativePositionBias(2)) is None
+    assert "RelativePositionBias" in b._why_not_fused(on_the_gpu(), None, Slope())

@@ -86,6 +86,8 @@ class FFTBlock(nn.Module):  # common_layers.py:148-185: post-norm self-attention
             return "it would not call the hooks on self_attn"
         if a.head_dim > MAX_HEAD_DIM:
             return f"head dimension {a.head_dim} is over {MAX_HEAD_DIM}"
+        if not isinstance(position_bias, (RelativePositionBias, type(None))):
+            return f"it takes a RelativePositionBias, not a {type(position_bias).__name__}"
         if torch._C._are_functorch_transforms_active():
             return "it does not go through the transforms of torch.func"
         if has_tangents(src, a.in_proj_weight, a.in_proj_bias, None if position_bias is None else position_bias.weight):
@@ -128,7 +130,7 @@ def set_attention_path(module: nn.Module, path: str) -> nn.Module:
     'stock'  nn.MultiheadAttention (the default);
     'fused'  wavernn_amd.attention, forward and backward: the scores never reach memory; an error where it does not apply (training with
              dropout > 0, which it has none of; head dimensions over 256; types other than float32 and bfloat16; masks that are not bool;
-             hooks on self_attn, which is not called; forward-mode derivatives and the transforms of torch.func);
+             hooks on self_attn, which is not called; position biases of another kind than RelativePositionBias; forward-mode derivatives and the transforms of torch.func);
     'auto'   'fused' where it applies, 'stock' elsewhere.
     They agree to rounding, but for batch rows whose every position is masked: 'stock' gives NaN there, 'fused' attends to nothing."""
     if path not in ATTENTION_PATHS:
