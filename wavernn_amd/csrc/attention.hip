@@ -28,7 +28,8 @@ static int lut_floats(const Params& p) { return p.table ? 2 * p.max_distance + 1
 // Workgroups that share one block of stationary rows, each with part of the `tiles` of the other side: as many as fill the compute units,
 // none with fewer than `least` tiles (1 x 2 heads, 128 x 128 x 128 in bfloat16: 13.5 us undivided, 17.7 with shares of two tiles, for the joining
 // launch).  Where the blocks alone fill the compute units one and a bit times, dividing them evens the last round out but
-// costs more than that gives: 32 x 2 heads, 640 x 640 x 128 in float32 102 us, 121 with two shares, 119 with three.
+// costs more than that gives: 32 x 2 heads, 640 x 640 x 128 in float32 102 us, 121 with two shares, 119 with three.  A compute unit counts as one
+// place, also for the kernels of which it holds two.
 static int shares(int64_t blocks, int64_t tiles, int least) {
   const int64_t want = kComputeUnits / (blocks > 0 ? blocks : 1), most = tiles / least;
   const int64_t n = want < most ? want : most;

@@ -7,12 +7,12 @@
 // in place of the five of a form that adds dq up in memory.
 //
 // Bound by the matrix instructions (the rates count all seven products):
-//   bfloat16  2 x 16 heads, 4096 x 4096 x 128  1247 us  771 TFLOP/s (a library product of 8192 x 8192 x 8192: 1173)
-//                                     x 64      623 us  772, and the eighth product of dS's second plane
-//             2 x 8 heads,  4096 x 4096 x 256  2300 us  420
-//   float32   2 x 16 heads, 2048 x 2048 x 128  1295 us  186 (six partial products: 195 is the library product's sixth)
-//                                     x 64      664 us  181
-//             2 x 8 heads,  2048 x 2048 x 256  1780 us  135
+//   bfloat16  2 x 16 heads, 4096 x 4096 x 128  1291 us  745 TFLOP/s (a library product of 8192 x 8192 x 8192: 1173)
+//                                     x 64      629 us  764, and the eighth product of dS's second plane
+//             2 x 8 heads,  4096 x 4096 x 256  2459 us  391
+//   float32   2 x 16 heads, 2048 x 2048 x 128  1317 us  183 (six partial products: 195 is the library product's sixth)
+//                                     x 64      663 us  181
+//             2 x 8 heads,  2048 x 2048 x 256  1749 us  138
 // Past 128 columns one tile buffer is all that fits in float32, so its conversion is not hidden, and the two waves of a row meet twice a round.
 #pragma once
 #include "attention_tile.h"
@@ -152,10 +152,10 @@ __device__ __forceinline__ void products_shadow(const char* x, const char* y, co
 
 // dq: queries stationary, key tiles through LDS.  delta = rowsum(dout * out) carries the rounding of out and of the probabilities behind it.  The table's
 // gradient adds it up over all rows in the buckets that hold most of a row's keys, and in bfloat16 dk shows it: with few keys (2.8e-3 of its
-// norm, without 2.4e-3), and at any length where the values lie far from zero beside their spread (30 +- 1: 3 .. 6e-2, without 2.3e-3).
+// norm, without 2.4e-3), and at any length where the values lie far from zero beside their spread (30 +- 1: 3 .. 6e-2, without 2.4e-3).
 // There the kernel also sums dS over each row - what delta is off by, as the probabilities add up to one - and the next kernel, which makes dk, dv and the
 // table's gradient, works with the corrected delta, the sum of the shares' planes: a second walk over the keys for it took twice the
-// time.  dq itself keeps the uncorrected delta.
+// time.  dq itself keeps the uncorrected delta, and is off by 4e-2 .. 1e-1 of its norm with such values.
 template <class T, int DP, int BIAS>
 __global__ __launch_bounds__(256, (BackwardShape<T, DP>::WAVES)) void attention_dq_kernel(Params p) {
   using S = BackwardShape<T, DP>;

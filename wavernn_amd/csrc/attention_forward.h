@@ -5,14 +5,14 @@
 //
 // Long sequences are bound by the matrix instructions and, the fewer columns the more, by the softmax's vector instructions between them (bfloat16
 // at 128 columns: 120 of those to 16 products a subtile).  Measured, forward only:
-//   bfloat16  2 x 16 heads, 4096 x 4096 x 128   302 us  910 TFLOP/s (a library product of 8192 x 8192 x 8192: 1173)
-//                                     x 64      183 us  750
-//             2 x 8 heads,  4096 x 4096 x 256   410 us  670
-//   float32   2 x 16 heads, 2048 x 2048 x 128   368 us  187 (six partial products: 195 is the library product's sixth)
-//                                     x 64      186 us  185
-//             2 x 8 heads,  2048 x 2048 x 256   457 us  150
-// Single tokens over a cache are bound by the reading of it: 8 rows, 16 heads on 4, 8191 keys of 128 columns in bfloat16 32 us, the joining kernel's 4
-// included (134 MB at 4.2 TB/s; a large copy moves 4.8).
+//   bfloat16  2 x 16 heads, 4096 x 4096 x 128   291 us  944 TFLOP/s (a library product of 8192 x 8192 x 8192: 1173)
+//                                     x 64      173 us  795
+//             2 x 8 heads,  4096 x 4096 x 256   412 us  667
+//   float32   2 x 16 heads, 2048 x 2048 x 128   354 us  194 (six partial products: 195 is the library product's sixth)
+//                                     x 64      178 us  193
+//             2 x 8 heads,  2048 x 2048 x 256   445 us  154
+// Single tokens over a cache are bound by the reading of it: 8 rows, 16 heads on 4, 8191 keys of 128 columns in bfloat16 31 us, the joining kernel's 4
+// included (134 MB at 4.3 TB/s; a large copy moves 4.8); in float32 104 us.
 #pragma once
 #include "attention_tile.h"
 

@@ -10,7 +10,8 @@ signatures.  The transformer blocks, predictors and projections are per-utteranc
 ops, written here from the reference's behaviour (models/common_layers.py:127-240); the expand runs in
 libwrnn_mi355.so (``LengthRegulator``), and so do the frame-recurrent ``lstm`` of the multispeaker
 ForwardTacotron (``BiLSTM``) and every CBHG / predictor GRU (``BiGRU``).  Those are forward/inference only; the transformer blocks
-can be trained.
+can be trained by themselves, in a ``TransformerPredictor`` and in ``postnet``.  ``LengthRegulator`` passes no gradient on: a loss on the
+mel spectrogram of a whole model gives what lies before it (prenet, embedding, the pitch and energy projections) none, without an error.
 
 The blocks' self-attention runs on ``nn.MultiheadAttention`` ('stock', the default) or in libwrnn_mi355.so, forward and backward
 (``set_attention_path``).  Build extension, not in the reference: ``rel_buckets`` > 0 gives each transformer a learned relative
