@@ -150,3 +150,21 @@ def test_traces_compute_on_their_inputs(grad, D):
         traced = torch.jit.trace(lambda x: A.attention(x, k, v, bias_table=table) * 2, (normal(0, 1, 2, 5, D).requires_grad_(grad),), check_trace=False)
         x = normal(4, 1, 2, 5, D)
         assert torch.equal(traced(x), A.attention(x, k, v, bias_table=table) * 2)
+
+
+def test_copies_of_rows_are_in_the_kernels_form():
+    """Whatever a tensor's strides and however few elements it has: what is not taken as it is comes back contiguous."""
+    wide = torch.zeros(2, 5, 3, 19)
+    for t in (wide[..., 1:17].permute(0, 2, 1, 3)[:, :, :0], wide[:, :1, :, 1:17].permute(0, 2, 1, 3), wide[:0, ..., 1:17], wide.flatten()[1:97].view(1, 2, 3, 16)):
+        rows = A._rows(t)
+        assert rows.shape == t.shape and torch.equal(rows, t)
+        assert all(s % 4 == 0 for s, n in zip(rows.stride()[:3], rows.shape) if n != 1) and rows.stride(3) == 1 and rows.data_ptr() % 16 == 0
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_no_keys_in_a_slice_of_odd_rows(dtype):
+    q = normal(0, 3, 16, 4, 99, dtype=dtype)[..., 1:97].permute(0, 2, 1, 3).requires_grad_()
+    k = normal(1, 3, 16, 2, 99, dtype=dtype)[:, :0, :, 1:97].permute(0, 2, 1, 3)
+    out = A.attention(q, k, k)
+    assert not out.any() and not torch.autograd.grad(out, q, torch.ones_like(out))[0].any()
