@@ -168,3 +168,24 @@ def test_no_keys_in_a_slice_of_odd_rows(dtype):
     k = normal(1, 3, 16, 2, 99, dtype=dtype)[:, :0, :, 1:97].permute(0, 2, 1, 3)
     out = A.attention(q, k, k)
     assert not out.any() and not torch.autograd.grad(out, q, torch.ones_like(out))[0].any()
+
+
+@pytest.mark.parametrize("D", [5, 6, 13, 16])
+def test_padded_copies_of_rows_with_the_heads_innermost(D):
+    """torch pads a tensor in the order in memory that it finds."""
+    t = torch.randn(2, 3, 4, D).to(memory_format=torch.channels_last)
+    rows = A._rows(t)
+    assert rows.is_contiguous() and torch.equal(rows[..., :D], t) and not rows[..., D:].any()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("D", [5, 13, 16])
+def test_heads_innermost(dtype, D):
+    q, k, v, dout = (normal(i, 2, 3, 9, D, dtype=dtype) for i in range(4))
+    inner = [x.to(memory_format=torch.channels_last).requires_grad_() for x in (q, k, v)]
+    got = A.attention(*inner)
+    want = A.attention(*(x.requires_grad_() for x in (q, k, v)))
+    assert torch.equal(got, want)
+    for a, b in zip(torch.autograd.grad(got, inner, dout.to(memory_format=torch.channels_last)), torch.autograd.grad(want, (q, k, v), dout)):
+        assert torch.equal(a, b)

@@ -77,7 +77,8 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
             and not ((s[0] % 4 and n[0] != 1) or (s[1] % 4 and n[1] != 1) or (s[2] % 4 and n[2] != 1))):
         return t
     pad = max(-n[3] % 4, 16 // t.element_size() - n[3])
-    return nn.functional.pad(t, (0, pad)) if pad else t.clone(memory_format=torch.contiguous_format)
+    # (pad keeps the order of a tensor whose heads lie innermost)
+    return nn.functional.pad(t, (0, pad)).contiguous() if pad else t.clone(memory_format=torch.contiguous_format)
 
 
 @functools.lru_cache(maxsize=1024)
