@@ -3,6 +3,7 @@ float32 past 128, masks whose tail spans several scans, the second plane of dS."
 import pytest
 import torch
 
+from attention_ref import buckets, check, reference
 from test_attention import BF16, F32, normal, run_case
 from wavernn_amd import attention as A
 
@@ -56,3 +57,47 @@ def test_score_gradients_in_two_planes(D, Tk):
     dp = x[3] @ x[2].transpose(-1, -2)
     want = (p * (dp - (p * dp).sum(-1, keepdim=True))) @ x[1] / D ** 0.5
     assert float((got - want).norm() / want.norm()) < torch.finfo(BF16).eps / 2 / 3 ** 0.5
+
+
+@gpu
+@pytest.mark.parametrize("Tq", [1, 40])
+def test_offsets_past_32_bits(Tq):
+    """A cache of 2.5e9 elements of which the last keys alone are left: the same as those keys by themselves (which another number of workgroups
+    sums in another order: the bounds are run_case's on both sides), gradients in their places, everything before them untouched by NaN."""
+    H, Tk, D, last = 32, 600_001, 128, 100
+    cache = torch.empty(1, Tk, H, D, dtype=BF16, device="cuda")
+    assert cache.numel() > 2 ** 31
+    cache[:, ::1000] = float("nan")
+    cache[:, -last:] = normal(1, 1, last, H, D, dtype=BF16)
+    k = cache.permute(0, 2, 1, 3)
+    q, dout = normal(0, 1, H, Tq, D, dtype=BF16), normal(2, 1, H, Tq, D, dtype=BF16)
+    mask = torch.arange(Tk, device="cuda")[None] < Tk - last
+    few = k[:, :, -last:].contiguous()
+    want = reference(q, few, few, dout)
+    leaves = [q.requires_grad_(), k.requires_grad_()]
+    out = A.attention(q, k, k, key_mask=mask)
+    check("out", out, want["out"])
+    dq, dk = torch.autograd.grad(out, leaves, dout)
+    check("dq", dq, want["dq"])
+    # dk + dv, added up in bfloat16 by autograd
+    value = want["dk"][0] + want["dv"][0]
+    check("dk + dv", dk[:, :, -last:], (value, want["dk"][1] + want["dv"][1] + torch.finfo(BF16).eps / 2 * (want["dk"][0].abs() + want["dv"][0].abs())))
+    assert not dk[:, :, :-last].any()
+
+
+@gpu
+def test_dense_bias_past_32_bits():
+    """3.2e9 values: the last rows, and the gradient of their sum, which counts the pairs of each bucket (whole numbers below 2^24 a workgroup,
+    then 64 bits; half a step of bfloat16 where it is stored)."""
+    H, T = 3, 32768
+    table = normal(0, 32, H, dtype=BF16).requires_grad_()
+    out = A.relative_position_bias(table, T, T)
+    rel = torch.arange(T) - (T - 1)
+    which = buckets(rel, 32, 128, True)
+    assert torch.equal(out[-1, -1].cpu(), table.detach()[:, -1].cpu()[which])
+    ahead = buckets(-rel, 32, 128, True)                      # of distances 0 .. T - 1 ahead, T - distance pairs each
+    pairs = (T + rel).double()
+    count = torch.zeros(32, dtype=torch.float64).index_add_(0, which, pairs)
+    count.index_add_(0, ahead[:-1], pairs[:-1])
+    got = torch.autograd.grad(out, table, torch.ones((), dtype=BF16, device="cuda").expand_as(out))[0].double().cpu()
+    assert bool(((got - count[:, None]).abs() <= torch.finfo(BF16).eps / 2 * count[:, None]).all())
