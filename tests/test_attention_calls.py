@@ -2,6 +2,7 @@
 past what the kernels count in, rules made at the same time."""
 import ctypes as C
 import gc
+import threading
 import weakref
 
 import pytest
@@ -189,3 +190,36 @@ def test_heads_innermost(dtype, D):
     assert torch.equal(got, want)
     for a, b in zip(torch.autograd.grad(got, inner, dout.to(memory_format=torch.channels_last)), torch.autograd.grad(want, (q, k, v), dout)):
         assert torch.equal(a, b)
+
+
+@gpu
+def test_calls_from_several_threads_and_streams_at_once():
+    """Each with a rule, sizes and a stream of its own: the bits of the calls one after the other."""
+    def case(n):
+        D, Tq, Tk = (16, 64, 100, 200)[n], (3, 70, 200, 40)[n], (900, 70, 300, 500)[n]
+        leaves = [normal(10 * n + i, 2, 4, Tq if i == 0 else Tk, D, dtype=(F32, BF16)[n % 2]).requires_grad_() for i in range(3)]
+        leaves.append(normal(10 * n + 3, 16, 4).requires_grad_())
+        return leaves, normal(10 * n + 4, 2, 4, Tq, D, dtype=(F32, BF16)[n % 2])
+
+    def step(leaves, dout, n, k):
+        out = A.attention(*leaves[:3], bias_table=leaves[3], max_distance=40 + n + 4 * k)
+        return [out.detach(), *torch.autograd.grad(out, leaves, dout)]
+
+    cases = [case(n) for n in range(4)]
+    want = [[step(*c, n, k) for k in range(20)] for n, c in enumerate(cases)]
+    torch.cuda.synchronize()
+    got = [None] * 4
+
+    def work(n):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got[n] = [step(*cases[n], n, k) for k in range(20)]
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(n,)) for n in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for a, b in zip(got, want):
+        for x, y in zip(a, b):
+            assert all(torch.equal(u, v) for u, v in zip(x, y))
